@@ -417,6 +417,31 @@ int cvh_embed_lookup_fwd(int dtype, const long long* tok, const float* table, co
 int cvh_embed_lookup_bwd(int dtype, const long long* tok, const void* dout, float* dtable, long long rows, int E, long long padding_idx,
                          void* stream);
 
+/* ---- attention over packed sequences ------------------------------------------------------------- */
+/* Softmax attention of sequences that lie one behind the other in the rows of q / k / v: sequence b has the rows cu[b] .. cu[b + 1] - 1.
+ * q [rows][heads_q][d], k / v [rows][heads_kv][d], heads_q % heads_kv == 0 (query head h reads key head h / (heads_q / heads_kv)); *_row and
+ * *_head are strides in elements; the d elements of a head are contiguous, d % 8 == 0, d <= 128; 16-byte aligned bases and strides.  Rows at or
+ * behind cu[seqs] are read by nothing; their results are zeros.  lse [heads_q][rows] (log2 of the softmax sums, with the maxima) is written by the
+ * forward and read by the backward, delta [heads_q][rows] is the backward's scratch.  plan: cvh_packed_plan of the same seqs, rows and block. */
+typedef struct cvh_packed_attn {
+  const void *q, *k, *v;
+  void* out; /* forward: written; backward: the forward's result */
+  const void* dout;
+  void *dq, *dk, *dv;
+  float *lse, *delta;
+  const int* plan;
+  long long q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head, dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+  int rows, seqs, heads_q, heads_kv, d, causal, block, places;
+  float scale; /* > 0 */
+} cvh_packed_attn;
+/* Work list of a batch of packed sequences in blocks of 32 or 128 rows: int32 plan[cvh_packed_plan_elems(...)] from cu[seqs + 1] (device, int32).
+ * Boundaries outside 0 .. rows are clamped and falling ones lifted to the largest before them, so that no list leads out of the buffers;
+ * `places` of the struct above is rows / block + seqs + 1.  Made once per batch, read by every layer and both directions. */
+long long cvh_packed_plan_elems(int seqs, int rows, int block);
+int cvh_packed_plan(const int* cu, int seqs, int rows, int block, int* plan, void* stream);
+int cvh_packed_attn_fwd(int dtype, const cvh_packed_attn* p, void* stream);
+int cvh_packed_attn_bwd(int dtype, const cvh_packed_attn* p, void* stream);
+
 /* ---- LayerNorm over channels -------------------------------------------------------------------- */
 /* Replaces nn.LayerNorm, channel-last branch (cvnets/layers/normalization/layer_norm.py:67-68). */
 int cvh_layernorm_fwd(int dtype, const void* x, const float* gamma, const float* beta, void* y, float* mean, float* rstd,

@@ -1,0 +1,673 @@
+// Softmax attention over PACKED sequences of different lengths (grouped query heads, causal or not), forward + backward, on MFMA.
+//
+//   s_ij = scale q_i . k_j  (j in i's sequence, j <= i when causal)    p = softmax_j(s)    o_i = sum_j p_ij v_j
+//   dv_j = sum_i p_ij do_i     ds_ij = p_ij (do_i . v_j - delta_i),  delta_i = do_i . o_i     dq_i = scale sum_j ds_ij k_j     dk_j = scale sum_i ds_ij q_i
+//
+// q [rows][hq][d], k / v [rows][hkv][d] (any row / head stride, d contiguous); the sequences lie one behind the other, sequence b in rows
+// cu[b] .. cu[b + 1] - 1.  The scores never reach memory: one pass over the keys with a running maximum and sum (forward), and a
+// recomputation from the stored log-sum in the two backward kernels.  dk / dv of a key head are summed over its query heads inside ONE
+// workgroup (a loop over the group), so nothing is accumulated with atomics and every result is bit-reproducible.
+//
+// A wave owns 32 queries (forward, dq) or 32 keys (dk / dv) and forms TRANSPOSED products: S^T = K Q^T has the query along lane & 31, so the
+// softmax statistics are per-lane scalars, and the accumulator rows of P^T are the contraction index of O^T = V^T P^T: the probabilities go
+// from accumulator to operand registers and never touch LDS.  The waves of a workgroup share the staged K / V (or Q / dO) tiles, which are
+// double-buffered in LDS and loaded a tile ahead through registers.
+//
+// Work items come from a plan (packed_plan_kernel) made once per batch: (sequence, block) pairs, most expensive first, so that the last
+// workgroups to start are the short ones; the list also has the rows behind the last sequence, whose results are written as zeros.
+#include "common.hpp"
+#include "cvnets_hip.h"
+
+namespace {
+
+typedef cvh_packed_attn PA;
+
+__device__ __forceinline__ float pexp2(float x) { return __builtin_amdgcn_exp2f(x); }
+constexpr float kL2E = 1.4426950408889634f;
+
+template <typename T> struct Chunk;  // 16 bytes
+template <> struct Chunk<bf16_t> {
+  static constexpr int N = 8;
+};
+template <> struct Chunk<float> {
+  static constexpr int N = 4;
+};
+__device__ __forceinline__ uint4 keep16(uint4 v, bool ok) {
+  const uint32_t m = ok ? 0xffffffffu : 0u;
+  return make_uint4(v.x & m, v.y & m, v.z & m, v.w & m);
+}
+
+// one MFMA operand (32 rows x 16 columns) straight from global memory: lane l holds columns k0 + 8 (l >> 5) .. + 7 of row (l & 31)
+__device__ __forceinline__ Frag<bf16_t> gfrag(const bf16_t* row, int c0, int d, bool ok) {
+  const bool in = ok && c0 < d;
+  const uint4 v = *reinterpret_cast<const uint4*>(row + (in ? c0 : 0));
+  Frag<bf16_t> f;
+  f.v = __builtin_bit_cast(bf16x8_t, keep16(v, in));
+  return f;
+}
+__device__ __forceinline__ Frag<float> gfrag(const float* row, int c0, int d, bool ok) {
+  const bool in = ok && c0 < d;
+  const float4 a = *reinterpret_cast<const float4*>(row + (in ? c0 : 0)), b = *reinterpret_cast<const float4*>(row + (in ? c0 + 4 : 0));
+  Frag<float> f;
+  f.v[0] = in ? a.x : 0.f; f.v[1] = in ? a.y : 0.f; f.v[2] = in ? a.z : 0.f; f.v[3] = in ? a.w : 0.f;
+  f.v[4] = in ? b.x : 0.f; f.v[5] = in ? b.y : 0.f; f.v[6] = in ? b.z : 0.f; f.v[7] = in ? b.w : 0.f;
+  return f;
+}
+__device__ __forceinline__ float frag_dot(const Frag<bf16_t>& a, const Frag<bf16_t>& b) {
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s += (float)a.v[j] * (float)b.v[j];
+  return s;
+}
+__device__ __forceinline__ float frag_dot(const Frag<float>& a, const Frag<float>& b) {
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s += a.v[j] * b.v[j];
+  return s;
+}
+
+// A tile of NROWS consecutive rows, loaded by NT threads into registers (load: only issues the reads) and written to LDS (store).  Rows at or
+// behind `live` and columns at or behind `d` become zeros: a masked probability is 0, and 0 times whatever another sequence holds there has to be 0.
+template <typename T, int CP, int NROWS, int NT> struct RowTile {
+  static constexpr int VN = Chunk<T>::N, CH = CP / VN, IT = (NROWS * CH + NT - 1) / NT;
+  static constexpr bool EXACT = (NROWS * CH) % NT == 0;
+  uint4 q[IT];
+  unsigned ok;
+  __device__ __forceinline__ void load(const T* __restrict__ base, long long row_stride, int live, int d, int tid) {
+    ok = 0;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int idx = tid + i * NT, r = idx / CH, c = (idx % CH) * VN;
+      const bool in = (EXACT || idx < NROWS * CH) && r < live && c < d;
+      ok |= (in ? 1u : 0u) << i;
+      q[i] = *reinterpret_cast<const uint4*>(base + (in ? (long long)r * row_stride + c : 0ll));
+    }
+  }
+  __device__ __forceinline__ void store(T* lds, int pitch, int tid) const {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int idx = tid + i * NT, r = idx / CH, c = (idx % CH) * VN;
+      if (EXACT || idx < NROWS * CH) *reinterpret_cast<uint4*>(lds + r * pitch + c) = keep16(q[i], (ok >> i) & 1u);
+    }
+  }
+};
+
+// operand fragment of the TRANSPOSE of a [k][n] LDS tile, the contraction index in the order in which a 32x32 accumulator holds its rows:
+// slot j of lane half h is tile row k0 + 8 (j >> 2) + 4 h + (j & 3).  bf16: two LDS transpose reads (lane 4r + q of a 16-lane group gives the
+// address of 4 columns of block row r and receives column 4r + q of the 4 x 16 block).
+typedef short v4s_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ Frag<bf16_t> tfrag(const bf16_t* tile, int pitch, int k0, int col0, int lane) {
+  const int i = lane & 15;
+  const bf16_t* p = tile + (k0 + 4 * (lane >> 5) + (i >> 2)) * pitch + col0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+  const v4s_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*)(p));
+  const v4s_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*)(p + 8 * pitch));
+  Frag<bf16_t> f;
+  f.v = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  return f;
+}
+__device__ __forceinline__ Frag<float> tfrag(const float* tile, int pitch, int k0, int col0, int lane) {
+  const float* p = tile + (k0 + 4 * (lane >> 5)) * pitch + col0 + (lane & 31);
+  Frag<float> f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f.v[j] = p[((j & 3) + 8 * (j >> 2)) * pitch];
+  return f;
+}
+// rows 16 t .. 16 t + 15 (in that order) of an accumulator as an operand.  bf16: the one rounding of P / dS to 8 bits, each probability off by
+// at most 2^-9 of itself; the sums it enters stay in 32 bits.
+template <typename T> __device__ __forceinline__ Frag<T> acc_frag(const f32x16_t& a, int t);
+template <> __device__ __forceinline__ Frag<bf16_t> acc_frag<bf16_t>(const f32x16_t& a, int t) {
+  Frag<bf16_t> f;
+  f.v = __builtin_bit_cast(bf16x8_t, make_uint4(f2bf_pk(a[8 * t], a[8 * t + 1]), f2bf_pk(a[8 * t + 2], a[8 * t + 3]), f2bf_pk(a[8 * t + 4], a[8 * t + 5]),
+                                                f2bf_pk(a[8 * t + 6], a[8 * t + 7])));
+  return f;
+}
+template <> __device__ __forceinline__ Frag<float> acc_frag<float>(const f32x16_t& a, int t) {
+  Frag<float> f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f.v[j] = a[8 * t + j];
+  return f;
+}
+
+// 4 consecutive columns of one row
+template <typename T> __device__ __forceinline__ void store4(T* p, const float* f) {
+  V4<T> v;
+  v4_pack(f, v);
+  v4_store<T>(p, v);
+}
+
+struct Item {
+  int seq, block, head, start, len;
+};
+// work item of this workgroup.  Blocks are dealt out tile by tile with the heads fastest: when the head count is a multiple of the 8 XCDs (block
+// b runs on XCD b % 8) neighbouring heads - the query heads of one key head - stay on one XCD and share its L2.
+__device__ __forceinline__ Item work_item(const PA& p, int heads) {
+  const int slot = blockIdx.x % heads, tile = blockIdx.x / heads;
+  Item w;
+  w.head = heads % 8 == 0 ? (slot & 7) * (heads >> 3) + (slot >> 3) : slot;
+  const int* list = p.plan + ((p.seqs + 2) & ~1);
+  w.seq = list[2 * tile];
+  w.block = list[2 * tile + 1];
+  w.start = w.seq >= 0 ? p.plan[w.seq] : p.plan[p.seqs];
+  w.len = (w.seq >= 0 ? p.plan[w.seq + 1] : p.rows) - w.start;
+  return w;
+}
+// rows behind the last sequence: zeros
+template <typename T> __device__ __forceinline__ void zero_rows(T* base, long long row_stride, int r0, int n, int d, int tid, int nt) {
+  constexpr int VN = Chunk<T>::N;
+  const int ch = d / VN;
+  for (int i = tid; i < n * ch; i += nt)
+    *reinterpret_cast<uint4*>(base + (long long)(r0 + i / ch) * row_stride + (i % ch) * VN) = make_uint4(0, 0, 0, 0);
+}
+
+// -----------------------------------------------------------------------------------------------------------------------------------------
+// forward: workgroup = NW x 32 consecutive queries of one (sequence, query head)
+// -----------------------------------------------------------------------------------------------------------------------------------------
+template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bounds__(64 * NW, OCC) void packed_attn_fwd_kernel(PA p) {
+  constexpr int PT = lds_pitch<T>(CP), NF = CP / 32, NK = CP / 16, NB = KB / 32, NT = 64 * NW;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  T* const Kl = reinterpret_cast<T*>(smem);  // [2][KB][PT]
+  T* const Vl = Kl + 2 * KB * PT;            // [2][KB][PT]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Item w = work_item(p, p.heads_q);
+  if (w.seq < -1) return;
+  T* const out = reinterpret_cast<T*>(p.out) + w.head * p.o_head;
+  const int first = w.block * (32 * NW);
+  if (w.seq < 0) {
+    zero_rows(out + (long long)w.start * p.o_row, p.o_row, first, min(32 * NW, w.len - first), p.d, tid, NT);
+    return;
+  }
+  const int q0 = first + wave * 32, my_q = q0 + (lane & 31);
+  const bool q_ok = my_q < w.len;
+  const int kv_head = w.head / (p.heads_q / p.heads_kv);
+  const T* const kb = reinterpret_cast<const T*>(p.k) + (long long)w.start * p.k_row + kv_head * p.k_head;
+  const T* const vb = reinterpret_cast<const T*>(p.v) + (long long)w.start * p.v_row + kv_head * p.v_head;
+  const int keys = p.causal ? min(w.len, first + 32 * NW) : w.len;
+  const int tiles = (keys + KB - 1) / KB;
+
+  RowTile<T, CP, KB, NT> kt, vt;
+  kt.load(kb, p.k_row, w.len, p.d, tid);
+  vt.load(vb, p.v_row, w.len, p.d, tid);
+  Frag<T> qf[NK];
+  {
+    const T* qrow = reinterpret_cast<const T*>(p.q) + (long long)(w.start + (q_ok ? my_q : 0)) * p.q_row + w.head * p.q_head;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) qf[k] = gfrag(qrow, 16 * k + 8 * (lane >> 5), p.d, q_ok);
+  }
+  kt.store(Kl, PT, tid);
+  vt.store(Vl, PT, tid);
+  if (tiles > 1) {
+    kt.load(kb + (long long)KB * p.k_row, p.k_row, w.len - KB, p.d, tid);
+    vt.load(vb + (long long)KB * p.v_row, p.v_row, w.len - KB, p.d, tid);
+  }
+
+  const float c = p.scale * kL2E;  // scores in powers of two: exp(x) is one v_exp_f32
+  float m = -INFINITY, l = 0.f;    // running maximum (of the unscaled scores) and sum
+  f32x16_t o[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) o[f] = acc_zero();
+
+  for (int t = 0; t < tiles; ++t) {
+    const int k0 = t * KB;
+    wg_barrier_lds();  // tile t is in LDS; everyone is done with tile t - 1, whose buffer tile t + 1 goes into
+    const T* const Kt = Kl + (t & 1) * KB * PT;
+    const T* const Vt = Vl + (t & 1) * KB * PT;
+    if (t + 1 < tiles) {
+      kt.store(Kl + ((t + 1) & 1) * KB * PT, PT, tid);
+      vt.store(Vl + ((t + 1) & 1) * KB * PT, PT, tid);
+    }
+    if (t + 2 < tiles) {
+      kt.load(kb + (long long)(k0 + 2 * KB) * p.k_row, p.k_row, w.len - k0 - 2 * KB, p.d, tid);
+      vt.load(vb + (long long)(k0 + 2 * KB) * p.v_row, p.v_row, w.len - k0 - 2 * KB, p.d, tid);
+    }
+    if (p.causal && k0 > q0 + 31) continue;  // in the future of all of this wave's queries
+    f32x16_t s[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) s[b] = acc_zero();
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) mma32(s[b], lds_frag(Kt, PT, 32 * b, 16 * k, lane), qf[k]);
+    if (k0 + KB > w.len || (p.causal && k0 + KB - 1 > q0)) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = k0 + 32 * b + acc_row(r, lane);
+          s[b][r] = key >= w.len || (p.causal && key > my_q) ? -INFINITY : s[b][r];
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    // key 0 is visible to every query (and to the rows past the end, which count as zeros), so the maximum is finite from the first tile on
+    const float m_new = fmaxf(m, mx);
+    if (__any(m_new > m)) {
+      const float alpha = pexp2((m - m_new) * c);
+      l *= alpha;
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[f][r] *= alpha;
+      m = m_new;
+    }
+    const float mc = m * c;
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[b][r] = pexp2(fmaf(s[b][r], c, -mc));
+        sum += s[b][r];
+      }
+    l += sum;  // this lane's half of the keys; the halves are joined once, at the end
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Frag<T> pf = acc_frag<T>(s[b], h);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) mma32(o[f], tfrag(Vt, PT, 32 * b + 16 * h, 32 * f, lane), pf);
+      }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (!q_ok) return;
+  const float inv = 1.0f / l;
+  T* const orow = out + (long long)(w.start + my_q) * p.o_row;
+#pragma unroll
+  for (int f = 0; f < NF; ++f)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c0 = 32 * f + 8 * i + 4 * (lane >> 5);
+      const float v[4] = {o[f][4 * i] * inv, o[f][4 * i + 1] * inv, o[f][4 * i + 2] * inv, o[f][4 * i + 3] * inv};
+      if (c0 < p.d) store4<T>(orow + c0, v);
+    }
+  if (lane < 32) p.lse[(long long)w.head * p.rows + w.start + my_q] = fmaf(m, c, __log2f(l));
+}
+
+// -----------------------------------------------------------------------------------------------------------------------------------------
+// backward, dq (and delta): workgroup = NW x 32 consecutive queries of one (sequence, query head)
+// -----------------------------------------------------------------------------------------------------------------------------------------
+template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bounds__(64 * NW, OCC) void packed_attn_dq_kernel(PA p) {
+  constexpr int PT = lds_pitch<T>(CP), NF = CP / 32, NK = CP / 16, NB = KB / 32, NT = 64 * NW;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  T* const Kl = reinterpret_cast<T*>(smem);
+  T* const Vl = Kl + 2 * KB * PT;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Item w = work_item(p, p.heads_q);
+  if (w.seq < -1) return;
+  T* const dq = reinterpret_cast<T*>(p.dq) + w.head * p.dq_head;
+  const int first = w.block * (32 * NW);
+  if (w.seq < 0) {
+    zero_rows(dq + (long long)w.start * p.dq_row, p.dq_row, first, min(32 * NW, w.len - first), p.d, tid, NT);
+    return;
+  }
+  const int q0 = first + wave * 32, my_q = q0 + (lane & 31);
+  const bool q_ok = my_q < w.len;
+  const int kv_head = w.head / (p.heads_q / p.heads_kv);
+  const T* const kb = reinterpret_cast<const T*>(p.k) + (long long)w.start * p.k_row + kv_head * p.k_head;
+  const T* const vb = reinterpret_cast<const T*>(p.v) + (long long)w.start * p.v_row + kv_head * p.v_head;
+  const int keys = p.causal ? min(w.len, first + 32 * NW) : w.len;
+  const int tiles = (keys + KB - 1) / KB;
+
+  RowTile<T, CP, KB, NT> kt, vt;
+  kt.load(kb, p.k_row, w.len, p.d, tid);
+  vt.load(vb, p.v_row, w.len, p.d, tid);
+  Frag<T> qf[NK], df[NK];
+  const long long row = w.start + (q_ok ? my_q : 0);
+  float delta = 0.f;
+  {
+    const T* qrow = reinterpret_cast<const T*>(p.q) + row * p.q_row + w.head * p.q_head;
+    const T* drow = reinterpret_cast<const T*>(p.dout) + row * p.do_row + w.head * p.do_head;
+    const T* orow = reinterpret_cast<const T*>(p.out) + row * p.o_row + w.head * p.o_head;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      const int c0 = 16 * k + 8 * (lane >> 5);
+      qf[k] = gfrag(qrow, c0, p.d, q_ok);
+      df[k] = gfrag(drow, c0, p.d, q_ok);
+      delta += frag_dot(df[k], gfrag(orow, c0, p.d, q_ok));
+    }
+  }
+  delta += __shfl_xor(delta, 32, 64);
+  const long long at = (long long)w.head * p.rows + row;
+  const float lse = p.lse[at];
+  if (lane < 32 && q_ok) p.delta[at] = delta;  // read by the dk / dv kernel behind this one
+  kt.store(Kl, PT, tid);
+  vt.store(Vl, PT, tid);
+  if (tiles > 1) {
+    kt.load(kb + (long long)KB * p.k_row, p.k_row, w.len - KB, p.d, tid);
+    vt.load(vb + (long long)KB * p.v_row, p.v_row, w.len - KB, p.d, tid);
+  }
+  const float c = p.scale * kL2E;
+  f32x16_t acc[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) acc[f] = acc_zero();
+
+  for (int t = 0; t < tiles; ++t) {
+    const int k0 = t * KB;
+    wg_barrier_lds();
+    const T* const Kt = Kl + (t & 1) * KB * PT;
+    const T* const Vt = Vl + (t & 1) * KB * PT;
+    if (t + 1 < tiles) {
+      kt.store(Kl + ((t + 1) & 1) * KB * PT, PT, tid);
+      vt.store(Vl + ((t + 1) & 1) * KB * PT, PT, tid);
+    }
+    if (t + 2 < tiles) {
+      kt.load(kb + (long long)(k0 + 2 * KB) * p.k_row, p.k_row, w.len - k0 - 2 * KB, p.d, tid);
+      vt.load(vb + (long long)(k0 + 2 * KB) * p.v_row, p.v_row, w.len - k0 - 2 * KB, p.d, tid);
+    }
+    if (p.causal && k0 > q0 + 31) continue;
+    const bool masked = k0 + KB > w.len || (p.causal && k0 + KB - 1 > q0);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      f32x16_t s = acc_zero(), dp = acc_zero();
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        mma32(s, lds_frag(Kt, PT, 32 * b, 16 * k, lane), qf[k]);
+        mma32(dp, lds_frag(Vt, PT, 32 * b, 16 * k, lane), df[k]);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = pexp2(fmaf(s[r], c, -lse));
+      if (masked) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = k0 + 32 * b + acc_row(r, lane);
+          s[r] = key >= w.len || (p.causal && key > my_q) ? 0.f : s[r];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Frag<T> sf = acc_frag<T>(s, h);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) mma32(acc[f], tfrag(Kt, PT, 32 * b + 16 * h, 32 * f, lane), sf);
+      }
+    }
+  }
+  if (!q_ok) return;
+  T* const orow = dq + row * p.dq_row;
+#pragma unroll
+  for (int f = 0; f < NF; ++f)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c0 = 32 * f + 8 * i + 4 * (lane >> 5);
+      const float v[4] = {acc[f][4 * i] * p.scale, acc[f][4 * i + 1] * p.scale, acc[f][4 * i + 2] * p.scale, acc[f][4 * i + 3] * p.scale};
+      if (c0 < p.d) store4<T>(orow + c0, v);
+    }
+}
+
+// -----------------------------------------------------------------------------------------------------------------------------------------
+// backward, dk and dv: workgroup = NW x 32 consecutive keys of one (sequence, key head); loops over the group's query heads and the queries
+// -----------------------------------------------------------------------------------------------------------------------------------------
+template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bounds__(64 * NW, OCC) void packed_attn_dkv_kernel(PA p) {
+  constexpr int PT = lds_pitch<T>(CP), NF = CP / 32, NK = CP / 16, NB = QB / 32, NT = 64 * NW;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  T* const Ql = reinterpret_cast<T*>(smem);
+  T* const Dl = Ql + 2 * QB * PT;
+  float* const Ll = reinterpret_cast<float*>(Dl + 2 * QB * PT);  // [2][QB] log-sums, [2][QB] deltas
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Item w = work_item(p, p.heads_kv);
+  if (w.seq < -1) return;
+  T* const dk = reinterpret_cast<T*>(p.dk) + w.head * p.dk_head;
+  T* const dv = reinterpret_cast<T*>(p.dv) + w.head * p.dv_head;
+  // the list has the blocks with the most keys in front of them first; a key block's cost is the queries BEHIND it: read the list mirrored
+  const int first = w.seq < 0 ? w.block * (32 * NW) : ((w.len + 32 * NW - 1) / (32 * NW) - 1 - w.block) * (32 * NW);
+  if (w.seq < 0) {
+    zero_rows(dk + (long long)w.start * p.dk_row, p.dk_row, first, min(32 * NW, w.len - first), p.d, tid, NT);
+    zero_rows(dv + (long long)w.start * p.dv_row, p.dv_row, first, min(32 * NW, w.len - first), p.d, tid, NT);
+    return;
+  }
+  const int k0 = first + wave * 32, my_k = k0 + (lane & 31);
+  const bool k_ok = my_k < w.len;
+  const int group = p.heads_q / p.heads_kv;
+  const long long row = w.start + (k_ok ? my_k : 0);
+  Frag<T> kf[NK], vf[NK];
+  {
+    const T* krow = reinterpret_cast<const T*>(p.k) + row * p.k_row + w.head * p.k_head;
+    const T* vrow = reinterpret_cast<const T*>(p.v) + row * p.v_row + w.head * p.v_head;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      kf[k] = gfrag(krow, 16 * k + 8 * (lane >> 5), p.d, k_ok);
+      vf[k] = gfrag(vrow, 16 * k + 8 * (lane >> 5), p.d, k_ok);
+    }
+  }
+  const int qfirst = p.causal ? first / QB * QB : 0;
+  const int per_head = (w.len - qfirst + QB - 1) / QB, tiles = group * per_head;
+
+  RowTile<T, CP, QB, NT> qt, dt;
+  constexpr int SPT = (2 * QB + NT - 1) / NT;
+  float stats[SPT];  // of the tile's queries: log-sums, then deltas
+  auto load = [&](int t) {
+    const int head = w.head * group + t / per_head, q0 = qfirst + (t % per_head) * QB;
+    qt.load(reinterpret_cast<const T*>(p.q) + (long long)(w.start + q0) * p.q_row + head * p.q_head, p.q_row, w.len - q0, p.d, tid);
+    dt.load(reinterpret_cast<const T*>(p.dout) + (long long)(w.start + q0) * p.do_row + head * p.do_head, p.do_row, w.len - q0, p.d, tid);
+#pragma unroll
+    for (int i = 0; i < SPT; ++i) {
+      const int idx = tid + i * NT, q = idx % QB;
+      const float* src = idx < QB ? p.lse : p.delta;
+      stats[i] = src[(long long)head * p.rows + w.start + (q0 + q < w.len ? q0 + q : w.len - 1)];
+    }
+  };
+  auto store = [&](int t) {
+    qt.store(Ql + (t & 1) * QB * PT, PT, tid);
+    dt.store(Dl + (t & 1) * QB * PT, PT, tid);
+#pragma unroll
+    for (int i = 0; i < SPT; ++i) {
+      const int idx = tid + i * NT;
+      if (idx < 2 * QB) Ll[(t & 1) * 2 * QB + idx] = stats[i];
+    }
+  };
+  load(0);
+  store(0);
+  if (tiles > 1) load(1);
+
+  const float c = p.scale * kL2E;
+  f32x16_t ak[NF], av[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) { ak[f] = acc_zero(); av[f] = acc_zero(); }
+
+  for (int t = 0; t < tiles; ++t) {
+    wg_barrier_lds();
+    if (t + 1 < tiles) store(t + 1);
+    if (t + 2 < tiles) load(t + 2);
+    const int q0 = qfirst + (t % per_head) * QB;
+    const T* const Qt = Ql + (t & 1) * QB * PT;
+    const T* const Dt = Dl + (t & 1) * QB * PT;
+    const float* const Lt = Ll + (t & 1) * 2 * QB;
+    if (k0 >= w.len || (p.causal && q0 + QB - 1 < k0)) continue;  // no key of this wave, or none of the tile's queries sees one
+    const bool masked = q0 + QB > w.len || (p.causal && q0 < k0 + 31);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      f32x16_t s = acc_zero(), dp = acc_zero();
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        mma32(s, lds_frag(Qt, PT, 32 * b, 16 * k, lane), kf[k]);
+        mma32(dp, lds_frag(Dt, PT, 32 * b, 16 * k, lane), vf[k]);
+      }
+      f32x16_t ds;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r0 = 32 * b + 8 * i + 4 * (lane >> 5);
+        const float4 ls = *reinterpret_cast<const float4*>(Lt + r0), de = *reinterpret_cast<const float4*>(Lt + QB + r0);
+        const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dl[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float pv = pexp2(fmaf(s[4 * i + e], c, -lv[e]));
+          if (masked) pv = q0 + r0 + e >= w.len || (p.causal && my_k > q0 + r0 + e) ? 0.f : pv;
+          s[4 * i + e] = pv;
+          ds[4 * i + e] = pv * (dp[4 * i + e] - dl[e]);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Frag<T> pf = acc_frag<T>(s, h), sf = acc_frag<T>(ds, h);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+          mma32(av[f], tfrag(Dt, PT, 32 * b + 16 * h, 32 * f, lane), pf);
+          mma32(ak[f], tfrag(Qt, PT, 32 * b + 16 * h, 32 * f, lane), sf);
+        }
+      }
+    }
+  }
+  if (!k_ok) return;
+  T* const krow = dk + row * p.dk_row;
+  T* const vrow = dv + row * p.dv_row;
+#pragma unroll
+  for (int f = 0; f < NF; ++f)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c0 = 32 * f + 8 * i + 4 * (lane >> 5);
+      const float a[4] = {ak[f][4 * i] * p.scale, ak[f][4 * i + 1] * p.scale, ak[f][4 * i + 2] * p.scale, ak[f][4 * i + 3] * p.scale};
+      const float b[4] = {av[f][4 * i], av[f][4 * i + 1], av[f][4 * i + 2], av[f][4 * i + 3]};
+      if (c0 < p.d) {
+        store4<T>(krow + c0, a);
+        store4<T>(vrow + c0, b);
+      }
+    }
+}
+
+// -----------------------------------------------------------------------------------------------------------------------------------------
+// plan: starts[0 .. seqs] (clamped into 0 .. rows and made monotone, so that no kernel can be led out of its buffers), then the list of
+// (sequence, block) pairs by falling block index, the filling blocks behind the last sequence as (-1, block), and (-2, 0) for unused places.
+// One workgroup; LDS counters give the places, whose order among equals does not matter (every item's results are its own).
+// -----------------------------------------------------------------------------------------------------------------------------------------
+constexpr int kPlanThreads = 1024, kClasses = 512;
+__global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(const int* __restrict__ cu, int seqs, int rows, int block, int* __restrict__ plan, int places) {
+  __shared__ int part[kPlanThreads];
+  __shared__ int count[kClasses], place[kClasses];
+  const int tid = threadIdx.x;
+  // starts: running maximum over chunks of consecutive entries
+  const int n = seqs + 1, per = (n + kPlanThreads - 1) / kPlanThreads, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+  int top = 0;
+  for (int i = i0; i < i1; ++i) top = max(top, min(max(cu[i], 0), rows));
+  part[tid] = top;
+  for (int c = tid; c < kClasses; c += kPlanThreads) count[c] = 0;
+  __syncthreads();
+  for (int o = 1; o < kPlanThreads; o <<= 1) {
+    const int v = tid >= o ? part[tid - o] : 0;
+    __syncthreads();
+    part[tid] = max(part[tid], v);
+    __syncthreads();
+  }
+  int run = tid ? part[tid - 1] : 0;
+  for (int i = i0; i < i1; ++i) {
+    run = max(run, min(max(cu[i], 0), rows));
+    plan[i] = run;
+  }
+  __threadfence_block();
+  __syncthreads();
+  const int lane = tid & 63, wave = tid >> 6;
+  for (int s = wave; s < seqs; s += kPlanThreads / 64) {
+    const int nb = (plan[s + 1] - plan[s] + block - 1) / block;
+    for (int b = lane; b < nb; b += 64) atomicAdd(&count[min(b, kClasses - 1)], 1);
+  }
+  __syncthreads();
+  part[tid] = tid < kClasses ? count[kClasses - 1 - tid] : 0;
+  __syncthreads();
+  for (int o = 1; o < kClasses; o <<= 1) {
+    const int v = tid >= o ? part[tid - o] : 0;
+    __syncthreads();
+    part[tid] += v;
+    __syncthreads();
+  }
+  if (tid < kClasses) place[kClasses - 1 - tid] = tid ? part[tid - 1] : 0;
+  __syncthreads();
+  const int used = part[kClasses - 1];
+  int* const list = plan + ((seqs + 2) & ~1);
+  for (int s = wave; s < seqs; s += kPlanThreads / 64) {
+    const int nb = (plan[s + 1] - plan[s] + block - 1) / block;
+    for (int b = lane; b < nb; b += 64) {
+      const int at = atomicAdd(&place[min(b, kClasses - 1)], 1);
+      list[2 * at] = s;
+      list[2 * at + 1] = b;
+    }
+  }
+  const int tail = (rows - plan[seqs] + block - 1) / block;
+  for (int i = used + tid; i < places; i += kPlanThreads) {
+    list[2 * i] = i < used + tail ? -1 : -2;
+    list[2 * i + 1] = i < used + tail ? i - used : 0;
+  }
+}
+
+// waves per SIMD that the register budget is set for: 2, and 1 where a lone wave stages wide tiles by itself or the accumulators are many
+template <typename T, int CP, int NW> constexpr int occ(bool two_accumulators) {
+  return NW == 1 ? (CP > 64 || (sizeof(T) == 4 && CP > 32) ? 1 : 2) : two_accumulators && (CP > 64 || (sizeof(T) == 4 && CP > 32)) ? 1 : sizeof(T) == 4 && CP > 64 ? 1 : 2;
+}
+template <typename T, int CP, int NW, int KB> int launch_fwd(const PA& p, hipStream_t st) {
+  constexpr auto kernel = packed_attn_fwd_kernel<T, CP, NW, KB, occ<T, CP, NW>(false)>;
+  static DynSmemAttr attr;
+  const size_t smem = (size_t)4 * KB * lds_pitch<T>(CP) * sizeof(T);
+  if (hipError_t e = attr.ensure((const void*)kernel, smem)) return (int)e;
+  kernel<<<dim3((unsigned)(p.places * p.heads_q)), dim3(64 * NW), smem, st>>>(p);
+  CVH_CHECK_LAUNCH();
+  return 0;
+}
+template <typename T, int CP, int NW, int KB> int launch_bwd(const PA& p, hipStream_t st) {
+  constexpr int QB = 32;
+  constexpr auto dq = packed_attn_dq_kernel<T, CP, NW, KB, occ<T, CP, NW>(false)>;
+  constexpr auto dkv = packed_attn_dkv_kernel<T, CP, NW, QB, occ<T, CP, NW>(true)>;
+  static DynSmemAttr aq, ak;
+  const size_t sq = (size_t)4 * KB * lds_pitch<T>(CP) * sizeof(T), sk = (size_t)4 * QB * lds_pitch<T>(CP) * sizeof(T) + 4 * QB * sizeof(float);
+  if (hipError_t e = aq.ensure((const void*)dq, sq)) return (int)e;
+  if (hipError_t e = ak.ensure((const void*)dkv, sk)) return (int)e;
+  dq<<<dim3((unsigned)(p.places * p.heads_q)), dim3(64 * NW), sq, st>>>(p);
+  dkv<<<dim3((unsigned)(p.places * p.heads_kv)), dim3(64 * NW), sk, st>>>(p);
+  CVH_CHECK_LAUNCH();
+  return 0;
+}
+template <typename T, int CP> int run_width(const PA& p, int backward, hipStream_t st) {
+  constexpr int KB4 = sizeof(T) == 2 && CP <= 64 ? 64 : 32;
+  if (p.block == 32) return backward ? launch_bwd<T, CP, 1, 32>(p, st) : launch_fwd<T, CP, 1, 32>(p, st);
+  return backward ? launch_bwd<T, CP, 4, KB4>(p, st) : launch_fwd<T, CP, 4, sizeof(T) == 2 ? 64 : 32>(p, st);
+}
+template <typename T> int run_type(const PA& p, int backward, hipStream_t st) {
+  switch ((p.d + 31) / 32) {
+    case 1: return run_width<T, 32>(p, backward, st);
+    case 2: return run_width<T, 64>(p, backward, st);
+    case 3: return run_width<T, 96>(p, backward, st);
+    default: return run_width<T, 128>(p, backward, st);
+  }
+}
+
+bool strides_ok(int dtype, const void* base, long long row, long long head) {
+  const long long n = dtype == CVH_DT_BF16 ? 8 : 4;  // 16-byte accesses
+  return base != nullptr && (reinterpret_cast<uintptr_t>(base) & 15) == 0 && row % n == 0 && head % n == 0 && row >= 0 && head >= 0;
+}
+int check(int dtype, const PA* p, int backward) {
+  if (dtype != CVH_DT_F32 && dtype != CVH_DT_BF16) return -1;
+  if (p == nullptr || p->plan == nullptr || p->lse == nullptr) return -2;
+  if (p->rows <= 0 || p->seqs <= 0 || p->heads_q <= 0 || p->heads_kv <= 0 || p->heads_q % p->heads_kv || p->d <= 0 || p->d > 128 || p->d % 8) return -2;
+  if (!(p->scale > 0.f) || (p->block != 32 && p->block != 128)) return -2;
+  if (p->places != p->rows / p->block + p->seqs + 1 || (long long)p->places * p->heads_q > 0x7fffffffll) return -2;
+  if (!strides_ok(dtype, p->q, p->q_row, p->q_head) || !strides_ok(dtype, p->k, p->k_row, p->k_head) || !strides_ok(dtype, p->v, p->v_row, p->v_head) ||
+      !strides_ok(dtype, p->out, p->o_row, p->o_head))
+    return -2;
+  if (backward && (p->delta == nullptr || !strides_ok(dtype, p->dout, p->do_row, p->do_head) || !strides_ok(dtype, p->dq, p->dq_row, p->dq_head) ||
+                   !strides_ok(dtype, p->dk, p->dk_row, p->dk_head) || !strides_ok(dtype, p->dv, p->dv_row, p->dv_head)))
+    return -2;
+  return 0;
+}
+
+}  // namespace
+
+extern "C" long long cvh_packed_plan_elems(int seqs, int rows, int block) {
+  if (seqs <= 0 || rows <= 0 || (block != 32 && block != 128)) return -2;
+  return ((long long)(seqs + 2) & ~1ll) + 2 * ((long long)rows / block + seqs + 1);
+}
+extern "C" int cvh_packed_plan(const int* cu, int seqs, int rows, int block, int* plan, void* stream) {
+  if (cu == nullptr || plan == nullptr || seqs <= 0 || rows <= 0 || (block != 32 && block != 128)) return -2;
+  hipLaunchKernelGGL(packed_plan_kernel, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, cu, seqs, rows, block, plan, rows / block + seqs + 1);
+  CVH_CHECK_LAUNCH();
+  return 0;
+}
+extern "C" int cvh_packed_attn_fwd(int dtype, const cvh_packed_attn* p, void* stream) {
+  if (int rc = check(dtype, p, 0)) return rc;
+  return dtype == CVH_DT_BF16 ? run_type<bf16_t>(*p, 0, (hipStream_t)stream) : run_type<float>(*p, 0, (hipStream_t)stream);
+}
+extern "C" int cvh_packed_attn_bwd(int dtype, const cvh_packed_attn* p, void* stream) {
+  if (int rc = check(dtype, p, 1)) return rc;
+  return dtype == CVH_DT_BF16 ? run_type<bf16_t>(*p, 1, (hipStream_t)stream) : run_type<float>(*p, 1, (hipStream_t)stream);
+}

@@ -3,7 +3,7 @@
 Host side: Python mirrors of cvnets.layers / cvnets.modules / MobileViT with identical signatures and
 state_dict keys; compute: hand-written HIP kernels for gfx950 in libcvnets_hip.so (C ABI: include/cvnets_hip.h).
 """
-from . import _lib, ops, optim  # noqa: F401
+from . import _lib, ops, optim, packed  # noqa: F401
 from .layers import (BatchNorm2d, Conv2d, ConvLayer2d, Dropout, GELU, GlobalPool, Identity, Embedding, LayerNorm, LayerNorm2D_NCHW,  # noqa: F401
                      LayerNormFP32, LinearLayer, LinearSelfAttention, MultiHeadAttention, PositionalEmbedding, Swish, build_activation_layer, default_opts, get_normalization_layer)
 from .models import (MobileViT, MobileViTv2, VisionTransformer, build_mobilevit, build_mobilevit_v2, build_vit,  # noqa: F401

@@ -135,6 +135,10 @@ SIGNATURES = {
     "cvh_attn_bwd_drop": [I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, F, P, U, P],
     "cvh_attn_fwd_mask": [I, P, P, P, P, P, L, I, I, I, I, I, I, I, I, I, F, I, F, P, U, P],
     "cvh_attn_bwd_mask": [I, P, P, P, P, P, P, P, P, L, I, I, I, I, I, I, I, I, I, F, I, F, P, U, P],
+    "cvh_packed_plan_elems": [I, I, I],
+    "cvh_packed_plan": [P, I, I, I, P, P],
+    "cvh_packed_attn_fwd": [I, P, P],
+    "cvh_packed_attn_bwd": [I, P, P],
     "cvh_comm_available": [],
     "cvh_comm_unique_id": [P],
     "cvh_comm_init": [P, I, I, P],
@@ -151,6 +155,13 @@ SIGNATURES = {
 class OperandXf(ctypes.Structure):
     """cvh_operand_xf (include/cvnets_hip.h): transform applied to a kernel operand while it is loaded."""
     _fields_ = [("mode", c_int), ("src2", c_void_p), ("c0", c_void_p), ("c1", c_void_p), ("c2", c_void_p), ("act", c_int)]
+
+
+class PackedAttn(ctypes.Structure):
+    """cvh_packed_attn (include/cvnets_hip.h)."""
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv", "lse", "delta", "plan")]
+                + [(n + s, c_longlong) for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for s in ("_row", "_head")]
+                + [(n, c_int) for n in ("rows", "seqs", "heads_q", "heads_kv", "d", "causal", "block", "places")] + [("scale", c_float)])
 
 
 class ReduceDesc(ctypes.Structure):

@@ -1,0 +1,194 @@
+"""Operators on PACKED sequences: sequences of different lengths that lie one behind the other in the rows of one matrix, instead of being
+padded to the longest (the text tower pads captions of 5 .. 77 tokens to its context length: cvnets/text_encoders/transformer.py:354-435).
+
+``PackedSeqs`` holds the boundaries and the kernels' work list of one batch; ``attention`` / ``attention_qkv`` and ``embed`` take it.
+Rows behind the last sequence (a buffer larger than its sequences) are read by nothing and come back as zeros."""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import _check_dev, _dt, _p
+
+_INT_MAX = 2 ** 31 - 1
+
+
+def _stream_of(t: Tensor) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+class PackedSeqs:
+    """Boundaries of a batch of packed sequences.
+
+    cu_seqlens: int32 [sequences + 1] on the GPU, sequence b has the rows ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1`` (empty ones are allowed);
+    rows: the number of rows of the matrices that are used with it (>= cu_seqlens[-1]); max_len: an upper bound of the lengths, if one is
+    known on the host - it only chooses the work list's block size, a wrong one costs time and no result.
+
+    The work list is made by one kernel on the current stream, from the boundaries on the device: ``refresh`` makes it again after they were
+    changed in place (inside a captured graph, too).  Boundaries that fall or leave 0 .. rows are clamped by that kernel (they are not read by
+    the host); ``from_lengths`` checks lengths that the host knows."""
+
+    def __init__(self, cu_seqlens: Tensor, rows: int, max_len: Optional[int] = None):
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_contiguous():
+            raise RuntimeError(f"cu_seqlens must be a contiguous int32 vector of sequences + 1 boundaries. Got: {cu_seqlens.dtype} {list(cu_seqlens.shape)}")
+        rows = int(rows)
+        if not 0 < rows <= _INT_MAX:
+            raise ValueError(f"rows must be in 1 .. {_INT_MAX}. Got: {rows}")
+        if max_len is not None and max_len < 0:
+            raise ValueError(f"max_len must not be negative. Got: {max_len}")
+        _check_dev(cu_seqlens)
+        self.cu_seqlens, self.rows, self.seqs = cu_seqlens, rows, cu_seqlens.numel() - 1
+        self.max_len = rows if max_len is None else min(int(max_len), rows)
+        # One wave per 32 rows where a 128-row workgroup would be mostly empty: captions (512 of 5 .. 77 tokens, 8 heads of 64).
+        self.block = 32 if self.max_len <= 128 else 128
+        self.places = rows // self.block + self.seqs + 1
+        with torch.cuda.device(cu_seqlens.device):
+            self.plan = torch.empty(_lib.query("cvh_packed_plan_elems", self.seqs, rows, self.block), dtype=torch.int32, device=cu_seqlens.device)
+            self.refresh()
+
+    @classmethod
+    def from_lengths(cls, lengths: Sequence[int], device, rows: Optional[int] = None) -> "PackedSeqs":
+        lengths = [int(n) for n in lengths]
+        if not lengths or min(lengths) < 0:
+            raise ValueError(f"lengths must be one or more non-negative numbers. Got: {lengths[:8]}")
+        cu = torch.zeros(len(lengths) + 1, dtype=torch.int64)
+        torch.cumsum(torch.tensor(lengths, dtype=torch.int64), 0, out=cu[1:])
+        total = int(cu[-1])
+        rows = max(total, 1) if rows is None else int(rows)
+        if not total <= rows <= _INT_MAX:
+            raise ValueError(f"{total} rows of sequences do not fit into rows = {rows} (at most {_INT_MAX})")
+        return cls(cu.to(torch.int32).to(device), rows, max_len=max(lengths))
+
+    def refresh(self) -> None:
+        with torch.cuda.device(self.plan.device):
+            _lib.call("cvh_packed_plan", _p(self.cu_seqlens), self.seqs, self.rows, self.block, _p(self.plan), _stream_of(self.plan))
+
+    def __repr__(self) -> str:
+        return f"PackedSeqs(sequences={self.seqs}, rows={self.rows}, max_len={self.max_len})"
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------------------------------------------------
+def _loadable(t: Tensor) -> Tensor:
+    """[rows, heads, d] as the kernels read it: d contiguous, base and strides on 16 bytes (any other layout is copied)"""
+    n = 16 // t.element_size()
+    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % n == 0 and t.stride(1) % n == 0 and t.stride(0) >= 0 and t.stride(1) >= 0
+    return t if ok else t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _launch(name: str, seqs: PackedSeqs, scale: float, causal: bool, lse: Tensor, delta: Optional[Tensor], **t: Tensor) -> None:
+    q, k = t["q"], t["k"]
+    a = _lib.PackedAttn(lse=_p(lse), delta=_p(delta), plan=_p(seqs.plan), rows=seqs.rows, seqs=seqs.seqs, heads_q=q.shape[1], heads_kv=k.shape[1],
+                        d=q.shape[2], causal=int(causal), block=seqs.block, places=seqs.places, scale=scale)
+    for n, x in t.items():
+        s = "o" if n == "out" else "do" if n == "dout" else n
+        setattr(a, n, x.data_ptr())
+        setattr(a, s + "_row", x.stride(0))
+        setattr(a, s + "_head", x.stride(1))
+    with torch.cuda.device(q.device):
+        _lib.call(name, _dt(q), ctypes.byref(a), _stream_of(q))
+
+
+def _check_heads(q: Tensor, k: Tensor, v: Tensor, seqs: PackedSeqs, scale: Optional[float]) -> float:
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise RuntimeError(f"packed attention takes q [rows, heads, d] and k, v [rows, kv_heads, d]. Got: {list(q.shape)}, {list(k.shape)}, {list(v.shape)}")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise RuntimeError(f"q, k and v must have one dtype. Got: {q.dtype}, {k.dtype}, {v.dtype}")
+    _dt(q)
+    hq, hkv, d = q.shape[1], k.shape[1], q.shape[2]
+    if hkv == 0 or hq == 0 or hq % hkv:
+        raise RuntimeError(f"the number of query heads must be a multiple of the number of key heads. Got: {hq} and {hkv}")
+    if d == 0 or d % 8 or d > 128:
+        raise NotImplementedError(f"packed attention: head_dim must be a multiple of 8 up to 128. Got: {d}")
+    scale = float(d) ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite. Got: {scale}")
+    if q.shape[0] != seqs.rows:
+        raise RuntimeError(f"the layout is of {seqs.rows} rows, the tensors have {q.shape[0]}")
+    for t in (q, k, v):
+        _check_dev(t)
+        if t.device != seqs.plan.device:
+            raise RuntimeError(f"tensors and layout must be on one device. Got: {t.device} and {seqs.plan.device}")
+    if seqs.places * hq > _INT_MAX:
+        raise RuntimeError(f"{seqs.places} blocks of {hq} heads are more workgroups than one launch takes")
+    return scale
+
+
+class PackedAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, seqs, causal, scale):
+        q, k, v = _loadable(q), _loadable(k), _loadable(v)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+        _launch("cvh_packed_attn_fwd", seqs, scale, causal, lse, None, q=q, k=k, v=v, out=out)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.cfg = (seqs, causal, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        seqs, causal, scale = ctx.cfg
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        _launch("cvh_packed_attn_bwd", seqs, scale, causal, lse, torch.empty_like(lse), q=q, k=k, v=v, out=out, dout=_loadable(dout), dq=dq, dk=dk, dv=dv)
+        return dq, dk, dv, None, None, None
+
+
+class PackedAttentionQKVFn(torch.autograd.Function):
+    """the same on the columns [q | k | v] of one projection's result: no copy on the way in, one gradient matrix on the way out"""
+
+    @staticmethod
+    def forward(ctx, qkv, heads, kv_heads, seqs, causal, scale):
+        q, k, v = _split_heads(qkv, heads, kv_heads)
+        out = torch.empty((qkv.shape[0], heads, q.shape[2]), dtype=qkv.dtype, device=qkv.device)
+        lse = torch.empty((heads, qkv.shape[0]), dtype=torch.float32, device=qkv.device)
+        _launch("cvh_packed_attn_fwd", seqs, scale, causal, lse, None, q=q, k=k, v=v, out=out)
+        ctx.save_for_backward(qkv, out, lse)
+        ctx.cfg = (heads, kv_heads, seqs, causal, scale)
+        return out.view(qkv.shape[0], -1)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        qkv, out, lse = ctx.saved_tensors
+        heads, kv_heads, seqs, causal, scale = ctx.cfg
+        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        q, k, v = _split_heads(qkv, heads, kv_heads)
+        dq, dk, dv = _split_heads(dqkv, heads, kv_heads)
+        _launch("cvh_packed_attn_bwd", seqs, scale, causal, lse, torch.empty_like(lse), q=q, k=k, v=v, out=out,
+                dout=_loadable(dout.view(out.shape) if dout.is_contiguous() else dout.reshape(out.shape)), dq=dq, dk=dk, dv=dv)
+        return dqkv, None, None, None, None, None
+
+
+def _split_heads(qkv: Tensor, heads: int, kv_heads: int):
+    d = qkv.shape[1] // (heads + 2 * kv_heads)
+    h = qkv.view(qkv.shape[0], heads + 2 * kv_heads, d)
+    return h[:, :heads], h[:, heads:heads + kv_heads], h[:, heads + kv_heads:]
+
+
+def attention(q: Tensor, k: Tensor, v: Tensor, seqs: PackedSeqs, causal: bool = True, scale: Optional[float] = None) -> Tensor:
+    """Softmax attention inside each sequence: q [rows, heads, d], k and v [rows, kv_heads, d] (heads a multiple of kv_heads: consecutive query
+    heads share a key head) -> [rows, heads, d], differentiable in q, k and v.  float32 or bfloat16, d a multiple of 8 up to 128; views with
+    d contiguous and rows on 16 bytes are read in place.  scale: default d ** -0.5.  causal: token i sees the tokens 0 .. i of its sequence.
+    A NaN or infinity reaches the results of its own sequence only (under the causal mask: of its 32-row block and behind it)."""
+    scale = _check_heads(q, k, v, seqs, scale)
+    return PackedAttentionFn.apply(q, k, v, seqs, bool(causal), scale)
+
+
+def attention_qkv(qkv: Tensor, heads: int, seqs: PackedSeqs, kv_heads: Optional[int] = None, causal: bool = True, scale: Optional[float] = None) -> Tensor:
+    """``attention`` on the result of one projection, columns [q | k | v] head by head: qkv [rows, (heads + 2 kv_heads) d] -> [rows, heads d]"""
+    kv_heads = heads if kv_heads is None else int(kv_heads)
+    if qkv.dim() != 2 or heads <= 0 or kv_heads <= 0 or qkv.shape[1] % (heads + 2 * kv_heads):
+        raise RuntimeError(f"qkv must be [rows, ({heads} + 2 x {kv_heads}) heads x d]. Got: {list(qkv.shape)}")
+    d = qkv.shape[1] // (heads + 2 * kv_heads)
+    if not qkv.is_contiguous() or qkv.data_ptr() % 16:
+        qkv = qkv.contiguous() if not qkv.is_contiguous() else qkv.clone()
+    scale = _check_heads(*_split_heads(qkv, int(heads), kv_heads), seqs, scale)
+    return PackedAttentionQKVFn.apply(qkv, int(heads), kv_heads, seqs, bool(causal), scale)
