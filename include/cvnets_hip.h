@@ -442,6 +442,20 @@ int cvh_packed_plan(const int* cu, int seqs, int rows, int block, int* plan, voi
 int cvh_packed_attn_fwd(int dtype, const cvh_packed_attn* p, void* stream);
 int cvh_packed_attn_bwd(int dtype, const cvh_packed_attn* p, void* stream);
 
+/* ---- token embedding on packed rows, its gradient by sorted tokens ------------------------------- */
+/* out[r] = scale * table[ids[r]] + pos[place of r in its sequence] (pos nullable), table / pos float32, e % 8 == 0.  plan: the work list of
+ * cvh_packed_plan (rows behind its last sequence become zeros), or NULL: every row counts and pos must be NULL.  A token outside 0 .. vocab - 1 or a
+ * place at or behind `positions` gives a row of NaN (never a read out of bounds).
+ * bwd: dtable[vocab][e] = scale * the sums of dout over the rows of each token, in row order (padding_idx's row: zero), every row written once;
+ * dpos[positions][e] = the sums over the sequences; either may be NULL.  sort / pieces: scratch of cvh_embed_sort_elems int32 /
+ * cvh_embed_pieces_elems float32.  No atomics on values: bit-reproducible. */
+long long cvh_embed_sort_elems(int rows);
+long long cvh_embed_pieces_elems(int rows, int e);
+int cvh_embed_packed_fwd(int dtype, const long long* ids, const float* table, const float* pos, const int* plan, int seqs, int block, int places,
+                         int rows, int vocab, int positions, int e, float scale, void* out, void* stream);
+int cvh_embed_packed_bwd(int dtype, const long long* ids, const void* dout, const int* plan, int seqs, int rows, int vocab, int e, long long padding_idx,
+                         float scale, float* dtable, int positions, float* dpos, int* sort, float* pieces, void* stream);
+
 /* ---- LayerNorm over channels -------------------------------------------------------------------- */
 /* Replaces nn.LayerNorm, channel-last branch (cvnets/layers/normalization/layer_norm.py:67-68). */
 int cvh_layernorm_fwd(int dtype, const void* x, const float* gamma, const float* beta, void* y, float* mean, float* rstd,

@@ -13,7 +13,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _check_dev, _dt, _p
+from .ops import _check_dev, _dt, _p, compute_dtype
 
 _INT_MAX = 2 ** 31 - 1
 
@@ -192,3 +192,76 @@ def attention_qkv(qkv: Tensor, heads: int, seqs: PackedSeqs, kv_heads: Optional[
         qkv = qkv.contiguous() if not qkv.is_contiguous() else qkv.clone()
     scale = _check_heads(*_split_heads(qkv, int(heads), kv_heads), seqs, scale)
     return PackedAttentionQKVFn.apply(qkv, int(heads), kv_heads, seqs, bool(causal), scale)
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------------
+# token embedding
+# ---------------------------------------------------------------------------------------------------------------------------------------
+class PackedEmbedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, pos, ids, seqs, scale, padding_idx, dtype):
+        rows, (vocab, e) = ids.shape[0], table.shape
+        out = torch.empty((rows, e), dtype=dtype, device=table.device)
+        positions = 0 if pos is None else pos.shape[0]
+        layout = (None, 0, 0, 0) if seqs is None else (_p(seqs.plan), seqs.seqs, seqs.block, seqs.places)
+        with torch.cuda.device(table.device):
+            _lib.call("cvh_embed_packed_fwd", _dt(out), _p(ids), _p(table), _p(pos), *layout, rows, vocab, positions, e, scale, _p(out), _stream_of(table))
+        ctx.save_for_backward(ids)
+        ctx.cfg = (seqs, scale, -1 if padding_idx is None else padding_idx, vocab, positions)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        (ids,) = ctx.saved_tensors
+        seqs, scale, padding, vocab, positions = ctx.cfg
+        dout = dout.contiguous()
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
+        (rows, e), dev = dout.shape, dout.device
+        dtable = dpos = sort = pieces = None
+        if ctx.needs_input_grad[0]:
+            dtable = torch.empty((vocab, e), dtype=torch.float32, device=dev)
+            sort = torch.empty(_lib.query("cvh_embed_sort_elems", rows), dtype=torch.int32, device=dev)
+            pieces = torch.empty(_lib.query("cvh_embed_pieces_elems", rows, e), dtype=torch.float32, device=dev)
+        if positions and ctx.needs_input_grad[1]:
+            dpos = torch.empty((positions, e), dtype=torch.float32, device=dev)
+        with torch.cuda.device(dev):
+            _lib.call("cvh_embed_packed_bwd", _dt(dout), _p(ids), _p(dout), None if seqs is None else _p(seqs.plan), 0 if seqs is None else seqs.seqs, rows,
+                      vocab, e, padding, scale, _p(dtable), positions, _p(dpos), _p(sort), _p(pieces), _stream_of(dout))
+        return dtable, dpos, None, None, None, None, None
+
+
+def embed(ids: Tensor, table: Tensor, seqs: Optional[PackedSeqs] = None, pos: Optional[Tensor] = None, scale: float = 1.0,
+          padding_idx: Optional[int] = None, dtype: Optional[torch.dtype] = None) -> Tensor:
+    """scale * table[ids] (+ pos[place in the sequence]): ids int64 [rows], table float32 [vocab, e], pos float32 [positions, e] ->
+    [rows, e] in ``dtype`` (default: the compute dtype), differentiable in table and pos.  The gradient of the table is dense; it is summed in
+    row order (bit-reproducible), and the row of ``padding_idx`` is zero, as with nn.Embedding.  pos needs ``seqs``.  The tokens live on the
+    device and are not read by the host: one outside the table (or a place behind the last position) gives a row of NaN and no gradient."""
+    if ids.dim() != 1 or ids.dtype != torch.int64:
+        raise RuntimeError(f"ids must be an int64 vector. Got: {ids.dtype} {list(ids.shape)}")
+    if table.dim() != 2 or table.dtype != torch.float32 or table.shape[0] == 0:
+        raise RuntimeError(f"table must be float32 [vocab, e]. Got: {table.dtype} {list(table.shape)}")
+    vocab, e = table.shape
+    if e == 0 or e % 8:
+        raise NotImplementedError(f"packed embedding: the width must be a multiple of 8. Got: {e}")
+    if not 0 < ids.shape[0] <= _INT_MAX or vocab > _INT_MAX - 1024:
+        raise RuntimeError(f"packed embedding takes 1 .. {_INT_MAX} rows and up to {_INT_MAX - 1024} tokens. Got: {ids.shape[0]} and {vocab}")
+    if pos is not None:
+        if pos.dim() != 2 or pos.dtype != torch.float32 or pos.shape[1] != e or pos.shape[0] == 0:
+            raise RuntimeError(f"pos must be float32 [positions, {e}]. Got: {pos.dtype} {list(pos.shape)}")
+        if seqs is None:
+            raise RuntimeError("pos needs the layout of the sequences (seqs)")
+    if seqs is not None and seqs.rows != ids.shape[0]:
+        raise RuntimeError(f"the layout is of {seqs.rows} rows, ids has {ids.shape[0]}")
+    if padding_idx is not None and not 0 <= padding_idx < vocab:
+        raise ValueError(f"padding_idx must be in 0 .. {vocab - 1}. Got: {padding_idx}")
+    dtype = compute_dtype() if dtype is None else dtype
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f"unsupported activation dtype {dtype}")
+    for t in (ids, table) + (() if pos is None else (pos,)):
+        _check_dev(t)
+        if t.device != table.device or (seqs is not None and t.device != seqs.plan.device):
+            raise RuntimeError(f"ids, tables and layout must be on one device. Got: {t.device} and {table.device}")
+    table, pos = (t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0) else t.contiguous() if not t.is_contiguous() else t.clone() for t in (table, pos))
+    return PackedEmbedFn.apply(table, pos, ids.contiguous(), seqs, float(scale), padding_idx, dtype)
