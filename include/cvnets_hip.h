@@ -367,6 +367,24 @@ int cvh_adamw_multi(const long long* table, int n_tensors, long long total, floa
 /* dst = dst*(1-momentum) + momentum*src over a table[n+1][4] = {dst ptr, src ptr, numel, prefix start}: EMA of the float buffers */
 int cvh_lerp_multi(const long long* table, int n_tensors, long long total, float momentum, void* stream);
 
+/* ---- orthogonalised updates ----------------------------------------------------------------------- */
+/* A list of matrices, row-major and contiguous: Newton-Schulz steps x <- (a I + b x x^T + c (x x^T)^2) x from x = u / (|u|_F + eps), the shorter
+ * side as rows.  cvh_orthogonalize: u = src, dst = x (both of `dtype`; dst may be src).  cvh_muon_step (float32): momentum <- mu momentum + src
+ * (src = the gradient), u = src + mu momentum (nesterov) or momentum, param <- (1 - lr wd) param - lr gain x, with {lr, wd} =
+ * group_hp[group] on the device.  Coefficients with |a| + |b| + |c| <= 15 whose steps keep singular values below 15.  `mats` is a HOST array (read
+ * during the call only); ws: cvh_ns_workspace_elems float32 of device memory, 256-byte aligned; its contents do not have to survive. */
+typedef struct cvh_ns_matrix {
+  const void* src;
+  void* dst;
+  float *momentum, *param;
+  int rows, cols, group;
+  float gain;
+} cvh_ns_matrix;
+long long cvh_ns_workspace_elems(const cvh_ns_matrix* mats, int n);
+int cvh_orthogonalize(int dtype, const cvh_ns_matrix* mats, int n, int steps, float a, float b, float c, float eps, float* ws, void* stream);
+int cvh_muon_step(const cvh_ns_matrix* mats, int n, int steps, float a, float b, float c, float eps, float momentum, int nesterov, const float* group_hp,
+                  float* ws, void* stream);
+
 /* ---- classification loss (SURVEY 8f "next" row 2) -------------------------------------------------- */
 /* CrossEntropy._compute_loss (loss_fn/classification/cross_entropy.py:65-92) = F.cross_entropy(logits[N][M], labels, weight=None,
  * ignore_index, label_smoothing), per-row part: loss_rows[N] (0 for ignored rows) and lse[N]; the mean over valid rows is the

@@ -143,6 +143,9 @@ SIGNATURES = {
     "cvh_embed_pieces_elems": [I, I],
     "cvh_embed_packed_fwd": [I, P, P, P, P, I, I, I, I, I, I, I, F, P, P],
     "cvh_embed_packed_bwd": [I, P, P, P, I, I, I, I, L, F, P, I, P, P, P, P],
+    "cvh_ns_workspace_elems": [P, I],
+    "cvh_orthogonalize": [I, P, I, I, F, F, F, F, P, P],
+    "cvh_muon_step": [P, I, I, F, F, F, F, F, I, P, P, P],
     "cvh_comm_available": [],
     "cvh_comm_unique_id": [P],
     "cvh_comm_init": [P, I, I, P],
@@ -166,6 +169,12 @@ class PackedAttn(ctypes.Structure):
     _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv", "lse", "delta", "plan")]
                 + [(n + s, c_longlong) for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for s in ("_row", "_head")]
                 + [(n, c_int) for n in ("rows", "seqs", "heads_q", "heads_kv", "d", "causal", "block", "places")] + [("scale", c_float)])
+
+
+class NsMatrix(ctypes.Structure):
+    """cvh_ns_matrix (include/cvnets_hip.h)."""
+    _fields_ = [("src", c_void_p), ("dst", c_void_p), ("momentum", c_void_p), ("param", c_void_p), ("rows", c_int), ("cols", c_int), ("group", c_int),
+                ("gain", c_float)]
 
 
 class ReduceDesc(ctypes.Structure):

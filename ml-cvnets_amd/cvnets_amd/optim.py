@@ -4,7 +4,9 @@ optim/scheduler/*) whose ``step()`` is ONE kernel launch over every parameter te
 ``EMA.update_parameters`` (cvnets/misc/averaging_utils.py:43-55) into the same pass."""
 from __future__ import annotations
 
-from typing import Iterable, Optional
+import ctypes
+import math
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -247,3 +249,157 @@ class EMABuffers:
             ops.invalidate_packed()
         for d, s in self.ints:  # averaging an integer counter is a copy after the cast back (ema_v.copy_(...) on an int64 tensor)
             d.copy_((d * (1.0 - self.momentum) + self.momentum * s).to(d.dtype))
+
+
+# ---- orthogonalised updates ------------------------------------------------------------------------------------------------------------
+NS_COEFFICIENTS = (3.4445, -4.775, 2.0315)  # of the quintic step: maps singular values from (0, 1] towards 1, fastest growth at zero
+
+
+def _check_ns(steps: int, coefficients: Sequence[float], eps: float) -> Tuple[int, float, float, float, float]:
+    a, b, c = (float(x) for x in coefficients)
+    if int(steps) < 1:
+        raise ValueError(f"steps must be at least 1. Got: {steps}")
+    if not abs(a) + abs(b) + abs(c) <= 15.0:
+        raise ValueError(f"coefficients with |a| + |b| + |c| <= 15 are supported. Got: {tuple(coefficients)}")
+    if not 0.0 <= eps < math.inf:
+        raise ValueError(f"eps must not be negative. Got: {eps}")
+    return int(steps), a, b, c, float(eps)
+
+
+def _check_matrix(rows: int, cols: int) -> None:
+    if rows < 1 or cols < 1 or min(rows, cols) > 1 << 14 or max(rows, cols) > 1 << 24:
+        raise NotImplementedError(f"matrices with a shorter side of 1 .. {1 << 14} and a longer one up to {1 << 24} are supported. Got: {rows} x {cols}")
+
+
+def _by_cost(sizes: Sequence[Tuple[int, int]]) -> List[int]:
+    """the longest products first: a launch over a list then ends with its short ones"""
+    return sorted(range(len(sizes)), key=lambda i: -max(sizes[i]))
+
+
+@torch.no_grad()
+def orthogonalize(matrices: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = 5, coefficients: Sequence[float] = NS_COEFFICIENTS,
+                  eps: float = 1e-7) -> Union[torch.Tensor, List[torch.Tensor]]:
+    """Newton-Schulz orthogonalisation of matrices (one or a list of any shapes, all float32 or all bfloat16): x = u / (|u|_F + eps), then ``steps``
+    times x <- (a I + b x x^T + c (x x^T)^2) x, the shorter side as rows.  The products are computed to float32 accuracy whatever the type
+    of the matrices; the result has their type.  A list takes as many launches as one matrix.  A NaN or an infinity in a matrix makes its whole
+    result NaN (and no other's).  Coefficients whose steps let singular values grow beyond 15 are not supported."""
+    single = isinstance(matrices, torch.Tensor)
+    mats = [matrices] if single else list(matrices)
+    cfg = _check_ns(steps, coefficients, eps)
+    for t in mats:
+        if t.dim() != 2 or t.dtype not in (torch.float32, torch.bfloat16) or t.dtype != mats[0].dtype:
+            raise RuntimeError(f"orthogonalize takes float32 or bfloat16 matrices of one dtype. Got: {t.dtype} {list(t.shape)}")
+        _check_matrix(*t.shape)
+    for t in mats:
+        ops._check_dev(t)
+        if t.device != mats[0].device:
+            raise RuntimeError(f"the matrices must be on one device. Got: {t.device} and {mats[0].device}")
+    if not mats:
+        return []
+    dev = mats[0].device
+    with torch.cuda.device(dev):
+        src = [t.contiguous() for t in mats]
+        out = [torch.empty_like(t) for t in src]
+        table = (_lib.NsMatrix * len(src))(*[_lib.NsMatrix(src=_p(src[i]), dst=_p(out[i]), rows=src[i].shape[0], cols=src[i].shape[1])
+                                             for i in _by_cost([t.shape for t in src])])
+        ws = torch.empty(_lib.query("cvh_ns_workspace_elems", ctypes.byref(table), len(src)), dtype=torch.float32, device=dev)
+        _lib.call("cvh_orthogonalize", ops._dt(src[0]), ctypes.byref(table), len(src), *cfg, _p(ws), _stream())
+    return out[0] if single else out
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum whose update is orthogonalised, for the matrices of a model (dimensions behind the first are flattened, as in a convolution's
+    [out, in, kh, kw]); vectors, embeddings and heads stay with ``AdamW``:
+
+        mom <- momentum mom + grad;   u = grad + momentum mom (nesterov) or mom
+        param <- (1 - lr weight_decay) param - lr max(1, rows / cols) ** 0.5 orthogonalize(u)
+
+    ``param_groups`` with their own lr and weight_decay, which a scheduler may rewrite; ``state[p]["momentum_buffer"]`` and the usual state dict.
+    One step is 2 + 3 ns_steps launches for up to 32 matrices.  Rates live on the device: a captured ``step(sync_hyperparameters=False)``
+    follows ``sync_hyperparameters()`` calls between replays."""
+
+    def __init__(self, params: Iterable, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, ns_steps: int = 5,
+                 ns_coefficients: Sequence[float] = NS_COEFFICIENTS, eps: float = 1e-7):
+        if not lr >= 0.0 or not weight_decay >= 0.0 or not 0.0 <= momentum < 1.0:
+            raise ValueError(f"lr and weight_decay must not be negative, momentum in [0, 1). Got: {lr}, {weight_decay}, {momentum}")
+        self._ns = _check_ns(ns_steps, ns_coefficients, eps)
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=bool(nesterov), weight_decay=weight_decay))
+        if len({(g["momentum"], g["nesterov"]) for g in self.param_groups}) != 1:
+            raise NotImplementedError("per-group momentum / nesterov are not supported")
+        for g in self.param_groups:
+            for p in g["params"]:
+                if p.dim() < 2:
+                    raise ValueError(f"Muon takes matrices (two or more dimensions); give vectors to AdamW. Got: {list(p.shape)}")
+                if p.dtype != torch.float32 or not p.is_contiguous():
+                    raise RuntimeError("parameters must be contiguous float32")
+                _check_matrix(p.shape[0], p.numel() // max(1, p.shape[0]))
+        self._plan = None
+        self._hp = self._hp_host = None
+
+    def _entries(self):
+        out = []
+        for gi, g in enumerate(self.param_groups):
+            for p in g["params"]:
+                if p.grad is not None:
+                    if p.grad.is_sparse or p.grad.dtype != torch.float32:
+                        raise RuntimeError("gradients must be dense float32")
+                    out.append((p, p.grad if p.grad.is_contiguous() else p.grad.contiguous(), gi))
+        return out
+
+    def _build(self, entries):
+        dev = entries[0][0].device
+        for p, _, _ in entries:
+            ops._check_dev(p)
+            if p.device != dev:
+                raise RuntimeError(f"the parameters must be on one device. Got: {p.device} and {dev}")
+            buf = self.state[p].get("momentum_buffer")
+            if buf is None or buf.dtype != torch.float32 or not buf.is_contiguous() or buf.device != dev:  # (a loaded state may be another type's)
+                self.state[p]["momentum_buffer"] = torch.zeros_like(p) if buf is None else buf.to(device=dev, dtype=torch.float32).contiguous()
+        sizes = [(p.shape[0], p.numel() // p.shape[0]) for p, _, _ in entries]
+        rows = [_lib.NsMatrix(src=_p(entries[i][1]), momentum=_p(self.state[entries[i][0]]["momentum_buffer"]), param=_p(entries[i][0]), rows=sizes[i][0],
+                              cols=sizes[i][1], group=entries[i][2], gain=math.sqrt(max(1.0, sizes[i][0] / sizes[i][1]))) for i in _by_cost(sizes)]
+        table = (_lib.NsMatrix * len(rows))(*rows)
+        need = _lib.query("cvh_ns_workspace_elems", ctypes.byref(table), len(rows))
+        ws = self._plan["ws"] if self._plan is not None and self._plan["ws"].numel() >= need and self._plan["ws"].device == dev else \
+            torch.empty(need, dtype=torch.float32, device=dev)
+        self._plan = {"table": table, "n": len(rows), "ws": ws, "key": self._key(entries)}
+        return self._plan
+
+    def _key(self, entries):
+        return [(p.data_ptr(), g.data_ptr(), self.state[p]["momentum_buffer"].data_ptr() if "momentum_buffer" in self.state[p] else 0, gi) for p, g, gi in entries]
+
+    def sync_hyperparameters(self) -> None:
+        """copy the groups' (lr, weight_decay) to the device table; call after a scheduler changed them (outside graph replay)"""
+        host = [[float(g["lr"]), float(g["weight_decay"])] for g in self.param_groups]
+        if self._hp is None or len(self._hp) != len(host):
+            self._hp = torch.zeros(len(host), 2, dtype=torch.float32, device=self.param_groups[0]["params"][0].device)
+            self._hp_host = None
+        if host != self._hp_host:
+            self._hp.copy_(torch.tensor(host, dtype=torch.float32), non_blocking=True)  # plumbing: 2 floats per group
+            self._hp_host = host
+
+    @torch.no_grad()
+    def step(self, closure=None, sync_hyperparameters: bool = True):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        ops.finish_backward()
+        import sys
+        _ddp = sys.modules.get(__package__ + ".ddp")
+        if _ddp is not None:
+            _ddp.exchange_pending()
+        entries = self._entries()
+        if not entries:
+            return loss
+        with torch.cuda.device(entries[0][0].device):
+            plan = self._plan
+            if plan is None or plan["key"] != self._key(entries):
+                plan = self._build(entries)
+            if sync_hyperparameters or self._hp is None:
+                self.sync_hyperparameters()
+            g0 = self.param_groups[0]
+            _lib.call("cvh_muon_step", ctypes.byref(plan["table"]), plan["n"], *self._ns, float(g0["momentum"]), int(g0["nesterov"]), _p(self._hp), _p(plan["ws"]),
+                      _stream())
+        ops.invalidate_packed()
+        return loss

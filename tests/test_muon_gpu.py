@@ -1,0 +1,170 @@
+"""optim.orthogonalize and optim.Muon against the same steps in float64.
+
+Tolerance of a float32 result, of the 2-norm: each of the three products of a step has entries that are off by about 2^-22 of the operands' norms
+(two roundings of pairs of 11 bits and a float32 accumulation), an error that the steps after it multiply by at most a = 3.45 each - as they do
+the matrix itself, whose norm grows from 1 to sqrt(m) by that same factor.  5 steps x 3 products x 2^-22 = 3.6e-6, doubled for the error's own
+spread over directions that grow more than the matrix: 2^-17 = 7.6e-6.  A bf16 result: one rounding more.  It is off by at
+most half a step, 2^-8 of a value (a step is 2^-7 of the power of two below it), so by at most 2^-8 in the 2-norm whatever the values are; over many
+values, spread evenly over their half steps, by 2^-8 / sqrt(3).  A matrix of a handful of values (1 x 1: 0.6970 became 0.6953, half a step of 2^-8
+being 0.00195 = 2.8e-3 of it) has no mean square: the first bound is the one that holds for it."""
+import copy
+import math
+
+import pytest
+import torch
+
+from cvnets_amd import optim
+
+pytestmark = pytest.mark.gpu
+TOL = {torch.float32: 2.0 ** -17}
+
+
+def tol(dtype, values):
+    if dtype == torch.float32:
+        return TOL[dtype]
+    return 2.0 ** -8 / (math.sqrt(3) if values >= 256 else 1.0) + TOL[torch.float32]
+
+
+def steps64(u, steps=5, coefficients=optim.NS_COEFFICIENTS, eps=1e-7):
+    a, b, c = coefficients
+    x = u.double().cpu()
+    flip = x.shape[0] > x.shape[1]
+    x = x.t() if flip else x
+    x = x / (x.norm() + eps)
+    for _ in range(steps):
+        g = x @ x.t()
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return x.t() if flip else x
+
+
+def err(got, want):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape and torch.isfinite(got).all()
+    return float((got - want).norm() / want.norm())
+
+
+def gradient(r, c, seed=0, dtype=torch.float32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    k = max(1, min(r, c) // 8)
+    strong = torch.randn(r, k, generator=g, device="cuda") * torch.logspace(0, -2, k, device="cuda")
+    return (torch.matmul(strong, torch.randn(k, c, generator=g, device="cuda")) * 1e-3 + torch.randn(r, c, generator=g, device="cuda") * 2e-4).to(dtype)
+
+
+SHAPES = [(1, 1), (1, 640), (640, 1), (2, 3), (63, 64), (64, 65), (65, 63), (144, 432), (257, 129), (129, 1000), (512, 512)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_one_matrix(dtype, shape):
+    u = gradient(*shape, dtype=dtype)
+    x = optim.orthogonalize(u)
+    assert x.dtype == dtype
+    assert err(x, steps64(u)) <= tol(dtype, x.numel())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_list_of_many_shapes_is_each_matrix_by_itself(dtype):
+    mats = [gradient(r, c, seed=i, dtype=dtype) for i, (r, c) in enumerate(SHAPES * 4)]  # more than one table of them
+    keep = [m.clone() for m in mats]
+    for x, u, k in zip(optim.orthogonalize(mats), mats, keep):
+        assert err(x, steps64(u)) <= tol(dtype, x.numel())
+        assert torch.equal(u, k)
+
+
+def test_wide_tiles():
+    mats = [gradient(1536, 512, seed=i) for i in range(6)] + [gradient(512, 2000, seed=9)] * 3 + [gradient(1100, 1030, seed=10)] * 2 + [gradient(1030, 1400, seed=11)] * 4
+    for x, u in zip(optim.orthogonalize(mats), mats):
+        assert err(x, steps64(u)) <= TOL[torch.float32]
+
+
+def test_steps_coefficients_and_eps():
+    u = gradient(100, 200)
+    assert err(optim.orthogonalize(u, steps=1), steps64(u, steps=1)) <= TOL[torch.float32]
+    assert err(optim.orthogonalize(u, steps=12, coefficients=(1.875, -1.25, 0.375)), steps64(u, steps=12, coefficients=(1.875, -1.25, 0.375))) <= TOL[torch.float32]
+    assert err(optim.orthogonalize(u, eps=0.5), steps64(u, eps=0.5)) <= TOL[torch.float32]
+
+
+def test_scale_zero_and_non_finite():
+    u = gradient(70, 90)
+    for s in (1e-30, 1e25):  # squares outside float32
+        assert err(optim.orthogonalize(u * s, eps=0.0), steps64(u.double() * s, eps=0.0)) <= TOL[torch.float32]
+    z, bad = torch.zeros(70, 90, device="cuda"), u.clone()
+    bad[3, 4] = float("inf")
+    x = optim.orthogonalize([z, bad, u])
+    assert torch.equal(x[0], z) and torch.isnan(x[1]).all() and err(x[2], steps64(u)) <= TOL[torch.float32]
+
+
+def test_views_and_order():
+    u = gradient(90, 200)
+    assert torch.equal(optim.orthogonalize(u[:, ::2]), optim.orthogonalize(u[:, ::2].contiguous()))
+    assert err(optim.orthogonalize(u.t()), steps64(u).t()) <= TOL[torch.float32]
+    assert torch.equal(optim.orthogonalize(u), optim.orthogonalize(u))
+    assert optim.orthogonalize([]) == []
+
+
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_muon_steps(nesterov):
+    shapes = [(96, 64), (64, 96), (40, 8, 3, 3), (1, 50)]
+    g = torch.Generator(device="cuda").manual_seed(7)
+    params = [torch.nn.Parameter(torch.randn(s, generator=g, device="cuda") * 0.1) for s in shapes]
+    opt = optim.Muon([{"params": params[:2], "lr": 0.05, "weight_decay": 0.1}, {"params": params[2:]}], lr=0.01, momentum=0.9, nesterov=nesterov)
+    want = [p.detach().double().cpu() for p in params]
+    mom = [torch.zeros_like(w) for w in want]
+    for it in range(3):
+        if it == 2:
+            opt.param_groups[0]["lr"] = 0.02  # a scheduler's rate
+        for i, p in enumerate(params):
+            grad = torch.randn(p.shape, generator=g, device="cuda")
+            p.grad = grad.clone(memory_format=torch.contiguous_format) if it else grad
+            g64 = grad.double().cpu()
+            mom[i] = 0.9 * mom[i] + g64
+            u = g64 + 0.9 * mom[i] if nesterov else mom[i]
+            lr, wd = ((0.02 if it == 2 else 0.05), 0.1) if i < 2 else (0.01, 0.0)
+            rows = p.shape[0]
+            x = steps64(u.reshape(rows, -1))
+            want[i] = want[i] * (1 - lr * wd) - lr * max(1.0, rows / x.shape[1]) ** 0.5 * x.view(p.shape)
+        opt.step()
+    for p, w, m in zip(params, want, mom):
+        assert err(p, w) <= 2.0 ** -17
+        assert err(opt.state[p]["momentum_buffer"], m) <= 2.0 ** -22
+
+
+def test_muon_state_dict_and_skipped_parameters():
+    params = [torch.nn.Parameter(gradient(30, 20, seed=i)) for i in range(2)]
+    opt = optim.Muon(params, lr=0.1)
+    params[0].grad = gradient(30, 20, seed=5)
+    before = params[1].detach().clone()
+    opt.step()
+    assert torch.equal(params[1], before) and params[1] not in opt.state
+    copies = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    other = optim.Muon(copies, lr=0.1)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))  # (torch's load shares the tensors it is given)
+    for o, ps in ((opt, params), (other, copies)):
+        for i, p in enumerate(ps):
+            p.grad = gradient(30, 20, seed=8 + i)
+        o.step()
+    for a, b in zip(params, copies):
+        assert torch.equal(a, b)
+
+
+def test_muon_step_in_a_graph():
+    p = torch.nn.Parameter(gradient(64, 100))
+    q = torch.nn.Parameter(p.detach().clone())
+    p.grad, q.grad = gradient(64, 100, seed=2), gradient(64, 100, seed=2)
+    a, b = optim.Muon([p], lr=0.1), optim.Muon([q], lr=0.1)
+    a.step()
+    b.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step(sync_hyperparameters=False)
+    for it in range(4):
+        new = gradient(64, 100, seed=10 + it)
+        p.grad.copy_(new)
+        q.grad.copy_(new)
+        for o in (a, b):
+            o.param_groups[0]["lr"] = 0.1 / (it + 1)
+            o.sync_hyperparameters()
+        graph.replay()
+        b.step()
+        torch.cuda.synchronize()
+        assert torch.equal(p, q)
