@@ -468,7 +468,7 @@ int cvh_packed_attn_bwd(int dtype, const cvh_packed_attn* p, void* stream);
  * dpos[positions][e] = the sums over the sequences; either may be NULL.  sort / pieces: scratch of cvh_embed_sort_elems int32 /
  * cvh_embed_pieces_elems float32.  No atomics on values: bit-reproducible. */
 long long cvh_embed_sort_elems(int rows);
-long long cvh_embed_pieces_elems(int rows, int e);
+long long cvh_embed_pieces_elems(int rows, int e, int positions, int seqs); /* positions, seqs: 0 without dpos */
 int cvh_embed_packed_fwd(int dtype, const long long* ids, const float* table, const float* pos, const int* plan, int seqs, int block, int places,
                          int rows, int vocab, int positions, int e, float scale, void* out, void* stream);
 int cvh_embed_packed_bwd(int dtype, const long long* ids, const void* dout, const int* plan, int seqs, int rows, int vocab, int e, long long padding_idx,

@@ -6,15 +6,15 @@
 // The gradient of the table is dense float32.  Scattering with float atomics makes its sums depend on the order in which they retire and needs
 // the table zeroed first; here the rows are sorted by token (stable radix sort, 8 bits a pass), every row of the table is then written exactly
 // once, as the sum of its run in a fixed order: bit-reproducible.  What bounds it: the write of the whole table (49408 x 512: 101 MB) next to
-// one read of dy.  A frequent token (the start mark of every caption) would leave its whole run to one wave: runs longer than kChunk are summed
-// in pieces of kChunk rows first, by as many waves, and joined in order.
+// one read of dy (two with positions).  The sorted rows are summed in equal chunks, not token by token: frequent tokens (the start mark of every
+// caption, the first words of a vocabulary in order of frequency) would otherwise leave their long runs to a few waves.
 #include "common.hpp"
 #include "cvnets_hip.h"
 
 namespace {
 
 constexpr int kItems = 2048;   // rows a sort workgroup takes: 4 waves x 8 rounds x 64 lanes
-constexpr int kChunk = 64;     // rows of a piece
+constexpr int kChunk = 32;     // sorted rows that are summed by one group of lanes
 constexpr int kTableRows = 32;  // rows of the table a workgroup writes
 
 // sort key of row r: its token, or `vocab` (sorted behind everything) where the row adds nothing: behind the last sequence, the padding token,
@@ -137,147 +137,178 @@ __device__ __forceinline__ int lower_bound_lane(const unsigned* keys, int lo, in
   return lo;
 }
 
-// acc[0 .. 8) += columns c .. c + 7 of dy rows order[a .. b), in order; four rows in flight
-template <typename T> __device__ __forceinline__ void add_rows(const T* __restrict__ dy, const int* __restrict__ order, int a, int b, int e, int c, float* acc) {
-  int i = a;
-  for (; i + 4 <= b; i += 4) {
-    V8<T> v[4];
+// ---- sums -------------------------------------------------------------------------------------------------------------------------------
+// Chunk c of the sorted rows is [kChunk c, kChunk c + kChunk).  A run of one token that begins and ends in a chunk is written to the table at once;
+// of a run that crosses borders every chunk leaves a piece: part[c][1] of the run that begins in chunk c and goes on, part[c][0] of the one
+// that came in.  `G` lanes (8 columns each) share a chunk, so narrow tables keep whole waves busy.
+__device__ __forceinline__ void put8(float* p, const float* acc, float scale) {
+  *reinterpret_cast<float4*>(p) = make_float4(acc[0] * scale, acc[1] * scale, acc[2] * scale, acc[3] * scale);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(acc[4] * scale, acc[5] * scale, acc[6] * scale, acc[7] * scale);
+}
+__device__ __forceinline__ void add8(float* acc, const float* f) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = v8_load<T>(dy + (size_t)order[i + j] * e + c);
+  for (int k = 0; k < 8; ++k) acc[k] += f[k];
+}
+
+struct Grad {
+  const unsigned* keys;  // sorted tokens
+  const int* order;      // and their rows
+  const int* starts;     // boundaries of the sequences
+  float *dtable, *part, *dpos, *pos_part;
+  int n, vocab, e, group, chunk_blocks, pos_blocks, seqs, pos_split;
+  float scale;
+};
+
+template <typename T> __device__ __forceinline__ void chunk_rows(const Grad& g, const T* __restrict__ dy, int block) {
+  const int G = g.group, chunk = block * (256 / G) + threadIdx.x / G, sl = threadIdx.x % G;
+  const int a = chunk * kChunk, b = min(a + kChunk, g.n);
+  if (a >= g.n) return;
+  const bool came_in = a > 0 && g.keys[a - 1] == g.keys[a], goes_on = b < g.n && g.keys[b] == g.keys[b - 1];
+  for (int c = sl * 8; c < g.e; c += G * 8) {
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    bool inside = !came_in;  // the run began in this chunk
+    for (int i = a; i < b; i += 8) {  // eight rows in flight; keys and order are padded to whole chunks
+      const uint4 k0 = *reinterpret_cast<const uint4*>(g.keys + i), k1 = *reinterpret_cast<const uint4*>(g.keys + i + 4);
+      const int4 o0 = *reinterpret_cast<const int4*>(g.order + i), o1 = *reinterpret_cast<const int4*>(g.order + i + 4);
+      const unsigned key[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+      const int row[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
+      V8<T> v[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float f[8];
-      v8_unpack(v[j], f);
+      for (int j = 0; j < 8; ++j) v[j] = v8_load_clamped<T>(dy, (size_t)row[j] * g.e + c, i + j < b);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) acc[k] += f[k];
+      for (int j = 0; j < 8; ++j) {
+        if (i + j >= b) break;
+        float f[8];
+        v8_unpack(v[j], f);
+        add8(acc, f);
+        const bool last = i + j + 1 == b;
+        const unsigned next = last ? 0xffffffffu : j < 7 ? key[(j + 1) & 7] : g.keys[i + 8];
+        if (last ? true : next != key[j]) {  // the run ends here, or the chunk does
+          if (key[j] < (unsigned)g.vocab) {
+            if (!inside) put8(g.part + ((size_t)chunk * 2) * g.e + c, acc, 1.f);
+            else if (last && goes_on) put8(g.part + ((size_t)chunk * 2 + 1) * g.e + c, acc, 1.f);
+            else put8(g.dtable + (size_t)key[j] * g.e + c, acc, g.scale);
+          }
+          inside = true;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+        }
+      }
     }
-  }
-  for (; i < b; ++i) {
-    float f[8];
-    v8_unpack(v8_load<T>(dy + (size_t)order[i] * e + c), f);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) acc[k] += f[k];
   }
 }
 
-// pieces of the long runs (more than kChunk rows): chunk c of the sorted rows has part[c][0] for the run its first row belongs to and part[c][1]
-// for the run its last row belongs to, where that is another one.  One wave a chunk.
-template <typename T>
-__global__ __launch_bounds__(256) void embed_pieces_kernel(const T* __restrict__ dy, const unsigned* __restrict__ keys, const int* __restrict__ order, int n,
-                                                           int vocab, int e, float* __restrict__ part) {
-  const int lane = threadIdx.x & 63, chunk = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int a = chunk * kChunk, b = min(a + kChunk, n);
-  if (a >= n) return;
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const unsigned v = keys[side ? b - 1 : a];
-    if (v >= (unsigned)vocab || (side && v == keys[a])) continue;
-    // long: the run reaches at least kChunk + 1 rows; inside this chunk it is [lo, hi)
-    const int from = max(0, a - kChunk), to = min(n, b + kChunk);
-    const int lo = lower_bound_wave(keys, from, to, v, lane), hi = lower_bound_wave(keys, from, to, v + 1, lane);
-    const bool is_long = hi - lo > kChunk || (lo == from && from > 0) || (hi == to && to < n);
-    if (!is_long) continue;
-    // (a run that only touches the window's end may still be short: the rows kernel decides by the run itself and then does not read this piece)
-    for (int c = lane * 8; c < e; c += 512) {
-      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      add_rows<T>(dy, order, max(lo, a), min(hi, b), e, c, acc);
-      float* p = part + ((size_t)chunk * 2 + side) * e + c;
-      *reinterpret_cast<float4*>(p) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      *reinterpret_cast<float4*>(p + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-    }
-  }
-}
-
-// rows v0 .. v0 + kTableRows - 1 of the gradient, each written once: zeros, the sum of a short run, or of a long run's pieces (by all four waves)
-template <typename T>
-__global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ dy, const unsigned* __restrict__ keys, const int* __restrict__ order, int n,
-                                                         int vocab, int e, float scale, const float* __restrict__ part, float* __restrict__ dtable, int group) {
+// rows of the table that no token names: zeros
+__device__ __forceinline__ void empty_rows(const Grad& g, int block) {
   __shared__ int bound[kTableRows + 1];
   __shared__ int range[2];
-  __shared__ __attribute__((aligned(16))) float joined[4][512];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int v0 = blockIdx.x * kTableRows, rows = min(kTableRows, vocab - v0);
+  const int v0 = block * kTableRows, rows = min(kTableRows, g.vocab - v0);
   if (wave < 2) {
-    const int at = lower_bound_wave(keys, 0, n, (unsigned)(wave ? v0 + rows : v0), lane);
+    const int at = lower_bound_wave(g.keys, 0, g.n, (unsigned)(wave ? v0 + rows : v0), lane);
     if (lane == 0) range[wave] = at;
   }
   __syncthreads();
-  if (tid <= rows) bound[tid] = lower_bound_lane(keys, range[0], range[1], (unsigned)(v0 + tid));
+  if (tid <= rows) bound[tid] = lower_bound_lane(g.keys, range[0], range[1], (unsigned)(v0 + tid));
   __syncthreads();
-  const int per = 256 / group, sub = tid / group, sl = tid % group;  // `group` lanes a row
-  for (int r = sub; r < rows; r += per) {
-    const int a = bound[r], b = bound[r + 1];
-    if (b - a > kChunk) continue;
-    for (int c = sl * 8; c < e; c += group * 8) {
-      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      add_rows<T>(dy, order, a, b, e, c, acc);
-      float* p = dtable + (size_t)(v0 + r) * e + c;
-      *reinterpret_cast<float4*>(p) = make_float4(acc[0] * scale, acc[1] * scale, acc[2] * scale, acc[3] * scale);
-      *reinterpret_cast<float4*>(p + 4) = make_float4(acc[4] * scale, acc[5] * scale, acc[6] * scale, acc[7] * scale);
-    }
-  }
-  for (int r = 0; r < rows; ++r) {
-    const int a = bound[r], b = bound[r + 1];
-    if (b - a <= kChunk) continue;  // the same for the whole workgroup
-    const int c0 = a / kChunk, c1 = (b - 1) / kChunk, first = a % kChunk ? 1 : 0;
-    for (int base = 0; base < e; base += 512) {
-      const int c = base + lane * 8;
-      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (c < e) {
-#pragma unroll 4
-        for (int k = c0 + wave; k <= c1; k += 4) {
-          // (of the run's first chunk the piece is the one of its last row, unless the run begins with the chunk)
-          const float* p = part + ((size_t)k * 2 + (k == c0 ? first : 0)) * e + c;
-          const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
-          acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
-          acc[4] += y.x; acc[5] += y.y; acc[6] += y.z; acc[7] += y.w;
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) joined[wave][lane * 8 + k] = acc[k];
-      __syncthreads();
-      for (int k = tid; k < 512 && base + k < e; k += 256)
-        dtable[(size_t)(v0 + r) * e + base + k] = ((joined[0][k] + joined[1][k]) + (joined[2][k] + joined[3][k])) * scale;
-      __syncthreads();
-    }
+  const int per = g.e / 4;
+  float4* const out = reinterpret_cast<float4*>(g.dtable + (size_t)v0 * g.e);
+  for (int i = tid; i < rows * per; i += 256) {
+    const int r = i / per;
+    if (bound[r] == bound[r + 1]) out[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
 
-// one workgroup a position: the rows at that place of all sequences, 16 waves over the sequences, joined in order
-template <typename T>
-__global__ __launch_bounds__(1024) void embed_pos_kernel(const T* __restrict__ dy, const int* __restrict__ starts, int seqs, int e, float* __restrict__ dpos) {
-  __shared__ __attribute__((aligned(16))) float joined[16][512];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.x;
-  for (int base = 0; base < e; base += 512) {
+// position t, one part of the sequences: the rows at that place; a wave takes 16 sequences at a time, eight rows in flight
+template <typename T> __device__ __forceinline__ void pos_rows(const Grad& g, const T* __restrict__ dy, int block) {
+  __shared__ __attribute__((aligned(16))) float joined[4][512];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = block / g.pos_split, part = block % g.pos_split;
+  const int per = ((g.seqs + g.pos_split - 1) / g.pos_split + 63) & ~63, s0 = part * per, s1 = min(s0 + per, g.seqs);
+  for (int base = 0; base < g.e; base += 512) {
     const int c = base + lane * 8;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c < e) {
-      for (int b = wave; b < seqs; b += 64) {  // four sequences in flight
-        V8<T> v[4];
-        bool ok[4];
+    for (int s = s0 + wave * 16; s < s1; s += 64) {
+      const int q = min(s + (lane & 15), g.seqs - 1), first = g.starts[q], row = first + t;
+      unsigned m = (unsigned)(__ballot(s + (lane & 15) < s1 && t < g.starts[q + 1] - first) & 0xffffu);
+      while (m) {
+        V8<T> v[8];
+        unsigned have = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int s = min(b + 16 * j, seqs - 1), a = starts[s];
-          ok[j] = b + 16 * j < seqs && t < starts[s + 1] - a;
-          v[j] = v8_load_clamped<T>(dy, (size_t)(a + t) * e + c, ok[j]);
+        for (int j = 0; j < 8; ++j) {
+          const int w = m ? __ffs(m) - 1 : 0;
+          have |= (m ? 1u : 0u) << j;
+          m &= m - 1;
+          v[j] = v8_load_clamped<T>(dy, (size_t)__shfl(row, w, 64) * g.e + c, ((have >> j) & 1u) && c < g.e);
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 8; ++j) {
           float f[8];
-          v8_unpack(v8_mask(v[j], ok[j]), f);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) acc[k] += f[k];
+          v8_unpack(v8_mask(v[j], (have >> j) & 1u), f);
+          add8(acc, f);
         }
       }
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) joined[wave][lane * 8 + k] = acc[k];
     __syncthreads();
-    for (int k = threadIdx.x; k < 512 && base + k < e; k += 1024) {
+    float* const out = g.pos_split > 1 ? g.pos_part + ((size_t)part * (g.pos_blocks / g.pos_split) + t) * g.e : g.dpos + (size_t)t * g.e;
+    for (int k = threadIdx.x; k < 512 && base + k < g.e; k += 256) out[base + k] = (joined[0][k] + joined[1][k]) + (joined[2][k] + joined[3][k]);
+    __syncthreads();
+  }
+}
+
+// the three kinds of workgroups of the backward pass: chunks (the longest ones) first, zeros last
+template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(Grad g, const T* __restrict__ dy) {
+  const int block = blockIdx.x;
+  if (block < g.chunk_blocks) chunk_rows<T>(g, dy, block);
+  else if (block < g.chunk_blocks + g.pos_blocks) pos_rows<T>(g, dy, block - g.chunk_blocks);
+  else empty_rows(g, block - g.chunk_blocks - g.pos_blocks);
+}
+
+// runs that cross chunks: the workgroup of the chunk that such a run begins in adds up its pieces, 256 / G of them side by side; and the parts of
+// the positions' sums
+__global__ __launch_bounds__(256) void embed_join_kernel(Grad g, int chunks) {
+  __shared__ __attribute__((aligned(16))) float joined[2048];
+  __shared__ int run_end;
+  const int tid = threadIdx.x, G = g.group, per = 256 / G, sub = tid / G, sl = tid % G;
+  if ((int)blockIdx.x >= chunks) {
+    const int t = blockIdx.x - chunks, positions = g.pos_blocks / g.pos_split;
+    for (int c = tid; c < g.e; c += 256) {
       float s = 0.f;
+      for (int q = 0; q < g.pos_split; ++q) s += g.pos_part[((size_t)q * positions + t) * g.e + c];
+      g.dpos[(size_t)t * g.e + c] = s;
+    }
+    return;
+  }
+  const int chunk = blockIdx.x, a = chunk * kChunk, b = a + kChunk;
+  if (b >= g.n) return;
+  const unsigned v = g.keys[b - 1];
+  if (v >= (unsigned)g.vocab || g.keys[b] != v || (a > 0 && g.keys[a - 1] == v)) return;  // does not go on, or came in (the same for all threads)
+  if (tid < 64) {
+    const int at = lower_bound_wave(g.keys, b, g.n, v + 1, tid);
+    if (tid == 0) run_end = at;
+  }
+  __syncthreads();
+  const int last = (run_end - 1) / kChunk;
+  for (int base = 0; base < g.e; base += G * 8) {
+    const int c = base + sl * 8;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (c < g.e) {
+#pragma unroll 8
+      for (int k = chunk + sub; k <= last; k += per) {
+        const float* p = g.part + ((size_t)k * 2 + (k == chunk ? 1 : 0)) * g.e + c;
+        const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
+        const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        add8(acc, f);
+      }
+    }
 #pragma unroll
-      for (int w = 0; w < 16; ++w) s += joined[w][k];
-      dpos[(size_t)t * e + base + k] = s;
+    for (int k = 0; k < 8; ++k) joined[tid * 8 + k] = acc[k];
+    __syncthreads();
+    for (int k = tid; k < G * 8 && base + k < g.e; k += 256) {
+      float s = 0.f;
+      for (int q = 0; q < per; ++q) s += joined[q * G * 8 + k];
+      g.dtable[(size_t)v * g.e + base + k] = s * g.scale;
     }
     __syncthreads();
   }
@@ -332,17 +363,21 @@ int sort_passes(int vocab) {
   return (bits + 7) / 8;
 }
 long long sort_blocks(long long n) { return (n + kItems - 1) / kItems; }
+long long padded(long long n) { return (n + kChunk - 1) / kChunk * kChunk; }
+int pos_split(int seqs) { return seqs <= 64 ? 1 : seqs >= 1024 ? 16 : (seqs + 63) / 64; }  // 64 sequences a workgroup, while that is at most 16 parts
 
 }  // namespace
 
-// int32 scratch: two key and two row arrays, the digit counts
+// int32 scratch: two key and two row arrays (in whole chunks), the digit counts
 extern "C" long long cvh_embed_sort_elems(int rows) {
   if (rows <= 0) return -2;
-  return 4ll * rows + sort_blocks(rows) * 256;
+  return 4 * padded(rows) + sort_blocks(rows) * 256;
 }
-extern "C" long long cvh_embed_pieces_elems(int rows, int e) {
-  if (rows <= 0 || e <= 0) return -2;
-  return ((long long)rows + kChunk - 1) / kChunk * 2 * e;
+// float32 scratch: two pieces a chunk, the parts of the positions' sums
+extern "C" long long cvh_embed_pieces_elems(int rows, int e, int positions, int seqs) {
+  if (rows <= 0 || e <= 0 || positions < 0 || seqs < 0) return -2;
+  const int split = pos_split(seqs);
+  return (padded(rows) / kChunk * 2 + (split > 1 ? (long long)split * positions : 0)) * e;
 }
 extern "C" int cvh_embed_packed_fwd(int dtype, const long long* ids, const float* table, const float* pos, const int* plan, int seqs, int block, int places,
                                     int rows, int vocab, int positions, int e, float scale, void* out, void* stream) {
@@ -362,25 +397,24 @@ extern "C" int cvh_embed_packed_fwd(int dtype, const long long* ids, const float
   return 0;
 }
 
-template <typename T> static void embed_bwd(const T* dy, const unsigned* keys, const int* order, int rows, int vocab, int e, float scale, float* part, float* dtable, hipStream_t st) {
-  const int chunks = (rows + kChunk - 1) / kChunk;
-  if (rows > kChunk) hipLaunchKernelGGL(embed_pieces_kernel<T>, dim3((chunks + 3) / 4), dim3(256), 0, st, dy, keys, order, rows, vocab, e, part);
-  int group = 4;
-  while (group < 64 && group * 8 < e) group *= 2;
-  hipLaunchKernelGGL(embed_rows_kernel<T>, dim3((vocab + kTableRows - 1) / kTableRows), dim3(256), 0, st, dy, keys, order, rows, vocab, e, scale, part, dtable, group);
-}
-
 extern "C" int cvh_embed_packed_bwd(int dtype, const long long* ids, const void* dout, const int* plan, int seqs, int rows, int vocab, int e, long long padding_idx,
                                     float scale, float* dtable, int positions, float* dpos, int* sort, float* pieces, void* stream) {
   if (dtype != CVH_DT_F32 && dtype != CVH_DT_BF16) return -1;
-  if (dout == nullptr || rows <= 0 || e <= 0 || e % 8 || (dpos != nullptr && (plan == nullptr || positions <= 0)) || (plan != nullptr && seqs <= 0)) return -2;
+  if (dout == nullptr || rows <= 0 || e <= 0 || e % 8 || (dpos != nullptr && (plan == nullptr || positions <= 0 || positions > (1 << 26) || pieces == nullptr)) || (plan != nullptr && seqs <= 0)) return -2;
   if (dtable != nullptr && (ids == nullptr || sort == nullptr || pieces == nullptr || vocab <= 0 || vocab >= 0x7fffffff - kTableRows)) return -2;
   hipStream_t st = (hipStream_t)stream;
+  Grad g = {};
+  g.n = rows; g.vocab = vocab; g.e = e; g.scale = scale; g.starts = plan; g.seqs = seqs;
+  g.dtable = dtable; g.part = pieces; g.dpos = dpos;
+  g.group = 4;
+  while (g.group < 64 && g.group * 8 < e) g.group *= 2;
+  int zero_blocks = 0, chunks = 0;
   if (dtable != nullptr) {
     const int blocks = (int)sort_blocks(rows), passes = sort_passes(vocab);
-    unsigned* keys[2] = {(unsigned*)sort, (unsigned*)sort + rows};
-    int* order[2] = {sort + 2ll * rows, sort + 3ll * rows};
-    int* count = sort + 4ll * rows;
+    const long long size = padded(rows);
+    unsigned* keys[2] = {(unsigned*)sort, (unsigned*)sort + size};
+    int* order[2] = {sort + 2 * size, sort + 3 * size};
+    int* count = sort + 4 * size;
     SortIn s = {ids, plan, nullptr, nullptr, padding_idx, rows, seqs, vocab, 0};
     for (int p = 0; p < passes; ++p) {
       s.shift = 8 * p;
@@ -389,13 +423,24 @@ extern "C" int cvh_embed_packed_bwd(int dtype, const long long* ids, const void*
       s.keys = keys[p & 1];
       s.rows = order[p & 1];
     }
-    if (dtype == CVH_DT_BF16) embed_bwd<bf16_t>((const bf16_t*)dout, s.keys, s.rows, rows, vocab, e, scale, pieces, dtable, st);
-    else embed_bwd<float>((const float*)dout, s.keys, s.rows, rows, vocab, e, scale, pieces, dtable, st);
+    g.keys = s.keys;
+    g.order = s.rows;
+    chunks = (int)(size / kChunk);
+    g.chunk_blocks = (chunks + 256 / g.group - 1) / (256 / g.group);
+    zero_blocks = (vocab + kTableRows - 1) / kTableRows;
   }
+  g.pos_split = 1;
   if (dpos != nullptr) {
-    if (dtype == CVH_DT_BF16) hipLaunchKernelGGL(embed_pos_kernel<bf16_t>, dim3(positions), dim3(1024), 0, st, (const bf16_t*)dout, plan, seqs, e, dpos);
-    else hipLaunchKernelGGL(embed_pos_kernel<float>, dim3(positions), dim3(1024), 0, st, (const float*)dout, plan, seqs, e, dpos);
+    g.pos_split = pos_split(seqs);
+    g.pos_blocks = positions * g.pos_split;
+    g.pos_part = pieces + (long long)padded(rows) / kChunk * 2 * e;
   }
+  const dim3 grid(g.chunk_blocks + g.pos_blocks + zero_blocks);
+  if (grid.x == 0) return 0;
+  if (dtype == CVH_DT_BF16) hipLaunchKernelGGL(embed_grad_kernel<bf16_t>, grid, dim3(256), 0, st, g, (const bf16_t*)dout);
+  else hipLaunchKernelGGL(embed_grad_kernel<float>, grid, dim3(256), 0, st, g, (const float*)dout);
+  const int joins = (chunks > 1 ? chunks : 0) + (g.pos_split > 1 ? positions : 0);
+  if (joins > 0) hipLaunchKernelGGL(embed_join_kernel, dim3(joins), dim3(256), 0, st, g, chunks > 1 ? chunks : 0);
   CVH_CHECK_LAUNCH();
   return 0;
 }

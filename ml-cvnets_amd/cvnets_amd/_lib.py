@@ -140,7 +140,7 @@ SIGNATURES = {
     "cvh_packed_attn_fwd": [I, P, P],
     "cvh_packed_attn_bwd": [I, P, P],
     "cvh_embed_sort_elems": [I],
-    "cvh_embed_pieces_elems": [I, I],
+    "cvh_embed_pieces_elems": [I, I, I, I],
     "cvh_embed_packed_fwd": [I, P, P, P, P, I, I, I, I, I, I, I, F, P, P],
     "cvh_embed_packed_bwd": [I, P, P, P, I, I, I, I, L, F, P, I, P, P, P, P],
     "cvh_ns_workspace_elems": [P, I],

@@ -223,9 +223,9 @@ class PackedEmbedFn(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             dtable = torch.empty((vocab, e), dtype=torch.float32, device=dev)
             sort = torch.empty(_lib.query("cvh_embed_sort_elems", rows), dtype=torch.int32, device=dev)
-            pieces = torch.empty(_lib.query("cvh_embed_pieces_elems", rows, e), dtype=torch.float32, device=dev)
         if positions and ctx.needs_input_grad[1]:
             dpos = torch.empty((positions, e), dtype=torch.float32, device=dev)
+        pieces = torch.empty(_lib.query("cvh_embed_pieces_elems", rows, e, positions, 0 if dpos is None else seqs.seqs), dtype=torch.float32, device=dev)
         with torch.cuda.device(dev):
             _lib.call("cvh_embed_packed_bwd", _dt(dout), _p(ids), _p(dout), None if seqs is None else _p(seqs.plan), 0 if seqs is None else seqs.seqs, rows,
                       vocab, e, padding, scale, _p(dtable), positions, _p(dpos), _p(sort), _p(pieces), _stream_of(dout))
