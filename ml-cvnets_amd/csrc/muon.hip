@@ -13,8 +13,9 @@
 //
 // (a x is added to the finished sum: with a I inside P the small terms of the long sum are rounded next to a x, 8e-6 instead of 2e-6 after 5
 // steps of a 1030 x 1100 matrix, whose float32 products give 2e-6, too.)
-// x is kept in both layouts, [m][n] and [n][m], so that every product is rows times rows with the contraction index contiguous; the epilogue
-// writes both.  Sides are padded to the tile with zeros, which the products keep zero, so that the main loop has no bounds.
+// x is kept once, [m][n] (contraction over n: rows times rows); P x reads its columns with LDS transpose reads.  The cross products hi lo + lo hi
+// have accumulators of their own: the large sum is then rounded once per 16 terms instead of three times.  Every epilogue goes through
+// LDS, so that global memory sees whole rows.  Sides are padded to the tile with zeros, which the products keep zero: the main loop has no bounds.
 // All matrices of a list go through one launch per product (a table in the kernel's arguments): 2 + 3 steps launches for up to kMats matrices.
 #include "common.hpp"
 #include "cvnets_hip.h"
@@ -22,6 +23,7 @@
 namespace {
 
 constexpr int kMats = 32;
+constexpr int kWideTiles = 512;
 constexpr int kMostRows = 1 << 14, kMostCols = 1 << 24;  // of the shorter and the longer side
 constexpr float kScale = 4096.f, kScaleP = 1024.f;  // of x and G; of P
 typedef _Float16 half_t;
@@ -32,7 +34,7 @@ struct Mat {
   const void* src;  // u, or the gradient (float32)
   void* dst;        // result (orthogonalize)
   float *mom, *par;
-  half_t* ws;       // x [2][mp][np], x^T [2][np][mp], the same again (ping-pong), G [2][mp][mp], P [2][mp][mp]; hi and lo planes
+  half_t* ws;       // x [2][mp][np] twice (ping-pong), G [2][mp][mp], P [2][mp][mp]; hi and lo planes
   double* norm;     // partial sums of squares
   int m, n, mp, np, rows, cols, group;
   float gain;
@@ -48,9 +50,8 @@ __device__ __forceinline__ int find(const Mats& t, int wg) {
   return i;
 }
 __device__ __forceinline__ size_t plane_x(const Mat& a) { return (size_t)a.mp * a.np; }
-__device__ __forceinline__ half_t* x_of(const Mat& a, int which) { return a.ws + (size_t)which * 4 * plane_x(a); }
-__device__ __forceinline__ half_t* xt_of(const Mat& a, int which) { return x_of(a, which) + 2 * plane_x(a); }
-__device__ __forceinline__ half_t* g_of(const Mat& a) { return a.ws + 8 * plane_x(a); }
+__device__ __forceinline__ half_t* x_of(const Mat& a, int which) { return a.ws + (size_t)which * 2 * plane_x(a); }
+__device__ __forceinline__ half_t* g_of(const Mat& a) { return a.ws + 4 * plane_x(a); }
 __device__ __forceinline__ half_t* p_of(const Mat& a) { return g_of(a) + 2 * (size_t)a.mp * a.mp; }
 
 __device__ __forceinline__ void split(float v, half_t& hi, half_t& lo) {
@@ -61,7 +62,7 @@ __device__ __forceinline__ void split(float v, half_t& hi, half_t& lo) {
 // -----------------------------------------------------------------------------------------------------------------------------------------
 // sums of squares (and the momentum), kNormItems elements a workgroup; in 64 bits, so that no gradient's square leaves the range
 // -----------------------------------------------------------------------------------------------------------------------------------------
-constexpr int kNormItems = 16384;
+constexpr int kNormItems = 8192;
 template <typename T, bool MOM> __device__ __forceinline__ float update_of(const Mat& a, size_t i, float mu, int nesterov) {
   const float g = to_f<T>(reinterpret_cast<const T*>(a.src)[i]);
   if (!MOM) return g;
@@ -73,11 +74,33 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_norm_k
   const int k = find(t, blockIdx.x), chunk = blockIdx.x - t.first[k];
   const Mat& a = t.mat[k];
   const size_t size = (size_t)a.m * a.n, i0 = (size_t)chunk * kNormItems, i1 = i0 + kNormItems < size ? i0 + kNormItems : size;
+  const T* const src = reinterpret_cast<const T*>(a.src);
   double s = 0.0;
-  for (size_t i = i0 + threadIdx.x; i < i1; i += 256) {
-    if (MOM) a.mom[i] = mu * a.mom[i] + to_f<T>(reinterpret_cast<const T*>(a.src)[i]);
-    const double u = update_of<T, MOM>(a, i, mu, nesterov);
+  auto one = [&](float g, float m) {
+    const double u = MOM ? (nesterov ? g + mu * m : m) : g;
     s += u * u;
+  };
+  size_t done = i0;
+  if (((reinterpret_cast<uintptr_t>(src) | (MOM ? reinterpret_cast<uintptr_t>(a.mom) : 0)) & 15) == 0) {
+    done = i0 + (i1 - i0) / 4 * 4;
+    for (size_t i = i0 + threadIdx.x * 4; i < done; i += 1024) {
+      float g[4], m[4] = {0.f, 0.f, 0.f, 0.f};
+      v4_unpack(v4_load<T>(src + i), g);
+      if (MOM) {
+        v4_unpack(v4_load<float>(a.mom + i), m);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[e] = mu * m[e] + g[e];
+        *reinterpret_cast<float4*>(a.mom + i) = make_float4(m[0], m[1], m[2], m[3]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) one(g[e], m[e]);
+    }
+  }
+  for (size_t i = done + threadIdx.x; i < i1; i += 256) {
+    const float g = to_f<T>(src[i]);
+    float m = 0.f;
+    if (MOM) a.mom[i] = m = mu * a.mom[i] + g;
+    one(g, m);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -87,7 +110,7 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_norm_k
 }
 
 // -----------------------------------------------------------------------------------------------------------------------------------------
-// x = u / (|u| + eps) into both layouts, 64 x 64 elements (of the padded matrix) a workgroup
+// x = u / (|u| + eps), 64 x 64 elements (of the padded matrix) a workgroup; through LDS where the matrix is taller than wide
 // -----------------------------------------------------------------------------------------------------------------------------------------
 template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_kernel(Mats t, float mu, int nesterov, float eps) {
   __shared__ float tile[64][65];
@@ -95,6 +118,14 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_
   const int k = find(t, blockIdx.x), at = blockIdx.x - t.first[k], tid = threadIdx.x;
   const Mat& a = t.mat[k];
   const int tn = a.np / 64, i0 = at / tn * 64, j0 = at % tn * 64;
+  const bool flip = a.rows > a.cols;  // x[i][j] = u[j][i]
+  float v[16];
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    const int r = q * 4 + (tid >> 6), c = tid & 63;  // of u's tile: c runs along u's rows
+    const int i = flip ? i0 + c : i0 + r, j = flip ? j0 + r : j0 + c;
+    v[q] = i < a.m && j < a.n ? update_of<T, MOM>(a, (size_t)(flip ? j : i) * a.cols + (flip ? i : j), mu, nesterov) : 0.f;
+  }
   if (tid < 64) {
     const int chunks = (int)(((size_t)a.m * a.n + kNormItems - 1) / kNormItems);
     double s = 0.0;
@@ -103,39 +134,46 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if (tid == 0) total = s;
   }
-  const bool flip = a.rows > a.cols;  // x[i][j] = u[j][i]
-  for (int e = tid; e < 4096; e += 256) {
-    const int r = e >> 6, c = e & 63;  // of u's tile: c runs along u's rows
-    const int i = flip ? i0 + c : i0 + r, j = flip ? j0 + r : j0 + c;
-    const float v = i < a.m && j < a.n ? update_of<T, MOM>(a, (size_t)(flip ? j : i) * a.cols + (flip ? i : j), mu, nesterov) : 0.f;
-    if (flip) tile[c][r] = v; else tile[r][c] = v;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    const int r = q * 4 + (tid >> 6), c = tid & 63;
+    if (flip) tile[c][r] = v[q]; else tile[r][c] = v[q];
   }
   __syncthreads();
   const double inv = (double)kScale / (sqrt(total) + (double)eps);
-  half_t *x = x_of(a, 0), *xt = xt_of(a, 0);
+  half_t* const x = x_of(a, 0);
   const size_t plane = plane_x(a);
-  for (int e = tid; e < 4096; e += 256) {
-    const int r = e >> 6, c = e & 63;
-    half_t hi, lo;
-    split((float)(tile[r][c] * inv), hi, lo);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int r = q * 16 + (tid >> 4), c = (tid & 15) * 4;
+    half4_t hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      half_t h, l;
+      split((float)(tile[r][c + e] * inv), h, l);
+      hi[e] = h;
+      lo[e] = l;
+    }
     const size_t o = (size_t)(i0 + r) * a.np + j0 + c;
-    x[o] = hi;
-    x[plane + o] = lo;
-    split((float)(tile[c][r] * inv), hi, lo);
-    const size_t p = (size_t)(j0 + r) * a.mp + i0 + c;
-    xt[p] = hi;
-    xt[plane + p] = lo;
+    *reinterpret_cast<half4_t*>(x + o) = hi;
+    *reinterpret_cast<half4_t*>(x + plane + o) = lo;
   }
 }
 
 // -----------------------------------------------------------------------------------------------------------------------------------------
-// rows-times-rows product of hi + lo operands: acc[i][j] = sum_k A[i][k] B[j][k] for a TILE x TILE tile, 4 waves of (TILE / 2)^2
+// product of hi + lo operands on a TILE x TILE tile, 4 waves of (TILE / 2)^2: acc[r][c] = sum_k A[r][k] B[c][k], B in rows; A in rows, or
+// (COLS) given as [k][r] and read with LDS transpose reads.  Double-buffered in LDS, loaded a step ahead through registers.
 // -----------------------------------------------------------------------------------------------------------------------------------------
-constexpr int BK = 32, PITCH = BK + 8;
-template <int TILE> struct Product {
-  static constexpr int W = TILE / 64;       // 32-wide fragments of a wave in each direction
+constexpr int BK = 32, PITCH = BK + 8;  // rows of 80 bytes: 16 lanes' 16-byte reads hit distinct banks
+typedef short v4s_t __attribute__((ext_vector_type(4)));
+template <int TILE, bool COLS> struct Product {
+  static constexpr int W = TILE / 64;               // 32-wide fragments of a wave in each direction
   static constexpr int CH = TILE * (BK / 8) / 256;  // 16-byte pieces a thread loads of each plane
-  half_t* lds;                              // [2 stages][4 planes: A hi, A lo, B hi, B lo][TILE][PITCH]
+  static constexpr int CPITCH = TILE + 16;          // [k][r] rows: 4 rows of a transpose read on distinct banks
+  static constexpr int AELEMS = COLS ? BK * CPITCH : TILE * PITCH, BELEMS = TILE * PITCH, STAGE = 2 * AELEMS + 2 * BELEMS;
+  static constexpr int OPITCH = TILE + 4;           // of the float tile of the epilogue
+  static constexpr size_t BYTES = sizeof(half_t) * 2 * STAGE > sizeof(float) * TILE * OPITCH ? sizeof(half_t) * 2 * STAGE : sizeof(float) * TILE * OPITCH;
+  half_t* lds;
   f32x16_t acc[W][W];
   uint4 q[4][CH];
 
@@ -143,30 +181,42 @@ template <int TILE> struct Product {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int idx = tid + c * 256, r = idx >> 2, col = k0 + (idx & 3) * 8;
-      q[0][c] = *reinterpret_cast<const uint4*>(a + (size_t)r * lda + col);
-      q[1][c] = *reinterpret_cast<const uint4*>(a + a_plane + (size_t)r * lda + col);
+      const half_t* pa = COLS ? a + (size_t)(k0 + idx / (TILE / 8)) * lda + idx % (TILE / 8) * 8 : a + (size_t)r * lda + col;
+      q[0][c] = *reinterpret_cast<const uint4*>(pa);
+      q[1][c] = *reinterpret_cast<const uint4*>(pa + a_plane);
       q[2][c] = *reinterpret_cast<const uint4*>(b + (size_t)r * ldb + col);
       q[3][c] = *reinterpret_cast<const uint4*>(b + b_plane + (size_t)r * ldb + col);
     }
   }
   __device__ __forceinline__ void store(int stage, int tid) {
+    half_t* const s = lds + stage * STAGE;
 #pragma unroll
-    for (int p = 0; p < 4; ++p)
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int idx = tid + c * 256;
-        *reinterpret_cast<uint4*>(lds + ((size_t)(stage * 4 + p) * TILE + (idx >> 2)) * PITCH + (idx & 3) * 8) = q[p][c];
-      }
+    for (int c = 0; c < CH; ++c) {
+      const int idx = tid + c * 256, rows = (idx >> 2) * PITCH + (idx & 3) * 8;
+      const int at = COLS ? idx / (TILE / 8) * CPITCH + idx % (TILE / 8) * 8 : rows;
+      *reinterpret_cast<uint4*>(s + at) = q[0][c];
+      *reinterpret_cast<uint4*>(s + AELEMS + at) = q[1][c];
+      *reinterpret_cast<uint4*>(s + 2 * AELEMS + rows) = q[2][c];
+      *reinterpret_cast<uint4*>(s + 2 * AELEMS + BELEMS + rows) = q[3][c];
+    }
   }
-  __device__ __forceinline__ half8_t frag(int stage, int plane, int row, int k, int lane) const {
-    return *reinterpret_cast<const half8_t*>(lds + ((size_t)(stage * 4 + plane) * TILE + row + (lane & 31)) * PITCH + k + 8 * (lane >> 5));
+  static __device__ __forceinline__ half8_t row_frag(const half_t* t, int row, int k, int lane) {
+    return *reinterpret_cast<const half8_t*>(t + (row + (lane & 31)) * PITCH + k + 8 * (lane >> 5));
+  }
+  static __device__ __forceinline__ half8_t col_frag(const half_t* t, int row, int k, int lane) {
+    const int i = lane & 15;
+    const half_t* p = t + (k + 8 * (lane >> 5) + (i >> 2)) * CPITCH + row + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+    const v4s_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*)(p));
+    const v4s_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*)(p + 4 * CPITCH));
+    return __builtin_bit_cast(half8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
   __device__ __forceinline__ void run(const half_t* a, size_t a_plane, int lda, const half_t* b, size_t b_plane, int ldb, int K, int tid) {
     const int lane = tid & 63, wr = (tid >> 7) * (TILE / 2), wc = ((tid >> 6) & 1) * (TILE / 2);
+    f32x16_t cross[W][W];
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
-      for (int j = 0; j < W; ++j) acc[i][j] = acc_zero();
+      for (int j = 0; j < W; ++j) acc[i][j] = cross[i][j] = acc_zero();
     load(a, a_plane, lda, b, b_plane, ldb, 0, tid);
     store(0, tid);
     if (K > BK) load(a, a_plane, lda, b, b_plane, ldb, BK, tid);
@@ -174,168 +224,218 @@ template <int TILE> struct Product {
       wg_barrier_lds();
       if (k0 + BK < K) store(s ^ 1, tid);
       if (k0 + 2 * BK < K) load(a, a_plane, lda, b, b_plane, ldb, k0 + 2 * BK, tid);
+      const half_t* const st = lds + s * STAGE;
 #pragma unroll
       for (int k = 0; k < BK; k += 16) {
         half8_t ah[W], al[W], bh[W], bl[W];
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-          ah[i] = frag(s, 0, wr + 32 * i, k, lane);
-          al[i] = frag(s, 1, wr + 32 * i, k, lane);
-          bh[i] = frag(s, 2, wc + 32 * i, k, lane);
-          bl[i] = frag(s, 3, wc + 32 * i, k, lane);
+          ah[i] = COLS ? col_frag(st, wr + 32 * i, k, lane) : row_frag(st, wr + 32 * i, k, lane);
+          al[i] = COLS ? col_frag(st + AELEMS, wr + 32 * i, k, lane) : row_frag(st + AELEMS, wr + 32 * i, k, lane);
+          bh[i] = row_frag(st + 2 * AELEMS, wc + 32 * i, k, lane);
+          bl[i] = row_frag(st + 2 * AELEMS + BELEMS, wc + 32 * i, k, lane);
         }
 #pragma unroll
         for (int i = 0; i < W; ++i)
 #pragma unroll
           for (int j = 0; j < W; ++j) {
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
+            cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], cross[i][j], 0, 0, 0);
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
           }
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+          for (int j = 0; j < W; ++j) cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], cross[i][j], 0, 0, 0);
       }
     }
-  }
-  // f(row, column, 4 values of rows row .. row + 3) over the tile
-  template <typename F> __device__ __forceinline__ void each(int tid, F&& f) const {
-    const int lane = tid & 63, wr = (tid >> 7) * (TILE / 2), wc = ((tid >> 6) & 1) * (TILE / 2);
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
       for (int j = 0; j < W; ++j)
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const float v[4] = {acc[i][j][4 * q4], acc[i][j][4 * q4 + 1], acc[i][j][4 * q4 + 2], acc[i][j][4 * q4 + 3]};
-          f(wr + 32 * i + 8 * q4 + 4 * (lane >> 5), wc + 32 * j + (lane & 31), v);
-        }
+        for (int r = 0; r < 16; ++r) acc[i][j][r] += cross[i][j][r];
+  }
+  // the tile as floats in LDS, transposed: out[c][r]
+  __device__ __forceinline__ float* spill(int tid) {
+    const int lane = tid & 63, wr = (tid >> 7) * (TILE / 2), wc = ((tid >> 6) & 1) * (TILE / 2);
+    float* const out = reinterpret_cast<float*>(lds);
+    __syncthreads();  // the operands are read
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<float4*>(out + (wc + 32 * j + (lane & 31)) * OPITCH + wr + 32 * i + 8 * e + 4 * (lane >> 5)) =
+              make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
+    __syncthreads();
+    return out;
   }
 };
 
-// value[i .. i + 3][j] as hi + lo into both an [i][j] and a [j][i] matrix
-__device__ __forceinline__ void put(half_t* ij, size_t ij_plane, int ld_ij, half_t* ji, size_t ji_plane, int ld_ji, int i, int j, const float* v) {
-  half4_t hi, lo;
+__device__ __forceinline__ void split8(const float* v, half8_t& hi, half8_t& lo) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < 8; ++e) {
     half_t h, l;
     split(v[e], h, l);
     hi[e] = h;
     lo[e] = l;
-    if (ij != nullptr) {
-      ij[(size_t)(i + e) * ld_ij + j] = h;
-      ij[ij_plane + (size_t)(i + e) * ld_ij + j] = l;
-    }
   }
-  if (ji != nullptr) {
-    *reinterpret_cast<half4_t*>(ji + (size_t)j * ld_ji + i) = hi;
-    *reinterpret_cast<half4_t*>(ji + ji_plane + (size_t)j * ld_ji + i) = lo;
-  }
+}
+// Four consecutive tiles (which share an operand panel) on one XCD: block b runs on XCD b % 8.  Groups of 32 blocks; the rest in order.
+__device__ __forceinline__ int near_tiles(int b, int n) {
+  const int whole = n & ~31;
+  return b < whole ? (b & ~31) + (b & 7) * 4 + ((b & 31) >> 3) : b;
 }
 
 // G = x x^T (POLY false) or P = b G + c G G (true): tiles (i, j <= i), written to both halves
 template <int TILE, bool POLY> __global__ __launch_bounds__(256, 2) void ns_sym_kernel(Mats t, int which, float cb, float cc) {
-  __shared__ __attribute__((aligned(16))) half_t lds[2 * 4 * TILE * PITCH];
-  const int k = find(t, blockIdx.x), tid = threadIdx.x;
+  typedef Product<TILE, false> Prod;
+  __shared__ __attribute__((aligned(16))) char smem[Prod::BYTES];
+  const int block = near_tiles(blockIdx.x, t.first[t.count]), k = find(t, block), tid = threadIdx.x;
   const Mat& a = t.mat[k];
-  int at = blockIdx.x - t.first[k], ti = 0;
+  int at = block - t.first[k], ti = 0;
   while (at > ti) at -= ++ti;  // (ti, at) of the lower triangle
   const int i0 = ti * TILE, j0 = at * TILE;
   const size_t plane = (size_t)a.mp * a.mp;
   half_t* const g = g_of(a);
-  Product<TILE> p;
-  p.lds = lds;
+  Prod p;
+  p.lds = reinterpret_cast<half_t*>(smem);
   if (POLY) p.run(g + (size_t)i0 * a.mp, plane, a.mp, g + (size_t)j0 * a.mp, plane, a.mp, a.mp, tid);
   else p.run(x_of(a, which) + (size_t)i0 * a.np, plane_x(a), a.np, x_of(a, which) + (size_t)j0 * a.np, plane_x(a), a.np, a.np, tid);
   half_t* const out = POLY ? p_of(a) : g;
-  p.each(tid, [&](int i, int j, const float* v) {
-    float w[4];
+  float* const v = p.spill(tid);  // v[j][i]
+  for (int idx = tid; idx < TILE * TILE / 8; idx += 256) {
+    const int j = idx / (TILE / 8), i = idx % (TILE / 8) * 8;
+    const size_t o = (size_t)(j0 + j) * a.mp + i0 + i;
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = v[j * Prod::OPITCH + i + e] * (1.f / kScale);
     if (POLY) {
-      const size_t o = (size_t)(j0 + j) * a.mp + i0 + i;  // G[j][i ..] = G[i ..][j]
-      const half4_t h = *reinterpret_cast<const half4_t*>(g + o), l = *reinterpret_cast<const half4_t*>(g + plane + o);
+      const half8_t h = *reinterpret_cast<const half8_t*>(g + o), l = *reinterpret_cast<const half8_t*>(g + plane + o);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = (kScaleP / kScale) * (cc * (v[e] * (1.f / kScale)) + cb * ((float)h[e] + (float)l[e]));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = v[e] * (1.f / kScale);
+      for (int e = 0; e < 8; ++e) w[e] = (kScaleP / kScale) * (cc * w[e] + cb * ((float)h[e] + (float)l[e]));
     }
-    put(i0 == j0 ? nullptr : out, plane, a.mp, out, plane, a.mp, i0 + i, j0 + j, w);
-  });
+    half8_t hi, lo;
+    split8(w, hi, lo);
+    *reinterpret_cast<half8_t*>(out + o) = hi;
+    *reinterpret_cast<half8_t*>(out + plane + o) = lo;
+    if (i0 != j0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[j * Prod::OPITCH + i + e] = w[e];
+    }
+  }
+  if (i0 == j0) return;
+  __syncthreads();
+  for (int idx = tid; idx < TILE * TILE / 8; idx += 256) {  // the mirror image
+    const int i = idx % TILE, j = idx / TILE * 8;
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = v[(j + e) * Prod::OPITCH + i];
+    half8_t hi, lo;
+    split8(w, hi, lo);
+    const size_t o = (size_t)(i0 + i) * a.mp + j0 + j;
+    *reinterpret_cast<half8_t*>(out + o) = hi;
+    *reinterpret_cast<half8_t*>(out + plane + o) = lo;
+  }
 }
 
 // x <- a x + P x; the last one writes the result instead
 template <int TILE, typename T, int LAST> __global__ __launch_bounds__(256, 2) void ns_apply_kernel(Mats t, int which, float ca, const float* __restrict__ hp) {
-  __shared__ __attribute__((aligned(16))) half_t lds[2 * 4 * TILE * PITCH];
-  const int k = find(t, blockIdx.x), tid = threadIdx.x, at = blockIdx.x - t.first[k];
+  typedef Product<TILE, true> Prod;
+  __shared__ __attribute__((aligned(16))) char smem[Prod::BYTES];
+  const int block = near_tiles(blockIdx.x, t.first[t.count]), k = find(t, block), tid = threadIdx.x, at = block - t.first[k];
   const Mat& a = t.mat[k];
   const int tm = a.mp / TILE, i0 = at % tm * TILE, j0 = at / tm * TILE;
-  Product<TILE> p;
-  p.lds = lds;
-  p.run(p_of(a) + (size_t)i0 * a.mp, (size_t)a.mp * a.mp, a.mp, xt_of(a, which) + (size_t)j0 * a.mp, plane_x(a), a.mp, a.mp, tid);
-  const half_t* const xt = xt_of(a, which);
+  const half_t* const x = x_of(a, which);
   const size_t plane = plane_x(a);
-  auto next = [&](int i, int j, const float* v, float* w) {  // kScale times the new x[i .. i + 3][j]
-    const size_t o = (size_t)(j0 + j) * a.mp + i0 + i;
-    const half4_t h = *reinterpret_cast<const half4_t*>(xt + o), l = *reinterpret_cast<const half4_t*>(xt + plane + o);
+  Prod p;
+  p.lds = reinterpret_cast<half_t*>(smem);
+  p.run(x + j0, plane, a.np, p_of(a) + (size_t)i0 * a.mp, (size_t)a.mp * a.mp, a.mp, a.mp, tid);
+  float* const v = p.spill(tid);  // v[i][j]
+  half_t* const next = x_of(a, which ^ 1);
+  for (int idx = tid; idx < TILE * TILE / 8; idx += 256) {
+    const int i = idx / (TILE / 8), j = idx % (TILE / 8) * 8;
+    const size_t o = (size_t)(i0 + i) * a.np + j0 + j;
+    const half8_t h = *reinterpret_cast<const half8_t*>(x + o), l = *reinterpret_cast<const half8_t*>(x + plane + o);
+    float w[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = fmaf(ca, (float)h[e] + (float)l[e], v[e] * (1.f / kScaleP));
-  };
-  if (LAST == 0) {
-    p.each(tid, [&](int i, int j, const float* v) {
-      float w[4];
-      next(i, j, v, w);
-      put(x_of(a, which ^ 1), plane_x(a), a.np, xt_of(a, which ^ 1), plane_x(a), a.mp, i0 + i, j0 + j, w);
-    });
-  } else {
-    const bool flip = a.rows > a.cols;
-    const float lr = LAST == 2 ? hp[2 * a.group] : 0.f, keep = LAST == 2 ? 1.f - lr * hp[2 * a.group + 1] : 0.f, step = lr * a.gain;
-    p.each(tid, [&](int i, int j, const float* v) {
-      float w[4];
-      next(i, j, v, w);
+    for (int e = 0; e < 8; ++e) w[e] = fmaf(ca, (float)h[e] + (float)l[e], v[i * Prod::OPITCH + j + e] * (1.f / kScaleP));
+    if (LAST == 0) {
+      half8_t hi, lo;
+      split8(w, hi, lo);
+      *reinterpret_cast<half8_t*>(next + o) = hi;
+      *reinterpret_cast<half8_t*>(next + plane + o) = lo;
+    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = i0 + i + e, c = j0 + j;
-        if (r >= a.m || c >= a.n) continue;
-        const size_t o = flip ? (size_t)c * a.cols + r : (size_t)r * a.cols + c;
-        const float x = w[e] * (1.f / kScale);
-        if (LAST == 1) reinterpret_cast<T*>(a.dst)[o] = from_f<T>(x);
-        else a.par[o] = a.par[o] * keep - step * x;
-      }
-    });
+      for (int e = 0; e < 8; ++e) v[i * Prod::OPITCH + j + e] = w[e] * (1.f / kScale);
+    }
+  }
+  if (LAST == 0) return;
+  __syncthreads();
+  const bool flip = a.rows > a.cols;
+  const float lr = LAST == 2 ? hp[2 * a.group] : 0.f, keep = LAST == 2 ? 1.f - lr * hp[2 * a.group + 1] : 0.f, step = lr * a.gain;
+  for (int idx = tid; idx < TILE * TILE; idx += 256) {
+    const int slow = idx / TILE, fast = idx % TILE, i = flip ? fast : slow, j = flip ? slow : fast;
+    if (i0 + i >= a.m || j0 + j >= a.n) continue;
+    const size_t o = flip ? (size_t)(j0 + j) * a.cols + i0 + i : (size_t)(i0 + i) * a.cols + j0 + j;
+    const float y = v[i * Prod::OPITCH + j];
+    if (LAST == 1) reinterpret_cast<T*>(a.dst)[o] = from_f<T>(y);
+    else a.par[o] = a.par[o] * keep - step * y;
   }
 }
 
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
-// 128-wide tiles unless the list has too few of them for the card; then 64-wide ones (and no side is padded to more than it has to be)
-int tile_of(const cvh_ns_matrix* mats, int n) {
-  long long tiles = 0;
-  for (int i = 0; i < n; ++i) {
-    const int m = mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols, w = mats[i].rows < mats[i].cols ? mats[i].cols : mats[i].rows;
-    tiles += (long long)(round_up(m, 128) / 128) * (round_up(w, 128) / 128);
-  }
-  return tiles >= 512 ? 128 : 64;
-}
-long long bytes_of(const cvh_ns_matrix& a, int tile) {
+// sides are padded to 64, or to 128 where that adds little: both tile widths then fit
+int pad_of(int v) { return v >= 512 ? round_up(v, 128) : round_up(v, 64); }
+long long bytes_of(const cvh_ns_matrix& a) {
   const long long m = a.rows < a.cols ? a.rows : a.cols, n = a.rows < a.cols ? a.cols : a.rows;
-  const long long mp = round_up((int)m, tile), np = round_up((int)n, tile), chunks = (m * n + kNormItems - 1) / kNormItems;
-  return (8 * mp * np + 4 * mp * mp) * 2 + (chunks * 8 + 255) / 256 * 256;
+  const long long mp = pad_of((int)m), np = pad_of((int)n), chunks = (m * n + kNormItems - 1) / kNormItems;
+  return (4 * mp * np + 4 * mp * mp) * 2 + (chunks * 8 + 255) / 256 * 256;
 }
 
-template <typename F> void prefix(Mats& t, F&& groups) {
+template <typename F> int prefix(Mats& t, F&& groups) {
   t.first[0] = 0;
   for (int i = 0; i < t.count; ++i) t.first[i + 1] = t.first[i] + groups(t.mat[i]);
+  return t.first[t.count];
 }
-template <int TILE, typename T, bool MOM> int run_list(Mats& t, int steps, float a, float b, float c, float eps, float mu, int nesterov, const float* hp, hipStream_t st) {
-  prefix(t, [](const Mat& q) { return (int)(((long long)q.m * q.n + kNormItems - 1) / kNormItems); });
-  ns_norm_kernel<T, MOM><<<dim3(t.first[t.count]), dim3(256), 0, st>>>(t, mu, nesterov);
-  prefix(t, [](const Mat& q) { return q.mp / 64 * (q.np / 64); });
-  ns_scale_kernel<T, MOM><<<dim3(t.first[t.count]), dim3(256), 0, st>>>(t, mu, nesterov, eps);
+// 128-wide tiles where the list has enough of them to fill the card (and every side takes them), else 64-wide ones
+template <typename F> bool wide_tiles(const Mats& t, int least, F&& tiles) {
+  long long n = 0;
+  for (int i = 0; i < t.count; ++i) {
+    if (t.mat[i].mp % 128 || t.mat[i].np % 128) return false;
+    n += tiles(t.mat[i]);
+  }
+  return n >= least;
+}
+template <int TILE> int sym_tiles(const Mat& q) { return q.mp / TILE * (q.mp / TILE + 1) / 2; }
+template <int TILE> int all_tiles(const Mat& q) { return q.mp / TILE * (q.np / TILE); }
+template <typename T, bool MOM> int run_list(Mats& t, int steps, float a, float b, float c, float eps, float mu, int nesterov, const float* hp, hipStream_t st) {
+  const dim3 wg(256);
+  int n = prefix(t, [](const Mat& q) { return (int)(((long long)q.m * q.n + kNormItems - 1) / kNormItems); });
+  ns_norm_kernel<T, MOM><<<dim3(n), wg, 0, st>>>(t, mu, nesterov);
+  n = prefix(t, all_tiles<64>);
+  ns_scale_kernel<T, MOM><<<dim3(n), wg, 0, st>>>(t, mu, nesterov, eps);
+  const bool ws = wide_tiles(t, kWideTiles, sym_tiles<128>), wa = wide_tiles(t, kWideTiles, all_tiles<128>);
   Mats sym = t;
-  prefix(sym, [](const Mat& q) { return q.mp / TILE * (q.mp / TILE + 1) / 2; });
-  prefix(t, [](const Mat& q) { return q.mp / TILE * (q.np / TILE); });
-  const dim3 gs(sym.first[sym.count]), ga(t.first[t.count]);
+  const dim3 gs(ws ? prefix(sym, sym_tiles<128>) : prefix(sym, sym_tiles<64>)), ga(wa ? prefix(t, all_tiles<128>) : prefix(t, all_tiles<64>));
   for (int s = 0; s < steps; ++s) {
-    ns_sym_kernel<TILE, false><<<gs, dim3(256), 0, st>>>(sym, s & 1, b, c);
-    ns_sym_kernel<TILE, true><<<gs, dim3(256), 0, st>>>(sym, s & 1, b, c);
-    if (s + 1 < steps) ns_apply_kernel<TILE, T, 0><<<ga, dim3(256), 0, st>>>(t, s & 1, a, hp);
-    else ns_apply_kernel<TILE, T, MOM ? 2 : 1><<<ga, dim3(256), 0, st>>>(t, s & 1, a, hp);
+    const int w = s & 1;
+    if (ws) {
+      ns_sym_kernel<128, false><<<gs, wg, 0, st>>>(sym, w, b, c);
+      ns_sym_kernel<128, true><<<gs, wg, 0, st>>>(sym, w, b, c);
+    } else {
+      ns_sym_kernel<64, false><<<gs, wg, 0, st>>>(sym, w, b, c);
+      ns_sym_kernel<64, true><<<gs, wg, 0, st>>>(sym, w, b, c);
+    }
+    constexpr int LAST = MOM ? 2 : 1;
+    if (s + 1 < steps) {
+      if (wa) ns_apply_kernel<128, T, 0><<<ga, wg, 0, st>>>(t, w, a, hp);
+      else ns_apply_kernel<64, T, 0><<<ga, wg, 0, st>>>(t, w, a, hp);
+    } else {
+      if (wa) ns_apply_kernel<128, T, LAST><<<ga, wg, 0, st>>>(t, w, a, hp);
+      else ns_apply_kernel<64, T, LAST><<<ga, wg, 0, st>>>(t, w, a, hp);
+    }
   }
   CVH_CHECK_LAUNCH();
   return 0;
@@ -343,7 +443,6 @@ template <int TILE, typename T, bool MOM> int run_list(Mats& t, int steps, float
 
 template <typename T, bool MOM>
 int run_all(const cvh_ns_matrix* mats, int n, int steps, float a, float b, float c, float eps, float mu, int nesterov, const float* hp, void* ws, hipStream_t st) {
-  const int tile = tile_of(mats, n);
   char* at = reinterpret_cast<char*>(ws);
   for (int i0 = 0; i0 < n; i0 += kMats) {
     Mats t;
@@ -355,13 +454,13 @@ int run_all(const cvh_ns_matrix* mats, int n, int steps, float a, float b, float
       d.rows = q.rows; d.cols = q.cols; d.group = q.group; d.gain = q.gain;
       d.m = q.rows < q.cols ? q.rows : q.cols;
       d.n = q.rows < q.cols ? q.cols : q.rows;
-      d.mp = round_up(d.m, tile);
-      d.np = round_up(d.n, tile);
+      d.mp = pad_of(d.m);
+      d.np = pad_of(d.n);
       d.ws = reinterpret_cast<half_t*>(at);
-      d.norm = reinterpret_cast<double*>(at + (8ll * d.mp * d.np + 4ll * d.mp * d.mp) * 2);
-      at += bytes_of(q, tile);
+      d.norm = reinterpret_cast<double*>(at + (4ll * d.mp * d.np + 4ll * d.mp * d.mp) * 2);
+      at += bytes_of(q);
     }
-    const int rc = tile == 128 ? run_list<128, T, MOM>(t, steps, a, b, c, eps, mu, nesterov, hp, st) : run_list<64, T, MOM>(t, steps, a, b, c, eps, mu, nesterov, hp, st);
+    const int rc = run_list<T, MOM>(t, steps, a, b, c, eps, mu, nesterov, hp, st);
     if (rc) return rc;
   }
   return 0;
@@ -382,8 +481,7 @@ int check(const cvh_ns_matrix* mats, int n, int steps, float a, float b, float c
 extern "C" long long cvh_ns_workspace_elems(const cvh_ns_matrix* mats, int n) {
   if (mats == nullptr || n <= 0) return -2;
   long long bytes = 0;
-  const int tile = tile_of(mats, n);
-  for (int i = 0; i < n; ++i) bytes += bytes_of(mats[i], tile);
+  for (int i = 0; i < n; ++i) bytes += bytes_of(mats[i]);
   return (bytes + 3) / 4;
 }
 extern "C" int cvh_orthogonalize(int dtype, const cvh_ns_matrix* mats, int n, int steps, float a, float b, float c, float eps, float* ws, void* stream) {
