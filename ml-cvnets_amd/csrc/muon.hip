@@ -23,7 +23,9 @@
 namespace {
 
 constexpr int kMats = 32;
-constexpr int kWideTiles = 512;
+#ifndef W8
+#define W8 100
+#endif
 constexpr int kMostRows = 1 << 14, kMostCols = 1 << 24;  // of the shorter and the longer side
 constexpr float kScale = 4096.f, kScaleP = 1024.f;  // of x and G; of P
 typedef _Float16 half_t;
@@ -161,43 +163,51 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_
 }
 
 // -----------------------------------------------------------------------------------------------------------------------------------------
-// product of hi + lo operands on a TILE x TILE tile, 4 waves of (TILE / 2)^2: acc[r][c] = sum_k A[r][k] B[c][k], B in rows; A in rows, or
-// (COLS) given as [k][r] and read with LDS transpose reads.  Double-buffered in LDS, loaded a step ahead through registers.
+// product of hi + lo operands on a TILE x TILE tile by WAVES waves: acc[r][c] = sum_k A[r][k] B[c][k], B in rows; A in rows, or (COLS) given as
+// [k][r] and read with LDS transpose reads.  Three LDS stages of BK: step t computes from one, the next one is complete (its first fragments are
+// read under t's last MFMAs), and t + 2 is written from registers that were loaded two steps before.  Fragments are read one 16-wide slice ahead of
+// their MFMAs: with reads and MFMAs of a slice in sequence the time was their sum, whatever the depth of the global prefetch.
 // -----------------------------------------------------------------------------------------------------------------------------------------
-constexpr int BK = 32, PITCH = BK + 8;  // rows of 80 bytes: 16 lanes' 16-byte reads hit distinct banks
 typedef short v4s_t __attribute__((ext_vector_type(4)));
-template <int TILE, bool COLS> struct Product {
-  static constexpr int W = TILE / 64;               // 32-wide fragments of a wave in each direction
-  static constexpr int CH = TILE * (BK / 8) / 256;  // 16-byte pieces a thread loads of each plane
-  static constexpr int CPITCH = TILE + 16;          // [k][r] rows: 4 rows of a transpose read on distinct banks
+template <int TILE, int WAVES, bool COLS> struct Product {
+  static constexpr int NT = 64 * WAVES, BK = 32, PITCH = BK + 8;  // rows of 80 bytes: 16 lanes' 16-byte reads hit distinct banks
+  static constexpr int WR = TILE * 2 / WAVES, WC = TILE / 2;  // rows and columns of a wave
+  static constexpr int FR = WR / 32, FC = WC / 32;            // 32-wide fragments of them
+  static constexpr int CH = TILE * (BK / 8) / NT;             // 16-byte pieces a thread loads of each plane
+  static constexpr int CPITCH = TILE + 16;                    // [k][r] rows: 4 rows of a transpose read on distinct banks
   static constexpr int AELEMS = COLS ? BK * CPITCH : TILE * PITCH, BELEMS = TILE * PITCH, STAGE = 2 * AELEMS + 2 * BELEMS;
-  static constexpr int OPITCH = TILE + 4;           // of the float tile of the epilogue
-  static constexpr size_t BYTES = sizeof(half_t) * 2 * STAGE > sizeof(float) * TILE * OPITCH ? sizeof(half_t) * 2 * STAGE : sizeof(float) * TILE * OPITCH;
+  static constexpr int OPITCH = TILE + 4;                     // of the float tile of the epilogue
+  static constexpr size_t BYTES = sizeof(half_t) * 3 * STAGE > sizeof(float) * TILE * OPITCH ? sizeof(half_t) * 3 * STAGE : sizeof(float) * TILE * OPITCH;
   half_t* lds;
-  f32x16_t acc[W][W];
-  uint4 q[4][CH];
+  f32x16_t acc[FR][FC];
+  uint4 q[2][4][CH];
+  struct Frags {
+    half8_t ah[FR], al[FR], bh[FC], bl[FC];
+  };
 
-  __device__ __forceinline__ void load(const half_t* a, size_t a_plane, int lda, const half_t* b, size_t b_plane, int ldb, int k0, int tid) {
+  static __device__ __forceinline__ int row0(int tid) { return (tid >> 7) * WR; }
+  static __device__ __forceinline__ int col0(int tid) { return ((tid >> 6) & 1) * WC; }
+  template <int S> __device__ __forceinline__ void load(const half_t* a, size_t a_plane, int lda, const half_t* b, size_t b_plane, int ldb, int k0, int tid) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int idx = tid + c * 256, r = idx >> 2, col = k0 + (idx & 3) * 8;
+      const int idx = tid + c * NT, r = idx / (BK / 8), col = k0 + idx % (BK / 8) * 8;
       const half_t* pa = COLS ? a + (size_t)(k0 + idx / (TILE / 8)) * lda + idx % (TILE / 8) * 8 : a + (size_t)r * lda + col;
-      q[0][c] = *reinterpret_cast<const uint4*>(pa);
-      q[1][c] = *reinterpret_cast<const uint4*>(pa + a_plane);
-      q[2][c] = *reinterpret_cast<const uint4*>(b + (size_t)r * ldb + col);
-      q[3][c] = *reinterpret_cast<const uint4*>(b + b_plane + (size_t)r * ldb + col);
+      q[S][0][c] = *reinterpret_cast<const uint4*>(pa);
+      q[S][1][c] = *reinterpret_cast<const uint4*>(pa + a_plane);
+      q[S][2][c] = *reinterpret_cast<const uint4*>(b + (size_t)r * ldb + col);
+      q[S][3][c] = *reinterpret_cast<const uint4*>(b + b_plane + (size_t)r * ldb + col);
     }
   }
-  __device__ __forceinline__ void store(int stage, int tid) {
+  template <int S> __device__ __forceinline__ void store(int stage, int tid) {
     half_t* const s = lds + stage * STAGE;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int idx = tid + c * 256, rows = (idx >> 2) * PITCH + (idx & 3) * 8;
+      const int idx = tid + c * NT, rows = idx / (BK / 8) * PITCH + idx % (BK / 8) * 8;
       const int at = COLS ? idx / (TILE / 8) * CPITCH + idx % (TILE / 8) * 8 : rows;
-      *reinterpret_cast<uint4*>(s + at) = q[0][c];
-      *reinterpret_cast<uint4*>(s + AELEMS + at) = q[1][c];
-      *reinterpret_cast<uint4*>(s + 2 * AELEMS + rows) = q[2][c];
-      *reinterpret_cast<uint4*>(s + 2 * AELEMS + BELEMS + rows) = q[3][c];
+      *reinterpret_cast<uint4*>(s + at) = q[S][0][c];
+      *reinterpret_cast<uint4*>(s + AELEMS + at) = q[S][1][c];
+      *reinterpret_cast<uint4*>(s + 2 * AELEMS + rows) = q[S][2][c];
+      *reinterpret_cast<uint4*>(s + 2 * AELEMS + BELEMS + rows) = q[S][3][c];
     }
   }
   static __device__ __forceinline__ half8_t row_frag(const half_t* t, int row, int k, int lane) {
@@ -210,60 +220,104 @@ template <int TILE, bool COLS> struct Product {
     const v4s_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*)(p + 4 * CPITCH));
     return __builtin_bit_cast(half8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
+  // order of the instructions since the last call: LDS reads, and the four instructions of class OTHER (LDS writes 0x200, global loads 0x020), between the MFMAs
+  template <int OTHER> static __device__ __forceinline__ void interleave() {
+    constexpr int MFMAS = 3 * FR * FC, READS = (COLS ? 4 : 2) * FR + 2 * FC, OTHERS = 4 * CH;
+    static_for<0, MFMAS>([](auto i) {
+      constexpr int r = (i + 1) * READS / MFMAS - i * READS / MFMAS, o = (i + 1) * OTHERS / MFMAS - i * OTHERS / MFMAS;
+      if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if constexpr (o > 0) __builtin_amdgcn_sched_group_barrier(OTHER, o, 0);
+    });
+    __builtin_amdgcn_sched_barrier(0);
+  }
   __device__ __forceinline__ void run(const half_t* a, size_t a_plane, int lda, const half_t* b, size_t b_plane, int ldb, int K, int tid) {
-    const int lane = tid & 63, wr = (tid >> 7) * (TILE / 2), wc = ((tid >> 6) & 1) * (TILE / 2);
-    f32x16_t cross[W][W];
+    const int lane = tid & 63, wr = row0(tid), wc = col0(tid);
+    f32x16_t cross[FR][FC];
 #pragma unroll
-    for (int i = 0; i < W; ++i)
+    for (int i = 0; i < FR; ++i)
 #pragma unroll
-      for (int j = 0; j < W; ++j) acc[i][j] = cross[i][j] = acc_zero();
-    load(a, a_plane, lda, b, b_plane, ldb, 0, tid);
-    store(0, tid);
-    if (K > BK) load(a, a_plane, lda, b, b_plane, ldb, BK, tid);
-    for (int k0 = 0, s = 0; k0 < K; k0 += BK, s ^= 1) {
-      wg_barrier_lds();
-      if (k0 + BK < K) store(s ^ 1, tid);
-      if (k0 + 2 * BK < K) load(a, a_plane, lda, b, b_plane, ldb, k0 + 2 * BK, tid);
-      const half_t* const st = lds + s * STAGE;
+      for (int j = 0; j < FC; ++j) acc[i][j] = cross[i][j] = acc_zero();
+    const int steps = K / BK;
+    auto request = [&](auto set, int t) { this->template load<decltype(set)::value>(a, a_plane, lda, b, b_plane, ldb, t * BK, tid); };
+    auto read = [&](int stage, int k) {
+      const half_t* const st = lds + stage * STAGE;
+      Frags f;
 #pragma unroll
-      for (int k = 0; k < BK; k += 16) {
-        half8_t ah[W], al[W], bh[W], bl[W];
+      for (int i = 0; i < FR; ++i) {
+        f.ah[i] = COLS ? col_frag(st, wr + 32 * i, k, lane) : row_frag(st, wr + 32 * i, k, lane);
+        f.al[i] = COLS ? col_frag(st + AELEMS, wr + 32 * i, k, lane) : row_frag(st + AELEMS, wr + 32 * i, k, lane);
+      }
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          ah[i] = COLS ? col_frag(st, wr + 32 * i, k, lane) : row_frag(st, wr + 32 * i, k, lane);
-          al[i] = COLS ? col_frag(st + AELEMS, wr + 32 * i, k, lane) : row_frag(st + AELEMS, wr + 32 * i, k, lane);
-          bh[i] = row_frag(st + 2 * AELEMS, wc + 32 * i, k, lane);
-          bl[i] = row_frag(st + 2 * AELEMS + BELEMS, wc + 32 * i, k, lane);
+      for (int j = 0; j < FC; ++j) {
+        f.bh[j] = row_frag(st + 2 * AELEMS, wc + 32 * j, k, lane);
+        f.bl[j] = row_frag(st + 2 * AELEMS + BELEMS, wc + 32 * j, k, lane);
+      }
+      return f;
+    };
+    auto multiply = [&](const Frags& f) {
+#pragma unroll
+      for (int i = 0; i < FR; ++i)
+#pragma unroll
+        for (int j = 0; j < FC; ++j) {
+          cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], cross[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bh[j], acc[i][j], 0, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < W; ++i)
+      for (int i = 0; i < FR; ++i)
 #pragma unroll
-          for (int j = 0; j < W; ++j) {
-            cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], cross[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
-          }
+        for (int j = 0; j < FC; ++j) cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bl[j], cross[i][j], 0, 0, 0);
+    };
+    typedef std::integral_constant<int, 0> S0;
+    typedef std::integral_constant<int, 1> S1;
+    // No branch inside the loop (steps is even: sides are multiples of 64): behind one the compiler's counts of outstanding loads are
+    // lower bounds and every wait becomes a wait for the newest load.  Steps past the end load the last one again, into stages nobody reads.
+    request(S0{}, 0);
+    request(S1{}, 1);
+    this->template store<0>(0, tid);
+    request(S0{}, min(2, steps - 1));
+    this->template store<1>(1, tid);
+    request(S1{}, min(3, steps - 1));
+    wg_barrier_lds();
+    Frags f = read(0, 0);
+    int s0 = 0, s1 = 1, s2 = 2;
+    for (int t0 = 0; t0 < steps; t0 += 2)
+      static_for<0, 2>([&](auto d) {
+        // A wave that issues its LDS instructions in a row waits for the LDS queue with its MFMAs behind it, as the other waves do at the same
+        // time, and the LDS is idle while they all multiply: one LDS instruction between two MFMAs keeps both busy.
+        Frags next;
+        this->template store<decltype(d)::value>(s2, tid);
+        next = read(s0, 16);
+        multiply(f);
+        interleave<0x200>();
+        f = next;
+        request(d, min(t0 + d + 4, steps - 1));
+        next = read(s1, 0);
+        multiply(f);
+        interleave<0x020>();
+        f = next;
+        wg_barrier_lds();
+        const int s = s0;
+        s0 = s1;
+        s1 = s2;
+        s2 = s;
+      });
 #pragma unroll
-        for (int i = 0; i < W; ++i)
+    for (int i = 0; i < FR; ++i)
 #pragma unroll
-          for (int j = 0; j < W; ++j) cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], cross[i][j], 0, 0, 0);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-#pragma unroll
-      for (int j = 0; j < W; ++j)
+      for (int j = 0; j < FC; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] += cross[i][j][r];
   }
   // the tile as floats in LDS, transposed: out[c][r]
   __device__ __forceinline__ float* spill(int tid) {
-    const int lane = tid & 63, wr = (tid >> 7) * (TILE / 2), wc = ((tid >> 6) & 1) * (TILE / 2);
+    const int lane = tid & 63, wr = row0(tid), wc = col0(tid);
     float* const out = reinterpret_cast<float*>(lds);
     __syncthreads();  // the operands are read
 #pragma unroll
-    for (int i = 0; i < W; ++i)
+    for (int i = 0; i < FR; ++i)
 #pragma unroll
-      for (int j = 0; j < W; ++j)
+      for (int j = 0; j < FC; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           *reinterpret_cast<float4*>(out + (wc + 32 * j + (lane & 31)) * OPITCH + wr + 32 * i + 8 * e + 4 * (lane >> 5)) =
@@ -282,21 +336,53 @@ __device__ __forceinline__ void split8(const float* v, half8_t& hi, half8_t& lo)
     lo[e] = l;
   }
 }
-// Four consecutive tiles (which share an operand panel) on one XCD: block b runs on XCD b % 8.  Groups of 32 blocks; the rest in order.
+// Tiles are numbered in squares of 4 x 4, and 16 consecutive ones run on one XCD (block b runs on XCD b % 8): they read 8 operand panels instead of
+// 32 into that XCD's L2, which the whole operand (4096 x 2048: 34 MB) does not fit.  In row order the products ran at the rate of the memory-side cache.
 __device__ __forceinline__ int near_tiles(int b, int n) {
-  const int whole = n & ~31;
-  return b < whole ? (b & ~31) + (b & 7) * 4 + ((b & 31) >> 3) : b;
+  const int whole = n & ~127;
+  if (b < whole) return (b & ~127) + (b & 7) * 16 + ((b & 127) >> 3);
+  const int r = b - whole, some = (n - whole) & ~31;
+  return whole + (r < some ? (r & ~31) + (r & 7) * 4 + ((r & 31) >> 3) : r);
+}
+// tile `at` of an nr x nc grid in that order: squares column by column, each column by column
+__device__ __forceinline__ void square_tile(int at, int nr, int nc, int& i, int& j) {
+  const int strip = at / (4 * nr), in = at - strip * 4 * nr, w = min(4, nc - strip * 4);  // a strip is 4 (the last one w) columns
+  const int band = in / (4 * w), r = in - band * 4 * w, h = min(4, nr - band * 4);
+  i = band * 4 + r % h;
+  j = strip * 4 + r / h;
+}
+// tile `at` of the lower triangle (j <= i) of an n x n grid: squares row by row, those on the diagonal being triangles themselves
+__device__ __forceinline__ void triangle_tile(int at, int n, int& i, int& j) {
+  int band = 0;
+  for (;; ++band) {  // band of 4 (the last one h) rows: 4 h tiles a square and a triangle
+    const int h = min(4, n - band * 4), size = 4 * h * band + h * (h + 1) / 2;
+    if (at < size) {
+      if (at < 4 * h * band) {
+        const int r = at % (4 * h);
+        i = band * 4 + r % h;
+        j = at / (4 * h) * 4 + r / h;
+      } else {
+        at -= 4 * h * band;
+        int ti = 0;
+        while (at > ti) at -= ++ti;
+        i = band * 4 + ti;
+        j = band * 4 + at;
+      }
+      return;
+    }
+    at -= size;
+  }
 }
 
 // G = x x^T (POLY false) or P = b G + c G G (true): tiles (i, j <= i), written to both halves
-template <int TILE, bool POLY> __global__ __launch_bounds__(256, 2) void ns_sym_kernel(Mats t, int which, float cb, float cc) {
-  typedef Product<TILE, false> Prod;
+template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVES, 2) void ns_sym_kernel(Mats t, int which, float cb, float cc) {
+  typedef Product<TILE, WAVES, false> Prod;
   __shared__ __attribute__((aligned(16))) char smem[Prod::BYTES];
   const int block = near_tiles(blockIdx.x, t.first[t.count]), k = find(t, block), tid = threadIdx.x;
   const Mat& a = t.mat[k];
-  int at = block - t.first[k], ti = 0;
-  while (at > ti) at -= ++ti;  // (ti, at) of the lower triangle
-  const int i0 = ti * TILE, j0 = at * TILE;
+  int ti, tj;
+  triangle_tile(block - t.first[k], a.mp / TILE, ti, tj);
+  const int i0 = ti * TILE, j0 = tj * TILE;
   const size_t plane = (size_t)a.mp * a.mp;
   half_t* const g = g_of(a);
   Prod p;
@@ -305,7 +391,7 @@ template <int TILE, bool POLY> __global__ __launch_bounds__(256, 2) void ns_sym_
   else p.run(x_of(a, which) + (size_t)i0 * a.np, plane_x(a), a.np, x_of(a, which) + (size_t)j0 * a.np, plane_x(a), a.np, a.np, tid);
   half_t* const out = POLY ? p_of(a) : g;
   float* const v = p.spill(tid);  // v[j][i]
-  for (int idx = tid; idx < TILE * TILE / 8; idx += 256) {
+  for (int idx = tid; idx < TILE * TILE / 8; idx += Prod::NT) {
     const int j = idx / (TILE / 8), i = idx % (TILE / 8) * 8;
     const size_t o = (size_t)(j0 + j) * a.mp + i0 + i;
     float w[8];
@@ -327,7 +413,7 @@ template <int TILE, bool POLY> __global__ __launch_bounds__(256, 2) void ns_sym_
   }
   if (i0 == j0) return;
   __syncthreads();
-  for (int idx = tid; idx < TILE * TILE / 8; idx += 256) {  // the mirror image
+  for (int idx = tid; idx < TILE * TILE / 8; idx += Prod::NT) {  // the mirror image
     const int i = idx % TILE, j = idx / TILE * 8;
     float w[8];
 #pragma unroll
@@ -341,12 +427,14 @@ template <int TILE, bool POLY> __global__ __launch_bounds__(256, 2) void ns_sym_
 }
 
 // x <- a x + P x; the last one writes the result instead
-template <int TILE, typename T, int LAST> __global__ __launch_bounds__(256, 2) void ns_apply_kernel(Mats t, int which, float ca, const float* __restrict__ hp) {
-  typedef Product<TILE, true> Prod;
+template <int TILE, int WAVES, typename T, int LAST> __global__ __launch_bounds__(64 * WAVES, 2) void ns_apply_kernel(Mats t, int which, float ca, const float* __restrict__ hp) {
+  typedef Product<TILE, WAVES, true> Prod;
   __shared__ __attribute__((aligned(16))) char smem[Prod::BYTES];
-  const int block = near_tiles(blockIdx.x, t.first[t.count]), k = find(t, block), tid = threadIdx.x, at = block - t.first[k];
+  const int block = near_tiles(blockIdx.x, t.first[t.count]), k = find(t, block), tid = threadIdx.x;
   const Mat& a = t.mat[k];
-  const int tm = a.mp / TILE, i0 = at % tm * TILE, j0 = at / tm * TILE;
+  int ti, tj;
+  square_tile(block - t.first[k], a.mp / TILE, a.np / TILE, ti, tj);
+  const int i0 = ti * TILE, j0 = tj * TILE;
   const half_t* const x = x_of(a, which);
   const size_t plane = plane_x(a);
   Prod p;
@@ -354,7 +442,7 @@ template <int TILE, typename T, int LAST> __global__ __launch_bounds__(256, 2) v
   p.run(x + j0, plane, a.np, p_of(a) + (size_t)i0 * a.mp, (size_t)a.mp * a.mp, a.mp, a.mp, tid);
   float* const v = p.spill(tid);  // v[i][j]
   half_t* const next = x_of(a, which ^ 1);
-  for (int idx = tid; idx < TILE * TILE / 8; idx += 256) {
+  for (int idx = tid; idx < TILE * TILE / 8; idx += Prod::NT) {
     const int i = idx / (TILE / 8), j = idx % (TILE / 8) * 8;
     const size_t o = (size_t)(i0 + i) * a.np + j0 + j;
     const half8_t h = *reinterpret_cast<const half8_t*>(x + o), l = *reinterpret_cast<const half8_t*>(x + plane + o);
@@ -375,13 +463,26 @@ template <int TILE, typename T, int LAST> __global__ __launch_bounds__(256, 2) v
   __syncthreads();
   const bool flip = a.rows > a.cols;
   const float lr = LAST == 2 ? hp[2 * a.group] : 0.f, keep = LAST == 2 ? 1.f - lr * hp[2 * a.group + 1] : 0.f, step = lr * a.gain;
-  for (int idx = tid; idx < TILE * TILE; idx += 256) {
-    const int slow = idx / TILE, fast = idx % TILE, i = flip ? fast : slow, j = flip ? slow : fast;
-    if (i0 + i >= a.m || j0 + j >= a.n) continue;
-    const size_t o = flip ? (size_t)(j0 + j) * a.cols + i0 + i : (size_t)(i0 + i) * a.cols + j0 + j;
-    const float y = v[i * Prod::OPITCH + j];
-    if (LAST == 1) reinterpret_cast<T*>(a.dst)[o] = from_f<T>(y);
-    else a.par[o] = a.par[o] * keep - step * y;
+  constexpr int IN_FLIGHT = 8;
+  for (int base = tid; base < TILE * TILE; base += Prod::NT * IN_FLIGHT) {
+    float old[IN_FLIGHT];
+    size_t o[IN_FLIGHT];
+    bool in[IN_FLIGHT];
+#pragma unroll
+    for (int q = 0; q < IN_FLIGHT; ++q) {
+      const int idx = base + q * Prod::NT, slow = idx / TILE, fast = idx % TILE, i = flip ? fast : slow, j = flip ? slow : fast;
+      in[q] = i0 + i < a.m && j0 + j < a.n;
+      o[q] = in[q] ? (flip ? (size_t)(j0 + j) * a.cols + i0 + i : (size_t)(i0 + i) * a.cols + j0 + j) : 0;
+      if (LAST == 2) old[q] = a.par[o[q]];
+    }
+#pragma unroll
+    for (int q = 0; q < IN_FLIGHT; ++q) {
+      const int idx = base + q * Prod::NT, slow = idx / TILE, fast = idx % TILE;
+      const float y = flip ? v[fast * Prod::OPITCH + slow] : v[slow * Prod::OPITCH + fast];
+      if (!in[q]) continue;
+      if (LAST == 1) reinterpret_cast<T*>(a.dst)[o[q]] = from_f<T>(y);
+      else a.par[o[q]] = old[q] * keep - step * y;
+    }
   }
 }
 
@@ -399,42 +500,43 @@ template <typename F> int prefix(Mats& t, F&& groups) {
   for (int i = 0; i < t.count; ++i) t.first[i + 1] = t.first[i] + groups(t.mat[i]);
   return t.first[t.count];
 }
-// 128-wide tiles where the list has enough of them to fill the card (and every side takes them), else 64-wide ones
-template <typename F> bool wide_tiles(const Mats& t, int least, F&& tiles) {
+// 128-wide tiles where the list has enough of them for the card (and every side takes them), else 64-wide ones
+template <typename F> bool wide_tiles(const Mats& t, F&& tiles) {
   long long n = 0;
   for (int i = 0; i < t.count; ++i) {
     if (t.mat[i].mp % 128 || t.mat[i].np % 128) return false;
     n += tiles(t.mat[i]);
   }
-  return n >= least;
+  return n >= W8;
 }
 template <int TILE> int sym_tiles(const Mat& q) { return q.mp / TILE * (q.mp / TILE + 1) / 2; }
 template <int TILE> int all_tiles(const Mat& q) { return q.mp / TILE * (q.np / TILE); }
+
+template <int TILE, int WAVES> void run_sym(Mats t, int which, float b, float c, hipStream_t st) {
+  const dim3 grid(prefix(t, sym_tiles<TILE>)), wg(64 * WAVES);
+  ns_sym_kernel<TILE, WAVES, false><<<grid, wg, 0, st>>>(t, which, b, c);
+  ns_sym_kernel<TILE, WAVES, true><<<grid, wg, 0, st>>>(t, which, b, c);
+}
+template <int TILE, int WAVES, typename T, int LAST> void run_apply(Mats t, int which, float a, const float* hp, hipStream_t st) {
+  const dim3 grid(prefix(t, all_tiles<TILE>)), wg(64 * WAVES);
+  ns_apply_kernel<TILE, WAVES, T, LAST><<<grid, wg, 0, st>>>(t, which, a, hp);
+}
 template <typename T, bool MOM> int run_list(Mats& t, int steps, float a, float b, float c, float eps, float mu, int nesterov, const float* hp, hipStream_t st) {
-  const dim3 wg(256);
   int n = prefix(t, [](const Mat& q) { return (int)(((long long)q.m * q.n + kNormItems - 1) / kNormItems); });
-  ns_norm_kernel<T, MOM><<<dim3(n), wg, 0, st>>>(t, mu, nesterov);
+  ns_norm_kernel<T, MOM><<<dim3(n), dim3(256), 0, st>>>(t, mu, nesterov);
   n = prefix(t, all_tiles<64>);
-  ns_scale_kernel<T, MOM><<<dim3(n), wg, 0, st>>>(t, mu, nesterov, eps);
-  const bool ws = wide_tiles(t, kWideTiles, sym_tiles<128>), wa = wide_tiles(t, kWideTiles, all_tiles<128>);
-  Mats sym = t;
-  const dim3 gs(ws ? prefix(sym, sym_tiles<128>) : prefix(sym, sym_tiles<64>)), ga(wa ? prefix(t, all_tiles<128>) : prefix(t, all_tiles<64>));
+  ns_scale_kernel<T, MOM><<<dim3(n), dim3(256), 0, st>>>(t, mu, nesterov, eps);
+  const bool ws = wide_tiles(t, sym_tiles<128>), wa = wide_tiles(t, all_tiles<128>);
+  constexpr int LAST = MOM ? 2 : 1;
   for (int s = 0; s < steps; ++s) {
-    const int w = s & 1;
-    if (ws) {
-      ns_sym_kernel<128, false><<<gs, wg, 0, st>>>(sym, w, b, c);
-      ns_sym_kernel<128, true><<<gs, wg, 0, st>>>(sym, w, b, c);
-    } else {
-      ns_sym_kernel<64, false><<<gs, wg, 0, st>>>(sym, w, b, c);
-      ns_sym_kernel<64, true><<<gs, wg, 0, st>>>(sym, w, b, c);
-    }
-    constexpr int LAST = MOM ? 2 : 1;
+    if (ws) run_sym<128, 8>(t, s & 1, b, c, st);
+    else run_sym<64, 4>(t, s & 1, b, c, st);
     if (s + 1 < steps) {
-      if (wa) ns_apply_kernel<128, T, 0><<<ga, wg, 0, st>>>(t, w, a, hp);
-      else ns_apply_kernel<64, T, 0><<<ga, wg, 0, st>>>(t, w, a, hp);
+      if (wa) run_apply<128, 8, T, 0>(t, s & 1, a, hp, st);
+      else run_apply<64, 4, T, 0>(t, s & 1, a, hp, st);
     } else {
-      if (wa) ns_apply_kernel<128, T, LAST><<<ga, wg, 0, st>>>(t, w, a, hp);
-      else ns_apply_kernel<64, T, LAST><<<ga, wg, 0, st>>>(t, w, a, hp);
+      if (wa) run_apply<128, 8, T, LAST>(t, s & 1, a, hp, st);
+      else run_apply<64, 4, T, LAST>(t, s & 1, a, hp, st);
     }
   }
   CVH_CHECK_LAUNCH();
