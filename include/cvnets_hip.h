@@ -438,12 +438,13 @@ int cvh_embed_lookup_bwd(int dtype, const long long* tok, const void* dout, floa
 /* ---- attention over packed sequences ------------------------------------------------------------- */
 /* Softmax attention of sequences that lie one behind the other in the rows of q / k / v: sequence b has the rows cu[b] .. cu[b + 1] - 1.
  * q [rows][heads_q][d], k / v [rows][heads_kv][d], heads_q % heads_kv == 0 (query head h reads key head h / (heads_q / heads_kv)); *_row and
- * *_head are strides in elements; the d elements of a head are contiguous, d % 8 == 0, d <= 128; 16-byte aligned bases and strides.  Rows at or
- * behind cu[seqs] are read by nothing; their results are zeros.  lse [heads_q][rows] (log2 of the softmax sums, with the maxima) is written by the
+ * *_head are strides in elements; the d elements of a head are contiguous, d % 8 == 0, d <= 128; 16-byte aligned bases and strides, *_row <= 2^21.  Rows at or
+ * behind cu[seqs] are read by nothing; their results are zeros.  lse [heads_q][rows] (log2 of the softmax sums, with the maxima; NULL: not wanted) is written by the
  * forward and read by the backward, delta [heads_q][rows] is the backward's scratch.  plan: cvh_packed_plan of the same seqs, rows and block. */
 typedef struct cvh_packed_attn {
   const void *q, *k, *v;
-  void* out; /* forward: written; backward: the forward's result */
+  void* out;    /* forward: written; backward: the forward's result */
+  void* out_lo; /* bf16, nullable: what the rounding of out left over, in out's layout; the backward's row sums dout . out are formed from both */
   const void* dout;
   void *dq, *dk, *dv;
   float *lse, *delta;

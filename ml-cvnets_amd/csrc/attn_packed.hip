@@ -32,25 +32,38 @@ template <> struct Chunk<bf16_t> {
 template <> struct Chunk<float> {
   static constexpr int N = 4;
 };
-__device__ __forceinline__ uint4 keep16(uint4 v, bool ok) {
-  const uint32_t m = ok ? 0xffffffffu : 0u;
-  return make_uint4(v.x & m, v.y & m, v.z & m, v.w & m);
+
+// Rows of one sequence through a buffer descriptor: what lies at or behind `bytes` reads as zero without an access.  A masked probability is 0, and
+// 0 times whatever another sequence holds there has to be 0; and no load of the loops needs a bounds test, a mask or a branch - behind a
+// branch the compiler's counts of outstanding loads are lower bounds and it waits for the newest load instead of the oldest.
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+constexpr int kBeyond = 0x7ffffff0;  // an offset that no descriptor covers
+__device__ __forceinline__ rsrc_t rows_of(const void* base, long long bytes) {
+  const long long most = kBeyond;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)(bytes < 0 ? 0 : bytes < most ? bytes : most), 0x00020000);
+}
+template <typename T> __device__ __forceinline__ rsrc_t tile_rows(const T* seq_base, long long row_stride, int row0, int len, int d) {
+  const long long rows = len - row0;
+  return rows_of(seq_base + (rows > 0 ? (long long)row0 * row_stride : 0ll), rows > 0 ? ((rows - 1) * row_stride + d) * (long long)sizeof(T) : 0ll);
+}
+__device__ __forceinline__ uint4 buf16(rsrc_t r, int offset) {
+  typedef unsigned u4 __attribute__((ext_vector_type(4)));
+  const u4 v = __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0);
+  return make_uint4(v.x, v.y, v.z, v.w);
 }
 
-// one MFMA operand (32 rows x 16 columns) straight from global memory: lane l holds columns k0 + 8 (l >> 5) .. + 7 of row (l & 31)
-__device__ __forceinline__ Frag<bf16_t> gfrag(const bf16_t* row, int c0, int d, bool ok) {
-  const bool in = ok && c0 < d;
-  const uint4 v = *reinterpret_cast<const uint4*>(row + (in ? c0 : 0));
+// one MFMA operand (32 rows x 16 columns) straight from global memory: lane l holds columns k0 + 8 (l >> 5) .. + 7 of row (l & 31); `offset` is the
+// byte offset of the lane's row, kBeyond for none
+__device__ __forceinline__ Frag<bf16_t> gfrag(rsrc_t r, int offset, int c0, int d, const bf16_t*) {
   Frag<bf16_t> f;
-  f.v = __builtin_bit_cast(bf16x8_t, keep16(v, in));
+  f.v = __builtin_bit_cast(bf16x8_t, buf16(r, c0 < d ? offset + c0 * 2 : kBeyond));
   return f;
 }
-__device__ __forceinline__ Frag<float> gfrag(const float* row, int c0, int d, bool ok) {
-  const bool in = ok && c0 < d;
-  const float4 a = *reinterpret_cast<const float4*>(row + (in ? c0 : 0)), b = *reinterpret_cast<const float4*>(row + (in ? c0 + 4 : 0));
+__device__ __forceinline__ Frag<float> gfrag(rsrc_t r, int offset, int c0, int d, const float*) {
   Frag<float> f;
-  f.v[0] = in ? a.x : 0.f; f.v[1] = in ? a.y : 0.f; f.v[2] = in ? a.z : 0.f; f.v[3] = in ? a.w : 0.f;
-  f.v[4] = in ? b.x : 0.f; f.v[5] = in ? b.y : 0.f; f.v[6] = in ? b.z : 0.f; f.v[7] = in ? b.w : 0.f;
+  const uint4 a = buf16(r, c0 < d ? offset + c0 * 4 : kBeyond), b = buf16(r, c0 < d ? offset + c0 * 4 + 16 : kBeyond);
+  f.v[0] = __uint_as_float(a.x); f.v[1] = __uint_as_float(a.y); f.v[2] = __uint_as_float(a.z); f.v[3] = __uint_as_float(a.w);
+  f.v[4] = __uint_as_float(b.x); f.v[5] = __uint_as_float(b.y); f.v[6] = __uint_as_float(b.z); f.v[7] = __uint_as_float(b.w);
   return f;
 }
 __device__ __forceinline__ float frag_dot(const Frag<bf16_t>& a, const Frag<bf16_t>& b) {
@@ -66,28 +79,29 @@ __device__ __forceinline__ float frag_dot(const Frag<float>& a, const Frag<float
   return s;
 }
 
-// A tile of NROWS consecutive rows, loaded by NT threads into registers (load: only issues the reads) and written to LDS (store).  Rows at or
-// behind `live` and columns at or behind `d` become zeros: a masked probability is 0, and 0 times whatever another sequence holds there has to be 0.
+// A tile of NROWS consecutive rows of a sequence, loaded by NT threads into registers (load: only issues the reads) and written to LDS (store);
+// rows behind the sequence and columns at or behind d are zeros
 template <typename T, int CP, int NROWS, int NT> struct RowTile {
   static constexpr int VN = Chunk<T>::N, CH = CP / VN, IT = (NROWS * CH + NT - 1) / NT;
   static constexpr bool EXACT = (NROWS * CH) % NT == 0;
   uint4 q[IT];
-  unsigned ok;
-  __device__ __forceinline__ void load(const T* __restrict__ base, long long row_stride, int live, int d, int tid) {
-    ok = 0;
+  int offset[IT];  // bytes
+  __device__ __forceinline__ void place(long long row_stride, int d, int tid) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int idx = tid + i * NT, r = idx / CH, c = (idx % CH) * VN;
-      const bool in = (EXACT || idx < NROWS * CH) && r < live && c < d;
-      ok |= (in ? 1u : 0u) << i;
-      q[i] = *reinterpret_cast<const uint4*>(base + (in ? (long long)r * row_stride + c : 0ll));
+      offset[i] = (EXACT || idx < NROWS * CH) && c < d ? (r * (int)row_stride + c) * (int)sizeof(T) : kBeyond;
     }
+  }
+  __device__ __forceinline__ void load(rsrc_t rows) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) q[i] = buf16(rows, offset[i]);
   }
   __device__ __forceinline__ void store(T* lds, int pitch, int tid) const {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int idx = tid + i * NT, r = idx / CH, c = (idx % CH) * VN;
-      if (EXACT || idx < NROWS * CH) *reinterpret_cast<uint4*>(lds + r * pitch + c) = keep16(q[i], (ok >> i) & 1u);
+      if (EXACT || idx < NROWS * CH) *reinterpret_cast<uint4*>(lds + r * pitch + c) = q[i];
     }
   }
 };
@@ -128,11 +142,54 @@ template <> __device__ __forceinline__ Frag<float> acc_frag<float>(const f32x16_
   return f;
 }
 
-// 4 consecutive columns of one row
-template <typename T> __device__ __forceinline__ void store4(T* p, const float* f) {
-  V4<T> v;
-  v4_pack(f, v);
-  v4_store<T>(p, v);
+// the halves of a wave hold 4 + 4 of 8 consecutive columns: lane l and l + 32 exchange, so that each has 8 of one 16-column group
+__device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  const u2 r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r.x;
+  b = r.y;
+}
+// f(x of the lane, x of the lane in the other half)
+__device__ __forceinline__ float both_halves_max(float x) {
+  uint32_t a = __float_as_uint(x), b = a;
+  swap_halves(a, b);
+  return fmaxf(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ float both_halves_sum(float x) {
+  uint32_t a = __float_as_uint(x), b = a;
+  swap_halves(a, b);
+  return __uint_as_float(a) + __uint_as_float(b);
+}
+// rows of a transposed accumulator: lane = row, registers = 32 columns from c0; `lo` (nullable): what the rounding to T left over, rounded itself
+__device__ __forceinline__ void store_rows(bf16_t* row, bf16_t* lo, const f32x16_t& v, float scale, int c0, int d, int lane, bool ok) {
+#pragma unroll
+  for (int pair = 0; pair < 2; ++pair) {
+    uint32_t w[4], x[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float f0 = v[8 * pair + 4 * i + 2 * e] * scale, f1 = v[8 * pair + 4 * i + 2 * e + 1] * scale;
+        w[2 * i + e] = f2bf_pk(f0, f1);
+        x[2 * i + e] = lo != nullptr ? f2bf_pk(f0 - __uint_as_float(w[2 * i + e] << 16), f1 - __uint_as_float(w[2 * i + e] & 0xffff0000u)) : 0u;
+      }
+    swap_halves(w[0], w[2]);
+    swap_halves(w[1], w[3]);
+    const int c = c0 + 16 * pair + 8 * (lane >> 5);
+    if (ok && c < d) *reinterpret_cast<uint4*>(row + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (lo != nullptr) {
+      swap_halves(x[0], x[2]);
+      swap_halves(x[1], x[3]);
+      if (ok && c < d) *reinterpret_cast<uint4*>(lo + c) = make_uint4(x[0], x[1], x[2], x[3]);
+    }
+  }
+}
+__device__ __forceinline__ void store_rows(float* row, float*, const f32x16_t& v, float scale, int c0, int d, int lane, bool ok) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = c0 + 8 * i + 4 * (lane >> 5);
+    if (ok && c < d) *reinterpret_cast<float4*>(row + c) = make_float4(v[4 * i] * scale, v[4 * i + 1] * scale, v[4 * i + 2] * scale, v[4 * i + 3] * scale);
+  }
 }
 
 struct Item {
@@ -145,10 +202,10 @@ __device__ __forceinline__ Item work_item(const PA& p, int heads) {
   Item w;
   w.head = heads % 8 == 0 ? (slot & 7) * (heads >> 3) + (slot >> 3) : slot;
   const int* list = p.plan + ((p.seqs + 2) & ~1);
-  w.seq = list[2 * tile];
-  w.block = list[2 * tile + 1];
-  w.start = w.seq >= 0 ? p.plan[w.seq] : p.plan[p.seqs];
-  w.len = (w.seq >= 0 ? p.plan[w.seq + 1] : p.rows) - w.start;
+  w.seq = __builtin_amdgcn_readfirstlane(list[2 * tile]);
+  w.block = __builtin_amdgcn_readfirstlane(list[2 * tile + 1]);
+  w.start = __builtin_amdgcn_readfirstlane(w.seq >= 0 ? p.plan[w.seq] : p.plan[p.seqs]);
+  w.len = __builtin_amdgcn_readfirstlane(w.seq >= 0 ? p.plan[w.seq + 1] : p.rows) - w.start;
   return w;
 }
 // rows behind the last sequence: zeros
@@ -167,7 +224,7 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* const Kl = reinterpret_cast<T*>(smem);  // [2][KB][PT]
   T* const Vl = Kl + 2 * KB * PT;            // [2][KB][PT]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Item w = work_item(p, p.heads_q);
   if (w.seq < -1) return;
   T* const out = reinterpret_cast<T*>(p.out) + w.head * p.o_head;
@@ -179,26 +236,30 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
   const int q0 = first + wave * 32, my_q = q0 + (lane & 31);
   const bool q_ok = my_q < w.len;
   const int kv_head = w.head / (p.heads_q / p.heads_kv);
+  const T* const qb = reinterpret_cast<const T*>(p.q) + (long long)w.start * p.q_row + w.head * p.q_head;
   const T* const kb = reinterpret_cast<const T*>(p.k) + (long long)w.start * p.k_row + kv_head * p.k_head;
   const T* const vb = reinterpret_cast<const T*>(p.v) + (long long)w.start * p.v_row + kv_head * p.v_head;
   const int keys = p.causal ? min(w.len, first + 32 * NW) : w.len;
   const int tiles = (keys + KB - 1) / KB;
 
   RowTile<T, CP, KB, NT> kt, vt;
-  kt.load(kb, p.k_row, w.len, p.d, tid);
-  vt.load(vb, p.v_row, w.len, p.d, tid);
+  kt.place(p.k_row, p.d, tid);
+  vt.place(p.v_row, p.d, tid);
+  auto request = [&](int t) {
+    kt.load(tile_rows(kb, p.k_row, t * KB, w.len, p.d));
+    vt.load(tile_rows(vb, p.v_row, t * KB, w.len, p.d));
+  };
+  request(0);
   Frag<T> qf[NK];
   {
-    const T* qrow = reinterpret_cast<const T*>(p.q) + (long long)(w.start + (q_ok ? my_q : 0)) * p.q_row + w.head * p.q_head;
+    const rsrc_t r = tile_rows(qb, p.q_row, q0, w.len, p.d);
+    const int offset = (lane & 31) * (int)p.q_row * (int)sizeof(T);
 #pragma unroll
-    for (int k = 0; k < NK; ++k) qf[k] = gfrag(qrow, 16 * k + 8 * (lane >> 5), p.d, q_ok);
+    for (int k = 0; k < NK; ++k) qf[k] = gfrag(r, offset, 16 * k + 8 * (lane >> 5), p.d, qb);
   }
   kt.store(Kl, PT, tid);
   vt.store(Vl, PT, tid);
-  if (tiles > 1) {
-    kt.load(kb + (long long)KB * p.k_row, p.k_row, w.len - KB, p.d, tid);
-    vt.load(vb + (long long)KB * p.v_row, p.v_row, w.len - KB, p.d, tid);
-  }
+  request(1);
 
   const float c = p.scale * kL2E;  // scores in powers of two: exp(x) is one v_exp_f32
   float m = -INFINITY, l = 0.f;    // running maximum (of the unscaled scores) and sum
@@ -211,14 +272,9 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
     wg_barrier_lds();  // tile t is in LDS; everyone is done with tile t - 1, whose buffer tile t + 1 goes into
     const T* const Kt = Kl + (t & 1) * KB * PT;
     const T* const Vt = Vl + (t & 1) * KB * PT;
-    if (t + 1 < tiles) {
-      kt.store(Kl + ((t + 1) & 1) * KB * PT, PT, tid);
-      vt.store(Vl + ((t + 1) & 1) * KB * PT, PT, tid);
-    }
-    if (t + 2 < tiles) {
-      kt.load(kb + (long long)(k0 + 2 * KB) * p.k_row, p.k_row, w.len - k0 - 2 * KB, p.d, tid);
-      vt.load(vb + (long long)(k0 + 2 * KB) * p.v_row, p.v_row, w.len - k0 - 2 * KB, p.d, tid);
-    }
+    kt.store(Kl + ((t + 1) & 1) * KB * PT, PT, tid);
+    vt.store(Vl + ((t + 1) & 1) * KB * PT, PT, tid);
+    request(t + 2);
     if (p.causal && k0 > q0 + 31) continue;  // in the future of all of this wave's queries
     f32x16_t s[NB];
 #pragma unroll
@@ -228,22 +284,19 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
 #pragma unroll
       for (int b = 0; b < NB; ++b) mma32(s[b], lds_frag(Kt, PT, 32 * b, 16 * k, lane), qf[k]);
     if (k0 + KB > w.len || (p.causal && k0 + KB - 1 > q0)) {
+      const int last = (p.causal ? min(my_q, w.len - 1) : w.len - 1) - k0 - 4 * (lane >> 5);  // the last key this lane's query sees, from its first row
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = k0 + 32 * b + acc_row(r, lane);
-          s[b][r] = key >= w.len || (p.causal && key > my_q) ? -INFINITY : s[b][r];
-        }
+        for (int r = 0; r < 16; ++r) s[b][r] = 32 * b + (r & 3) + 8 * (r >> 2) > last ? -INFINITY : s[b][r];
     }
     float mx = s[0][0];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     // key 0 is visible to every query (and to the rows past the end, which count as zeros), so the maximum is finite from the first tile on
-    const float m_new = fmaxf(m, mx);
+    const float m_new = fmaxf(m, both_halves_max(mx));
     if (__any(m_new > m)) {
       const float alpha = pexp2((m - m_new) * c);
       l *= alpha;
@@ -272,19 +325,13 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
         for (int f = 0; f < NF; ++f) mma32(o[f], tfrag(Vt, PT, 32 * b + 16 * h, 32 * f, lane), pf);
       }
   }
-  l += __shfl_xor(l, 32, 64);
-  if (!q_ok) return;
+  l = both_halves_sum(l);
   const float inv = 1.0f / l;
-  T* const orow = out + (long long)(w.start + my_q) * p.o_row;
+  const long long row = w.start + (q_ok ? my_q : 0);
+  T* const lo = p.out_lo != nullptr ? reinterpret_cast<T*>(p.out_lo) + w.head * p.o_head + row * p.o_row : nullptr;
 #pragma unroll
-  for (int f = 0; f < NF; ++f)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c0 = 32 * f + 8 * i + 4 * (lane >> 5);
-      const float v[4] = {o[f][4 * i] * inv, o[f][4 * i + 1] * inv, o[f][4 * i + 2] * inv, o[f][4 * i + 3] * inv};
-      if (c0 < p.d) store4<T>(orow + c0, v);
-    }
-  if (lane < 32) p.lse[(long long)w.head * p.rows + w.start + my_q] = fmaf(m, c, __log2f(l));
+  for (int f = 0; f < NF; ++f) store_rows(out + row * p.o_row, lo, o[f], inv, 32 * f, p.d, lane, q_ok);
+  if (lane < 32 && q_ok && p.lse != nullptr) p.lse[(long long)w.head * p.rows + row] = fmaf(m, c, __log2f(l));
 }
 
 // -----------------------------------------------------------------------------------------------------------------------------------------
@@ -295,7 +342,7 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* const Kl = reinterpret_cast<T*>(smem);
   T* const Vl = Kl + 2 * KB * PT;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Item w = work_item(p, p.heads_q);
   if (w.seq < -1) return;
   T* const dq = reinterpret_cast<T*>(p.dq) + w.head * p.dq_head;
@@ -307,39 +354,44 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
   const int q0 = first + wave * 32, my_q = q0 + (lane & 31);
   const bool q_ok = my_q < w.len;
   const int kv_head = w.head / (p.heads_q / p.heads_kv);
+  const T* const qb = reinterpret_cast<const T*>(p.q) + (long long)w.start * p.q_row + w.head * p.q_head;
+  const T* const db = reinterpret_cast<const T*>(p.dout) + (long long)w.start * p.do_row + w.head * p.do_head;
+  const T* const ob = reinterpret_cast<const T*>(p.out) + (long long)w.start * p.o_row + w.head * p.o_head;
+  const T* const lb = reinterpret_cast<const T*>(p.out_lo != nullptr ? p.out_lo : p.out) + (long long)w.start * p.o_row + w.head * p.o_head;
   const T* const kb = reinterpret_cast<const T*>(p.k) + (long long)w.start * p.k_row + kv_head * p.k_head;
   const T* const vb = reinterpret_cast<const T*>(p.v) + (long long)w.start * p.v_row + kv_head * p.v_head;
   const int keys = p.causal ? min(w.len, first + 32 * NW) : w.len;
   const int tiles = (keys + KB - 1) / KB;
 
   RowTile<T, CP, KB, NT> kt, vt;
-  kt.load(kb, p.k_row, w.len, p.d, tid);
-  vt.load(vb, p.v_row, w.len, p.d, tid);
+  kt.place(p.k_row, p.d, tid);
+  vt.place(p.v_row, p.d, tid);
+  auto request = [&](int t) {
+    kt.load(tile_rows(kb, p.k_row, t * KB, w.len, p.d));
+    vt.load(tile_rows(vb, p.v_row, t * KB, w.len, p.d));
+  };
+  request(0);
   Frag<T> qf[NK], df[NK];
-  const long long row = w.start + (q_ok ? my_q : 0);
   float delta = 0.f;
   {
-    const T* qrow = reinterpret_cast<const T*>(p.q) + row * p.q_row + w.head * p.q_head;
-    const T* drow = reinterpret_cast<const T*>(p.dout) + row * p.do_row + w.head * p.do_head;
-    const T* orow = reinterpret_cast<const T*>(p.out) + row * p.o_row + w.head * p.o_head;
+    const rsrc_t rq = tile_rows(qb, p.q_row, q0, w.len, p.d), rd = tile_rows(db, p.do_row, q0, w.len, p.d), ro = tile_rows(ob, p.o_row, q0, w.len, p.d);
+    const rsrc_t rl = p.out_lo != nullptr ? tile_rows(lb, p.o_row, q0, w.len, p.d) : rows_of(lb, 0);
+    const int r = (lane & 31) * (int)sizeof(T), oq = r * (int)p.q_row, od = r * (int)p.do_row, oo = r * (int)p.o_row;
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
       const int c0 = 16 * k + 8 * (lane >> 5);
-      qf[k] = gfrag(qrow, c0, p.d, q_ok);
-      df[k] = gfrag(drow, c0, p.d, q_ok);
-      delta += frag_dot(df[k], gfrag(orow, c0, p.d, q_ok));
+      qf[k] = gfrag(rq, oq, c0, p.d, qb);
+      df[k] = gfrag(rd, od, c0, p.d, qb);
+      delta += frag_dot(df[k], gfrag(ro, oo, c0, p.d, qb)) + frag_dot(df[k], gfrag(rl, oo, c0, p.d, qb));
     }
   }
-  delta += __shfl_xor(delta, 32, 64);
-  const long long at = (long long)w.head * p.rows + row;
+  delta = both_halves_sum(delta);
+  const long long row = w.start + (q_ok ? my_q : 0), at = (long long)w.head * p.rows + row;
   const float lse = p.lse[at];
   if (lane < 32 && q_ok) p.delta[at] = delta;  // read by the dk / dv kernel behind this one
   kt.store(Kl, PT, tid);
   vt.store(Vl, PT, tid);
-  if (tiles > 1) {
-    kt.load(kb + (long long)KB * p.k_row, p.k_row, w.len - KB, p.d, tid);
-    vt.load(vb + (long long)KB * p.v_row, p.v_row, w.len - KB, p.d, tid);
-  }
+  request(1);
   const float c = p.scale * kL2E;
   f32x16_t acc[NF];
 #pragma unroll
@@ -350,14 +402,9 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
     wg_barrier_lds();
     const T* const Kt = Kl + (t & 1) * KB * PT;
     const T* const Vt = Vl + (t & 1) * KB * PT;
-    if (t + 1 < tiles) {
-      kt.store(Kl + ((t + 1) & 1) * KB * PT, PT, tid);
-      vt.store(Vl + ((t + 1) & 1) * KB * PT, PT, tid);
-    }
-    if (t + 2 < tiles) {
-      kt.load(kb + (long long)(k0 + 2 * KB) * p.k_row, p.k_row, w.len - k0 - 2 * KB, p.d, tid);
-      vt.load(vb + (long long)(k0 + 2 * KB) * p.v_row, p.v_row, w.len - k0 - 2 * KB, p.d, tid);
-    }
+    kt.store(Kl + ((t + 1) & 1) * KB * PT, PT, tid);
+    vt.store(Vl + ((t + 1) & 1) * KB * PT, PT, tid);
+    request(t + 2);
     if (p.causal && k0 > q0 + 31) continue;
     const bool masked = k0 + KB > w.len || (p.causal && k0 + KB - 1 > q0);
 #pragma unroll
@@ -369,16 +416,12 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
         mma32(dp, lds_frag(Vt, PT, 32 * b, 16 * k, lane), df[k]);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = pexp2(fmaf(s[r], c, -lse));
+      for (int r = 0; r < 16; ++r) s[r] = pexp2(fmaf(s[r], c, -lse)) * (dp[r] - delta);
       if (masked) {
+        const int last = (p.causal ? min(my_q, w.len - 1) : w.len - 1) - k0 - 32 * b - 4 * (lane >> 5);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = k0 + 32 * b + acc_row(r, lane);
-          s[r] = key >= w.len || (p.causal && key > my_q) ? 0.f : s[r];
-        }
+        for (int r = 0; r < 16; ++r) s[r] = (r & 3) + 8 * (r >> 2) > last ? 0.f : s[r];
       }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const Frag<T> sf = acc_frag<T>(s, h);
@@ -387,16 +430,8 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
       }
     }
   }
-  if (!q_ok) return;
-  T* const orow = dq + row * p.dq_row;
 #pragma unroll
-  for (int f = 0; f < NF; ++f)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c0 = 32 * f + 8 * i + 4 * (lane >> 5);
-      const float v[4] = {acc[f][4 * i] * p.scale, acc[f][4 * i + 1] * p.scale, acc[f][4 * i + 2] * p.scale, acc[f][4 * i + 3] * p.scale};
-      if (c0 < p.d) store4<T>(orow + c0, v);
-    }
+  for (int f = 0; f < NF; ++f) store_rows(dq + row * p.dq_row, (T*)nullptr, acc[f], p.scale, 32 * f, p.d, lane, q_ok);
 }
 
 // -----------------------------------------------------------------------------------------------------------------------------------------
@@ -404,12 +439,13 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
 // -----------------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bounds__(64 * NW, OCC) void packed_attn_dkv_kernel(PA p) {
   constexpr int PT = lds_pitch<T>(CP), NF = CP / 32, NK = CP / 16, NB = QB / 32, NT = 64 * NW;
+  static_assert(NT >= QB, "one thread a query's statistics");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* const Ql = reinterpret_cast<T*>(smem);
   T* const Dl = Ql + 2 * QB * PT;
-  float* const Ll = reinterpret_cast<float*>(Dl + 2 * QB * PT);  // [2][QB] log-sums, [2][QB] deltas
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  Item w = work_item(p, p.heads_kv);
+  float* const Ll = reinterpret_cast<float*>(Dl + 2 * QB * PT);  // [2][2][NT]: log-sums and deltas of a tile's queries
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Item w = work_item(p, p.heads_kv);
   if (w.seq < -1) return;
   T* const dk = reinterpret_cast<T*>(p.dk) + w.head * p.dk_head;
   T* const dv = reinterpret_cast<T*>(p.dv) + w.head * p.dv_head;
@@ -423,60 +459,64 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
   const int k0 = first + wave * 32, my_k = k0 + (lane & 31);
   const bool k_ok = my_k < w.len;
   const int group = p.heads_q / p.heads_kv;
-  const long long row = w.start + (k_ok ? my_k : 0);
-  Frag<T> kf[NK], vf[NK];
-  {
-    const T* krow = reinterpret_cast<const T*>(p.k) + row * p.k_row + w.head * p.k_head;
-    const T* vrow = reinterpret_cast<const T*>(p.v) + row * p.v_row + w.head * p.v_head;
-#pragma unroll
-    for (int k = 0; k < NK; ++k) {
-      kf[k] = gfrag(krow, 16 * k + 8 * (lane >> 5), p.d, k_ok);
-      vf[k] = gfrag(vrow, 16 * k + 8 * (lane >> 5), p.d, k_ok);
-    }
-  }
-  const int qfirst = p.causal ? first / QB * QB : 0;
+  const T* const kb = reinterpret_cast<const T*>(p.k) + (long long)w.start * p.k_row + w.head * p.k_head;
+  const T* const vb = reinterpret_cast<const T*>(p.v) + (long long)w.start * p.v_row + w.head * p.v_head;
+  const int qfirst = p.causal ? first : 0;
   const int per_head = (w.len - qfirst + QB - 1) / QB, tiles = group * per_head;
 
   RowTile<T, CP, QB, NT> qt, dt;
-  constexpr int SPT = (2 * QB + NT - 1) / NT;
-  float stats[SPT];  // of the tile's queries: log-sums, then deltas
-  auto load = [&](int t) {
-    const int head = w.head * group + t / per_head, q0 = qfirst + (t % per_head) * QB;
-    qt.load(reinterpret_cast<const T*>(p.q) + (long long)(w.start + q0) * p.q_row + head * p.q_head, p.q_row, w.len - q0, p.d, tid);
-    dt.load(reinterpret_cast<const T*>(p.dout) + (long long)(w.start + q0) * p.do_row + head * p.do_head, p.do_row, w.len - q0, p.d, tid);
-#pragma unroll
-    for (int i = 0; i < SPT; ++i) {
-      const int idx = tid + i * NT, q = idx % QB;
-      const float* src = idx < QB ? p.lse : p.delta;
-      stats[i] = src[(long long)head * p.rows + w.start + (q0 + q < w.len ? q0 + q : w.len - 1)];
+  qt.place(p.q_row, p.d, tid);
+  dt.place(p.do_row, p.d, tid);
+  float lse, delta;
+  int next_head = w.head * group, next_q = qfirst, left = tiles;  // of the tile that is requested next
+  auto request = [&]() {
+    const int len = left > 0 ? w.len : 0;
+    const long long at = (long long)next_head * p.rows + w.start;
+    qt.load(tile_rows(reinterpret_cast<const T*>(p.q) + (long long)w.start * p.q_row + next_head * p.q_head, p.q_row, next_q, len, p.d));
+    dt.load(tile_rows(reinterpret_cast<const T*>(p.dout) + (long long)w.start * p.do_row + next_head * p.do_head, p.do_row, next_q, len, p.d));
+    const rsrc_t rl = tile_rows(p.lse + at, 1, next_q, len, 1), rd = tile_rows(p.delta + at, 1, next_q, len, 1);
+    const int offset = tid < QB ? tid * 4 : kBeyond;
+    lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rl, offset, 0, 0));
+    delta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rd, offset, 0, 0));
+    --left;
+    next_q += QB;
+    if (next_q >= w.len) {
+      next_q = qfirst;
+      next_head += left > 0 ? 1 : 0;
     }
   };
   auto store = [&](int t) {
     qt.store(Ql + (t & 1) * QB * PT, PT, tid);
     dt.store(Dl + (t & 1) * QB * PT, PT, tid);
-#pragma unroll
-    for (int i = 0; i < SPT; ++i) {
-      const int idx = tid + i * NT;
-      if (idx < 2 * QB) Ll[(t & 1) * 2 * QB + idx] = stats[i];
-    }
+    Ll[(t & 1) * 2 * NT + tid] = lse;
+    Ll[(t & 1) * 2 * NT + NT + tid] = delta;
   };
-  load(0);
+  request();
+  Frag<T> kf[NK], vf[NK];
+  {
+    const rsrc_t rk = tile_rows(kb, p.k_row, k0, w.len, p.d), rv = tile_rows(vb, p.v_row, k0, w.len, p.d);
+    const int r = (lane & 31) * (int)sizeof(T);
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      kf[k] = gfrag(rk, r * (int)p.k_row, 16 * k + 8 * (lane >> 5), p.d, kb);
+      vf[k] = gfrag(rv, r * (int)p.v_row, 16 * k + 8 * (lane >> 5), p.d, kb);
+    }
+  }
   store(0);
-  if (tiles > 1) load(1);
+  request();
 
   const float c = p.scale * kL2E;
   f32x16_t ak[NF], av[NF];
 #pragma unroll
   for (int f = 0; f < NF; ++f) { ak[f] = acc_zero(); av[f] = acc_zero(); }
 
-  for (int t = 0; t < tiles; ++t) {
+  for (int t = 0, q0 = qfirst; t < tiles; ++t, q0 = q0 + QB < w.len ? q0 + QB : qfirst) {
     wg_barrier_lds();
-    if (t + 1 < tiles) store(t + 1);
-    if (t + 2 < tiles) load(t + 2);
-    const int q0 = qfirst + (t % per_head) * QB;
+    store(t + 1);
+    request();
     const T* const Qt = Ql + (t & 1) * QB * PT;
     const T* const Dt = Dl + (t & 1) * QB * PT;
-    const float* const Lt = Ll + (t & 1) * 2 * QB;
+    const float* const Lt = Ll + (t & 1) * 2 * NT;
     if (k0 >= w.len || (p.causal && q0 + QB - 1 < k0)) continue;  // no key of this wave, or none of the tile's queries sees one
     const bool masked = q0 + QB > w.len || (p.causal && q0 < k0 + 31);
 #pragma unroll
@@ -487,23 +527,31 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
         mma32(s, lds_frag(Qt, PT, 32 * b, 16 * k, lane), kf[k]);
         mma32(dp, lds_frag(Dt, PT, 32 * b, 16 * k, lane), vf[k]);
       }
-      f32x16_t ds;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r0 = 32 * b + 8 * i + 4 * (lane >> 5);
-        const float4 ls = *reinterpret_cast<const float4*>(Lt + r0), de = *reinterpret_cast<const float4*>(Lt + QB + r0);
+        const float4 ls = *reinterpret_cast<const float4*>(Lt + r0), de = *reinterpret_cast<const float4*>(Lt + NT + r0);
         const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dl[4] = {de.x, de.y, de.z, de.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float pv = pexp2(fmaf(s[4 * i + e], c, -lv[e]));
-          if (masked) pv = q0 + r0 + e >= w.len || (p.causal && my_k > q0 + r0 + e) ? 0.f : pv;
-          s[4 * i + e] = pv;
-          ds[4 * i + e] = pv * (dp[4 * i + e] - dl[e]);
+          s[4 * i + e] = pexp2(fmaf(s[4 * i + e], c, -lv[e]));
+          dp[4 * i + e] = s[4 * i + e] * (dp[4 * i + e] - dl[e]);
+        }
+      }
+      if (masked) {
+        // queries from `lo` on (from this lane's first row) see this lane's key, those from `hi` on lie behind the sequence
+        const int base = q0 + 32 * b + 4 * (lane >> 5), lo = p.causal ? my_k - base : -64, hi = w.len - base;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int q = (r & 3) + 8 * (r >> 2);
+          const bool hide = q < lo || q >= hi;
+          s[r] = hide ? 0.f : s[r];
+          dp[r] = hide ? 0.f : dp[r];
         }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const Frag<T> pf = acc_frag<T>(s, h), sf = acc_frag<T>(ds, h);
+        const Frag<T> pf = acc_frag<T>(s, h), sf = acc_frag<T>(dp, h);
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
           mma32(av[f], tfrag(Dt, PT, 32 * b + 16 * h, 32 * f, lane), pf);
@@ -512,21 +560,12 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
       }
     }
   }
-  if (!k_ok) return;
-  T* const krow = dk + row * p.dk_row;
-  T* const vrow = dv + row * p.dv_row;
+  const long long row = w.start + (k_ok ? my_k : 0);
 #pragma unroll
-  for (int f = 0; f < NF; ++f)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c0 = 32 * f + 8 * i + 4 * (lane >> 5);
-      const float a[4] = {ak[f][4 * i] * p.scale, ak[f][4 * i + 1] * p.scale, ak[f][4 * i + 2] * p.scale, ak[f][4 * i + 3] * p.scale};
-      const float b[4] = {av[f][4 * i], av[f][4 * i + 1], av[f][4 * i + 2], av[f][4 * i + 3]};
-      if (c0 < p.d) {
-        store4<T>(krow + c0, a);
-        store4<T>(vrow + c0, b);
-      }
-    }
+  for (int f = 0; f < NF; ++f) {
+    store_rows(dk + row * p.dk_row, (T*)nullptr, ak[f], p.scale, 32 * f, p.d, lane, k_ok);
+    store_rows(dv + row * p.dv_row, (T*)nullptr, av[f], 1.f, 32 * f, p.d, lane, k_ok);
+  }
 }
 
 // -----------------------------------------------------------------------------------------------------------------------------------------
@@ -606,11 +645,11 @@ template <typename T, int CP, int NW, int KB> int launch_fwd(const PA& p, hipStr
   return 0;
 }
 template <typename T, int CP, int NW, int KB> int launch_bwd(const PA& p, hipStream_t st) {
-  constexpr int QB = 32;
+  constexpr int QB = KB;
   constexpr auto dq = packed_attn_dq_kernel<T, CP, NW, KB, occ<T, CP, NW>(false)>;
   constexpr auto dkv = packed_attn_dkv_kernel<T, CP, NW, QB, occ<T, CP, NW>(true)>;
   static DynSmemAttr aq, ak;
-  const size_t sq = (size_t)4 * KB * lds_pitch<T>(CP) * sizeof(T), sk = (size_t)4 * QB * lds_pitch<T>(CP) * sizeof(T) + 4 * QB * sizeof(float);
+  const size_t sq = (size_t)4 * KB * lds_pitch<T>(CP) * sizeof(T), sk = (size_t)4 * QB * lds_pitch<T>(CP) * sizeof(T) + 4 * 64 * NW * sizeof(float);
   if (hipError_t e = aq.ensure((const void*)dq, sq)) return (int)e;
   if (hipError_t e = ak.ensure((const void*)dkv, sk)) return (int)e;
   dq<<<dim3((unsigned)(p.places * p.heads_q)), dim3(64 * NW), sq, st>>>(p);
@@ -634,18 +673,19 @@ template <typename T> int run_type(const PA& p, int backward, hipStream_t st) {
 
 bool strides_ok(int dtype, const void* base, long long row, long long head) {
   const long long n = dtype == CVH_DT_BF16 ? 8 : 4;  // 16-byte accesses
-  return base != nullptr && (reinterpret_cast<uintptr_t>(base) & 15) == 0 && row % n == 0 && head % n == 0 && row >= 0 && head >= 0;
+  return base != nullptr && (reinterpret_cast<uintptr_t>(base) & 15) == 0 && row % n == 0 && head % n == 0 && row >= 0 && head >= 0 && row <= (1 << 21);  // (128 rows in 31 bits of bytes)
 }
 int check(int dtype, const PA* p, int backward) {
   if (dtype != CVH_DT_F32 && dtype != CVH_DT_BF16) return -1;
-  if (p == nullptr || p->plan == nullptr || p->lse == nullptr) return -2;
+  if (p == nullptr || p->plan == nullptr) return -2;
   if (p->rows <= 0 || p->seqs <= 0 || p->heads_q <= 0 || p->heads_kv <= 0 || p->heads_q % p->heads_kv || p->d <= 0 || p->d > 128 || p->d % 8) return -2;
   if (!(p->scale > 0.f) || (p->block != 32 && p->block != 128)) return -2;
   if (p->places != p->rows / p->block + p->seqs + 1 || (long long)p->places * p->heads_q > 0x7fffffffll) return -2;
   if (!strides_ok(dtype, p->q, p->q_row, p->q_head) || !strides_ok(dtype, p->k, p->k_row, p->k_head) || !strides_ok(dtype, p->v, p->v_row, p->v_head) ||
       !strides_ok(dtype, p->out, p->o_row, p->o_head))
     return -2;
-  if (backward && (p->delta == nullptr || !strides_ok(dtype, p->dout, p->do_row, p->do_head) || !strides_ok(dtype, p->dq, p->dq_row, p->dq_head) ||
+  if (p->out_lo != nullptr && (dtype != CVH_DT_BF16 || (reinterpret_cast<uintptr_t>(p->out_lo) & 15))) return -2;
+  if (backward && (p->lse == nullptr || p->delta == nullptr || !strides_ok(dtype, p->dout, p->do_row, p->do_head) || !strides_ok(dtype, p->dq, p->dq_row, p->dq_head) ||
                    !strides_ok(dtype, p->dk, p->dk_row, p->dk_head) || !strides_ok(dtype, p->dv, p->dv_row, p->dv_head)))
     return -2;
   return 0;

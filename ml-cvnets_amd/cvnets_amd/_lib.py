@@ -166,7 +166,7 @@ class OperandXf(ctypes.Structure):
 
 class PackedAttn(ctypes.Structure):
     """cvh_packed_attn (include/cvnets_hip.h)."""
-    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv", "lse", "delta", "plan")]
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "out", "out_lo", "dout", "dq", "dk", "dv", "lse", "delta", "plan")]
                 + [(n + s, c_longlong) for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for s in ("_row", "_head")]
                 + [(n, c_int) for n in ("rows", "seqs", "heads_q", "heads_kv", "d", "causal", "block", "places")] + [("scale", c_float)])
 

@@ -16,10 +16,16 @@ from . import _lib
 from .ops import _check_dev, _dt, _p, compute_dtype
 
 _INT_MAX = 2 ** 31 - 1
+_MOST_ROW = 1 << 21  # elements between two rows
 
 
-def _stream_of(t: Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _call(dev: torch.device, name: str, *args) -> None:
+    """an entry point on `dev` and its current stream, whatever device is the current one"""
+    if torch.cuda.current_device() == dev.index:
+        _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
 
 
 class PackedSeqs:
@@ -47,9 +53,8 @@ class PackedSeqs:
         # One wave per 32 rows where a 128-row workgroup would be mostly empty: captions (512 of 5 .. 77 tokens, 8 heads of 64).
         self.block = 32 if self.max_len <= 128 else 128
         self.places = rows // self.block + self.seqs + 1
-        with torch.cuda.device(cu_seqlens.device):
-            self.plan = torch.empty(_lib.query("cvh_packed_plan_elems", self.seqs, rows, self.block), dtype=torch.int32, device=cu_seqlens.device)
-            self.refresh()
+        self.plan = torch.empty(_lib.query("cvh_packed_plan_elems", self.seqs, rows, self.block), dtype=torch.int32, device=cu_seqlens.device)
+        self.refresh()
 
     @classmethod
     def from_lengths(cls, lengths: Sequence[int], device, rows: Optional[int] = None) -> "PackedSeqs":
@@ -65,8 +70,7 @@ class PackedSeqs:
         return cls(cu.to(torch.int32).to(device), rows, max_len=max(lengths))
 
     def refresh(self) -> None:
-        with torch.cuda.device(self.plan.device):
-            _lib.call("cvh_packed_plan", _p(self.cu_seqlens), self.seqs, self.rows, self.block, _p(self.plan), _stream_of(self.plan))
+        _call(self.plan.device, "cvh_packed_plan", _p(self.cu_seqlens), self.seqs, self.rows, self.block, _p(self.plan))
 
     def __repr__(self) -> str:
         return f"PackedSeqs(sequences={self.seqs}, rows={self.rows}, max_len={self.max_len})"
@@ -78,21 +82,29 @@ class PackedSeqs:
 def _loadable(t: Tensor) -> Tensor:
     """[rows, heads, d] as the kernels read it: d contiguous, base and strides on 16 bytes (any other layout is copied)"""
     n = 16 // t.element_size()
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % n == 0 and t.stride(1) % n == 0 and t.stride(0) >= 0 and t.stride(1) >= 0
+    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % n == 0 and t.stride(1) % n == 0 and t.stride(1) >= 0 and 0 <= t.stride(0) <= _MOST_ROW
     return t if ok else t.contiguous() if not t.is_contiguous() else t.clone()
 
 
-def _launch(name: str, seqs: PackedSeqs, scale: float, causal: bool, lse: Tensor, delta: Optional[Tensor], **t: Tensor) -> None:
-    q, k = t["q"], t["k"]
-    a = _lib.PackedAttn(lse=_p(lse), delta=_p(delta), plan=_p(seqs.plan), rows=seqs.rows, seqs=seqs.seqs, heads_q=q.shape[1], heads_kv=k.shape[1],
-                        d=q.shape[2], causal=int(causal), block=seqs.block, places=seqs.places, scale=scale)
-    for n, x in t.items():
-        s = "o" if n == "out" else "do" if n == "dout" else n
-        setattr(a, n, x.data_ptr())
-        setattr(a, s + "_row", x.stride(0))
-        setattr(a, s + "_head", x.stride(1))
-    with torch.cuda.device(q.device):
-        _lib.call(name, _dt(q), ctypes.byref(a), _stream_of(q))
+def _layout(t: Optional[Tensor]):
+    return (0, 0) if t is None else (t.stride(0), t.stride(1))
+
+
+def _launch(name: str, seqs: PackedSeqs, scale: float, causal: bool, q, k, v, out, out_lo, lse, delta=None, dout=None, dq=None, dk=None, dv=None) -> None:
+    a = _lib.PackedAttn(_p(q), _p(k), _p(v), _p(out), _p(out_lo), _p(dout), _p(dq), _p(dk), _p(dv), _p(lse), _p(delta), seqs.plan.data_ptr(),
+                        *_layout(q), *_layout(k), *_layout(v), *_layout(out), *_layout(dout), *_layout(dq), *_layout(dk), *_layout(dv),
+                        seqs.rows, seqs.seqs, q.shape[1], k.shape[1], q.shape[2], int(causal), seqs.block, seqs.places, scale)
+    _call(q.device, name, _dt(q), ctypes.byref(a))
+
+
+def _forward(q: Tensor, k: Tensor, v: Tensor, seqs: PackedSeqs, causal: bool, scale: float, grad: bool):
+    """(out, out_lo, lse); the last two are for the backward only: in bf16 the row sums dout . out are formed from 16 bits of out, not 8"""
+    rows, heads, d = q.shape
+    out = torch.empty((rows, heads, d), dtype=q.dtype, device=q.device)
+    out_lo = torch.empty((rows, heads, d), dtype=q.dtype, device=q.device) if grad and q.dtype == torch.bfloat16 else None
+    lse = torch.empty((heads, rows), dtype=torch.float32, device=q.device) if grad else None
+    _launch("cvh_packed_attn_fwd", seqs, scale, causal, q, k, v, out, out_lo, lse)
+    return out, out_lo, lse
 
 
 def _check_heads(q: Tensor, k: Tensor, v: Tensor, seqs: PackedSeqs, scale: Optional[float]) -> float:
@@ -101,22 +113,23 @@ def _check_heads(q: Tensor, k: Tensor, v: Tensor, seqs: PackedSeqs, scale: Optio
     if not (q.dtype == k.dtype == v.dtype):
         raise RuntimeError(f"q, k and v must have one dtype. Got: {q.dtype}, {k.dtype}, {v.dtype}")
     _dt(q)
-    hq, hkv, d = q.shape[1], k.shape[1], q.shape[2]
+    rows, hq, d = q.shape
+    hkv = k.shape[1]
     if hkv == 0 or hq == 0 or hq % hkv:
         raise RuntimeError(f"the number of query heads must be a multiple of the number of key heads. Got: {hq} and {hkv}")
     if d == 0 or d % 8 or d > 128:
         raise NotImplementedError(f"packed attention: head_dim must be a multiple of 8 up to 128. Got: {d}")
-    scale = float(d) ** -0.5 if scale is None else float(scale)
+    scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale must be positive and finite. Got: {scale}")
-    if q.shape[0] != seqs.rows:
-        raise RuntimeError(f"the layout is of {seqs.rows} rows, the tensors have {q.shape[0]}")
-    for t in (q, k, v):
-        _check_dev(t)
-        if t.device != seqs.plan.device:
-            raise RuntimeError(f"tensors and layout must be on one device. Got: {t.device} and {seqs.plan.device}")
-    if seqs.places * hq > _INT_MAX:
-        raise RuntimeError(f"{seqs.places} blocks of {hq} heads are more workgroups than one launch takes")
+    if rows != seqs.rows:
+        raise RuntimeError(f"the layout is of {seqs.rows} rows, the tensors have {rows}")
+    if hq * d > _MOST_ROW or seqs.places * hq > _INT_MAX:
+        raise NotImplementedError(f"packed attention: {hq} heads of {d} on {seqs.places} blocks are more than one launch takes")
+    dev = seqs.plan.device
+    if q.device != dev or k.device != dev or v.device != dev:
+        _check_dev(q), _check_dev(k), _check_dev(v)
+        raise RuntimeError(f"tensors and layout must be on one device. Got: {q.device}, {k.device}, {v.device} and {dev}")
     return scale
 
 
@@ -124,20 +137,18 @@ class PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, seqs, causal, scale):
         q, k, v = _loadable(q), _loadable(k), _loadable(v)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
-        _launch("cvh_packed_attn_fwd", seqs, scale, causal, lse, None, q=q, k=k, v=v, out=out)
-        ctx.save_for_backward(q, k, v, out, lse)
+        out, out_lo, lse = _forward(q, k, v, seqs, causal, scale, True)
+        ctx.save_for_backward(q, k, v, out, out_lo, lse)
         ctx.cfg = (seqs, causal, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, out_lo, lse = ctx.saved_tensors
         seqs, causal, scale = ctx.cfg
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        _launch("cvh_packed_attn_bwd", seqs, scale, causal, lse, torch.empty_like(lse), q=q, k=k, v=v, out=out, dout=_loadable(dout), dq=dq, dk=dk, dv=dv)
+        _launch("cvh_packed_attn_bwd", seqs, scale, causal, q, k, v, out, out_lo, lse, torch.empty_like(lse), _loadable(dout), dq, dk, dv)
         return dq, dk, dv, None, None, None
 
 
@@ -146,24 +157,20 @@ class PackedAttentionQKVFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, heads, kv_heads, seqs, causal, scale):
-        q, k, v = _split_heads(qkv, heads, kv_heads)
-        out = torch.empty((qkv.shape[0], heads, q.shape[2]), dtype=qkv.dtype, device=qkv.device)
-        lse = torch.empty((heads, qkv.shape[0]), dtype=torch.float32, device=qkv.device)
-        _launch("cvh_packed_attn_fwd", seqs, scale, causal, lse, None, q=q, k=k, v=v, out=out)
-        ctx.save_for_backward(qkv, out, lse)
+        out, out_lo, lse = _forward(*_split_heads(qkv, heads, kv_heads), seqs, causal, scale, True)
+        ctx.save_for_backward(qkv, out, out_lo, lse)
         ctx.cfg = (heads, kv_heads, seqs, causal, scale)
         return out.view(qkv.shape[0], -1)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        qkv, out, lse = ctx.saved_tensors
+        qkv, out, out_lo, lse = ctx.saved_tensors
         heads, kv_heads, seqs, causal, scale = ctx.cfg
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        q, k, v = _split_heads(qkv, heads, kv_heads)
-        dq, dk, dv = _split_heads(dqkv, heads, kv_heads)
-        _launch("cvh_packed_attn_bwd", seqs, scale, causal, lse, torch.empty_like(lse), q=q, k=k, v=v, out=out,
-                dout=_loadable(dout.view(out.shape) if dout.is_contiguous() else dout.reshape(out.shape)), dq=dq, dk=dk, dv=dv)
+        out = out.view(qkv.shape[0], heads, -1)
+        _launch("cvh_packed_attn_bwd", seqs, scale, causal, *_split_heads(qkv, heads, kv_heads), out, out_lo, lse, torch.empty_like(lse),
+                _loadable(dout.reshape(out.shape)), *_split_heads(dqkv, heads, kv_heads))
         return dqkv, None, None, None, None, None
 
 
@@ -179,7 +186,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, seqs: PackedSeqs, causal: bool = 
     d contiguous and rows on 16 bytes are read in place.  scale: default d ** -0.5.  causal: token i sees the tokens 0 .. i of its sequence.
     A NaN or infinity reaches the results of its own sequence only (under the causal mask: of its 32-row block and behind it)."""
     scale = _check_heads(q, k, v, seqs, scale)
-    return PackedAttentionFn.apply(q, k, v, seqs, bool(causal), scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return PackedAttentionFn.apply(q, k, v, seqs, bool(causal), scale)
+    return _forward(_loadable(q), _loadable(k), _loadable(v), seqs, bool(causal), scale, False)[0]
 
 
 def attention_qkv(qkv: Tensor, heads: int, seqs: PackedSeqs, kv_heads: Optional[int] = None, causal: bool = True, scale: Optional[float] = None) -> Tensor:
@@ -187,27 +196,34 @@ def attention_qkv(qkv: Tensor, heads: int, seqs: PackedSeqs, kv_heads: Optional[
     kv_heads = heads if kv_heads is None else int(kv_heads)
     if qkv.dim() != 2 or heads <= 0 or kv_heads <= 0 or qkv.shape[1] % (heads + 2 * kv_heads):
         raise RuntimeError(f"qkv must be [rows, ({heads} + 2 x {kv_heads}) heads x d]. Got: {list(qkv.shape)}")
-    d = qkv.shape[1] // (heads + 2 * kv_heads)
     if not qkv.is_contiguous() or qkv.data_ptr() % 16:
         qkv = qkv.contiguous() if not qkv.is_contiguous() else qkv.clone()
-    scale = _check_heads(*_split_heads(qkv, int(heads), kv_heads), seqs, scale)
-    return PackedAttentionQKVFn.apply(qkv, int(heads), kv_heads, seqs, bool(causal), scale)
+    q, k, v = _split_heads(qkv, int(heads), kv_heads)
+    scale = _check_heads(q, k, v, seqs, scale)
+    if qkv.shape[1] > _MOST_ROW:
+        raise NotImplementedError(f"packed attention: rows of more than {_MOST_ROW} elements. Got: {qkv.shape[1]}")
+    if torch.is_grad_enabled() and qkv.requires_grad:
+        return PackedAttentionQKVFn.apply(qkv, int(heads), kv_heads, seqs, bool(causal), scale)
+    return _forward(q, k, v, seqs, bool(causal), scale, False)[0].view(qkv.shape[0], -1)
 
 
 # ---------------------------------------------------------------------------------------------------------------------------------------
 # token embedding
 # ---------------------------------------------------------------------------------------------------------------------------------------
+def _lookup(table, pos, ids, seqs, scale, dtype) -> Tensor:
+    rows, (vocab, e) = ids.shape[0], table.shape
+    out = torch.empty((rows, e), dtype=dtype, device=table.device)
+    layout = (None, 0, 0, 0) if seqs is None else (_p(seqs.plan), seqs.seqs, seqs.block, seqs.places)
+    _call(table.device, "cvh_embed_packed_fwd", _dt(out), _p(ids), _p(table), _p(pos), *layout, rows, vocab, 0 if pos is None else pos.shape[0], e, scale, _p(out))
+    return out
+
+
 class PackedEmbedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, pos, ids, seqs, scale, padding_idx, dtype):
-        rows, (vocab, e) = ids.shape[0], table.shape
-        out = torch.empty((rows, e), dtype=dtype, device=table.device)
-        positions = 0 if pos is None else pos.shape[0]
-        layout = (None, 0, 0, 0) if seqs is None else (_p(seqs.plan), seqs.seqs, seqs.block, seqs.places)
-        with torch.cuda.device(table.device):
-            _lib.call("cvh_embed_packed_fwd", _dt(out), _p(ids), _p(table), _p(pos), *layout, rows, vocab, positions, e, scale, _p(out), _stream_of(table))
+        out = _lookup(table, pos, ids, seqs, scale, dtype)
         ctx.save_for_backward(ids)
-        ctx.cfg = (seqs, scale, -1 if padding_idx is None else padding_idx, vocab, positions)
+        ctx.cfg = (seqs, scale, -1 if padding_idx is None else padding_idx, table.shape[0], 0 if pos is None else pos.shape[0])
         return out
 
     @staticmethod
@@ -226,9 +242,8 @@ class PackedEmbedFn(torch.autograd.Function):
         if positions and ctx.needs_input_grad[1]:
             dpos = torch.empty((positions, e), dtype=torch.float32, device=dev)
         pieces = torch.empty(_lib.query("cvh_embed_pieces_elems", rows, e, positions, 0 if dpos is None else seqs.seqs), dtype=torch.float32, device=dev)
-        with torch.cuda.device(dev):
-            _lib.call("cvh_embed_packed_bwd", _dt(dout), _p(ids), _p(dout), None if seqs is None else _p(seqs.plan), 0 if seqs is None else seqs.seqs, rows,
-                      vocab, e, padding, scale, _p(dtable), positions, _p(dpos), _p(sort), _p(pieces), _stream_of(dout))
+        _call(dev, "cvh_embed_packed_bwd", _dt(dout), _p(ids), _p(dout), None if seqs is None else _p(seqs.plan), 0 if seqs is None else seqs.seqs, rows,
+              vocab, e, padding, scale, _p(dtable), positions, _p(dpos), _p(sort), _p(pieces))
         return dtable, dpos, None, None, None, None, None
 
 
@@ -259,9 +274,15 @@ def embed(ids: Tensor, table: Tensor, seqs: Optional[PackedSeqs] = None, pos: Op
     dtype = compute_dtype() if dtype is None else dtype
     if dtype not in (torch.float32, torch.bfloat16):
         raise RuntimeError(f"unsupported activation dtype {dtype}")
-    for t in (ids, table) + (() if pos is None else (pos,)):
-        _check_dev(t)
-        if t.device != table.device or (seqs is not None and t.device != seqs.plan.device):
-            raise RuntimeError(f"ids, tables and layout must be on one device. Got: {t.device} and {table.device}")
-    table, pos = (t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0) else t.contiguous() if not t.is_contiguous() else t.clone() for t in (table, pos))
-    return PackedEmbedFn.apply(table, pos, ids.contiguous(), seqs, float(scale), padding_idx, dtype)
+    dev = table.device
+    if ids.device != dev or (pos is not None and pos.device != dev) or (seqs is not None and seqs.plan.device != dev):
+        raise RuntimeError(f"ids, tables and layout must be on one device. Got: {ids.device} and {dev}")
+    _check_dev(table)
+    if not table.is_contiguous() or table.data_ptr() % 16:
+        table = table.contiguous() if not table.is_contiguous() else table.clone()
+    if pos is not None and (not pos.is_contiguous() or pos.data_ptr() % 16):
+        pos = pos.contiguous() if not pos.is_contiguous() else pos.clone()
+    ids = ids.contiguous()
+    if torch.is_grad_enabled() and (table.requires_grad or (pos is not None and pos.requires_grad)):
+        return PackedEmbedFn.apply(table, pos, ids, seqs, float(scale), padding_idx, dtype)
+    return _lookup(table, pos, ids, seqs, float(scale), dtype)
