@@ -79,13 +79,68 @@ __device__ __forceinline__ float frag_dot(const Frag<float>& a, const Frag<float
   return s;
 }
 
+// LDS tiles of rows x CP columns and their two kinds of operand fragments:
+//   rows(row0, k0):  lane l reads columns k0 + 8 (l >> 5) .. + 7 of row row0 + (l & 31)
+//   cols(k0, col0):  the TRANSPOSE: column col0 + (l & 31), its rows in the order in which a 32x32 accumulator holds them: slot j of lane half h is row
+//                    k0 + 8 (j >> 2) + 4 h + (j & 3).  bf16: two LDS transpose reads (lane 4 r + q of a 16-lane group gives the address of 4 columns of
+//                    block row r and receives column 4 r + q of the 4 x 16 block).
+// bf16 rows are padded so that both kinds of reads find distinct banks: 16 rows x 16 bytes (the pitch an odd number of 16-byte units) and 4 rows x 32
+// bytes (0, 1, 2, 3 pitches at least 32 bytes apart in the 256 bytes of the banks).  16 bytes of padding do for 64 and 96 columns; with 128 they make
+// half of the forward's LDS cycles bank conflicts, 48 bytes none.  (An XOR of the 16-byte chunks with the row does the same without padding, at 30
+// more registers for the addresses: 164 instead of 128 and spills at 128 columns.)
+typedef short v4s_t __attribute__((ext_vector_type(4)));
+template <typename T, int CP> struct Tile;
+template <int CP> struct Tile<bf16_t, CP> {
+  static constexpr int PT = CP == 128 || CP == 32 ? CP + 24 : CP + 8;  // elements a row
+  int row_at, col_at;
+  static __device__ __forceinline__ int chunk_at(int row, int chunk) { return row * PT + chunk * 8; }
+  __device__ __forceinline__ explicit Tile(int lane) {
+    const int i = lane & 15;
+    row_at = (lane & 31) * PT + 8 * (lane >> 5);
+    col_at = (4 * (lane >> 5) + (i >> 2)) * PT + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+  }
+  __device__ __forceinline__ Frag<bf16_t> rows(const bf16_t* tile, int row0, int k0) const {
+    Frag<bf16_t> r;
+    r.v = *reinterpret_cast<const bf16x8_t*>(tile + row_at + row0 * PT + k0);
+    return r;
+  }
+  __device__ __forceinline__ Frag<bf16_t> cols(const bf16_t* tile, int k0, int col0) const {
+    const bf16_t* const p = tile + col_at + k0 * PT + col0;
+    const v4s_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*)(p));
+    const v4s_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*)(p + 8 * PT));
+    Frag<bf16_t> r;
+    r.v = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    return r;
+  }
+};
+template <int CP> struct Tile<float, CP> {
+  static constexpr int PT = lds_pitch<float>(CP);
+  int lane;
+  static __device__ __forceinline__ int chunk_at(int row, int chunk) { return row * PT + chunk * 4; }
+  __device__ __forceinline__ explicit Tile(int l) : lane(l) {}
+  __device__ __forceinline__ Frag<float> rows(const float* tile, int row0, int k0) const { return lds_frag(tile, PT, row0, k0, lane); }
+  __device__ __forceinline__ Frag<float> cols(const float* tile, int k0, int col0) const {
+    const float* p = tile + (k0 + 4 * (lane >> 5)) * PT + col0 + (lane & 31);
+    Frag<float> r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.v[j] = p[((j & 3) + 8 * (j >> 2)) * PT];
+    return r;
+  }
+};
 // A tile of NROWS consecutive rows of a sequence, loaded by NT threads into registers (load: only issues the reads) and written to LDS (store);
 // rows behind the sequence and columns at or behind d are zeros
 template <typename T, int CP, int NROWS, int NT> struct RowTile {
   static constexpr int VN = Chunk<T>::N, CH = CP / VN, IT = (NROWS * CH + NT - 1) / NT;
   static constexpr bool EXACT = (NROWS * CH) % NT == 0;
   uint4 q[IT];
-  int offset[IT];  // bytes
+  int offset[IT];        // bytes
+  const T* base;         // of the tile that is loaded next
+  long long left, step;  // bytes of the sequence from there, and of a tile's rows
+  __device__ __forceinline__ void start(const T* seq_base, long long row_stride, int row0, int len, int d) {
+    base = seq_base + (long long)row0 * row_stride;
+    left = ((long long)(len - row0 - 1) * row_stride + d) * (long long)sizeof(T);
+    step = NROWS * row_stride * (long long)sizeof(T);
+  }
   __device__ __forceinline__ void place(long long row_stride, int d, int tid) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
@@ -93,39 +148,22 @@ template <typename T, int CP, int NROWS, int NT> struct RowTile {
       offset[i] = (EXACT || idx < NROWS * CH) && c < d ? (r * (int)row_stride + c) * (int)sizeof(T) : kBeyond;
     }
   }
-  __device__ __forceinline__ void load(rsrc_t rows) {
+  __device__ __forceinline__ void load() {
+    const rsrc_t rows = rows_of(base, left);
 #pragma unroll
     for (int i = 0; i < IT; ++i) q[i] = buf16(rows, offset[i]);
+    base = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + step);
+    left -= step;
   }
-  __device__ __forceinline__ void store(T* lds, int pitch, int tid) const {
+  __device__ __forceinline__ void store(T* lds, int tid) const {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int idx = tid + i * NT, r = idx / CH, c = (idx % CH) * VN;
-      if (EXACT || idx < NROWS * CH) *reinterpret_cast<uint4*>(lds + r * pitch + c) = q[i];
+      const int idx = tid + i * NT;
+      if (EXACT || idx < NROWS * CH) *reinterpret_cast<uint4*>(lds + Tile<T, CP>::chunk_at(idx / CH, idx % CH)) = q[i];
     }
   }
 };
 
-// operand fragment of the TRANSPOSE of a [k][n] LDS tile, the contraction index in the order in which a 32x32 accumulator holds its rows:
-// slot j of lane half h is tile row k0 + 8 (j >> 2) + 4 h + (j & 3).  bf16: two LDS transpose reads (lane 4r + q of a 16-lane group gives the
-// address of 4 columns of block row r and receives column 4r + q of the 4 x 16 block).
-typedef short v4s_t __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ Frag<bf16_t> tfrag(const bf16_t* tile, int pitch, int k0, int col0, int lane) {
-  const int i = lane & 15;
-  const bf16_t* p = tile + (k0 + 4 * (lane >> 5) + (i >> 2)) * pitch + col0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
-  const v4s_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*)(p));
-  const v4s_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*)(p + 8 * pitch));
-  Frag<bf16_t> f;
-  f.v = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-  return f;
-}
-__device__ __forceinline__ Frag<float> tfrag(const float* tile, int pitch, int k0, int col0, int lane) {
-  const float* p = tile + (k0 + 4 * (lane >> 5)) * pitch + col0 + (lane & 31);
-  Frag<float> f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f.v[j] = p[((j & 3) + 8 * (j >> 2)) * pitch];
-  return f;
-}
 // rows 16 t .. 16 t + 15 (in that order) of an accumulator as an operand.  bf16: the one rounding of P / dS to 8 bits, each probability off by
 // at most 2^-9 of itself; the sums it enters stay in 32 bits.
 template <typename T> __device__ __forceinline__ Frag<T> acc_frag(const f32x16_t& a, int t);
@@ -220,7 +258,7 @@ template <typename T> __device__ __forceinline__ void zero_rows(T* base, long lo
 // forward: workgroup = NW x 32 consecutive queries of one (sequence, query head)
 // -----------------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bounds__(64 * NW, OCC) void packed_attn_fwd_kernel(PA p) {
-  constexpr int PT = lds_pitch<T>(CP), NF = CP / 32, NK = CP / 16, NB = KB / 32, NT = 64 * NW;
+  constexpr int PT = Tile<T, CP>::PT, NF = CP / 32, NK = CP / 16, NB = KB / 32, NT = 64 * NW;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* const Kl = reinterpret_cast<T*>(smem);  // [2][KB][PT]
   T* const Vl = Kl + 2 * KB * PT;            // [2][KB][PT]
@@ -245,11 +283,14 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
   RowTile<T, CP, KB, NT> kt, vt;
   kt.place(p.k_row, p.d, tid);
   vt.place(p.v_row, p.d, tid);
-  auto request = [&](int t) {
-    kt.load(tile_rows(kb, p.k_row, t * KB, w.len, p.d));
-    vt.load(tile_rows(vb, p.v_row, t * KB, w.len, p.d));
+  kt.start(kb, p.k_row, 0, w.len, p.d);
+  vt.start(vb, p.v_row, 0, w.len, p.d);
+  const Tile<T, CP> tile(lane);
+  auto request = [&]() {
+    kt.load();
+    vt.load();
   };
-  request(0);
+  request();
   Frag<T> qf[NK];
   {
     const rsrc_t r = tile_rows(qb, p.q_row, q0, w.len, p.d);
@@ -257,9 +298,9 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
 #pragma unroll
     for (int k = 0; k < NK; ++k) qf[k] = gfrag(r, offset, 16 * k + 8 * (lane >> 5), p.d, qb);
   }
-  kt.store(Kl, PT, tid);
-  vt.store(Vl, PT, tid);
-  request(1);
+  kt.store(Kl, tid);
+  vt.store(Vl, tid);
+  request();
 
   const float c = p.scale * kL2E;  // scores in powers of two: exp(x) is one v_exp_f32
   float m = -INFINITY, l = 0.f;    // running maximum (of the unscaled scores) and sum
@@ -272,9 +313,9 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
     wg_barrier_lds();  // tile t is in LDS; everyone is done with tile t - 1, whose buffer tile t + 1 goes into
     const T* const Kt = Kl + (t & 1) * KB * PT;
     const T* const Vt = Vl + (t & 1) * KB * PT;
-    kt.store(Kl + ((t + 1) & 1) * KB * PT, PT, tid);
-    vt.store(Vl + ((t + 1) & 1) * KB * PT, PT, tid);
-    request(t + 2);
+    kt.store(Kl + ((t + 1) & 1) * KB * PT, tid);
+    vt.store(Vl + ((t + 1) & 1) * KB * PT, tid);
+    request();
     if (p.causal && k0 > q0 + 31) continue;  // in the future of all of this wave's queries
     f32x16_t s[NB];
 #pragma unroll
@@ -282,7 +323,7 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
 #pragma unroll
     for (int k = 0; k < NK; ++k)
 #pragma unroll
-      for (int b = 0; b < NB; ++b) mma32(s[b], lds_frag(Kt, PT, 32 * b, 16 * k, lane), qf[k]);
+      for (int b = 0; b < NB; ++b) mma32(s[b], tile.rows(Kt, 32 * b, 16 * k), qf[k]);
     if (k0 + KB > w.len || (p.causal && k0 + KB - 1 > q0)) {
       const int last = (p.causal ? min(my_q, w.len - 1) : w.len - 1) - k0 - 4 * (lane >> 5);  // the last key this lane's query sees, from its first row
 #pragma unroll
@@ -322,7 +363,7 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
       for (int h = 0; h < 2; ++h) {
         const Frag<T> pf = acc_frag<T>(s[b], h);
 #pragma unroll
-        for (int f = 0; f < NF; ++f) mma32(o[f], tfrag(Vt, PT, 32 * b + 16 * h, 32 * f, lane), pf);
+        for (int f = 0; f < NF; ++f) mma32(o[f], tile.cols(Vt, 32 * b + 16 * h, 32 * f), pf);
       }
   }
   l = both_halves_sum(l);
@@ -338,7 +379,7 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
 // backward, dq (and delta): workgroup = NW x 32 consecutive queries of one (sequence, query head)
 // -----------------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bounds__(64 * NW, OCC) void packed_attn_dq_kernel(PA p) {
-  constexpr int PT = lds_pitch<T>(CP), NF = CP / 32, NK = CP / 16, NB = KB / 32, NT = 64 * NW;
+  constexpr int PT = Tile<T, CP>::PT, NF = CP / 32, NK = CP / 16, NB = KB / 32, NT = 64 * NW;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* const Kl = reinterpret_cast<T*>(smem);
   T* const Vl = Kl + 2 * KB * PT;
@@ -366,11 +407,14 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
   RowTile<T, CP, KB, NT> kt, vt;
   kt.place(p.k_row, p.d, tid);
   vt.place(p.v_row, p.d, tid);
-  auto request = [&](int t) {
-    kt.load(tile_rows(kb, p.k_row, t * KB, w.len, p.d));
-    vt.load(tile_rows(vb, p.v_row, t * KB, w.len, p.d));
+  kt.start(kb, p.k_row, 0, w.len, p.d);
+  vt.start(vb, p.v_row, 0, w.len, p.d);
+  const Tile<T, CP> tile(lane);
+  auto request = [&]() {
+    kt.load();
+    vt.load();
   };
-  request(0);
+  request();
   Frag<T> qf[NK], df[NK];
   float delta = 0.f;
   {
@@ -389,9 +433,9 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
   const long long row = w.start + (q_ok ? my_q : 0), at = (long long)w.head * p.rows + row;
   const float lse = p.lse[at];
   if (lane < 32 && q_ok) p.delta[at] = delta;  // read by the dk / dv kernel behind this one
-  kt.store(Kl, PT, tid);
-  vt.store(Vl, PT, tid);
-  request(1);
+  kt.store(Kl, tid);
+  vt.store(Vl, tid);
+  request();
   const float c = p.scale * kL2E;
   f32x16_t acc[NF];
 #pragma unroll
@@ -402,9 +446,9 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
     wg_barrier_lds();
     const T* const Kt = Kl + (t & 1) * KB * PT;
     const T* const Vt = Vl + (t & 1) * KB * PT;
-    kt.store(Kl + ((t + 1) & 1) * KB * PT, PT, tid);
-    vt.store(Vl + ((t + 1) & 1) * KB * PT, PT, tid);
-    request(t + 2);
+    kt.store(Kl + ((t + 1) & 1) * KB * PT, tid);
+    vt.store(Vl + ((t + 1) & 1) * KB * PT, tid);
+    request();
     if (p.causal && k0 > q0 + 31) continue;
     const bool masked = k0 + KB > w.len || (p.causal && k0 + KB - 1 > q0);
 #pragma unroll
@@ -412,8 +456,8 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
       f32x16_t s = acc_zero(), dp = acc_zero();
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
-        mma32(s, lds_frag(Kt, PT, 32 * b, 16 * k, lane), qf[k]);
-        mma32(dp, lds_frag(Vt, PT, 32 * b, 16 * k, lane), df[k]);
+        mma32(s, tile.rows(Kt, 32 * b, 16 * k), qf[k]);
+        mma32(dp, tile.rows(Vt, 32 * b, 16 * k), df[k]);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = pexp2(fmaf(s[r], c, -lse)) * (dp[r] - delta);
@@ -426,7 +470,7 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
       for (int h = 0; h < 2; ++h) {
         const Frag<T> sf = acc_frag<T>(s, h);
 #pragma unroll
-        for (int f = 0; f < NF; ++f) mma32(acc[f], tfrag(Kt, PT, 32 * b + 16 * h, 32 * f, lane), sf);
+        for (int f = 0; f < NF; ++f) mma32(acc[f], tile.cols(Kt, 32 * b + 16 * h, 32 * f), sf);
       }
     }
   }
@@ -438,7 +482,7 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
 // backward, dk and dv: workgroup = NW x 32 consecutive keys of one (sequence, key head); loops over the group's query heads and the queries
 // -----------------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bounds__(64 * NW, OCC) void packed_attn_dkv_kernel(PA p) {
-  constexpr int PT = lds_pitch<T>(CP), NF = CP / 32, NK = CP / 16, NB = QB / 32, NT = 64 * NW;
+  constexpr int PT = Tile<T, CP>::PT, NF = CP / 32, NK = CP / 16, NB = QB / 32, NT = 64 * NW;
   static_assert(NT >= QB, "one thread a query's statistics");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* const Ql = reinterpret_cast<T*>(smem);
@@ -467,27 +511,29 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
   RowTile<T, CP, QB, NT> qt, dt;
   qt.place(p.q_row, p.d, tid);
   dt.place(p.do_row, p.d, tid);
+  const Tile<T, CP> tile(lane);
   float lse, delta;
-  int next_head = w.head * group, next_q = qfirst, left = tiles;  // of the tile that is requested next
+  int next_head = w.head * group, next_q = w.len;  // of the tile that is requested next; behind a head's last one: start the next head
+  const int end_head = next_head + group, offset = tid < QB ? tid * 4 : kBeyond;
   auto request = [&]() {
-    const int len = left > 0 ? w.len : 0;
-    const long long at = (long long)next_head * p.rows + w.start;
-    qt.load(tile_rows(reinterpret_cast<const T*>(p.q) + (long long)w.start * p.q_row + next_head * p.q_head, p.q_row, next_q, len, p.d));
-    dt.load(tile_rows(reinterpret_cast<const T*>(p.dout) + (long long)w.start * p.do_row + next_head * p.do_head, p.do_row, next_q, len, p.d));
-    const rsrc_t rl = tile_rows(p.lse + at, 1, next_q, len, 1), rd = tile_rows(p.delta + at, 1, next_q, len, 1);
-    const int offset = tid < QB ? tid * 4 : kBeyond;
-    lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rl, offset, 0, 0));
-    delta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rd, offset, 0, 0));
-    --left;
-    next_q += QB;
     if (next_q >= w.len) {
-      next_q = qfirst;
-      next_head += left > 0 ? 1 : 0;
+      const int head = min(next_head, end_head - 1), len = next_head < end_head ? w.len : qfirst;  // (behind the last head: nothing)
+      qt.start(reinterpret_cast<const T*>(p.q) + (long long)w.start * p.q_row + head * p.q_head, p.q_row, qfirst, len, p.d);
+      dt.start(reinterpret_cast<const T*>(p.dout) + (long long)w.start * p.do_row + head * p.do_head, p.do_row, qfirst, len, p.d);
+      if (next_head < end_head) next_q = qfirst;
+      ++next_head;
     }
+    qt.load();
+    dt.load();
+    const long long at = (long long)min(next_head - 1, end_head - 1) * p.rows + w.start + next_q;
+    const long long bytes = next_head <= end_head ? (long long)(w.len - next_q) * 4 : 0;
+    lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows_of(p.lse + at, bytes), offset, 0, 0));
+    delta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows_of(p.delta + at, bytes), offset, 0, 0));
+    next_q += QB;
   };
   auto store = [&](int t) {
-    qt.store(Ql + (t & 1) * QB * PT, PT, tid);
-    dt.store(Dl + (t & 1) * QB * PT, PT, tid);
+    qt.store(Ql + (t & 1) * QB * PT, tid);
+    dt.store(Dl + (t & 1) * QB * PT, tid);
     Ll[(t & 1) * 2 * NT + tid] = lse;
     Ll[(t & 1) * 2 * NT + NT + tid] = delta;
   };
@@ -524,8 +570,8 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
       f32x16_t s = acc_zero(), dp = acc_zero();
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
-        mma32(s, lds_frag(Qt, PT, 32 * b, 16 * k, lane), kf[k]);
-        mma32(dp, lds_frag(Dt, PT, 32 * b, 16 * k, lane), vf[k]);
+        mma32(s, tile.rows(Qt, 32 * b, 16 * k), kf[k]);
+        mma32(dp, tile.rows(Dt, 32 * b, 16 * k), vf[k]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -554,8 +600,8 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
         const Frag<T> pf = acc_frag<T>(s, h), sf = acc_frag<T>(dp, h);
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
-          mma32(av[f], tfrag(Dt, PT, 32 * b + 16 * h, 32 * f, lane), pf);
-          mma32(ak[f], tfrag(Qt, PT, 32 * b + 16 * h, 32 * f, lane), sf);
+          mma32(av[f], tile.cols(Dt, 32 * b + 16 * h, 32 * f), pf);
+          mma32(ak[f], tile.cols(Qt, 32 * b + 16 * h, 32 * f), sf);
         }
       }
     }
@@ -638,7 +684,7 @@ template <typename T, int CP, int NW> constexpr int occ(bool two_accumulators) {
 template <typename T, int CP, int NW, int KB> int launch_fwd(const PA& p, hipStream_t st) {
   constexpr auto kernel = packed_attn_fwd_kernel<T, CP, NW, KB, occ<T, CP, NW>(false)>;
   static DynSmemAttr attr;
-  const size_t smem = (size_t)4 * KB * lds_pitch<T>(CP) * sizeof(T);
+  const size_t smem = (size_t)4 * KB * Tile<T, CP>::PT * sizeof(T);
   if (hipError_t e = attr.ensure((const void*)kernel, smem)) return (int)e;
   kernel<<<dim3((unsigned)(p.places * p.heads_q)), dim3(64 * NW), smem, st>>>(p);
   CVH_CHECK_LAUNCH();
@@ -649,7 +695,7 @@ template <typename T, int CP, int NW, int KB> int launch_bwd(const PA& p, hipStr
   constexpr auto dq = packed_attn_dq_kernel<T, CP, NW, KB, occ<T, CP, NW>(false)>;
   constexpr auto dkv = packed_attn_dkv_kernel<T, CP, NW, QB, occ<T, CP, NW>(true)>;
   static DynSmemAttr aq, ak;
-  const size_t sq = (size_t)4 * KB * lds_pitch<T>(CP) * sizeof(T), sk = (size_t)4 * QB * lds_pitch<T>(CP) * sizeof(T) + 4 * 64 * NW * sizeof(float);
+  const size_t sq = (size_t)4 * KB * Tile<T, CP>::PT * sizeof(T), sk = (size_t)4 * QB * Tile<T, CP>::PT * sizeof(T) + 4 * 64 * NW * sizeof(float);
   if (hipError_t e = aq.ensure((const void*)dq, sq)) return (int)e;
   if (hipError_t e = ak.ensure((const void*)dkv, sk)) return (int)e;
   dq<<<dim3((unsigned)(p.places * p.heads_q)), dim3(64 * NW), sq, st>>>(p);
