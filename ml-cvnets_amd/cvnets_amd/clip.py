@@ -7,12 +7,12 @@ forward/backward run the HIP kernels (token embedding, causal fused attention, G
 from __future__ import annotations
 
 import math
-from typing import Dict, Optional, Sequence
+from typing import Dict, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor, nn
 
-from . import ops
+from . import ops, packed
 from .layers import Dropout, Embedding, PositionalEmbedding, get_normalization_layer, opt
 from .modules import TransformerEncoder
 
@@ -110,6 +110,38 @@ class TextTransformer(nn.Module):
         emb = ops.linear(eot, self.projection_layer.t())  # x @ P
         return ops.l2_normalize(emb)
 
+    @staticmethod
+    def pack_captions(text_tokens: Tensor, device=None) -> Tuple[Tensor, packed.PackedSeqs]:
+        """[B, S] padded captions -> (tokens [rows], layout): each caption up to and including its end mark (its largest token, as in
+        ``encode_text``).  A host function for the data loader's batch; on a tensor of the device it waits for it."""
+        if text_tokens.dim() != 2 or text_tokens.numel() == 0:
+            raise RuntimeError(f"captions must be [batch, sequence] token ids. Got: {list(text_tokens.shape)}")
+        host = text_tokens.cpu()
+        lengths = host.argmax(dim=-1) + 1
+        rows = host[torch.arange(host.shape[1])[None, :] < lengths[:, None]]
+        device = device if device is not None else text_tokens.device if text_tokens.is_cuda else torch.device("cuda", torch.cuda.current_device())
+        return rows.to(device=device, dtype=torch.int64), packed.PackedSeqs.from_lengths(lengths.tolist(), device)
+
+    def encode_packed(self, text_tokens: Tensor, seqs: packed.PackedSeqs, context_length: Optional[int] = None) -> Tensor:
+        """``encode_text`` of packed captions (``pack_captions``): under the causal mask nothing behind a caption's end mark reaches its
+        embedding, so the tower runs on the captions' own tokens only.  Every sequence has at least its end mark.  context_length: the
+        padded length whose positional table is meant (default: the table's own)."""
+        if not self.causal_masking:
+            raise NotImplementedError("packed captions need model.text.transformer.causal_masking: without it the padding tokens take part")
+        if context_length is not None and context_length < 1:
+            raise ValueError(f"context_length must be positive. Got: {context_length}")
+        pos = None
+        if self.positional_embedding is not None:
+            pos = self.positional_embedding.table(context_length or self.positional_embedding.pos_embed.num_embeddings)
+        emb = self.embedding_layer
+        t = packed.embed(text_tokens, emb.weight, seqs, pos=pos, padding_idx=emb.padding_idx)
+        t = self.embedding_dropout(t)
+        for layer in self.transformer:
+            t = layer.forward_tokens(t, ops.NO_SEQMAP, causal=True, seqs=seqs)
+        t = ops.layer_norm_tokens(t, self.final_layer_norm, ops.NO_SEQMAP)
+        ends = (seqs.cu_seqlens[1:].long() - 1).clamp(min=0)  # plumbing: EOT index arithmetic
+        return ops.l2_normalize(ops.linear(ops.RowsGatherIdx.apply(t, ends), self.projection_layer.t()))
+
     def forward_zero_shot(self, text_tokens: Tensor, key_padding_mask: Optional[Tensor] = None, *args, **kwargs) -> Tensor:
         raise NotImplementedError("zero-shot class-template averaging is an evaluation utility, not the HIP training hot path")
 
@@ -169,7 +201,11 @@ class CLIP(nn.Module):
             raise NotImplementedError("zero-shot evaluation is not on the HIP training hot path")
         ops.pack_all(self.text_encoder)  # the image encoder packs its own weights; without this the text tower would run on the packs of
         #                                  whatever step its per-layer cache was filled in (the fused optimizer writes through raw pointers)
-        text_embeddings = self.text_encoder(text_tokens=text_tokens, key_padding_mask=padding_mask)
+        seqs = input.get("text_seqs", None)  # layout of packed captions (TextTransformer.pack_captions): "text" then is their tokens [rows]
+        if seqs is not None:
+            text_embeddings = self.text_encoder.encode_packed(text_tokens, seqs)
+        else:
+            text_embeddings = self.text_encoder(text_tokens=text_tokens, key_padding_mask=padding_mask)
         return {"image": image_embeddings, "text": text_embeddings, "logit_scale": self._exponentiate_and_clip_logits(),
                 "zero_shot_image_logits": None, "augmented_tensor": None}
 

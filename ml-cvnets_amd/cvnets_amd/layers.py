@@ -13,7 +13,7 @@ from typing import Optional, Tuple, Union
 import torch
 from torch import Tensor, nn
 
-from . import ops
+from . import ops, packed
 
 # ---------------------------------------------------------------------------------------------
 # opts helpers: the reference reads dotted names off an argparse.Namespace with getattr
@@ -609,9 +609,15 @@ class MultiHeadAttention(nn.Module):
         return "{}(head_dim={}, num_heads={}, attn_dropout={})".format(self.__class__.__name__, self.head_dim, self.num_heads, self.attn_dropout.p)
 
     def forward_tokens(self, x2d: Tensor, seqmap, causal: bool = False, key_padding_mask: Optional[Tensor] = None, out_drop_p: float = 0.0,
-                       residual: Optional[Tensor] = None, attn_bias: Optional[Tensor] = None) -> Tensor:
-        """qkv projection -> fused attention -> output projection (+dropout +residual in its epilogue)."""
+                       residual: Optional[Tensor] = None, attn_bias: Optional[Tensor] = None, seqs: Optional[packed.PackedSeqs] = None) -> Tensor:
+        """qkv projection -> fused attention -> output projection (+dropout +residual in its epilogue).  `seqs`: the rows are packed sequences
+        of these lengths instead of those of `seqmap`."""
         qkv = ops.linear(x2d, self.qkv_proj.weight, self.qkv_proj.bias)
+        if seqs is not None:
+            if key_padding_mask is not None or attn_bias is not None or (self.training and self.attn_dropout.p > 0.0):
+                raise NotImplementedError("packed sequences take no key padding mask, no attention mask and no dropout on the attention probabilities")
+            o = packed.attention_qkv(qkv, self.num_heads, seqs, causal=causal)
+            return ops.linear(o, self.out_proj.weight, self.out_proj.bias, drop_p=out_drop_p, residual=residual)
         # attn_dropout (multi_head_attention.py:217-218) acts on the softmax output inside the fused kernel; the mask is regenerated in backward
         o = ops.attention(qkv, self.num_heads, seqmap, causal=causal, key_padding_mask=key_padding_mask,
                           drop_p=float(self.attn_dropout.p) if self.training else 0.0, attn_bias=attn_bias)

@@ -155,13 +155,16 @@ class TransformerEncoder(nn.Module):
             self.attn_fn_name, self.act_fn_name, self.norm_type)
 
     def forward_tokens(self, x: Tensor, seqmap, causal: bool = False, key_padding_mask: Optional[Tensor] = None,
-                       attn_bias: Optional[Tensor] = None) -> Tensor:
+                       attn_bias: Optional[Tensor] = None, seqs=None) -> Tensor:
+        """`seqs` (packed.PackedSeqs): the rows of x are packed sequences; `seqmap` then names no sequences (ops.NO_SEQMAP)"""
         ln1, mha, drop1 = self.pre_norm_mha[0], self.pre_norm_mha[1], self.pre_norm_mha[2]
         if not isinstance(ln1, nn.LayerNorm):
             raise NotImplementedError("transformer_norm_layer must be layer_norm on the HIP hot path")
         p1 = drop1.p if self.training else 0.0
         sd = self.drop_path.p if (self.training and isinstance(self.drop_path, StochasticDepth)) else 0.0
         if sd > 0.0:
+            if seqs is not None:
+                raise NotImplementedError("stochastic depth on packed sequences")
             # x = x + StochasticDepth(Dropout(branch(LN(x)))): one Bernoulli draw per sample scales the whole branch; the residual add rides in
             # the drop-path kernel instead of the GEMM epilogue (transformer.py:140-155)
             y = ops.layer_norm_tokens(x, ln1, seqmap)
@@ -171,7 +174,7 @@ class TransformerEncoder(nn.Module):
         # x = x + Dropout(MHA(LN(x)))   — dropout and residual live in the out_proj GEMM epilogue; the fork x -> (x, LN(x)) is one autograd
         # node, so the two gradients of x meet inside the LayerNorm backward kernel
         x, y = ops.layer_norm_fork(x, ln1, seqmap)
-        x = mha.forward_tokens(y, seqmap, causal=causal, key_padding_mask=key_padding_mask, out_drop_p=p1, residual=x, attn_bias=attn_bias)
+        x = mha.forward_tokens(y, seqmap, causal=causal, key_padding_mask=key_padding_mask, out_drop_p=p1, residual=x, attn_bias=attn_bias, seqs=seqs)
         return self._ffn_tokens(x, seqmap, 0.0)
 
     def _ffn_tokens(self, x: Tensor, seqmap, sd: float) -> Tensor:

@@ -82,6 +82,15 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+def call_on(dev: torch.device, name: str, *args) -> None:
+    """an entry point on `dev` and its current stream, whatever device is the current one"""
+    if torch.cuda.current_device() == dev.index:
+        _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _check_dev(t: torch.Tensor):
     if not t.is_cuda:
         raise RuntimeError("cvnets_amd ops run on the GPU only (HIP kernels; there is no CPU fallback)")
@@ -1258,6 +1267,9 @@ class LayerNormChannelFirstFn(torch.autograd.Function):
 
 def layer_norm_channel_first(x2d, gamma, beta, eps):
     return LayerNormChannelFirstFn.apply(x2d.contiguous(), gamma, beta, float(eps))
+
+
+NO_SEQMAP = (0, 0, 1, 1, 0, 1, 0)  # the `seqmap` of a token matrix without equally long sequences: LayerNorm is channel-last
 
 
 def layer_norm_tokens(x2d, ln, seqmap):

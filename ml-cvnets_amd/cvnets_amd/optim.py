@@ -297,13 +297,11 @@ def orthogonalize(matrices: Union[torch.Tensor, Sequence[torch.Tensor]], steps: 
     if not mats:
         return []
     dev = mats[0].device
-    with torch.cuda.device(dev):
-        src = [t.contiguous() for t in mats]
-        out = [torch.empty_like(t) for t in src]
-        table = (_lib.NsMatrix * len(src))(*[_lib.NsMatrix(src=_p(src[i]), dst=_p(out[i]), rows=src[i].shape[0], cols=src[i].shape[1])
-                                             for i in _by_cost([t.shape for t in src])])
-        ws = torch.empty(_lib.query("cvh_ns_workspace_elems", ctypes.byref(table), len(src)), dtype=torch.float32, device=dev)
-        _lib.call("cvh_orthogonalize", ops._dt(src[0]), ctypes.byref(table), len(src), *cfg, _p(ws), _stream())
+    src = [t.contiguous() for t in mats]
+    out = [torch.empty_like(t) for t in src]
+    table = (_lib.NsMatrix * len(src))(*[_lib.NsMatrix(_p(src[i]), _p(out[i]), None, None, *src[i].shape, 0, 1.0) for i in _by_cost([t.shape for t in src])])
+    ws = torch.empty(_lib.query("cvh_ns_workspace_elems", ctypes.byref(table), len(src)), dtype=torch.float32, device=dev)
+    ops.call_on(dev, "cvh_orthogonalize", ops._dt(src[0]), ctypes.byref(table), len(src), *cfg, _p(ws))
     return out[0] if single else out
 
 
@@ -392,14 +390,14 @@ class Muon(torch.optim.Optimizer):
         entries = self._entries()
         if not entries:
             return loss
-        with torch.cuda.device(entries[0][0].device):
-            plan = self._plan
-            if plan is None or plan["key"] != self._key(entries):
-                plan = self._build(entries)
-            if sync_hyperparameters or self._hp is None:
-                self.sync_hyperparameters()
-            g0 = self.param_groups[0]
-            _lib.call("cvh_muon_step", ctypes.byref(plan["table"]), plan["n"], *self._ns, float(g0["momentum"]), int(g0["nesterov"]), _p(self._hp), _p(plan["ws"]),
-                      _stream())
+        dev = entries[0][0].device
+        ops._check_dev(entries[0][0])
+        plan = self._plan
+        if plan is None or plan["key"] != self._key(entries):
+            plan = self._build(entries)
+        if sync_hyperparameters or self._hp is None:
+            self.sync_hyperparameters()
+        g0 = self.param_groups[0]
+        ops.call_on(dev, "cvh_muon_step", ctypes.byref(plan["table"]), plan["n"], *self._ns, float(g0["momentum"]), int(g0["nesterov"]), _p(self._hp), _p(plan["ws"]))
         ops.invalidate_packed()
         return loss

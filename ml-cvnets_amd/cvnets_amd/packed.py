@@ -13,19 +13,10 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _check_dev, _dt, _p, compute_dtype
+from .ops import _check_dev, _dt, _p, call_on, compute_dtype
 
 _INT_MAX = 2 ** 31 - 1
 _MOST_ROW = 1 << 21  # elements between two rows
-
-
-def _call(dev: torch.device, name: str, *args) -> None:
-    """an entry point on `dev` and its current stream, whatever device is the current one"""
-    if torch.cuda.current_device() == dev.index:
-        _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
-    else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
 
 
 class PackedSeqs:
@@ -70,7 +61,7 @@ class PackedSeqs:
         return cls(cu.to(torch.int32).to(device), rows, max_len=max(lengths))
 
     def refresh(self) -> None:
-        _call(self.plan.device, "cvh_packed_plan", _p(self.cu_seqlens), self.seqs, self.rows, self.block, _p(self.plan))
+        call_on(self.plan.device, "cvh_packed_plan", _p(self.cu_seqlens), self.seqs, self.rows, self.block, _p(self.plan))
 
     def __repr__(self) -> str:
         return f"PackedSeqs(sequences={self.seqs}, rows={self.rows}, max_len={self.max_len})"
@@ -94,7 +85,7 @@ def _launch(name: str, seqs: PackedSeqs, scale: float, causal: bool, q, k, v, ou
     a = _lib.PackedAttn(_p(q), _p(k), _p(v), _p(out), _p(out_lo), _p(dout), _p(dq), _p(dk), _p(dv), _p(lse), _p(delta), seqs.plan.data_ptr(),
                         *_layout(q), *_layout(k), *_layout(v), *_layout(out), *_layout(dout), *_layout(dq), *_layout(dk), *_layout(dv),
                         seqs.rows, seqs.seqs, q.shape[1], k.shape[1], q.shape[2], int(causal), seqs.block, seqs.places, scale)
-    _call(q.device, name, _dt(q), ctypes.byref(a))
+    call_on(q.device, name, _dt(q), ctypes.byref(a))
 
 
 def _forward(q: Tensor, k: Tensor, v: Tensor, seqs: PackedSeqs, causal: bool, scale: float, grad: bool):
@@ -214,7 +205,7 @@ def _lookup(table, pos, ids, seqs, scale, dtype) -> Tensor:
     rows, (vocab, e) = ids.shape[0], table.shape
     out = torch.empty((rows, e), dtype=dtype, device=table.device)
     layout = (None, 0, 0, 0) if seqs is None else (_p(seqs.plan), seqs.seqs, seqs.block, seqs.places)
-    _call(table.device, "cvh_embed_packed_fwd", _dt(out), _p(ids), _p(table), _p(pos), *layout, rows, vocab, 0 if pos is None else pos.shape[0], e, scale, _p(out))
+    call_on(table.device, "cvh_embed_packed_fwd", _dt(out), _p(ids), _p(table), _p(pos), *layout, rows, vocab, 0 if pos is None else pos.shape[0], e, scale, _p(out))
     return out
 
 
@@ -242,7 +233,7 @@ class PackedEmbedFn(torch.autograd.Function):
         if positions and ctx.needs_input_grad[1]:
             dpos = torch.empty((positions, e), dtype=torch.float32, device=dev)
         pieces = torch.empty(_lib.query("cvh_embed_pieces_elems", rows, e, positions, 0 if dpos is None else seqs.seqs), dtype=torch.float32, device=dev)
-        _call(dev, "cvh_embed_packed_bwd", _dt(dout), _p(ids), _p(dout), None if seqs is None else _p(seqs.plan), 0 if seqs is None else seqs.seqs, rows,
+        call_on(dev, "cvh_embed_packed_bwd", _dt(dout), _p(ids), _p(dout), None if seqs is None else _p(seqs.plan), 0 if seqs is None else seqs.seqs, rows,
               vocab, e, padding, scale, _p(dtable), positions, _p(dpos), _p(sort), _p(pieces))
         return dtable, dpos, None, None, None, None, None
 

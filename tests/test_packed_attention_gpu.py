@@ -88,3 +88,177 @@ def test_head_widths(dtype, d, hq, hkv):
         out = packed.attention(q, k, v, packed.PackedSeqs(cu, 261, max_len=max_len), scale=0.2)
         for what, a, b in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, (q, k, v), dout)), want):
             close(a, b, dtype, (what, max_len))
+
+
+def test_projection_columns_are_read_in_place_and_give_one_gradient():
+    lens, hq, hkv, d = [45, 1, 130], 6, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(5)
+    qkv = torch.randn(sum(lens), (hq + 2 * hkv) * d, generator=g, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    dout = torch.randn(sum(lens), hq * d, generator=g, device="cuda").to(torch.bfloat16)
+    seqs = packed.PackedSeqs.from_lengths(lens, "cuda")
+    out = packed.attention_qkv(qkv, hq, seqs, kv_heads=hkv)
+    (dqkv,) = torch.autograd.grad(out, (qkv,), dout)
+    q, k, v = (t.reshape(sum(lens), -1, d).requires_grad_(True) for t in qkv.detach().split([hq * d, hkv * d, hkv * d], 1))
+    one = packed.attention(q, k, v, seqs)
+    assert torch.equal(out, one.view(sum(lens), -1))
+    assert torch.equal(dqkv, torch.cat([t.view(sum(lens), -1) for t in torch.autograd.grad(one, (q, k, v), dout.view(one.shape))], 1))
+    with torch.no_grad():
+        assert torch.equal(packed.attention_qkv(qkv, hq, seqs, kv_heads=hkv), out)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_any_strides(dtype):
+    """heads first, spaced rows, an unaligned base, an expanded key head, a transposed incoming gradient: read in place or copied, the same values"""
+    lens, d = [33, 70], 32
+    rows = sum(lens)
+    q, k, v, dout = make(rows, 4, 2, d, dtype, seed=9)
+    seqs = packed.PackedSeqs.from_lengths(lens, "cuda")
+    want = reference(q, k, v, lens, True, d ** -0.5, dout)
+    heads_first = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+    wide = [torch.empty(rows, t.shape[1], d + 24, dtype=dtype, device="cuda")[..., 8:8 + d].copy_(t) for t in (q, k, v)]
+    odd = [torch.empty(t.numel() + 1, dtype=dtype, device="cuda")[1:].view(t.shape).copy_(t) for t in (q, k, v)]
+    last = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    for case in (heads_first, wide, odd, last):
+        case = [t.detach().requires_grad_(True) for t in case]
+        out = packed.attention(*case, seqs)
+        grads = torch.autograd.grad(out, case, dout.transpose(1, 2).contiguous().transpose(1, 2))
+        for what, a, b in zip(("out", "dq", "dk", "dv"), (out, *grads), want):
+            close(a, b, dtype, what)
+    shared = k[:, :1].expand(-1, 2, -1).detach().requires_grad_(True)
+    want = reference(q, shared, v, lens, True, d ** -0.5, dout)
+    out = packed.attention(q, shared, v, seqs)
+    close(out, want[0], dtype, "expanded")
+    close(torch.autograd.grad(out, (shared,), dout)[0], want[2], dtype, "expanded gradient")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("causal", [True, False])
+def test_other_sequences_and_filling_rows_do_not_reach_a_sequence(dtype, causal):
+    """NaN and infinities in one sequence and behind the last one: the other sequences' results do not change by a bit; the filling rows are zeros"""
+    lens, rows, d = [40, 37, 61], 170, 64
+    q, k, v, dout = make(rows, 4, 2, d, dtype, seed=2)
+    for max_len in (61, None):
+        cu = torch.tensor([0, 40, 77, 138], dtype=torch.int32, device="cuda")
+        seqs = packed.PackedSeqs(cu, rows, max_len=max_len)
+
+        def run(*t):
+            t = [x.detach().clone().requires_grad_(True) for x in t]
+            out = packed.attention(*t, seqs, causal=causal)
+            return (out.detach(), *torch.autograd.grad(out, t, dout))
+
+        clean = run(q, k, v)
+        for a, b in zip(clean, reference(q, k, v, lens, causal, d ** -0.5, dout)):
+            close(a[:138], b[:138], dtype, "clean")
+            assert bool((a[138:] == 0).all())
+        dirty = [t.clone() for t in (q, k, v)]
+        for t in dirty:
+            t[40:77:3] = float("nan")
+            t[41:77:3] = float("inf")
+            t[138:] = float("nan")
+        for a, b in zip(run(*dirty), clean):
+            assert torch.equal(a[:40], b[:40]) and torch.equal(a[77:], b[77:])
+
+
+def test_boundaries_from_the_device_are_clamped():
+    """falling boundaries and such outside the rows: sequences as if lifted to the largest before and cut at the rows; every row is written"""
+    rows, d = 100, 32
+    q, k, v, _ = make(rows, 2, 2, d, torch.float32, seed=3)
+    for cu, lens in (([-5, 30, 20, 400], [30, 0, 70]), ([10, 10, 50, 60], [40, 10]), ([0, 0, 0, 0], [])):
+        seqs = packed.PackedSeqs(torch.tensor(cu, dtype=torch.int32, device="cuda"), rows)
+        out = packed.attention(q, k, v, seqs)
+        a = max(0, cu[0])
+        want = reference(q[a:], k[a:], v[a:], lens, True, d ** -0.5)[0]
+        n = sum(lens)
+        if n:
+            close(out[a:a + n], want[:n], torch.float32, cu)
+        assert bool((out[a + n:] == 0).all())
+
+
+def test_offsets_beyond_32_bits():
+    """rows 2^17 elements apart: the last sequence lies 5 GB behind the base"""
+    rows, stride, d = 20000, 1 << 17, 64
+    big = torch.empty(rows, stride, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(11)
+    q, k, v = (big[:, i * 256:i * 256 + 128].view(rows, 2, d) for i in range(3))
+    for t in (q, k, v):
+        t.copy_(torch.randn(rows, 2, d, generator=g, device="cuda"))
+    dout = torch.randn(rows, 2, d, generator=g, device="cuda").to(torch.bfloat16)
+    lens = [19000, 900, 100]
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    out = packed.attention(q, k, v, packed.PackedSeqs.from_lengths(lens, "cuda"))
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    want = reference(q[19000:], k[19000:], v[19000:], lens[1:], True, d ** -0.5, dout[19000:])
+    for a, b in zip((out, *grads), want):
+        close(a[19000:], b, torch.bfloat16, "far rows")
+
+
+def test_gradients_against_differences():
+    lens, d = [9, 1, 40], 16
+    q, k, v, dout = make(sum(lens), 4, 2, d, torch.float32, seed=21)
+    seqs = packed.PackedSeqs.from_lengths(lens, "cuda")
+    for i in range(3):
+        t = [x.detach().clone() for x in (q, k, v)]
+        t[i].requires_grad_(True)
+        (g,) = torch.autograd.grad(packed.attention(*t, seqs, scale=0.3), (t[i],), dout)
+        step = torch.randn(t[i].shape, generator=torch.Generator(device="cuda").manual_seed(i), device="cuda")
+        # Central differences of the sum f = out . dout along `step`: h^2 / 6 of the third derivative (h = 2^-7, the derivatives of one magnitude: 1e-5
+        # of the slope) and the rounding of out, 2^-22 of |out| |dout| at random, over h: 2^-22 sqrt(n) / (sqrt(2) h) = 2e-5 sqrt(n) * sqrt(out's mean square)
+        h, diff = 2.0 ** -7, 0.0
+        for sign in (1, -1):
+            u = [x.detach().clone() for x in t]
+            u[i] += sign * h * step
+            diff += sign * float((packed.attention(*u, seqs, scale=0.3).double() * dout.double()).sum())
+        slope, n = float((g.double() * step.double()).sum()), dout.numel()
+        size = float(g.double().norm())  # of the slope: a sum of |g| times a normal number
+        assert abs(diff / (2 * h) - slope) <= 1e-4 * size + 4 * 2e-5 * math.sqrt(n), (i, diff / (2 * h), slope)
+
+
+def test_repeats_are_equal_and_other_streams():
+    lens = [77, 300, 5, 128] * 4
+    q, k, v, dout = make(sum(lens), 8, 2, 64, torch.bfloat16, seed=6)
+
+    def run():
+        t = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        out = packed.attention(*t, packed.PackedSeqs.from_lengths(lens, "cuda"))
+        return (out.detach(), *torch.autograd.grad(out, t, dout))
+
+    first = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)
+
+
+def test_a_captured_step_follows_changed_boundaries():
+    """plan, forward and backward in a graph: replays with other boundaries and inputs equal the eager results, with eager work between the replays"""
+    rows, d = 512, 64
+    q, k, v, dout = make(rows, 4, 4, d, torch.bfloat16, seed=8)
+    cu = torch.tensor([0, 100, 300, 512], dtype=torch.int32, device="cuda")
+    seqs = packed.PackedSeqs(cu, rows)
+
+    def step():
+        seqs.refresh()
+        t = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        out = packed.attention(*t, seqs)
+        return (out.detach(), *torch.autograd.grad(out, t, dout))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i, bounds in enumerate(([0, 1, 2, 512], [0, 256, 256, 400], [0, 511, 511, 511], [0, 0, 0, 5])):
+        cu.copy_(torch.tensor(bounds, dtype=torch.int32))
+        q.copy_(make(rows, 4, 4, d, torch.bfloat16, seed=30 + i)[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), bounds
