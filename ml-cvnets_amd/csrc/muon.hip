@@ -41,20 +41,38 @@ struct Mat {
   int m, n, mp, np, rows, cols, group;
   float gain;
 };
+// The list: an argument of the first kernel, which leaves a copy in the workspace for the others (arguments lie in host memory: a workgroup's two
+// dependent reads of them cost more than a small matrix's product).
+enum { NORM, SCALE, SYM, APPLY, PHASES };
 struct Mats {
   Mat mat[kMats];
-  int first[kMats + 1];  // prefix of workgroups
+  int first[PHASES][kMats + 1];  // prefixes of workgroups; behind the last matrix: their number
   int count;
 };
-__device__ __forceinline__ int find(const Mats& t, int wg) {
-  int i = 0;
-  while (i + 1 < t.count && wg >= t.first[i + 1]) ++i;
-  return i;
+// the matrix that workgroup `wg` of a phase works on, for all of its waves: lane i compares the end of matrix i
+__device__ __forceinline__ int find(const Mats& t, int phase, int wg) {
+  const int lane = threadIdx.x & 63;
+  return __popcll(__ballot(lane < kMats && wg >= t.first[phase][min(lane, kMats - 1) + 1]));
+}
+// Pointers that were loaded from memory have no address space, and accesses through them would be flat ones, which count as LDS instructions, too
+// (10 % of the products' time): they are cast to global ones.
+#define GLOBAL __attribute__((address_space(1)))
+typedef GLOBAL half_t ghalf_t;
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+template <typename V> __device__ __forceinline__ V gload(const ghalf_t* p) { return *(const GLOBAL V*)p; }
+template <typename V> __device__ __forceinline__ void gstore(ghalf_t* p, V v) { *(GLOBAL V*)p = v; }
+template <typename T> __device__ __forceinline__ float gvalue(const void* p, size_t i) {
+  if constexpr (sizeof(T) == 4) return ((const GLOBAL float*)p)[i];
+  else return bf2f(((const GLOBAL uint16_t*)p)[i]);
+}
+template <typename T> __device__ __forceinline__ void gput(void* p, size_t i, float v) {
+  if constexpr (sizeof(T) == 4) ((GLOBAL float*)p)[i] = v;
+  else ((GLOBAL uint16_t*)p)[i] = f2bf(v);
 }
 __device__ __forceinline__ size_t plane_x(const Mat& a) { return (size_t)a.mp * a.np; }
-__device__ __forceinline__ half_t* x_of(const Mat& a, int which) { return a.ws + (size_t)which * 2 * plane_x(a); }
-__device__ __forceinline__ half_t* g_of(const Mat& a) { return a.ws + 4 * plane_x(a); }
-__device__ __forceinline__ half_t* p_of(const Mat& a) { return g_of(a) + 2 * (size_t)a.mp * a.mp; }
+__device__ __forceinline__ ghalf_t* x_of(const Mat& a, int which) { return (ghalf_t*)a.ws + (size_t)which * 2 * plane_x(a); }
+__device__ __forceinline__ ghalf_t* g_of(const Mat& a) { return (ghalf_t*)a.ws + 4 * plane_x(a); }
+__device__ __forceinline__ ghalf_t* p_of(const Mat& a) { return g_of(a) + 2 * (size_t)a.mp * a.mp; }
 
 __device__ __forceinline__ void split(float v, half_t& hi, half_t& lo) {
   hi = (half_t)v;
@@ -66,14 +84,16 @@ __device__ __forceinline__ void split(float v, half_t& hi, half_t& lo) {
 // -----------------------------------------------------------------------------------------------------------------------------------------
 constexpr int kNormItems = 8192;
 template <typename T, bool MOM> __device__ __forceinline__ float update_of(const Mat& a, size_t i, float mu, int nesterov) {
-  const float g = to_f<T>(reinterpret_cast<const T*>(a.src)[i]);
+  const float g = gvalue<T>(a.src, i);
   if (!MOM) return g;
-  const float m = a.mom[i];
+  const float m = gvalue<float>(a.mom, i);
   return nesterov ? g + mu * m : m;
 }
-template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_norm_kernel(Mats t, float mu, int nesterov) {
+template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_norm_kernel(Mats t, Mats* copy, float mu, int nesterov) {
   __shared__ double sums[4];
-  const int k = find(t, blockIdx.x), chunk = blockIdx.x - t.first[k];
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < (int)(sizeof(Mats) / 4); i += 256) reinterpret_cast<int*>(copy)[i] = reinterpret_cast<const int*>(&t)[i];
+  const int k = find(t, NORM, blockIdx.x), chunk = blockIdx.x - t.first[NORM][k];
   const Mat& a = t.mat[k];
   const size_t size = (size_t)a.m * a.n, i0 = (size_t)chunk * kNormItems, i1 = i0 + kNormItems < size ? i0 + kNormItems : size;
   const T* const src = reinterpret_cast<const T*>(a.src);
@@ -114,10 +134,11 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_norm_k
 // -----------------------------------------------------------------------------------------------------------------------------------------
 // x = u / (|u| + eps), 64 x 64 elements (of the padded matrix) a workgroup; through LDS where the matrix is taller than wide
 // -----------------------------------------------------------------------------------------------------------------------------------------
-template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_kernel(Mats t, float mu, int nesterov, float eps) {
+template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_kernel(const Mats* __restrict__ list, float mu, int nesterov, float eps) {
+  const Mats& t = *list;
   __shared__ float tile[64][65];
   __shared__ double total;
-  const int k = find(t, blockIdx.x), at = blockIdx.x - t.first[k], tid = threadIdx.x;
+  const int k = find(t, SCALE, blockIdx.x), at = blockIdx.x - t.first[SCALE][k], tid = threadIdx.x;
   const Mat& a = t.mat[k];
   const int tn = a.np / 64, i0 = at / tn * 64, j0 = at % tn * 64;
   const bool flip = a.rows > a.cols;  // x[i][j] = u[j][i]
@@ -131,7 +152,7 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_
   if (tid < 64) {
     const int chunks = (int)(((size_t)a.m * a.n + kNormItems - 1) / kNormItems);
     double s = 0.0;
-    for (int c = tid; c < chunks; c += 64) s += a.norm[c];
+    for (int c = tid; c < chunks; c += 64) s += ((const GLOBAL double*)a.norm)[c];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if (tid == 0) total = s;
@@ -143,7 +164,7 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_
   }
   __syncthreads();
   const double inv = (double)kScale / (sqrt(total) + (double)eps);
-  half_t* const x = x_of(a, 0);
+  ghalf_t* const x = x_of(a, 0);
   const size_t plane = plane_x(a);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -157,8 +178,8 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_
       lo[e] = l;
     }
     const size_t o = (size_t)(i0 + r) * a.np + j0 + c;
-    *reinterpret_cast<half4_t*>(x + o) = hi;
-    *reinterpret_cast<half4_t*>(x + plane + o) = lo;
+    gstore(x + o, hi);
+    gstore(x + plane + o, lo);
   }
 }
 
@@ -180,22 +201,22 @@ template <int TILE, int WAVES, bool COLS> struct Product {
   static constexpr size_t BYTES = sizeof(half_t) * 3 * STAGE > sizeof(float) * TILE * OPITCH ? sizeof(half_t) * 3 * STAGE : sizeof(float) * TILE * OPITCH;
   half_t* lds;
   f32x16_t acc[FR][FC];
-  uint4 q[2][4][CH];
+  u32x4_t q[2][4][CH];
   struct Frags {
     half8_t ah[FR], al[FR], bh[FC], bl[FC];
   };
 
   static __device__ __forceinline__ int row0(int tid) { return (tid >> 7) * WR; }
   static __device__ __forceinline__ int col0(int tid) { return ((tid >> 6) & 1) * WC; }
-  template <int S> __device__ __forceinline__ void load(const half_t* a, size_t a_plane, int lda, const half_t* b, size_t b_plane, int ldb, int k0, int tid) {
+  template <int S> __device__ __forceinline__ void load(const ghalf_t* a, size_t a_plane, int lda, const ghalf_t* b, size_t b_plane, int ldb, int k0, int tid) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int idx = tid + c * NT, r = idx / (BK / 8), col = k0 + idx % (BK / 8) * 8;
-      const half_t* pa = COLS ? a + (size_t)(k0 + idx / (TILE / 8)) * lda + idx % (TILE / 8) * 8 : a + (size_t)r * lda + col;
-      q[S][0][c] = *reinterpret_cast<const uint4*>(pa);
-      q[S][1][c] = *reinterpret_cast<const uint4*>(pa + a_plane);
-      q[S][2][c] = *reinterpret_cast<const uint4*>(b + (size_t)r * ldb + col);
-      q[S][3][c] = *reinterpret_cast<const uint4*>(b + b_plane + (size_t)r * ldb + col);
+      const ghalf_t* pa = COLS ? a + (size_t)(k0 + idx / (TILE / 8)) * lda + idx % (TILE / 8) * 8 : a + (size_t)r * lda + col;
+      q[S][0][c] = gload<u32x4_t>(pa);
+      q[S][1][c] = gload<u32x4_t>(pa + a_plane);
+      q[S][2][c] = gload<u32x4_t>(b + (size_t)r * ldb + col);
+      q[S][3][c] = gload<u32x4_t>(b + b_plane + (size_t)r * ldb + col);
     }
   }
   template <int S> __device__ __forceinline__ void store(int stage, int tid) {
@@ -204,10 +225,10 @@ template <int TILE, int WAVES, bool COLS> struct Product {
     for (int c = 0; c < CH; ++c) {
       const int idx = tid + c * NT, rows = idx / (BK / 8) * PITCH + idx % (BK / 8) * 8;
       const int at = COLS ? idx / (TILE / 8) * CPITCH + idx % (TILE / 8) * 8 : rows;
-      *reinterpret_cast<uint4*>(s + at) = q[S][0][c];
-      *reinterpret_cast<uint4*>(s + AELEMS + at) = q[S][1][c];
-      *reinterpret_cast<uint4*>(s + 2 * AELEMS + rows) = q[S][2][c];
-      *reinterpret_cast<uint4*>(s + 2 * AELEMS + BELEMS + rows) = q[S][3][c];
+      *reinterpret_cast<u32x4_t*>(s + at) = q[S][0][c];
+      *reinterpret_cast<u32x4_t*>(s + AELEMS + at) = q[S][1][c];
+      *reinterpret_cast<u32x4_t*>(s + 2 * AELEMS + rows) = q[S][2][c];
+      *reinterpret_cast<u32x4_t*>(s + 2 * AELEMS + BELEMS + rows) = q[S][3][c];
     }
   }
   static __device__ __forceinline__ half8_t row_frag(const half_t* t, int row, int k, int lane) {
@@ -231,7 +252,7 @@ template <int TILE, int WAVES, bool COLS> struct Product {
     });
     __builtin_amdgcn_sched_barrier(0);
   }
-  __device__ __forceinline__ void run(const half_t* a, size_t a_plane, int lda, const half_t* b, size_t b_plane, int ldb, int K, int tid) {
+  __device__ __forceinline__ void run(const ghalf_t* a, size_t a_plane, int lda, const ghalf_t* b, size_t b_plane, int ldb, int K, int tid) {
     const int lane = tid & 63, wr = row0(tid), wc = col0(tid);
     f32x16_t cross[FR][FC];
 #pragma unroll
@@ -375,37 +396,49 @@ __device__ __forceinline__ void triangle_tile(int at, int n, int& i, int& j) {
 }
 
 // G = x x^T (POLY false) or P = b G + c G G (true): tiles (i, j <= i), written to both halves
-template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVES, 2) void ns_sym_kernel(Mats t, int which, float cb, float cc) {
+template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVES, 2) void ns_sym_kernel(const Mats* __restrict__ list, int which, float cb, float cc) {
+  const Mats& t = *list;
   typedef Product<TILE, WAVES, false> Prod;
   __shared__ __attribute__((aligned(16))) char smem[Prod::BYTES];
-  const int block = near_tiles(blockIdx.x, t.first[t.count]), k = find(t, block), tid = threadIdx.x;
-  const Mat& a = t.mat[k];
+  const int block = near_tiles(blockIdx.x, gridDim.x), k = find(t, SYM, block), tid = threadIdx.x;
+  const Mat a = t.mat[k];
   int ti, tj;
-  triangle_tile(block - t.first[k], a.mp / TILE, ti, tj);
+  triangle_tile(block - t.first[SYM][k], a.mp / TILE, ti, tj);
   const int i0 = ti * TILE, j0 = tj * TILE;
   const size_t plane = (size_t)a.mp * a.mp;
-  half_t* const g = g_of(a);
+  ghalf_t* const g = g_of(a);
   Prod p;
   p.lds = reinterpret_cast<half_t*>(smem);
   if (POLY) p.run(g + (size_t)i0 * a.mp, plane, a.mp, g + (size_t)j0 * a.mp, plane, a.mp, a.mp, tid);
   else p.run(x_of(a, which) + (size_t)i0 * a.np, plane_x(a), a.np, x_of(a, which) + (size_t)j0 * a.np, plane_x(a), a.np, a.np, tid);
-  half_t* const out = POLY ? p_of(a) : g;
+  ghalf_t* const out = POLY ? p_of(a) : g;
+  constexpr int PIECES = TILE * TILE / 8 / Prod::NT;
+  half8_t gh[PIECES], gl[PIECES];
+  if (POLY) {
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) {
+      const int idx = tid + q * Prod::NT;
+      const size_t o = (size_t)(j0 + idx / (TILE / 8)) * a.mp + i0 + idx % (TILE / 8) * 8;
+      gh[q] = gload<half8_t>(g + o);
+      gl[q] = gload<half8_t>(g + plane + o);
+    }
+  }
   float* const v = p.spill(tid);  // v[j][i]
-  for (int idx = tid; idx < TILE * TILE / 8; idx += Prod::NT) {
-    const int j = idx / (TILE / 8), i = idx % (TILE / 8) * 8;
+#pragma unroll
+  for (int q = 0; q < PIECES; ++q) {
+    const int idx = tid + q * Prod::NT, j = idx / (TILE / 8), i = idx % (TILE / 8) * 8;
     const size_t o = (size_t)(j0 + j) * a.mp + i0 + i;
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = v[j * Prod::OPITCH + i + e] * (1.f / kScale);
     if (POLY) {
-      const half8_t h = *reinterpret_cast<const half8_t*>(g + o), l = *reinterpret_cast<const half8_t*>(g + plane + o);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = (kScaleP / kScale) * (cc * w[e] + cb * ((float)h[e] + (float)l[e]));
+      for (int e = 0; e < 8; ++e) w[e] = (kScaleP / kScale) * (cc * w[e] + cb * ((float)gh[q][e] + (float)gl[q][e]));
     }
     half8_t hi, lo;
     split8(w, hi, lo);
-    *reinterpret_cast<half8_t*>(out + o) = hi;
-    *reinterpret_cast<half8_t*>(out + plane + o) = lo;
+    gstore(out + o, hi);
+    gstore(out + plane + o, lo);
     if (i0 != j0) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[j * Prod::OPITCH + i + e] = w[e];
@@ -421,39 +454,49 @@ template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVE
     half8_t hi, lo;
     split8(w, hi, lo);
     const size_t o = (size_t)(i0 + i) * a.mp + j0 + j;
-    *reinterpret_cast<half8_t*>(out + o) = hi;
-    *reinterpret_cast<half8_t*>(out + plane + o) = lo;
+    gstore(out + o, hi);
+    gstore(out + plane + o, lo);
   }
 }
 
 // x <- a x + P x; the last one writes the result instead
-template <int TILE, int WAVES, typename T, int LAST> __global__ __launch_bounds__(64 * WAVES, 2) void ns_apply_kernel(Mats t, int which, float ca, const float* __restrict__ hp) {
+template <int TILE, int WAVES, typename T, int LAST> __global__ __launch_bounds__(64 * WAVES, 2) void ns_apply_kernel(const Mats* __restrict__ list, int which, float ca, const float* __restrict__ hp) {
+  const Mats& t = *list;
   typedef Product<TILE, WAVES, true> Prod;
   __shared__ __attribute__((aligned(16))) char smem[Prod::BYTES];
-  const int block = near_tiles(blockIdx.x, t.first[t.count]), k = find(t, block), tid = threadIdx.x;
-  const Mat& a = t.mat[k];
+  const int block = near_tiles(blockIdx.x, gridDim.x), k = find(t, APPLY, block), tid = threadIdx.x;
+  const Mat a = t.mat[k];
   int ti, tj;
-  square_tile(block - t.first[k], a.mp / TILE, a.np / TILE, ti, tj);
+  square_tile(block - t.first[APPLY][k], a.mp / TILE, a.np / TILE, ti, tj);
   const int i0 = ti * TILE, j0 = tj * TILE;
-  const half_t* const x = x_of(a, which);
+  const ghalf_t* const x = x_of(a, which);
   const size_t plane = plane_x(a);
   Prod p;
   p.lds = reinterpret_cast<half_t*>(smem);
   p.run(x + j0, plane, a.np, p_of(a) + (size_t)i0 * a.mp, (size_t)a.mp * a.mp, a.mp, a.mp, tid);
+  constexpr int PIECES = TILE * TILE / 8 / Prod::NT;
+  half8_t xh[PIECES], xl[PIECES];
+#pragma unroll
+  for (int q = 0; q < PIECES; ++q) {
+    const int idx = tid + q * Prod::NT;
+    const size_t o = (size_t)(i0 + idx / (TILE / 8)) * a.np + j0 + idx % (TILE / 8) * 8;
+    xh[q] = gload<half8_t>(x + o);
+    xl[q] = gload<half8_t>(x + plane + o);
+  }
   float* const v = p.spill(tid);  // v[i][j]
-  half_t* const next = x_of(a, which ^ 1);
-  for (int idx = tid; idx < TILE * TILE / 8; idx += Prod::NT) {
-    const int i = idx / (TILE / 8), j = idx % (TILE / 8) * 8;
+  ghalf_t* const next = x_of(a, which ^ 1);
+#pragma unroll
+  for (int q = 0; q < PIECES; ++q) {
+    const int idx = tid + q * Prod::NT, i = idx / (TILE / 8), j = idx % (TILE / 8) * 8;
     const size_t o = (size_t)(i0 + i) * a.np + j0 + j;
-    const half8_t h = *reinterpret_cast<const half8_t*>(x + o), l = *reinterpret_cast<const half8_t*>(x + plane + o);
     float w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = fmaf(ca, (float)h[e] + (float)l[e], v[i * Prod::OPITCH + j + e] * (1.f / kScaleP));
+    for (int e = 0; e < 8; ++e) w[e] = fmaf(ca, (float)xh[q][e] + (float)xl[q][e], v[i * Prod::OPITCH + j + e] * (1.f / kScaleP));
     if (LAST == 0) {
       half8_t hi, lo;
       split8(w, hi, lo);
-      *reinterpret_cast<half8_t*>(next + o) = hi;
-      *reinterpret_cast<half8_t*>(next + plane + o) = lo;
+      gstore(next + o, hi);
+      gstore(next + plane + o, lo);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i * Prod::OPITCH + j + e] = w[e] * (1.f / kScale);
@@ -473,15 +516,15 @@ template <int TILE, int WAVES, typename T, int LAST> __global__ __launch_bounds_
       const int idx = base + q * Prod::NT, slow = idx / TILE, fast = idx % TILE, i = flip ? fast : slow, j = flip ? slow : fast;
       in[q] = i0 + i < a.m && j0 + j < a.n;
       o[q] = in[q] ? (flip ? (size_t)(j0 + j) * a.cols + i0 + i : (size_t)(i0 + i) * a.cols + j0 + j) : 0;
-      if (LAST == 2) old[q] = a.par[o[q]];
+      if (LAST == 2) old[q] = gvalue<float>(a.par, o[q]);
     }
 #pragma unroll
     for (int q = 0; q < IN_FLIGHT; ++q) {
       const int idx = base + q * Prod::NT, slow = idx / TILE, fast = idx % TILE;
       const float y = flip ? v[fast * Prod::OPITCH + slow] : v[slow * Prod::OPITCH + fast];
       if (!in[q]) continue;
-      if (LAST == 1) reinterpret_cast<T*>(a.dst)[o[q]] = from_f<T>(y);
-      else a.par[o[q]] = old[q] * keep - step * y;
+      if (LAST == 1) gput<T>(a.dst, o[q], y);
+      else gput<float>(a.par, o[q], old[q] * keep - step * y);
     }
   }
 }
@@ -495,10 +538,14 @@ long long bytes_of(const cvh_ns_matrix& a) {
   return (4 * mp * np + 4 * mp * mp) * 2 + (chunks * 8 + 255) / 256 * 256;
 }
 
-template <typename F> int prefix(Mats& t, F&& groups) {
-  t.first[0] = 0;
-  for (int i = 0; i < t.count; ++i) t.first[i + 1] = t.first[i] + groups(t.mat[i]);
-  return t.first[t.count];
+constexpr long long kListBytes = (sizeof(Mats) + 255) / 256 * 256;
+template <typename F> int prefix(Mats& t, int phase, F&& groups) {
+  int n = 0;
+  for (int i = 0; i <= kMats; ++i) {
+    t.first[phase][i] = i <= t.count ? n : 0x7fffffff;
+    if (i < t.count) n += groups(t.mat[i]);
+  }
+  return n;
 }
 // 128-wide tiles where the list has enough of them for the card (and every side takes them), else 64-wide ones
 template <typename F> bool wide_tiles(const Mats& t, F&& tiles) {
@@ -512,31 +559,31 @@ template <typename F> bool wide_tiles(const Mats& t, F&& tiles) {
 template <int TILE> int sym_tiles(const Mat& q) { return q.mp / TILE * (q.mp / TILE + 1) / 2; }
 template <int TILE> int all_tiles(const Mat& q) { return q.mp / TILE * (q.np / TILE); }
 
-template <int TILE, int WAVES> void run_sym(Mats t, int which, float b, float c, hipStream_t st) {
-  const dim3 grid(prefix(t, sym_tiles<TILE>)), wg(64 * WAVES);
-  ns_sym_kernel<TILE, WAVES, false><<<grid, wg, 0, st>>>(t, which, b, c);
-  ns_sym_kernel<TILE, WAVES, true><<<grid, wg, 0, st>>>(t, which, b, c);
+template <int TILE, int WAVES> void run_sym(const Mats* list, int n, int which, float b, float c, hipStream_t st) {
+  ns_sym_kernel<TILE, WAVES, false><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, which, b, c);
+  ns_sym_kernel<TILE, WAVES, true><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, which, b, c);
 }
-template <int TILE, int WAVES, typename T, int LAST> void run_apply(Mats t, int which, float a, const float* hp, hipStream_t st) {
-  const dim3 grid(prefix(t, all_tiles<TILE>)), wg(64 * WAVES);
-  ns_apply_kernel<TILE, WAVES, T, LAST><<<grid, wg, 0, st>>>(t, which, a, hp);
+template <int TILE, int WAVES, typename T, int LAST> void run_apply(const Mats* list, int n, int which, float a, const float* hp, hipStream_t st) {
+  ns_apply_kernel<TILE, WAVES, T, LAST><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, which, a, hp);
 }
-template <typename T, bool MOM> int run_list(Mats& t, int steps, float a, float b, float c, float eps, float mu, int nesterov, const float* hp, hipStream_t st) {
-  int n = prefix(t, [](const Mat& q) { return (int)(((long long)q.m * q.n + kNormItems - 1) / kNormItems); });
-  ns_norm_kernel<T, MOM><<<dim3(n), dim3(256), 0, st>>>(t, mu, nesterov);
-  n = prefix(t, all_tiles<64>);
-  ns_scale_kernel<T, MOM><<<dim3(n), dim3(256), 0, st>>>(t, mu, nesterov, eps);
+template <typename T, bool MOM> int run_list(Mats& t, Mats* list, int steps, float a, float b, float c, float eps, float mu, int nesterov, const float* hp, hipStream_t st) {
   const bool ws = wide_tiles(t, sym_tiles<128>), wa = wide_tiles(t, all_tiles<128>);
+  const int norms = prefix(t, NORM, [](const Mat& q) { return (int)(((long long)q.m * q.n + kNormItems - 1) / kNormItems); });
+  const int scales = prefix(t, SCALE, all_tiles<64>);
+  const int syms = ws ? prefix(t, SYM, sym_tiles<128>) : prefix(t, SYM, sym_tiles<64>);
+  const int applies = wa ? prefix(t, APPLY, all_tiles<128>) : prefix(t, APPLY, all_tiles<64>);
+  ns_norm_kernel<T, MOM><<<dim3(norms), dim3(256), 0, st>>>(t, list, mu, nesterov);
+  ns_scale_kernel<T, MOM><<<dim3(scales), dim3(256), 0, st>>>(list, mu, nesterov, eps);
   constexpr int LAST = MOM ? 2 : 1;
   for (int s = 0; s < steps; ++s) {
-    if (ws) run_sym<128, 8>(t, s & 1, b, c, st);
-    else run_sym<64, 4>(t, s & 1, b, c, st);
+    if (ws) run_sym<128, 8>(list, syms, s & 1, b, c, st);
+    else run_sym<64, 4>(list, syms, s & 1, b, c, st);
     if (s + 1 < steps) {
-      if (wa) run_apply<128, 8, T, 0>(t, s & 1, a, hp, st);
-      else run_apply<64, 4, T, 0>(t, s & 1, a, hp, st);
+      if (wa) run_apply<128, 8, T, 0>(list, applies, s & 1, a, hp, st);
+      else run_apply<64, 4, T, 0>(list, applies, s & 1, a, hp, st);
     } else {
-      if (wa) run_apply<128, 8, T, LAST>(t, s & 1, a, hp, st);
-      else run_apply<64, 4, T, LAST>(t, s & 1, a, hp, st);
+      if (wa) run_apply<128, 8, T, LAST>(list, applies, s & 1, a, hp, st);
+      else run_apply<64, 4, T, LAST>(list, applies, s & 1, a, hp, st);
     }
   }
   CVH_CHECK_LAUNCH();
@@ -547,7 +594,9 @@ template <typename T, bool MOM>
 int run_all(const cvh_ns_matrix* mats, int n, int steps, float a, float b, float c, float eps, float mu, int nesterov, const float* hp, void* ws, hipStream_t st) {
   char* at = reinterpret_cast<char*>(ws);
   for (int i0 = 0; i0 < n; i0 += kMats) {
-    Mats t;
+    Mats t = {};
+    Mats* const list = reinterpret_cast<Mats*>(at);
+    at += kListBytes;
     t.count = n - i0 < kMats ? n - i0 : kMats;
     for (int i = 0; i < t.count; ++i) {
       const cvh_ns_matrix& q = mats[i0 + i];
@@ -562,7 +611,7 @@ int run_all(const cvh_ns_matrix* mats, int n, int steps, float a, float b, float
       d.norm = reinterpret_cast<double*>(at + (4ll * d.mp * d.np + 4ll * d.mp * d.mp) * 2);
       at += bytes_of(q);
     }
-    const int rc = run_list<T, MOM>(t, steps, a, b, c, eps, mu, nesterov, hp, st);
+    const int rc = run_list<T, MOM>(t, list, steps, a, b, c, eps, mu, nesterov, hp, st);
     if (rc) return rc;
   }
   return 0;
@@ -582,7 +631,7 @@ int check(const cvh_ns_matrix* mats, int n, int steps, float a, float b, float c
 
 extern "C" long long cvh_ns_workspace_elems(const cvh_ns_matrix* mats, int n) {
   if (mats == nullptr || n <= 0) return -2;
-  long long bytes = 0;
+  long long bytes = (n + kMats - 1) / kMats * kListBytes;
   for (int i = 0; i < n; ++i) bytes += bytes_of(mats[i]);
   return (bytes + 3) / 4;
 }
