@@ -13,7 +13,7 @@
 
 namespace {
 
-constexpr int kItems = 2048;   // rows a sort workgroup takes: 4 waves x 8 rounds x 64 lanes
+constexpr int kItems = 1024;   // rows a sort workgroup takes: 4 waves x 4 rounds x 64 lanes
 constexpr int kChunk = 32;     // sorted rows that are summed by one group of lanes
 constexpr int kTableRows = 32;  // rows of the table a workgroup writes
 
@@ -70,10 +70,16 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(SortIn s, const int* 
   if (gridDim.x == 1) {
     total = at[0][tid] + at[1][tid] + at[2][tid] + at[3][tid];
   } else {
-    for (int b = 0; b < (int)gridDim.x; ++b) {
-      const int v = count[b * 256 + tid];
-      before += b < (int)blockIdx.x ? v : 0;
-      total += v;
+    for (int b0 = 0; b0 < (int)gridDim.x; b0 += 16) {
+      int v[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = count[min(b0 + j, (int)gridDim.x - 1) * 256 + tid];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int b = b0 + j, n = b < (int)gridDim.x ? v[j] : 0;
+        before += b < (int)blockIdx.x ? n : 0;
+        total += n;
+      }
     }
   }
   scan[tid] = total;
@@ -275,6 +281,7 @@ __global__ __launch_bounds__(256) void embed_join_kernel(Grad g, int chunks) {
     const int t = blockIdx.x - chunks, positions = g.pos_blocks / g.pos_split;
     for (int c = tid; c < g.e; c += 256) {
       float s = 0.f;
+#pragma unroll 8
       for (int q = 0; q < g.pos_split; ++q) s += g.pos_part[((size_t)q * positions + t) * g.e + c];
       g.dpos[(size_t)t * g.e + c] = s;
     }
@@ -314,11 +321,11 @@ __global__ __launch_bounds__(256) void embed_join_kernel(Grad g, int chunks) {
   }
 }
 
-// forward: a workgroup takes one item of the layout's work list (or, without a layout, 32 consecutive rows); 8 columns a thread
+// forward: a workgroup takes `share` rows of one item of the layout's work list (or, without a layout, of 32 consecutive rows); 8 columns a thread
 template <typename T>
 __global__ __launch_bounds__(256) void embed_packed_fwd_kernel(const long long* __restrict__ ids, const float* __restrict__ table, const float* __restrict__ pos,
-                                                               const int* __restrict__ plan, int seqs, int block, int rows, int vocab, int positions, int e,
-                                                               float scale, T* __restrict__ out) {
+                                                               const int* __restrict__ plan, int seqs, int block, int share, int rows, int vocab, int positions,
+                                                               int e, float scale, T* __restrict__ out) {
   int start = 0, len = rows, first = blockIdx.x * block, seq = 0;
   if (plan != nullptr) {
     const int* list = plan + ((seqs + 2) & ~1);
@@ -328,7 +335,8 @@ __global__ __launch_bounds__(256) void embed_packed_fwd_kernel(const long long* 
     start = plan[seq >= 0 ? seq : seqs];
     len = (seq >= 0 ? plan[seq + 1] : rows) - start;
   }
-  const int groups = e / 8, count = min(block, len - first);
+  first += blockIdx.y * share;
+  const int groups = e / 8, count = min(share, len - first);
   for (int i = threadIdx.x; i < count * groups; i += 256) {
     const int r = i / groups, c = (i - r * groups) * 8, place = first + r;
     const size_t row = (size_t)start + place;
@@ -389,10 +397,13 @@ extern "C" int cvh_embed_packed_fwd(int dtype, const long long* ids, const float
     places = (rows + block - 1) / block;
   }
   hipStream_t st = (hipStream_t)stream;
+  int share = block;  // about 2048 pieces of 8 columns a workgroup: 25 k rows of 768 in 128-row items are 232 workgroups otherwise, fewer than CUs
+  while (share > 8 && share * (e / 8) > 2048) share /= 2;
+  const dim3 grid(places, block / share);
   if (dtype == CVH_DT_BF16)
-    hipLaunchKernelGGL(embed_packed_fwd_kernel<bf16_t>, dim3(places), dim3(256), 0, st, ids, table, pos, plan, seqs, block, rows, vocab, positions, e, scale, (bf16_t*)out);
+    hipLaunchKernelGGL(embed_packed_fwd_kernel<bf16_t>, grid, dim3(256), 0, st, ids, table, pos, plan, seqs, block, share, rows, vocab, positions, e, scale, (bf16_t*)out);
   else
-    hipLaunchKernelGGL(embed_packed_fwd_kernel<float>, dim3(places), dim3(256), 0, st, ids, table, pos, plan, seqs, block, rows, vocab, positions, e, scale, (float*)out);
+    hipLaunchKernelGGL(embed_packed_fwd_kernel<float>, grid, dim3(256), 0, st, ids, table, pos, plan, seqs, block, share, rows, vocab, positions, e, scale, (float*)out);
   CVH_CHECK_LAUNCH();
   return 0;
 }

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_double, c_float, c_int, c_longlong, c_uint, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -169,6 +170,7 @@ class PackedAttn(ctypes.Structure):
     _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "out", "out_lo", "dout", "dq", "dk", "dv", "lse", "delta", "plan")]
                 + [(n + s, c_longlong) for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for s in ("_row", "_head")]
                 + [(n, c_int) for n in ("rows", "seqs", "heads_q", "heads_kv", "d", "causal", "block", "places")] + [("scale", c_float)])
+    PACK = struct.Struct("@12P16q8if4x").pack  # the same as bytes, which ctypes hands on as a pointer: a third of the time of filling the structure
 
 
 class NsMatrix(ctypes.Structure):

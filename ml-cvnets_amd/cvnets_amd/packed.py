@@ -5,7 +5,6 @@ padded to the longest (the text tower pads captions of 5 .. 77 tokens to its con
 Rows behind the last sequence (a buffer larger than its sequences) are read by nothing and come back as zeros."""
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Sequence
 
 import torch
@@ -77,15 +76,13 @@ def _loadable(t: Tensor) -> Tensor:
     return t if ok else t.contiguous() if not t.is_contiguous() else t.clone()
 
 
-def _layout(t: Optional[Tensor]):
-    return (0, 0) if t is None else (t.stride(0), t.stride(1))
-
-
 def _launch(name: str, seqs: PackedSeqs, scale: float, causal: bool, q, k, v, out, out_lo, lse, delta=None, dout=None, dq=None, dk=None, dv=None) -> None:
-    a = _lib.PackedAttn(_p(q), _p(k), _p(v), _p(out), _p(out_lo), _p(dout), _p(dq), _p(dk), _p(dv), _p(lse), _p(delta), seqs.plan.data_ptr(),
-                        *_layout(q), *_layout(k), *_layout(v), *_layout(out), *_layout(dout), *_layout(dq), *_layout(dk), *_layout(dv),
-                        seqs.rows, seqs.seqs, q.shape[1], k.shape[1], q.shape[2], int(causal), seqs.block, seqs.places, scale)
-    call_on(q.device, name, _dt(q), ctypes.byref(a))
+    grads = (0, 0) * 4 if dout is None else (*dout.stride()[:2], *dq.stride()[:2], *dk.stride()[:2], *dv.stride()[:2])
+    rows, heads, d = q.shape
+    call_on(q.device, name, _dt(q), _lib.PackedAttn.PACK(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _p(out_lo) or 0, _p(dout) or 0, _p(dq) or 0, _p(dk) or 0, _p(dv) or 0, _p(lse) or 0, _p(delta) or 0,
+        seqs.plan.data_ptr(), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2], *grads, rows, seqs.seqs, heads, k.shape[1], d, causal, seqs.block,
+        seqs.places, scale))
 
 
 def _forward(q: Tensor, k: Tensor, v: Tensor, seqs: PackedSeqs, causal: bool, scale: float, grad: bool):

@@ -134,3 +134,11 @@ def test_packed_captions_need_the_causal_mask():
         tower.encode_packed(torch.zeros(5, dtype=torch.int64), layout(5))
     with pytest.raises(RuntimeError):
         tower.pack_captions(torch.zeros(5, dtype=torch.int64))
+
+
+def test_the_packed_bytes_are_the_structure():
+    values = list(range(1, 13)) + list(range(2 ** 40, 2 ** 40 + 16)) + list(range(200, 208)) + [0.5]
+    data = _lib.PackedAttn.PACK(*values)
+    assert len(data) == ctypes.sizeof(_lib.PackedAttn)
+    a = _lib.PackedAttn.from_buffer_copy(data)
+    assert [getattr(a, name) for name, _ in a._fields_] == values
