@@ -36,7 +36,7 @@ struct Mat {
   const void* src;  // u, or the gradient (float32)
   void* dst;        // result (orthogonalize)
   float *mom, *par;
-  half_t* ws;       // x [2][mp][np] twice (ping-pong), G [2][mp][mp], P [2][mp][mp]; hi and lo planes
+  half_t* ws;       // x [mp][2 np] twice (ping-pong), G [mp][2 mp], P [mp][2 mp]; see place()
   double* norm;     // partial sums of squares
   int m, n, mp, np, rows, cols, group;
   float gain;
@@ -73,6 +73,11 @@ __device__ __forceinline__ size_t plane_x(const Mat& a) { return (size_t)a.mp * 
 __device__ __forceinline__ ghalf_t* x_of(const Mat& a, int which) { return (ghalf_t*)a.ws + (size_t)which * 2 * plane_x(a); }
 __device__ __forceinline__ ghalf_t* g_of(const Mat& a) { return (ghalf_t*)a.ws + 4 * plane_x(a); }
 __device__ __forceinline__ ghalf_t* p_of(const Mat& a) { return g_of(a) + 2 * (size_t)a.mp * a.mp; }
+
+// A row of pairs is in blocks of 32 columns, 32 hi and then their 32 lo: one 128-byte line.  A step of 32 columns of the products reads whole lines;
+// with the two halves in matrices of their own it reads half lines, each of them twice.  place(): of the hi of 8 columns; lo is kLo behind it.
+constexpr int kLo = 32;
+__device__ __forceinline__ size_t place(int row, int col, int ld) { return (size_t)row * 2 * ld + (col >> 5) * 64 + (col & 31); }
 
 __device__ __forceinline__ void split(float v, half_t& hi, half_t& lo) {
   hi = (half_t)v;
@@ -165,7 +170,6 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_
   __syncthreads();
   const double inv = (double)kScale / (sqrt(total) + (double)eps);
   ghalf_t* const x = x_of(a, 0);
-  const size_t plane = plane_x(a);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int r = q * 16 + (tid >> 4), c = (tid & 15) * 4;
@@ -177,9 +181,9 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_
       hi[e] = h;
       lo[e] = l;
     }
-    const size_t o = (size_t)(i0 + r) * a.np + j0 + c;
+    const size_t o = place(i0 + r, j0 + c, a.np);
     gstore(x + o, hi);
-    gstore(x + plane + o, lo);
+    gstore(x + o + kLo, lo);
   }
 }
 
@@ -194,41 +198,37 @@ template <int TILE, int WAVES, bool COLS> struct Product {
   static constexpr int NT = 64 * WAVES, BK = 32, PITCH = BK + 8;  // rows of 80 bytes: 16 lanes' 16-byte reads hit distinct banks
   static constexpr int WR = TILE * 2 / WAVES, WC = TILE / 2;  // rows and columns of a wave
   static constexpr int FR = WR / 32, FC = WC / 32;            // 32-wide fragments of them
-  static constexpr int CH = TILE * (BK / 8) / NT;             // 16-byte pieces a thread loads of each plane
+  static constexpr int CH = 2 * TILE * (BK / 8) / NT;         // 16-byte pieces a thread loads of each operand
   static constexpr int CPITCH = TILE + 16;                    // [k][r] rows: 4 rows of a transpose read on distinct banks
   static constexpr int AELEMS = COLS ? BK * CPITCH : TILE * PITCH, BELEMS = TILE * PITCH, STAGE = 2 * AELEMS + 2 * BELEMS;
   static constexpr int OPITCH = TILE + 4;                     // of the float tile of the epilogue
   static constexpr size_t BYTES = sizeof(half_t) * 3 * STAGE > sizeof(float) * TILE * OPITCH ? sizeof(half_t) * 3 * STAGE : sizeof(float) * TILE * OPITCH;
   half_t* lds;
   f32x16_t acc[FR][FC];
-  u32x4_t q[2][4][CH];
+  u32x4_t q[2][2][CH];
   struct Frags {
     half8_t ah[FR], al[FR], bh[FC], bl[FC];
   };
 
   static __device__ __forceinline__ int row0(int tid) { return (tid >> 7) * WR; }
   static __device__ __forceinline__ int col0(int tid) { return ((tid >> 6) & 1) * WC; }
-  template <int S> __device__ __forceinline__ void load(const ghalf_t* a, size_t a_plane, int lda, const ghalf_t* b, size_t b_plane, int ldb, int k0, int tid) {
+  // pieces of 16 bytes, in the order of the global lines: row r = 4 hi and 4 lo pieces (COLS: row k = TILE / 4 pieces)
+  template <int S> __device__ __forceinline__ void load(const ghalf_t* a, int lda, const ghalf_t* b, int ldb, int k0, int tid) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int idx = tid + c * NT, r = idx / (BK / 8), col = k0 + idx % (BK / 8) * 8;
-      const ghalf_t* pa = COLS ? a + (size_t)(k0 + idx / (TILE / 8)) * lda + idx % (TILE / 8) * 8 : a + (size_t)r * lda + col;
-      q[S][0][c] = gload<u32x4_t>(pa);
-      q[S][1][c] = gload<u32x4_t>(pa + a_plane);
-      q[S][2][c] = gload<u32x4_t>(b + (size_t)r * ldb + col);
-      q[S][3][c] = gload<u32x4_t>(b + b_plane + (size_t)r * ldb + col);
+      const int idx = tid + c * NT, r = idx >> 3, in = (idx & 7) * 8;
+      q[S][0][c] = gload<u32x4_t>(COLS ? a + (size_t)(k0 + idx / (TILE / 4)) * 2 * lda + idx % (TILE / 4) * 8 : a + (size_t)r * 2 * lda + k0 * 2 + in);
+      q[S][1][c] = gload<u32x4_t>(b + (size_t)r * 2 * ldb + k0 * 2 + in);
     }
   }
   template <int S> __device__ __forceinline__ void store(int stage, int tid) {
     half_t* const s = lds + stage * STAGE;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int idx = tid + c * NT, rows = idx / (BK / 8) * PITCH + idx % (BK / 8) * 8;
-      const int at = COLS ? idx / (TILE / 8) * CPITCH + idx % (TILE / 8) * 8 : rows;
-      *reinterpret_cast<u32x4_t*>(s + at) = q[S][0][c];
-      *reinterpret_cast<u32x4_t*>(s + AELEMS + at) = q[S][1][c];
-      *reinterpret_cast<u32x4_t*>(s + 2 * AELEMS + rows) = q[S][2][c];
-      *reinterpret_cast<u32x4_t*>(s + 2 * AELEMS + BELEMS + rows) = q[S][3][c];
+      const int idx = tid + c * NT, lo = (idx >> 2) & 1, rows = (idx >> 3) * PITCH + (idx & 3) * 8, in = idx % (TILE / 4);
+      const int at = COLS ? idx / (TILE / 4) * CPITCH + (in >> 3) * 32 + (idx & 3) * 8 : rows;
+      *reinterpret_cast<u32x4_t*>(s + lo * AELEMS + at) = q[S][0][c];
+      *reinterpret_cast<u32x4_t*>(s + 2 * AELEMS + lo * BELEMS + rows) = q[S][1][c];
     }
   }
   static __device__ __forceinline__ half8_t row_frag(const half_t* t, int row, int k, int lane) {
@@ -243,7 +243,7 @@ template <int TILE, int WAVES, bool COLS> struct Product {
   }
   // order of the instructions since the last call: LDS reads, and the four instructions of class OTHER (LDS writes 0x200, global loads 0x020), between the MFMAs
   template <int OTHER> static __device__ __forceinline__ void interleave() {
-    constexpr int MFMAS = 3 * FR * FC, READS = (COLS ? 4 : 2) * FR + 2 * FC, OTHERS = 4 * CH;
+    constexpr int MFMAS = 3 * FR * FC, READS = (COLS ? 4 : 2) * FR + 2 * FC, OTHERS = 2 * CH;
     static_for<0, MFMAS>([](auto i) {
       constexpr int r = (i + 1) * READS / MFMAS - i * READS / MFMAS, o = (i + 1) * OTHERS / MFMAS - i * OTHERS / MFMAS;
       if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
@@ -252,7 +252,7 @@ template <int TILE, int WAVES, bool COLS> struct Product {
     });
     __builtin_amdgcn_sched_barrier(0);
   }
-  __device__ __forceinline__ void run(const ghalf_t* a, size_t a_plane, int lda, const ghalf_t* b, size_t b_plane, int ldb, int K, int tid) {
+  __device__ __forceinline__ void run(const ghalf_t* a, int lda, const ghalf_t* b, int ldb, int K, int tid) {
     const int lane = tid & 63, wr = row0(tid), wc = col0(tid);
     f32x16_t cross[FR][FC];
 #pragma unroll
@@ -260,7 +260,7 @@ template <int TILE, int WAVES, bool COLS> struct Product {
 #pragma unroll
       for (int j = 0; j < FC; ++j) acc[i][j] = cross[i][j] = acc_zero();
     const int steps = K / BK;
-    auto request = [&](auto set, int t) { this->template load<decltype(set)::value>(a, a_plane, lda, b, b_plane, ldb, t * BK, tid); };
+    auto request = [&](auto set, int t) { this->template load<decltype(set)::value>(a, lda, b, ldb, t * BK, tid); };
     auto read = [&](int stage, int k) {
       const half_t* const st = lds + stage * STAGE;
       Frags f;
@@ -405,12 +405,11 @@ template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVE
   int ti, tj;
   triangle_tile(block - t.first[SYM][k], a.mp / TILE, ti, tj);
   const int i0 = ti * TILE, j0 = tj * TILE;
-  const size_t plane = (size_t)a.mp * a.mp;
   ghalf_t* const g = g_of(a);
   Prod p;
   p.lds = reinterpret_cast<half_t*>(smem);
-  if (POLY) p.run(g + (size_t)i0 * a.mp, plane, a.mp, g + (size_t)j0 * a.mp, plane, a.mp, a.mp, tid);
-  else p.run(x_of(a, which) + (size_t)i0 * a.np, plane_x(a), a.np, x_of(a, which) + (size_t)j0 * a.np, plane_x(a), a.np, a.np, tid);
+  if (POLY) p.run(g + place(i0, 0, a.mp), a.mp, g + place(j0, 0, a.mp), a.mp, a.mp, tid);
+  else p.run(x_of(a, which) + place(i0, 0, a.np), a.np, x_of(a, which) + place(j0, 0, a.np), a.np, a.np, tid);
   ghalf_t* const out = POLY ? p_of(a) : g;
   constexpr int PIECES = TILE * TILE / 8 / Prod::NT;
   half8_t gh[PIECES], gl[PIECES];
@@ -418,16 +417,16 @@ template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVE
 #pragma unroll
     for (int q = 0; q < PIECES; ++q) {
       const int idx = tid + q * Prod::NT;
-      const size_t o = (size_t)(j0 + idx / (TILE / 8)) * a.mp + i0 + idx % (TILE / 8) * 8;
+      const size_t o = place(j0 + idx / (TILE / 8), i0 + idx % (TILE / 8) * 8, a.mp);
       gh[q] = gload<half8_t>(g + o);
-      gl[q] = gload<half8_t>(g + plane + o);
+      gl[q] = gload<half8_t>(g + o + kLo);
     }
   }
   float* const v = p.spill(tid);  // v[j][i]
 #pragma unroll
   for (int q = 0; q < PIECES; ++q) {
     const int idx = tid + q * Prod::NT, j = idx / (TILE / 8), i = idx % (TILE / 8) * 8;
-    const size_t o = (size_t)(j0 + j) * a.mp + i0 + i;
+    const size_t o = place(j0 + j, i0 + i, a.mp);
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = v[j * Prod::OPITCH + i + e] * (1.f / kScale);
@@ -438,7 +437,7 @@ template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVE
     half8_t hi, lo;
     split8(w, hi, lo);
     gstore(out + o, hi);
-    gstore(out + plane + o, lo);
+    gstore(out + o + kLo, lo);
     if (i0 != j0) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[j * Prod::OPITCH + i + e] = w[e];
@@ -453,9 +452,9 @@ template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVE
     for (int e = 0; e < 8; ++e) w[e] = v[(j + e) * Prod::OPITCH + i];
     half8_t hi, lo;
     split8(w, hi, lo);
-    const size_t o = (size_t)(i0 + i) * a.mp + j0 + j;
+    const size_t o = place(i0 + i, j0 + j, a.mp);
     gstore(out + o, hi);
-    gstore(out + plane + o, lo);
+    gstore(out + o + kLo, lo);
   }
 }
 
@@ -470,25 +469,24 @@ template <int TILE, int WAVES, typename T, int LAST> __global__ __launch_bounds_
   square_tile(block - t.first[APPLY][k], a.mp / TILE, a.np / TILE, ti, tj);
   const int i0 = ti * TILE, j0 = tj * TILE;
   const ghalf_t* const x = x_of(a, which);
-  const size_t plane = plane_x(a);
   Prod p;
   p.lds = reinterpret_cast<half_t*>(smem);
-  p.run(x + j0, plane, a.np, p_of(a) + (size_t)i0 * a.mp, (size_t)a.mp * a.mp, a.mp, a.mp, tid);
+  p.run(x + place(0, j0, a.np), a.np, p_of(a) + place(i0, 0, a.mp), a.mp, a.mp, tid);
   constexpr int PIECES = TILE * TILE / 8 / Prod::NT;
   half8_t xh[PIECES], xl[PIECES];
 #pragma unroll
   for (int q = 0; q < PIECES; ++q) {
     const int idx = tid + q * Prod::NT;
-    const size_t o = (size_t)(i0 + idx / (TILE / 8)) * a.np + j0 + idx % (TILE / 8) * 8;
+    const size_t o = place(i0 + idx / (TILE / 8), j0 + idx % (TILE / 8) * 8, a.np);
     xh[q] = gload<half8_t>(x + o);
-    xl[q] = gload<half8_t>(x + plane + o);
+    xl[q] = gload<half8_t>(x + o + kLo);
   }
   float* const v = p.spill(tid);  // v[i][j]
   ghalf_t* const next = x_of(a, which ^ 1);
 #pragma unroll
   for (int q = 0; q < PIECES; ++q) {
     const int idx = tid + q * Prod::NT, i = idx / (TILE / 8), j = idx % (TILE / 8) * 8;
-    const size_t o = (size_t)(i0 + i) * a.np + j0 + j;
+    const size_t o = place(i0 + i, j0 + j, a.np);
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = fmaf(ca, (float)xh[q][e] + (float)xl[q][e], v[i * Prod::OPITCH + j + e] * (1.f / kScaleP));
@@ -496,7 +494,7 @@ template <int TILE, int WAVES, typename T, int LAST> __global__ __launch_bounds_
       half8_t hi, lo;
       split8(w, hi, lo);
       gstore(next + o, hi);
-      gstore(next + plane + o, lo);
+      gstore(next + o + kLo, lo);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i * Prod::OPITCH + j + e] = w[e] * (1.f / kScale);
