@@ -717,6 +717,7 @@ template <typename T> int run_type(const PA& p, int backward, hipStream_t st) {
   }
 }
 
+constexpr int kMostRows = 0x7fffffff - 4096;  // and sequences: blocks are counted in 32 bits
 bool strides_ok(int dtype, const void* base, long long row, long long head) {
   const long long n = dtype == CVH_DT_BF16 ? 8 : 4;  // 16-byte accesses
   return base != nullptr && (reinterpret_cast<uintptr_t>(base) & 15) == 0 && row % n == 0 && head % n == 0 && row >= 0 && head >= 0 && row <= (1 << 21);  // (128 rows in 31 bits of bytes)
@@ -724,9 +725,9 @@ bool strides_ok(int dtype, const void* base, long long row, long long head) {
 int check(int dtype, const PA* p, int backward) {
   if (dtype != CVH_DT_F32 && dtype != CVH_DT_BF16) return -1;
   if (p == nullptr || p->plan == nullptr) return -2;
-  if (p->rows <= 0 || p->seqs <= 0 || p->heads_q <= 0 || p->heads_kv <= 0 || p->heads_q % p->heads_kv || p->d <= 0 || p->d > 128 || p->d % 8) return -2;
+  if (p->rows <= 0 || p->rows > kMostRows || p->seqs <= 0 || p->seqs > kMostRows || p->heads_q <= 0 || p->heads_kv <= 0 || p->heads_q % p->heads_kv || p->d <= 0 || p->d > 128 || p->d % 8) return -2;
   if (!(p->scale > 0.f) || (p->block != 32 && p->block != 128)) return -2;
-  if (p->places != p->rows / p->block + p->seqs + 1 || (long long)p->places * p->heads_q > 0x7fffffffll) return -2;
+  if (p->places != p->rows / p->block + p->seqs + 1 || (long long)p->places * p->heads_q >= (1 << 24)) return -2;  // (a grid has fewer than 2^32 threads)
   if (!strides_ok(dtype, p->q, p->q_row, p->q_head) || !strides_ok(dtype, p->k, p->k_row, p->k_head) || !strides_ok(dtype, p->v, p->v_row, p->v_head) ||
       !strides_ok(dtype, p->out, p->o_row, p->o_head))
     return -2;
@@ -740,11 +741,11 @@ int check(int dtype, const PA* p, int backward) {
 }  // namespace
 
 extern "C" long long cvh_packed_plan_elems(int seqs, int rows, int block) {
-  if (seqs <= 0 || rows <= 0 || (block != 32 && block != 128)) return -2;
+  if (seqs <= 0 || seqs > kMostRows || rows <= 0 || rows > kMostRows || (block != 32 && block != 128)) return -2;
   return ((long long)(seqs + 2) & ~1ll) + 2 * ((long long)rows / block + seqs + 1);
 }
 extern "C" int cvh_packed_plan(const int* cu, int seqs, int rows, int block, int* plan, void* stream) {
-  if (cu == nullptr || plan == nullptr || seqs <= 0 || rows <= 0 || (block != 32 && block != 128)) return -2;
+  if (cu == nullptr || plan == nullptr || seqs <= 0 || seqs > kMostRows || rows <= 0 || rows > kMostRows || (block != 32 && block != 128)) return -2;
   hipLaunchKernelGGL(packed_plan_kernel, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, cu, seqs, rows, block, plan, rows / block + seqs + 1);
   CVH_CHECK_LAUNCH();
   return 0;

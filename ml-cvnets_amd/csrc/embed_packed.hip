@@ -16,6 +16,7 @@ namespace {
 constexpr int kItems = 1024;   // rows a sort workgroup takes: 4 waves x 4 rounds x 64 lanes
 constexpr int kChunk = 32;     // sorted rows that are summed by one group of lanes
 constexpr int kTableRows = 32;  // rows of the table a workgroup writes
+constexpr int kMostRows = 0x7fffffff - 4096, kMostBlocks = 1 << 24;  // (a grid has fewer than 2^32 threads)
 
 // sort key of row r: its token, or `vocab` (sorted behind everything) where the row adds nothing: behind the last sequence, the padding token,
 // a token outside the table
@@ -378,24 +379,25 @@ int pos_split(int seqs) { return seqs <= 64 ? 1 : seqs >= 1024 ? 16 : (seqs + 63
 
 // int32 scratch: two key and two row arrays (in whole chunks), the digit counts
 extern "C" long long cvh_embed_sort_elems(int rows) {
-  if (rows <= 0) return -2;
+  if (rows <= 0 || rows > kMostRows) return -2;
   return 4 * padded(rows) + sort_blocks(rows) * 256;
 }
 // float32 scratch: two pieces a chunk, the parts of the positions' sums
 extern "C" long long cvh_embed_pieces_elems(int rows, int e, int positions, int seqs) {
-  if (rows <= 0 || e <= 0 || positions < 0 || seqs < 0) return -2;
+  if (rows <= 0 || rows > kMostRows || e <= 0 || positions < 0 || seqs < 0) return -2;
   const int split = pos_split(seqs);
   return (padded(rows) / kChunk * 2 + (split > 1 ? (long long)split * positions : 0)) * e;
 }
 extern "C" int cvh_embed_packed_fwd(int dtype, const long long* ids, const float* table, const float* pos, const int* plan, int seqs, int block, int places,
                                     int rows, int vocab, int positions, int e, float scale, void* out, void* stream) {
   if (dtype != CVH_DT_F32 && dtype != CVH_DT_BF16) return -1;
-  if (ids == nullptr || table == nullptr || out == nullptr || rows <= 0 || vocab <= 0 || e <= 0 || e % 8 || (pos != nullptr && (plan == nullptr || positions <= 0))) return -2;
+  if (ids == nullptr || table == nullptr || out == nullptr || rows <= 0 || rows > kMostRows || vocab <= 0 || e <= 0 || e % 8 || (pos != nullptr && (plan == nullptr || positions <= 0))) return -2;
   if (plan != nullptr && (seqs <= 0 || (block != 32 && block != 128) || places != rows / block + seqs + 1)) return -2;
   if (plan == nullptr) {
     block = 32;
     places = (rows + block - 1) / block;
   }
+  if (places >= kMostBlocks) return -2;
   hipStream_t st = (hipStream_t)stream;
   int share = block;  // about 2048 pieces of 8 columns a workgroup: 25 k rows of 768 in 128-row items are 232 workgroups otherwise, fewer than CUs
   while (share > 8 && share * (e / 8) > 2048) share /= 2;
@@ -411,8 +413,8 @@ extern "C" int cvh_embed_packed_fwd(int dtype, const long long* ids, const float
 extern "C" int cvh_embed_packed_bwd(int dtype, const long long* ids, const void* dout, const int* plan, int seqs, int rows, int vocab, int e, long long padding_idx,
                                     float scale, float* dtable, int positions, float* dpos, int* sort, float* pieces, void* stream) {
   if (dtype != CVH_DT_F32 && dtype != CVH_DT_BF16) return -1;
-  if (dout == nullptr || rows <= 0 || e <= 0 || e % 8 || (dpos != nullptr && (plan == nullptr || positions <= 0 || positions > (1 << 26) || pieces == nullptr)) || (plan != nullptr && seqs <= 0)) return -2;
-  if (dtable != nullptr && (ids == nullptr || sort == nullptr || pieces == nullptr || vocab <= 0 || vocab >= 0x7fffffff - kTableRows)) return -2;
+  if (dout == nullptr || rows <= 0 || rows > kMostRows || e <= 0 || e % 8 || (dpos != nullptr && (plan == nullptr || positions <= 0 || positions > kMostBlocks / 64 || pieces == nullptr)) || (plan != nullptr && seqs <= 0)) return -2;
+  if (dtable != nullptr && (ids == nullptr || sort == nullptr || pieces == nullptr || vocab <= 0 || vocab / kTableRows >= kMostBlocks / 2)) return -2;
   hipStream_t st = (hipStream_t)stream;
   Grad g = {};
   g.n = rows; g.vocab = vocab; g.e = e; g.scale = scale; g.starts = plan; g.seqs = seqs;

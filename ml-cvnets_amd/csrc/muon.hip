@@ -26,7 +26,7 @@ constexpr int kMats = 32;
 #ifndef W8
 #define W8 100
 #endif
-constexpr int kMostRows = 1 << 14, kMostCols = 1 << 24;  // of the shorter and the longer side
+constexpr int kMostRows = 1 << 14, kMostCols = 1 << 20;  // of the shorter and the longer side
 constexpr float kScale = 4096.f, kScaleP = 1024.f;  // of x and G; of P
 typedef _Float16 half_t;
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));

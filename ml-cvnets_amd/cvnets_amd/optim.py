@@ -267,8 +267,8 @@ def _check_ns(steps: int, coefficients: Sequence[float], eps: float) -> Tuple[in
 
 
 def _check_matrix(rows: int, cols: int) -> None:
-    if rows < 1 or cols < 1 or min(rows, cols) > 1 << 14 or max(rows, cols) > 1 << 24:
-        raise NotImplementedError(f"matrices with a shorter side of 1 .. {1 << 14} and a longer one up to {1 << 24} are supported. Got: {rows} x {cols}")
+    if rows < 1 or cols < 1 or min(rows, cols) > 1 << 14 or max(rows, cols) > 1 << 20:
+        raise NotImplementedError(f"matrices with a shorter side of 1 .. {1 << 14} and a longer one up to {1 << 20} are supported. Got: {rows} x {cols}")
 
 
 def _by_cost(sizes: Sequence[Tuple[int, int]]) -> List[int]:
@@ -321,18 +321,26 @@ class Muon(torch.optim.Optimizer):
         if not lr >= 0.0 or not weight_decay >= 0.0 or not 0.0 <= momentum < 1.0:
             raise ValueError(f"lr and weight_decay must not be negative, momentum in [0, 1). Got: {lr}, {weight_decay}, {momentum}")
         self._ns = _check_ns(ns_steps, ns_coefficients, eps)
+        self._plan = None
+        self._hp = self._hp_host = None
+        self._workspaces = []  # every one that was handed to the kernels: a captured step goes on using its own
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=bool(nesterov), weight_decay=weight_decay))
-        if len({(g["momentum"], g["nesterov"]) for g in self.param_groups}) != 1:
-            raise NotImplementedError("per-group momentum / nesterov are not supported")
-        for g in self.param_groups:
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        try:
+            g, g0 = self.param_groups[-1], self.param_groups[0]
+            if (g["momentum"], g["nesterov"]) != (g0["momentum"], g0["nesterov"]):
+                raise NotImplementedError("per-group momentum / nesterov are not supported")
             for p in g["params"]:
                 if p.dim() < 2:
                     raise ValueError(f"Muon takes matrices (two or more dimensions); give vectors to AdamW. Got: {list(p.shape)}")
                 if p.dtype != torch.float32 or not p.is_contiguous():
                     raise RuntimeError("parameters must be contiguous float32")
                 _check_matrix(p.shape[0], p.numel() // max(1, p.shape[0]))
-        self._plan = None
-        self._hp = self._hp_host = None
+        except Exception:
+            self.param_groups.pop()
+            raise
 
     def _entries(self):
         out = []
@@ -358,8 +366,10 @@ class Muon(torch.optim.Optimizer):
                               cols=sizes[i][1], group=entries[i][2], gain=math.sqrt(max(1.0, sizes[i][0] / sizes[i][1]))) for i in _by_cost(sizes)]
         table = (_lib.NsMatrix * len(rows))(*rows)
         need = _lib.query("cvh_ns_workspace_elems", ctypes.byref(table), len(rows))
-        ws = self._plan["ws"] if self._plan is not None and self._plan["ws"].numel() >= need and self._plan["ws"].device == dev else \
-            torch.empty(need, dtype=torch.float32, device=dev)
+        ws = next((w for w in self._workspaces if w.numel() >= need and w.device == dev), None)
+        if ws is None:
+            ws = torch.empty(need, dtype=torch.float32, device=dev)
+            self._workspaces.append(ws)
         self._plan = {"table": table, "n": len(rows), "ws": ws, "key": self._key(entries)}
         return self._plan
 

@@ -14,7 +14,8 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .ops import _check_dev, _dt, _p, call_on, compute_dtype
 
-_INT_MAX = 2 ** 31 - 1
+_MOST_ROWS = 2 ** 31 - 4097  # rows are counted in 32 bits
+_MOST_BLOCKS = (1 << 24) - 1  # a grid has fewer than 2^32 threads
 _MOST_ROW = 1 << 21  # elements between two rows
 
 
@@ -33,8 +34,8 @@ class PackedSeqs:
         if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_contiguous():
             raise RuntimeError(f"cu_seqlens must be a contiguous int32 vector of sequences + 1 boundaries. Got: {cu_seqlens.dtype} {list(cu_seqlens.shape)}")
         rows = int(rows)
-        if not 0 < rows <= _INT_MAX:
-            raise ValueError(f"rows must be in 1 .. {_INT_MAX}. Got: {rows}")
+        if not 0 < rows <= _MOST_ROWS:
+            raise ValueError(f"rows must be in 1 .. {_MOST_ROWS}. Got: {rows}")
         if max_len is not None and max_len < 0:
             raise ValueError(f"max_len must not be negative. Got: {max_len}")
         _check_dev(cu_seqlens)
@@ -55,8 +56,8 @@ class PackedSeqs:
         torch.cumsum(torch.tensor(lengths, dtype=torch.int64), 0, out=cu[1:])
         total = int(cu[-1])
         rows = max(total, 1) if rows is None else int(rows)
-        if not total <= rows <= _INT_MAX:
-            raise ValueError(f"{total} rows of sequences do not fit into rows = {rows} (at most {_INT_MAX})")
+        if not total <= rows <= _MOST_ROWS:
+            raise ValueError(f"{total} rows of sequences do not fit into rows = {rows} (at most {_MOST_ROWS})")
         return cls(cu.to(torch.int32).to(device), rows, max_len=max(lengths))
 
     def refresh(self) -> None:
@@ -112,7 +113,7 @@ def _check_heads(q: Tensor, k: Tensor, v: Tensor, seqs: PackedSeqs, scale: Optio
         raise ValueError(f"scale must be positive and finite. Got: {scale}")
     if rows != seqs.rows:
         raise RuntimeError(f"the layout is of {seqs.rows} rows, the tensors have {rows}")
-    if hq * d > _MOST_ROW or seqs.places * hq > _INT_MAX:
+    if hq * d > _MOST_ROW or seqs.places * hq > _MOST_BLOCKS:
         raise NotImplementedError(f"packed attention: {hq} heads of {d} on {seqs.places} blocks are more than one launch takes")
     dev = seqs.plan.device
     if q.device != dev or k.device != dev or v.device != dev:
@@ -248,8 +249,8 @@ def embed(ids: Tensor, table: Tensor, seqs: Optional[PackedSeqs] = None, pos: Op
     vocab, e = table.shape
     if e == 0 or e % 8:
         raise NotImplementedError(f"packed embedding: the width must be a multiple of 8. Got: {e}")
-    if not 0 < ids.shape[0] <= _INT_MAX or vocab > _INT_MAX - 1024:
-        raise RuntimeError(f"packed embedding takes 1 .. {_INT_MAX} rows and up to {_INT_MAX - 1024} tokens. Got: {ids.shape[0]} and {vocab}")
+    if not 0 < ids.shape[0] <= _MOST_ROWS or vocab > 1 << 28:
+        raise RuntimeError(f"packed embedding takes 1 .. {_MOST_ROWS} rows and up to {1 << 28} tokens. Got: {ids.shape[0]} and {vocab}")
     if pos is not None:
         if pos.dim() != 2 or pos.dtype != torch.float32 or pos.shape[1] != e or pos.shape[0] == 0:
             raise RuntimeError(f"pos must be float32 [positions, {e}]. Got: {pos.dtype} {list(pos.shape)}")

@@ -168,3 +168,28 @@ def test_muon_step_in_a_graph():
         b.step()
         torch.cuda.synchronize()
         assert torch.equal(p, q)
+
+
+def test_a_captured_step_keeps_its_workspace():
+    """a larger list after the capture takes another workspace; the replays still give the eager result"""
+    small, large = torch.nn.Parameter(gradient(64, 80)), torch.nn.Parameter(gradient(600, 700))
+    twin = torch.nn.Parameter(small.detach().clone())
+    opt, eager = optim.Muon([small, large], lr=0.1), optim.Muon([twin], lr=0.1)
+    small.grad, twin.grad = gradient(64, 80, seed=2), gradient(64, 80, seed=2)
+    opt.step()
+    eager.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step(sync_hyperparameters=False)
+    keep = small.grad
+    small.grad, large.grad = None, gradient(600, 700, seed=3)
+    opt.step()
+    torch.cuda.synchronize()
+    filler = [torch.full((1 << 18,), float("nan"), device="cuda") for _ in range(64)]  # would lie in a freed workspace
+    small.grad, large.grad = keep, None
+    for _ in range(3):
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert torch.equal(small, twin)
+    assert all(torch.isnan(f).all() for f in filler)

@@ -21,7 +21,7 @@ def qkv(rows=10, hq=4, hkv=2, d=16, dtype=torch.float32):
 @pytest.mark.parametrize("cu,rows,max_len,error", [
     (torch.zeros(3, dtype=torch.int64), 5, None, RuntimeError), (torch.zeros(1, dtype=torch.int32), 5, None, RuntimeError),
     (torch.zeros(2, 2, dtype=torch.int32), 5, None, RuntimeError), (torch.zeros(6, dtype=torch.int32)[::2], 5, None, RuntimeError),
-    (torch.zeros(3, dtype=torch.int32), 0, None, ValueError), (torch.zeros(3, dtype=torch.int32), 2 ** 31, None, ValueError),
+    (torch.zeros(3, dtype=torch.int32), 0, None, ValueError), (torch.zeros(3, dtype=torch.int32), 2 ** 31 - 4096, None, ValueError),
     (torch.zeros(3, dtype=torch.int32), 5, -1, ValueError), (torch.zeros(3, dtype=torch.int32), 5, None, RuntimeError)])
 def test_layout_refuses(cu, rows, max_len, error):
     with pytest.raises(error):
@@ -89,6 +89,10 @@ def test_muon_refuses():
         with pytest.raises(error):
             optim.Muon(params, **kw)
     opt = optim.Muon([p])
+    for bad, error in ((dict(params=[torch.nn.Parameter(torch.zeros(4))]), ValueError), (dict(params=[torch.nn.Parameter(torch.zeros(3, 3))], momentum=0.1), NotImplementedError)):
+        with pytest.raises(error):
+            opt.add_param_group(bad)
+        assert len(opt.param_groups) == 1
     assert opt.step() is None  # nothing has a gradient
     p.grad = torch.zeros(4, 6)
     with pytest.raises(RuntimeError):

@@ -92,3 +92,12 @@ def test_tokens_outside_the_table_are_nan_rows_without_gradient():
     assert torch.isnan(out[[1, 3, 4]]).all() and torch.equal(out[[0, 2, 5]], table.detach()[[0, 5, 5]])
     (g,) = torch.autograd.grad(out, (table,), torch.ones_like(out))
     assert torch.equal(g, torch.tensor([1.0, 0, 0, 0, 0, 2]).cuda()[:, None].expand(6, 8))
+
+
+def test_places_without_a_position_are_nan_rows():
+    table, pos = torch.randn(6, 8, device="cuda", requires_grad=True), torch.randn(3, 8, device="cuda", requires_grad=True)
+    ids = torch.tensor([0, 1, 2, 3, 4, 5, 1], device="cuda")
+    out = packed.embed(ids, table, layout([5, 2]), pos=pos, dtype=torch.float32)
+    assert torch.isnan(out[3:5]).all() and torch.isfinite(out[[0, 1, 2, 5, 6]]).all()
+    _, dpos = torch.autograd.grad(out, (table, pos), torch.ones_like(out))
+    assert torch.equal(dpos, torch.tensor([2.0, 2, 1]).cuda()[:, None].expand(3, 8))
