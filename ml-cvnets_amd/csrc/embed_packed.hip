@@ -8,6 +8,8 @@
 // once, as the sum of its run in a fixed order: bit-reproducible.  What bounds it: the write of the whole table (49408 x 512: 101 MB) next to
 // one read of dy (two with positions).  The sorted rows are summed in equal chunks, not token by token: frequent tokens (the start mark of every
 // caption, the first words of a vocabulary in order of frequency) would otherwise leave their long runs to a few waves.
+// Measured (26.7 k caption tokens, 49408 x 512, bf16 rows, positions): forward 14 us, two sort passes 12 us each, the gradient kernel 24 us for 101 MB of
+// table and 55 MB of dy (positions read it again), joins 6 us.
 #include "common.hpp"
 #include "cvnets_hip.h"
 
