@@ -16,17 +16,16 @@
 // x is kept once, [m][n] (contraction over n: rows times rows); P x reads its columns with LDS transpose reads.  The cross products hi lo + lo hi
 // have accumulators of their own: the large sum is then rounded once per 16 terms instead of three times.  Every epilogue goes through
 // LDS, so that global memory sees whole rows.  Sides are padded to the tile with zeros, which the products keep zero: the main loop has no bounds.
-// All matrices of a list go through one launch per product (a table in the kernel's arguments): 2 + 3 steps launches for up to kMats matrices.
+// All matrices of a list go through one launch per product: 2 + 3 steps launches for up to kMats matrices.
 //
-// Measured: 24 matrices of a 6-layer text tower of 512 (1536 x 512 .. 512 x 2048, float32): 905 us, of 526 at the library's rates; 4096 x 2048 in bf16: 1216 of
-// 842 us (P x at 870 TFLOP/s of MFMA; x x^T has 136 tiles for 256 CUs); 21 matrices of 144 .. 720: 177 us, 17 dependent launches of 8 .. 16 us.
+// Measured: 24 matrices of a 6-layer text tower of 512 (1536 x 512 .. 512 x 2048, float32): 870 us, of 526 at the library's rates; 4096 x 2048 in bf16: 1205 of
+// 842 us (P x at 860 .. 900 TFLOP/s of MFMA; x x^T has 136 tiles for 256 units); 21 matrices of 144 .. 720: 159 us, 17 dependent launches of 5 .. 10 us.
 #include "common.hpp"
 #include "cvnets_hip.h"
 
 namespace {
 
 constexpr int kMats = 32;
-constexpr int kWideLeast = 100;  // 128-wide tiles from this number of them on (136 of them: 110 us for a product that takes 124 in 64-wide ones)
 constexpr int kMostRows = 1 << 14, kMostCols = 1 << 20;  // of the shorter and the longer side
 constexpr float kScale = 4096.f, kScaleP = 1024.f;  // of x and G; of P
 typedef _Float16 half_t;
@@ -189,24 +188,27 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_
 }
 
 // -----------------------------------------------------------------------------------------------------------------------------------------
-// product of hi + lo operands on a TILE x TILE tile by WAVES waves: acc[r][c] = sum_k A[r][k] B[c][k], B in rows; A in rows, or (COLS) given as
-// [k][r] and read with LDS transpose reads.  Three LDS stages of BK: step t computes from one, the next one is complete (its first fragments are
-// read under t's last MFMAs), and t + 2 is written from registers that were loaded two steps before.  Fragments are read one 16-wide slice ahead of
-// their MFMAs: with reads and MFMAs of a slice in sequence the time was their sum, whatever the depth of the global prefetch.
+// product of hi + lo operands on a TR x TC tile by WAVES waves: acc[r][c] = sum_k A[r][k] B[c][k], B in rows; A in rows, or (COLS) given as
+// [k][r] and read with LDS transpose reads.  Two LDS stages of BK.  First half of step t: its second 16-wide slice is read and its first one multiplied;
+// barrier: its stage is free and step t + 1's complete; second half: t + 2 goes from registers (requested a step and a half before) into the free stage,
+// and the first slice of t + 1 is read under t's last MFMAs.  With reads and MFMAs of a slice in sequence the time was their sum, whatever the depth
+// of the global prefetch.  The lo halves lie 16 banks off the hi halves (+ 32): eight lanes of a write, a global line of 32 hi and 32 lo, hit 32 banks
+// instead of 16 twice (with the pitch of the transpose reads: LDS conflicts from 30 % of its busy cycles to 0, the products 1 .. 4 % faster).
+// 4096 x 2048: MFMA busy in 61 % of the cycles in x x^T, 53 % in P x, at 2.0 .. 2.1 GHz (the library's large product reaches 43 % of the peak).
 // -----------------------------------------------------------------------------------------------------------------------------------------
 typedef short v4s_t __attribute__((ext_vector_type(4)));
-template <int TILE, int WAVES, bool COLS> struct Product {
+template <int TR, int TC, int WAVES, bool COLS> struct Product {
   static constexpr int NT = 64 * WAVES, BK = 32, PITCH = BK + 8;  // rows of 80 bytes: 16 lanes' 16-byte reads hit distinct banks
-  static constexpr int WR = TILE * 2 / WAVES, WC = TILE / 2;  // rows and columns of a wave
+  static constexpr int WR = TR * 2 / WAVES, WC = TC / 2;  // rows and columns of a wave
   static constexpr int FR = WR / 32, FC = WC / 32;            // 32-wide fragments of them
-  static constexpr int CH = 2 * TILE * (BK / 8) / NT;         // 16-byte pieces a thread loads of each operand
-  static constexpr int CPITCH = TILE + 16;                    // [k][r] rows: 4 rows of a transpose read on distinct banks
-  static constexpr int AELEMS = COLS ? BK * CPITCH : TILE * PITCH, BELEMS = TILE * PITCH, STAGE = 2 * AELEMS + 2 * BELEMS;
-  static constexpr int OPITCH = TILE + 4;                     // of the float tile of the epilogue
-  static constexpr size_t BYTES = sizeof(half_t) * 3 * STAGE > sizeof(float) * TILE * OPITCH ? sizeof(half_t) * 3 * STAGE : sizeof(float) * TILE * OPITCH;
+  static constexpr int CA = 8 * TR / NT, CB = 8 * TC / NT;    // 16-byte pieces a thread loads of each operand
+  static constexpr int CPITCH = TR + 32;                      // [k][r] rows: the 4 rows of a transpose read are 16 banks apart
+  static constexpr int AELEMS = (COLS ? BK * CPITCH : TR * PITCH) + 32, BELEMS = TC * PITCH + 32, STAGE = 2 * AELEMS + 2 * BELEMS;
+  static constexpr int OPITCH = TR + 4;                     // of the float tile of the epilogue
+  static constexpr size_t BYTES = sizeof(half_t) * 2 * STAGE > sizeof(float) * TC * OPITCH ? sizeof(half_t) * 2 * STAGE : sizeof(float) * TC * OPITCH;
   half_t* lds;
   f32x16_t acc[FR][FC];
-  u32x4_t q[2][2][CH];
+  u32x4_t qa[2][CA], qb[2][CB];
   struct Frags {
     half8_t ah[FR], al[FR], bh[FC], bl[FC];
   };
@@ -216,20 +218,28 @@ template <int TILE, int WAVES, bool COLS> struct Product {
   // pieces of 16 bytes, in the order of the global lines: row r = 4 hi and 4 lo pieces (COLS: row k = TILE / 4 pieces)
   template <int S> __device__ __forceinline__ void load(const ghalf_t* a, int lda, const ghalf_t* b, int ldb, int k0, int tid) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
+    for (int c = 0; c < CA; ++c) {
       const int idx = tid + c * NT, r = idx >> 3, in = (idx & 7) * 8;
-      q[S][0][c] = gload<u32x4_t>(COLS ? a + (size_t)(k0 + idx / (TILE / 4)) * 2 * lda + idx % (TILE / 4) * 8 : a + (size_t)r * 2 * lda + k0 * 2 + in);
-      q[S][1][c] = gload<u32x4_t>(b + (size_t)r * 2 * ldb + k0 * 2 + in);
+      qa[S][c] = gload<u32x4_t>(COLS ? a + (size_t)(k0 + idx / (TR / 4)) * 2 * lda + idx % (TR / 4) * 8 : a + (size_t)r * 2 * lda + k0 * 2 + in);
+    }
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+      const int idx = tid + c * NT;
+      qb[S][c] = gload<u32x4_t>(b + (size_t)(idx >> 3) * 2 * ldb + k0 * 2 + (idx & 7) * 8);
     }
   }
   template <int S> __device__ __forceinline__ void store(int stage, int tid) {
     half_t* const s = lds + stage * STAGE;
+    auto rows = [&](int idx) { return (idx >> 3) * PITCH + (idx & 3) * 8; };
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int idx = tid + c * NT, lo = (idx >> 2) & 1, rows = (idx >> 3) * PITCH + (idx & 3) * 8, in = idx % (TILE / 4);
-      const int at = COLS ? idx / (TILE / 4) * CPITCH + (in >> 3) * 32 + (idx & 3) * 8 : rows;
-      *reinterpret_cast<u32x4_t*>(s + lo * AELEMS + at) = q[S][0][c];
-      *reinterpret_cast<u32x4_t*>(s + 2 * AELEMS + lo * BELEMS + rows) = q[S][1][c];
+    for (int c = 0; c < CA; ++c) {
+      const int idx = tid + c * NT, in = idx % (TR / 4);
+      *reinterpret_cast<u32x4_t*>(s + ((idx >> 2) & 1) * AELEMS + (COLS ? idx / (TR / 4) * CPITCH + (in >> 3) * 32 + (idx & 3) * 8 : rows(idx))) = qa[S][c];
+    }
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+      const int idx = tid + c * NT;
+      *reinterpret_cast<u32x4_t*>(s + 2 * AELEMS + ((idx >> 2) & 1) * BELEMS + rows(idx)) = qb[S][c];
     }
   }
   static __device__ __forceinline__ half8_t row_frag(const half_t* t, int row, int k, int lane) {
@@ -244,7 +254,7 @@ template <int TILE, int WAVES, bool COLS> struct Product {
   }
   // order of the instructions since the last call: LDS reads, and the four instructions of class OTHER (LDS writes 0x200, global loads 0x020), between the MFMAs
   template <int OTHER> static __device__ __forceinline__ void interleave() {
-    constexpr int MFMAS = 3 * FR * FC, READS = (COLS ? 4 : 2) * FR + 2 * FC, OTHERS = 2 * CH;
+    constexpr int MFMAS = 3 * FR * FC, READS = (COLS ? 4 : 2) * FR + 2 * FC, OTHERS = CA + CB;
     static_for<0, MFMAS>([](auto i) {
       constexpr int r = (i + 1) * READS / MFMAS - i * READS / MFMAS, o = (i + 1) * OTHERS / MFMAS - i * OTHERS / MFMAS;
       if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
@@ -299,30 +309,25 @@ template <int TILE, int WAVES, bool COLS> struct Product {
     this->template store<0>(0, tid);
     request(S0{}, min(2, steps - 1));
     this->template store<1>(1, tid);
-    request(S1{}, min(3, steps - 1));
     wg_barrier_lds();
     Frags f = read(0, 0);
-    int s0 = 0, s1 = 1, s2 = 2;
     for (int t0 = 0; t0 < steps; t0 += 2)
       static_for<0, 2>([&](auto d) {
         // A wave that issues its LDS instructions in a row waits for the LDS queue with its MFMAs behind it, as the other waves do at the same
         // time, and the LDS is idle while they all multiply: one LDS instruction between two MFMAs keeps both busy.
+        constexpr int D = decltype(d)::value;
         Frags next;
-        this->template store<decltype(d)::value>(s2, tid);
-        next = read(s0, 16);
-        multiply(f);
-        interleave<0x200>();
-        f = next;
-        request(d, min(t0 + d + 4, steps - 1));
-        next = read(s1, 0);
+        request(std::integral_constant<int, 1 - D>{}, min(t0 + D + 3, steps - 1));
+        next = read(D, 16);
         multiply(f);
         interleave<0x020>();
         f = next;
         wg_barrier_lds();
-        const int s = s0;
-        s0 = s1;
-        s1 = s2;
-        s2 = s;
+        this->template store<D>(D, tid);
+        next = read(1 - D, 0);
+        multiply(f);
+        interleave<0x200>();
+        f = next;
       });
 #pragma unroll
     for (int i = 0; i < FR; ++i)
@@ -399,7 +404,7 @@ __device__ __forceinline__ void triangle_tile(int at, int n, int& i, int& j) {
 // G = x x^T (POLY false) or P = b G + c G G (true): tiles (i, j <= i), written to both halves
 template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVES, 2) void ns_sym_kernel(const Mats* __restrict__ list, int which, float cb, float cc) {
   const Mats& t = *list;
-  typedef Product<TILE, WAVES, false> Prod;
+  typedef Product<TILE, TILE, WAVES, false> Prod;
   __shared__ __attribute__((aligned(16))) char smem[Prod::BYTES];
   const int block = near_tiles(blockIdx.x, gridDim.x), k = find(t, SYM, block), tid = threadIdx.x;
   const Mat a = t.mat[k];
@@ -446,8 +451,9 @@ template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVE
   }
   if (i0 == j0) return;
   __syncthreads();
-  for (int idx = tid; idx < TILE * TILE / 8; idx += Prod::NT) {  // the mirror image
-    const int i = idx % TILE, j = idx / TILE * 8;
+#pragma unroll
+  for (int q = 0; q < PIECES; ++q) {  // the mirror image, four lanes to the 64 bytes of a row's 32 hi (lo)
+    const int idx = tid + q * Prod::NT, i = (idx >> 2) % TILE, j = idx / (4 * TILE) * 32 + (idx & 3) * 8;
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = v[(j + e) * Prod::OPITCH + i];
@@ -460,25 +466,25 @@ template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVE
 }
 
 // x <- a x + P x; the last one writes the result instead
-template <int TILE, int WAVES, typename T, int LAST> __global__ __launch_bounds__(64 * WAVES, 2) void ns_apply_kernel(const Mats* __restrict__ list, int which, float ca, const float* __restrict__ hp) {
+template <int TI, int TJ, int WAVES, typename T, int LAST> __global__ __launch_bounds__(64 * WAVES, 2) void ns_apply_kernel(const Mats* __restrict__ list, int which, float ca, const float* __restrict__ hp) {
   const Mats& t = *list;
-  typedef Product<TILE, WAVES, true> Prod;
+  typedef Product<TJ, TI, WAVES, true> Prod;
   __shared__ __attribute__((aligned(16))) char smem[Prod::BYTES];
   const int block = near_tiles(blockIdx.x, gridDim.x), k = find(t, APPLY, block), tid = threadIdx.x;
   const Mat a = t.mat[k];
   int ti, tj;
-  square_tile(block - t.first[APPLY][k], a.mp / TILE, a.np / TILE, ti, tj);
-  const int i0 = ti * TILE, j0 = tj * TILE;
+  square_tile(block - t.first[APPLY][k], a.mp / TI, a.np / TJ, ti, tj);
+  const int i0 = ti * TI, j0 = tj * TJ;
   const ghalf_t* const x = x_of(a, which);
   Prod p;
   p.lds = reinterpret_cast<half_t*>(smem);
   p.run(x + place(0, j0, a.np), a.np, p_of(a) + place(i0, 0, a.mp), a.mp, a.mp, tid);
-  constexpr int PIECES = TILE * TILE / 8 / Prod::NT;
+  constexpr int PIECES = TI * TJ / 8 / Prod::NT;
   half8_t xh[PIECES], xl[PIECES];
 #pragma unroll
   for (int q = 0; q < PIECES; ++q) {
     const int idx = tid + q * Prod::NT;
-    const size_t o = place(i0 + idx / (TILE / 8), j0 + idx % (TILE / 8) * 8, a.np);
+    const size_t o = place(i0 + idx / (TJ / 8), j0 + idx % (TJ / 8) * 8, a.np);
     xh[q] = gload<half8_t>(x + o);
     xl[q] = gload<half8_t>(x + o + kLo);
   }
@@ -486,7 +492,7 @@ template <int TILE, int WAVES, typename T, int LAST> __global__ __launch_bounds_
   ghalf_t* const next = x_of(a, which ^ 1);
 #pragma unroll
   for (int q = 0; q < PIECES; ++q) {
-    const int idx = tid + q * Prod::NT, i = idx / (TILE / 8), j = idx % (TILE / 8) * 8;
+    const int idx = tid + q * Prod::NT, i = idx / (TJ / 8), j = idx % (TJ / 8) * 8;
     const size_t o = place(i0 + i, j0 + j, a.np);
     float w[8];
 #pragma unroll
@@ -505,21 +511,22 @@ template <int TILE, int WAVES, typename T, int LAST> __global__ __launch_bounds_
   __syncthreads();
   const bool flip = a.rows > a.cols;
   const float lr = LAST == 2 ? hp[2 * a.group] : 0.f, keep = LAST == 2 ? 1.f - lr * hp[2 * a.group + 1] : 0.f, step = lr * a.gain;
+  const int across = flip ? TI : TJ;
   constexpr int IN_FLIGHT = 8;
-  for (int base = tid; base < TILE * TILE; base += Prod::NT * IN_FLIGHT) {
+  for (int base = tid; base < TI * TJ; base += Prod::NT * IN_FLIGHT) {
     float old[IN_FLIGHT];
     size_t o[IN_FLIGHT];
     bool in[IN_FLIGHT];
 #pragma unroll
     for (int q = 0; q < IN_FLIGHT; ++q) {
-      const int idx = base + q * Prod::NT, slow = idx / TILE, fast = idx % TILE, i = flip ? fast : slow, j = flip ? slow : fast;
+      const int idx = base + q * Prod::NT, slow = idx / across, fast = idx % across, i = flip ? fast : slow, j = flip ? slow : fast;
       in[q] = i0 + i < a.m && j0 + j < a.n;
       o[q] = in[q] ? (flip ? (size_t)(j0 + j) * a.cols + i0 + i : (size_t)(i0 + i) * a.cols + j0 + j) : 0;
       if (LAST == 2) old[q] = gvalue<float>(a.par, o[q]);
     }
 #pragma unroll
     for (int q = 0; q < IN_FLIGHT; ++q) {
-      const int idx = base + q * Prod::NT, slow = idx / TILE, fast = idx % TILE;
+      const int idx = base + q * Prod::NT, slow = idx / across, fast = idx % across;
       const float y = flip ? v[fast * Prod::OPITCH + slow] : v[slow * Prod::OPITCH + fast];
       if (!in[q]) continue;
       if (LAST == 1) gput<T>(a.dst, o[q], y);
@@ -546,44 +553,51 @@ template <typename F> int prefix(Mats& t, int phase, F&& groups) {
   }
   return n;
 }
-// 128-wide tiles where the list has enough of them for the card (and every side takes them), else 64-wide ones
-template <typename F> bool wide_tiles(const Mats& t, F&& tiles) {
+// 128-wide tiles of the symmetric products where there is one for half of the card's 256 units; fewer of them leave more of it idle than the smaller
+// tiles cost (all five steps of one matrix, 64- / 128-wide: 1792 x 1792, 105 tiles: 589 / 650 us; 2048 x 2048, 136 tiles: 818 / 754 us).
+constexpr int kWideSym = 128;
+// P x: 128 x 128 where they come in one round of half of the card or more (1536 x 1536, 144 tiles: 463 us, with 128 x 64 tiles 499, with 64 x 64 486).
+// Below and above that 128 x 64, two workgroups a unit: twice as many of them (1280 x 1280, 100 tiles: 287, 322, 302 us), and in several rounds one's
+// loads and epilogue under the other's MFMAs (a text tower's 24 matrices, 1152 tiles: 837, 872, 883 us).  64 x 64 below 72 (1024 x 1024, 64 tiles:
+// 207 us, with 128 x 64 tiles 230).
+enum { SQUARE_64, TALL, SQUARE_128 };
+constexpr int kTallLeast = 72, kSquareLeast = 128, kSquareMost = 256;
+template <typename F> long long wide_tiles(const Mats& t, F&& tiles) {  // 0: not every side takes them
   long long n = 0;
   for (int i = 0; i < t.count; ++i) {
-    if (t.mat[i].mp % 128 || t.mat[i].np % 128) return false;
+    if (t.mat[i].mp % 128 || t.mat[i].np % 128) return 0;
     n += tiles(t.mat[i]);
   }
-  return n >= kWideLeast;
+  return n;
 }
 template <int TILE> int sym_tiles(const Mat& q) { return q.mp / TILE * (q.mp / TILE + 1) / 2; }
-template <int TILE> int all_tiles(const Mat& q) { return q.mp / TILE * (q.np / TILE); }
+template <int TI, int TJ> int all_tiles(const Mat& q) { return q.mp / TI * (q.np / TJ); }
 
 template <int TILE, int WAVES> void run_sym(const Mats* list, int n, int which, float b, float c, hipStream_t st) {
   ns_sym_kernel<TILE, WAVES, false><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, which, b, c);
   ns_sym_kernel<TILE, WAVES, true><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, which, b, c);
 }
-template <int TILE, int WAVES, typename T, int LAST> void run_apply(const Mats* list, int n, int which, float a, const float* hp, hipStream_t st) {
-  ns_apply_kernel<TILE, WAVES, T, LAST><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, which, a, hp);
+template <typename T, int LAST> void run_apply(int tile, const Mats* list, int n, int which, float a, const float* hp, hipStream_t st) {
+  if (tile == SQUARE_128) ns_apply_kernel<128, 128, 8, T, LAST><<<dim3(n), dim3(512), 0, st>>>(list, which, a, hp);
+  else if (tile == TALL) ns_apply_kernel<128, 64, 4, T, LAST><<<dim3(n), dim3(256), 0, st>>>(list, which, a, hp);
+  else ns_apply_kernel<64, 64, 4, T, LAST><<<dim3(n), dim3(256), 0, st>>>(list, which, a, hp);
 }
 template <typename T, bool MOM> int run_list(Mats& t, Mats* list, int steps, float a, float b, float c, float eps, float mu, int nesterov, const float* hp, hipStream_t st) {
-  const bool ws = wide_tiles(t, sym_tiles<128>), wa = wide_tiles(t, all_tiles<128>);
+  const bool ws = wide_tiles(t, sym_tiles<128>) >= kWideSym;
+  const long long wide = wide_tiles(t, all_tiles<128, 128>);
+  const int wa = wide < kTallLeast ? SQUARE_64 : wide < kSquareLeast || wide > kSquareMost ? TALL : SQUARE_128;
   const int norms = prefix(t, NORM, [](const Mat& q) { return (int)(((long long)q.m * q.n + kNormItems - 1) / kNormItems); });
-  const int scales = prefix(t, SCALE, all_tiles<64>);
+  const int scales = prefix(t, SCALE, all_tiles<64, 64>);
   const int syms = ws ? prefix(t, SYM, sym_tiles<128>) : prefix(t, SYM, sym_tiles<64>);
-  const int applies = wa ? prefix(t, APPLY, all_tiles<128>) : prefix(t, APPLY, all_tiles<64>);
+  const int applies = wa == SQUARE_128 ? prefix(t, APPLY, all_tiles<128, 128>) : wa == TALL ? prefix(t, APPLY, all_tiles<128, 64>) : prefix(t, APPLY, all_tiles<64, 64>);
   ns_norm_kernel<T, MOM><<<dim3(norms), dim3(256), 0, st>>>(t, list, mu, nesterov);
   ns_scale_kernel<T, MOM><<<dim3(scales), dim3(256), 0, st>>>(list, mu, nesterov, eps);
   constexpr int LAST = MOM ? 2 : 1;
   for (int s = 0; s < steps; ++s) {
     if (ws) run_sym<128, 8>(list, syms, s & 1, b, c, st);
     else run_sym<64, 4>(list, syms, s & 1, b, c, st);
-    if (s + 1 < steps) {
-      if (wa) run_apply<128, 8, T, 0>(list, applies, s & 1, a, hp, st);
-      else run_apply<64, 4, T, 0>(list, applies, s & 1, a, hp, st);
-    } else {
-      if (wa) run_apply<128, 8, T, LAST>(list, applies, s & 1, a, hp, st);
-      else run_apply<64, 4, T, LAST>(list, applies, s & 1, a, hp, st);
-    }
+    if (s + 1 < steps) run_apply<T, 0>(wa, list, applies, s & 1, a, hp, st);
+    else run_apply<T, LAST>(wa, list, applies, s & 1, a, hp, st);
   }
   CVH_CHECK_LAUNCH();
   return 0;

@@ -50,6 +50,13 @@ def make(rows, hq, hkv, d, dtype, seed=0):
     return [torch.randn(rows, h, d, generator=g, device="cuda").to(dtype) for h in (hq, hkv, hkv, hq)]
 
 
+def layout(cu, rows, block):
+    """the sequences with either size of the work list's blocks (their choice costs time and no result)"""
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(packed, "_block_rows", lambda *_: block)
+        return packed.PackedSeqs(cu, rows)
+
+
 LENGTHS = {"one": [1], "tile edges": [31, 32, 33, 64, 65, 1, 0, 127, 128, 129, 0], "captions": [5, 77, 12, 40, 9, 31, 8, 77], "long": [700, 3, 257], "even": [128, 256]}
 
 
@@ -63,15 +70,15 @@ def test_against_float64(dtype, causal, name, hq, hkv, d):
     for t in (q, k, v):
         t.requires_grad_(True)
     want = reference(q, k, v, lens, causal, d ** -0.5, dout)
-    for max_len in (max(lens), None) if max(lens) <= 128 else (None,):  # both block sizes
+    for block in (32, 128):
         cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device="cuda")
-        out = packed.attention(q, k, v, packed.PackedSeqs(cu, sum(lens), max_len=max_len), causal=causal)
+        out = packed.attention(q, k, v, layout(cu, sum(lens), block), causal=causal)
         grads = torch.autograd.grad(out, (q, k, v), dout)
         for what, a, b in zip(("out", "dq", "dk", "dv"), (out, *grads), want):
             if what in ("dq", "dk") and max(lens) == 1:  # a softmax over one key: the exact gradient is zero
                 assert float(a.abs().max()) <= TOL[dtype] * d, what
             else:
-                close(a, b, dtype, (what, max_len))
+                close(a, b, dtype, (what, block))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -83,11 +90,11 @@ def test_head_widths(dtype, d, hq, hkv):
     for t in (q, k, v):
         t.requires_grad_(True)
     want = reference(q, k, v, lens, True, 0.2, dout)
-    for max_len in (100, None):  # (a max_len that is too small costs no result)
+    for block in (32, 128):
         cu = torch.tensor([0, 70, 71, 261], dtype=torch.int32, device="cuda")
-        out = packed.attention(q, k, v, packed.PackedSeqs(cu, 261, max_len=max_len), scale=0.2)
+        out = packed.attention(q, k, v, layout(cu, 261, block), scale=0.2)
         for what, a, b in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, (q, k, v), dout)), want):
-            close(a, b, dtype, (what, max_len))
+            close(a, b, dtype, (what, block))
 
 
 def test_projection_columns_are_read_in_place_and_give_one_gradient():
@@ -137,9 +144,9 @@ def test_other_sequences_and_filling_rows_do_not_reach_a_sequence(dtype, causal)
     """NaN and infinities in one sequence and behind the last one: the other sequences' results do not change by a bit; the filling rows are zeros"""
     lens, rows, d = [40, 37, 61], 170, 64
     q, k, v, dout = make(rows, 4, 2, d, dtype, seed=2)
-    for max_len in (61, None):
+    for block in (32, 128):
         cu = torch.tensor([0, 40, 77, 138], dtype=torch.int32, device="cuda")
-        seqs = packed.PackedSeqs(cu, rows, max_len=max_len)
+        seqs = layout(cu, rows, block)
 
         def run(*t):
             t = [x.detach().clone().requires_grad_(True) for x in t]
