@@ -13,11 +13,11 @@
 // from accumulator to operand registers and never touch LDS.  The waves of a workgroup share the staged K / V (or Q / dO) tiles, which are
 // double-buffered in LDS and loaded a tile ahead through registers.
 //
-// What bounds it (measured, MI355X): 128 columns, 20 k rows in 3 documents, 16 / 4 heads, causal forward: 638 us = 908 TFLOP/s of the 4 d a pair that have to
-// be computed; 40 % of the cycles MFMA, 43 % softmax arithmetic, which two waves a SIMD overlap only in part.  64 columns, 24.6 k rows, 12 / 4 heads,
-// training: forward 103, dq 132, dk / dv 197 us; a score costs an exponential (16 cycles a wave) and three other operations next to 1 / 4 of an MFMA.  128-row
-// workgroups: 4 waves share each staged tile; 64 keys (queries) a tile: 32 cost 20 %, 128 cost 10 % (registers, LDS).  Captions (5 .. 77 tokens):
-// one wave per 32 rows, 20 + 27 + 22 us for 13 k rows x 8 heads, latency.
+// What bounds it (measured, MI355X): 128 columns, 20 k rows in 3 documents, 16 / 4 heads, causal forward: 613 us = 945 TFLOP/s of the 4 d a pair that have to
+// be computed; about half of the cycles MFMA, the other half softmax arithmetic, which two waves a SIMD overlap only in part.  64 columns, 24.6 k rows,
+// 12 / 4 heads, training: forward 98, dq 130, dk / dv 191 us; a score costs an exponential and three other operations next to 1 / 4 of an MFMA.  128-row
+// workgroups: 4 waves share each staged tile; 64 keys (queries) a tile: at 64 columns 32 cost 20 % and 128 10 % in dk / dv, at 96 and 128 columns 32 cost 5 .. 8 % of
+// a whole training pass.  Captions (5 .. 77 tokens): one wave per 32 rows, 20 + 27 + 22 us for 13 k rows x 8 heads, latency.
 //
 // Work items come from a plan (packed_plan_kernel) made once per batch: (sequence, block) pairs, most expensive first, so that the last
 // workgroups to start are the short ones; the list also has the rows behind the last sequence, whose results are written as zeros.
@@ -171,7 +171,7 @@ template <typename T, int CP, int NROWS, int NT> struct RowTile {
 };
 
 // rows 16 t .. 16 t + 15 (in that order) of an accumulator as an operand.  bf16: the one rounding of P / dS to 8 bits, each probability off by
-// at most 2^-9 of itself; the sums it enters stay in 32 bits.
+// at most 2^-8 of itself; the sums it enters stay in 32 bits.
 template <typename T> __device__ __forceinline__ Frag<T> acc_frag(const f32x16_t& a, int t);
 template <> __device__ __forceinline__ Frag<bf16_t> acc_frag<bf16_t>(const f32x16_t& a, int t) {
   Frag<bf16_t> f;
@@ -233,6 +233,15 @@ __device__ __forceinline__ void store_rows(float* row, float*, const f32x16_t& v
   for (int i = 0; i < 4; ++i) {
     const int c = c0 + 8 * i + 4 * (lane >> 5);
     if (ok && c < d) *reinterpret_cast<float4*>(row + c) = make_float4(v[4 * i] * scale, v[4 * i + 1] * scale, v[4 * i + 2] * scale, v[4 * i + 3] * scale);
+  }
+}
+
+// One wave a SIMD has 256 ordinary and 256 accumulation registers.  The matrix instructions take their sums from either, but where values meet (the
+// loop, the skipped tiles) the compiler wants ordinary ones: without this it moved 128 of them there and back in every tile.
+template <bool ONE_WAVE, int N> __device__ __forceinline__ void accumulators(f32x16_t (&a)[N]) {
+  if constexpr (ONE_WAVE) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+a"(a[i]));
   }
 }
 
@@ -343,15 +352,19 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
     // key 0 is visible to every query (and to the rows past the end, which count as zeros), so the maximum is finite from the first tile on
+    // The reference point moves when a query's maximum is more than 2^8 past it: probabilities up to 2^8 instead of 1 have the same relative rounding, and
+    // l and o stay far from float32's range; moved with every new maximum, half of the tiles scale o, 16 d / 32 multiplications (see above).
+    // Per query, so that no result depends on the other queries of its wave.  (The negation: the first tile's -inf, and NaN, move.)
     const float m_new = fmaxf(m, both_halves_max(mx));
-    if (__any(m_new > m)) {
-      const float alpha = pexp2((m - m_new) * c);
+    const bool move = !((m_new - m) * c <= 8.f);
+    if (__any(move)) {
+      const float to = move ? m_new : m, alpha = pexp2((m - to) * c);
       l *= alpha;
 #pragma unroll
       for (int f = 0; f < NF; ++f)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[f][r] *= alpha;
-      m = m_new;
+      m = to;
     }
     const float mc = m * c;
     float sum = 0.f;
@@ -447,8 +460,12 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
 #pragma unroll
   for (int f = 0; f < NF; ++f) acc[f] = acc_zero();
 
+  f32x16_t minus_delta;  // the products with V start from it
+#pragma unroll
+  for (int r = 0; r < 16; ++r) minus_delta[r] = -delta;
   for (int t = 0; t < tiles; ++t) {
     const int k0 = t * KB;
+    accumulators<OCC == 1>(acc);
     wg_barrier_lds();
     const T* const Kt = Kl + (t & 1) * KB * PT;
     const T* const Vt = Vl + (t & 1) * KB * PT;
@@ -459,14 +476,14 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
     const bool masked = k0 + KB > w.len || (p.causal && k0 + KB - 1 > q0);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      f32x16_t s = acc_zero(), dp = acc_zero();
+      f32x16_t s = acc_zero(), dp = minus_delta;
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
         mma32(s, tile.rows(Kt, 32 * b, 16 * k), qf[k]);
         mma32(dp, tile.rows(Vt, 32 * b, 16 * k), df[k]);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = pexp2(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+      for (int r = 0; r < 16; ++r) s[r] = pexp2(fmaf(s[r], c, -lse)) * dp[r];
       if (masked) {
         const int last = (p.causal ? min(my_q, w.len - 1) : w.len - 1) - k0 - 32 * b - 4 * (lane >> 5);
 #pragma unroll
@@ -480,6 +497,7 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
       }
     }
   }
+  accumulators<OCC == 1>(acc);
 #pragma unroll
   for (int f = 0; f < NF; ++f) store_rows(dq + row * p.dq_row, (T*)nullptr, acc[f], p.scale, 32 * f, p.d, lane, q_ok);
 }
@@ -489,11 +507,13 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
 // -----------------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bounds__(64 * NW, OCC) void packed_attn_dkv_kernel(PA p) {
   constexpr int PT = Tile<T, CP>::PT, NF = CP / 32, NK = CP / 16, NB = QB / 32, NT = 64 * NW;
+  // 32-query blocks whose scores are held at once: a lone wave has nothing else to put under their MFMAs (96 and 128 columns: 2 % off the pass)
+  constexpr int SB = OCC == 1 ? NB : 1;
   static_assert(NT >= QB, "one thread a query's statistics");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* const Ql = reinterpret_cast<T*>(smem);
   T* const Dl = Ql + 2 * QB * PT;
-  float* const Ll = reinterpret_cast<float*>(Dl + 2 * QB * PT);  // [2][2][NT]: log-sums and deltas of a tile's queries
+  float* const Ll = reinterpret_cast<float*>(Dl + 2 * QB * PT);  // [2][2][NT]: log-sums and -deltas of a tile's queries
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Item w = work_item(p, p.heads_kv);
   if (w.seq < -1) return;
@@ -541,7 +561,7 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
     qt.store(Ql + (t & 1) * QB * PT, tid);
     dt.store(Dl + (t & 1) * QB * PT, tid);
     Ll[(t & 1) * 2 * NT + tid] = lse;
-    Ll[(t & 1) * 2 * NT + NT + tid] = delta;
+    Ll[(t & 1) * 2 * NT + NT + tid] = -delta;
   };
   request();
   Frag<T> kf[NK], vf[NK];
@@ -563,6 +583,8 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
   for (int f = 0; f < NF; ++f) { ak[f] = acc_zero(); av[f] = acc_zero(); }
 
   for (int t = 0, q0 = qfirst; t < tiles; ++t, q0 = q0 + QB < w.len ? q0 + QB : qfirst) {
+    accumulators<OCC == 1>(ak);
+    accumulators<OCC == 1>(av);
     wg_barrier_lds();
     store(t + 1);
     request();
@@ -572,46 +594,61 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
     if (k0 >= w.len || (p.causal && q0 + QB - 1 < k0)) continue;  // no key of this wave, or none of the tile's queries sees one
     const bool masked = q0 + QB > w.len || (p.causal && q0 < k0 + 31);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      f32x16_t s = acc_zero(), dp = acc_zero();
+    for (int b0 = 0; b0 < NB; b0 += SB) {
+      f32x16_t s[SB], dp[SB];  // dp starts from -delta
 #pragma unroll
-      for (int k = 0; k < NK; ++k) {
-        mma32(s, tile.rows(Qt, 32 * b, 16 * k), kf[k]);
-        mma32(dp, tile.rows(Dt, 32 * b, 16 * k), vf[k]);
-      }
+      for (int b = 0; b < SB; ++b) {
+        s[b] = acc_zero();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r0 = 32 * b + 8 * i + 4 * (lane >> 5);
-        const float4 ls = *reinterpret_cast<const float4*>(Lt + r0), de = *reinterpret_cast<const float4*>(Lt + NT + r0);
-        const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dl[4] = {de.x, de.y, de.z, de.w};
+        for (int i = 0; i < 4; ++i) {
+          const float4 de = *reinterpret_cast<const float4*>(Lt + NT + 32 * (b0 + b) + 8 * i + 4 * (lane >> 5));
+          dp[b][4 * i] = de.x; dp[b][4 * i + 1] = de.y; dp[b][4 * i + 2] = de.z; dp[b][4 * i + 3] = de.w;
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[4 * i + e] = pexp2(fmaf(s[4 * i + e], c, -lv[e]));
-          dp[4 * i + e] = s[4 * i + e] * (dp[4 * i + e] - dl[e]);
+        for (int k = 0; k < NK; ++k) {
+          mma32(s[b], tile.rows(Qt, 32 * (b0 + b), 16 * k), kf[k]);
+          mma32(dp[b], tile.rows(Dt, 32 * (b0 + b), 16 * k), vf[k]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 ls = *reinterpret_cast<const float4*>(Lt + 32 * (b0 + b) + 8 * i + 4 * (lane >> 5));
+          const float lv[4] = {ls.x, ls.y, ls.z, ls.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[b][4 * i + e] = pexp2(fmaf(s[b][4 * i + e], c, -lv[e]));
+            dp[b][4 * i + e] *= s[b][4 * i + e];
+          }
         }
       }
       if (masked) {
-        // queries from `lo` on (from this lane's first row) see this lane's key, those from `hi` on lie behind the sequence
-        const int base = q0 + 32 * b + 4 * (lane >> 5), lo = p.causal ? my_k - base : -64, hi = w.len - base;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int q = (r & 3) + 8 * (r >> 2);
-          const bool hide = q < lo || q >= hi;
-          s[r] = hide ? 0.f : s[r];
-          dp[r] = hide ? 0.f : dp[r];
+        for (int b = 0; b < SB; ++b) {
+          // queries from `lo` on (from this lane's first row) see this lane's key, those from `hi` on lie behind the sequence
+          const int base = q0 + 32 * (b0 + b) + 4 * (lane >> 5), lo = p.causal ? my_k - base : -64, hi = w.len - base;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int q = (r & 3) + 8 * (r >> 2);
+            const bool hide = q < lo || q >= hi;
+            s[b][r] = hide ? 0.f : s[b][r];
+            dp[b][r] = hide ? 0.f : dp[b][r];
+          }
         }
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const Frag<T> pf = acc_frag<T>(s, h), sf = acc_frag<T>(dp, h);
+      for (int b = 0; b < SB; ++b)
 #pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          mma32(av[f], tile.cols(Dt, 32 * b + 16 * h, 32 * f), pf);
-          mma32(ak[f], tile.cols(Qt, 32 * b + 16 * h, 32 * f), sf);
+        for (int h = 0; h < 2; ++h) {
+          const Frag<T> pf = acc_frag<T>(s[b], h), sf = acc_frag<T>(dp[b], h);
+#pragma unroll
+          for (int f = 0; f < NF; ++f) {
+            mma32(av[f], tile.cols(Dt, 32 * (b0 + b) + 16 * h, 32 * f), pf);
+            mma32(ak[f], tile.cols(Qt, 32 * (b0 + b) + 16 * h, 32 * f), sf);
+          }
         }
-      }
     }
   }
+  accumulators<OCC == 1>(ak);
+  accumulators<OCC == 1>(av);
   const long long row = w.start + (k_ok ? my_k : 0);
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
@@ -697,7 +734,7 @@ template <typename T, int CP, int NW, int KB> int launch_fwd(const PA& p, hipStr
   return 0;
 }
 template <typename T, int CP, int NW, int KB> int launch_bwd(const PA& p, hipStream_t st) {
-  constexpr int QB = KB;
+  constexpr int QB = sizeof(T) == 2 && NW == 4 ? 64 : KB;
   constexpr auto dq = packed_attn_dq_kernel<T, CP, NW, KB, occ<T, CP, NW>(false)>;
   constexpr auto dkv = packed_attn_dkv_kernel<T, CP, NW, QB, occ<T, CP, NW>(true)>;
   static DynSmemAttr aq, ak;
