@@ -139,7 +139,7 @@ class TextTransformer(nn.Module):
         for layer in self.transformer:
             t = layer.forward_tokens(t, ops.NO_SEQMAP, causal=True, seqs=seqs)
         t = ops.layer_norm_tokens(t, self.final_layer_norm, ops.NO_SEQMAP)
-        ends = (seqs.cu_seqlens[1:].long() - 1).clamp(min=0)  # plumbing: EOT index arithmetic
+        ends = (seqs.plan[1:seqs.seqs + 1].long() - 1).clamp(min=0)  # plumbing: EOT index arithmetic, on the clamped boundaries
         return ops.l2_normalize(ops.linear(ops.RowsGatherIdx.apply(t, ends), self.projection_layer.t()))
 
     def forward_zero_shot(self, text_tokens: Tensor, key_padding_mask: Optional[Tensor] = None, *args, **kwargs) -> Tensor:

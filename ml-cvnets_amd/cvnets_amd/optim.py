@@ -359,6 +359,9 @@ class Muon(torch.optim.Optimizer):
             if p.device != dev:
                 raise RuntimeError(f"the parameters must be on one device. Got: {p.device} and {dev}")
             buf = self.state[p].get("momentum_buffer")
+            if not p.is_contiguous() or (buf is not None and buf.shape != p.shape):
+                raise RuntimeError(f"a parameter became another matrix: {list(p.shape)}, contiguous {p.is_contiguous()}, its momentum {None if buf is None else list(buf.shape)}")
+            _check_matrix(p.shape[0], p.numel() // max(1, p.shape[0]))
             if buf is None or buf.dtype != torch.float32 or not buf.is_contiguous() or buf.device != dev:  # (a loaded state may be another type's)
                 self.state[p]["momentum_buffer"] = torch.zeros_like(p) if buf is None else buf.to(device=dev, dtype=torch.float32).contiguous()
         sizes = [(p.shape[0], p.numel() // p.shape[0]) for p, _, _ in entries]
@@ -374,7 +377,7 @@ class Muon(torch.optim.Optimizer):
         return self._plan
 
     def _key(self, entries):
-        return [(p.data_ptr(), g.data_ptr(), self.state[p]["momentum_buffer"].data_ptr() if "momentum_buffer" in self.state[p] else 0, gi) for p, g, gi in entries]
+        return [(p.data_ptr(), p.shape, g.data_ptr(), self.state[p]["momentum_buffer"].data_ptr() if "momentum_buffer" in self.state[p] else 0, gi) for p, g, gi in entries]
 
     def sync_hyperparameters(self) -> None:
         """copy the groups' (lr, weight_decay) to the device table; call after a scheduler changed them (outside graph replay)"""
@@ -408,6 +411,9 @@ class Muon(torch.optim.Optimizer):
         if sync_hyperparameters or self._hp is None:
             self.sync_hyperparameters()
         g0 = self.param_groups[0]
+        for g in self.param_groups:  # (they may be rewritten, or loaded)
+            if (g["momentum"], g["nesterov"]) != (g0["momentum"], g0["nesterov"]):
+                raise NotImplementedError("per-group momentum / nesterov are not supported")
         ops.call_on(dev, "cvh_muon_step", ctypes.byref(plan["table"]), plan["n"], *self._ns, float(g0["momentum"]), int(g0["nesterov"]), _p(self._hp), _p(plan["ws"]))
         ops.invalidate_packed()
         return loss

@@ -49,6 +49,7 @@ class PackedSeqs:
         self.cu_seqlens, self.rows, self.seqs = cu_seqlens, rows, cu_seqlens.numel() - 1
         self.max_len = rows if max_len is None else min(int(max_len), rows)
         self.block = _block_rows(rows, self.seqs, self.max_len)
+        self.version = 0  # of the work list: a backward pass with another one than its forward is refused
         self.places = rows // self.block + self.seqs + 1
         self.plan = torch.empty(_lib.query("cvh_packed_plan_elems", self.seqs, rows, self.block), dtype=torch.int32, device=cu_seqlens.device)
         self.refresh()
@@ -67,10 +68,16 @@ class PackedSeqs:
         return cls(cu.to(torch.int32).to(device), rows, max_len=max(lengths))
 
     def refresh(self) -> None:
+        self.version += 1
         call_on(self.plan.device, "cvh_packed_plan", _p(self.cu_seqlens), self.seqs, self.rows, self.block, _p(self.plan))
 
     def __repr__(self) -> str:
         return f"PackedSeqs(sequences={self.seqs}, rows={self.rows}, max_len={self.max_len})"
+
+
+def _check_version(seqs: PackedSeqs, version: int) -> None:
+    if seqs.version != version:
+        raise RuntimeError("the layout of the packed sequences was refreshed between forward and backward: batches in flight need layouts of their own")
 
 
 # ---------------------------------------------------------------------------------------------------------------------------------------
@@ -134,14 +141,15 @@ class PackedAttentionFn(torch.autograd.Function):
         q, k, v = _loadable(q), _loadable(k), _loadable(v)
         out, out_lo, lse = _forward(q, k, v, seqs, causal, scale, True)
         ctx.save_for_backward(q, k, v, out, out_lo, lse)
-        ctx.cfg = (seqs, causal, scale)
+        ctx.cfg = (seqs, seqs.version, causal, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, out_lo, lse = ctx.saved_tensors
-        seqs, causal, scale = ctx.cfg
+        seqs, version, causal, scale = ctx.cfg
+        _check_version(seqs, version)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         _launch("cvh_packed_attn_bwd", seqs, scale, causal, q, k, v, out, out_lo, lse, torch.empty_like(lse), _loadable(dout), dq, dk, dv)
         return dq, dk, dv, None, None, None
@@ -154,14 +162,15 @@ class PackedAttentionQKVFn(torch.autograd.Function):
     def forward(ctx, qkv, heads, kv_heads, seqs, causal, scale):
         out, out_lo, lse = _forward(*_split_heads(qkv, heads, kv_heads), seqs, causal, scale, True)
         ctx.save_for_backward(qkv, out, out_lo, lse)
-        ctx.cfg = (heads, kv_heads, seqs, causal, scale)
+        ctx.cfg = (heads, kv_heads, seqs, seqs.version, causal, scale)
         return out.view(qkv.shape[0], -1)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         qkv, out, out_lo, lse = ctx.saved_tensors
-        heads, kv_heads, seqs, causal, scale = ctx.cfg
+        heads, kv_heads, seqs, version, causal, scale = ctx.cfg
+        _check_version(seqs, version)
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         out = out.view(qkv.shape[0], heads, -1)
         _launch("cvh_packed_attn_bwd", seqs, scale, causal, *_split_heads(qkv, heads, kv_heads), out, out_lo, lse, torch.empty_like(lse),
@@ -218,14 +227,16 @@ class PackedEmbedFn(torch.autograd.Function):
     def forward(ctx, table, pos, ids, seqs, scale, padding_idx, dtype):
         out = _lookup(table, pos, ids, seqs, scale, dtype)
         ctx.save_for_backward(ids)
-        ctx.cfg = (seqs, scale, -1 if padding_idx is None else padding_idx, table.shape[0], 0 if pos is None else pos.shape[0])
+        ctx.cfg = (seqs, 0 if seqs is None else seqs.version, scale, -1 if padding_idx is None else padding_idx, table.shape[0], 0 if pos is None else pos.shape[0])
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
-        seqs, scale, padding, vocab, positions = ctx.cfg
+        seqs, version, scale, padding, vocab, positions = ctx.cfg
+        if seqs is not None:
+            _check_version(seqs, version)
         dout = dout.contiguous()
         if dout.data_ptr() % 16:
             dout = dout.clone()

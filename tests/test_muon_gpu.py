@@ -77,6 +77,19 @@ def test_wide_tiles():
         assert err(x, steps64(u)) <= TOL[torch.float32]
 
 
+@pytest.mark.parametrize("shape", [(1100, 1150), (1700, 1500), (1930, 1950)])
+def test_tiles_of_single_large_matrices(shape):
+    """each kind of tile of the products, in both types and in the optimizer step; the values are bf16 ones, so that one reference serves all"""
+    u = gradient(*shape, seed=3, dtype=torch.bfloat16)
+    want = steps64(u)
+    assert err(optim.orthogonalize(u.float()), want) <= TOL[torch.float32]
+    assert err(optim.orthogonalize(u), want) <= tol(torch.bfloat16, u.numel())
+    p = torch.nn.Parameter(torch.zeros(shape, device="cuda"))
+    p.grad = u.float()
+    optim.Muon([p], lr=1.0, momentum=0.5, nesterov=False).step()
+    assert err(p, -max(1.0, shape[0] / shape[1]) ** 0.5 * want) <= TOL[torch.float32] + 2.0 ** -23  # (lr times gain, and the product with it)
+
+
 def test_steps_coefficients_and_eps():
     u = gradient(100, 200)
     assert err(optim.orthogonalize(u, steps=1), steps64(u, steps=1)) <= TOL[torch.float32]
@@ -145,6 +158,24 @@ def test_muon_state_dict_and_skipped_parameters():
         o.step()
     for a, b in zip(params, copies):
         assert torch.equal(a, b)
+
+
+def test_muon_refuses_what_changed_behind_its_back():
+    p, q = (torch.nn.Parameter(gradient(40, 30, seed=i)) for i in range(2))
+    opt = optim.Muon([{"params": [p]}, {"params": [q]}], lr=0.1)
+    p.grad = gradient(40, 30, seed=4)
+    opt.step()
+    before = p.detach().clone()
+    opt.param_groups[1]["momentum"] = 0.5
+    with pytest.raises(NotImplementedError, match="per-group momentum"):
+        opt.step()
+    opt.param_groups[1]["momentum"] = 0.95
+    p.grad = None
+    p.data = p.data[:20]  # the same address, another matrix
+    p.grad = gradient(20, 30, seed=4)
+    with pytest.raises(RuntimeError, match="another matrix"):
+        opt.step()
+    assert torch.equal(p, before[:20])
 
 
 def test_muon_step_in_a_graph():

@@ -199,6 +199,56 @@ def test_offsets_beyond_32_bits():
         close(a[19000:], b, torch.bfloat16, "far rows")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("course", ["rises", "falls", "jumps"])
+def test_scores_that_move_the_running_maximum(dtype, course):
+    """scores of up to 22 (32 in powers of two) that grow over the keys in small steps, fall, or jump from tile to tile
+
+    The keys are one direction times a height here, and the ds of a query add up to zero: dq = scale sum_j ds_j k_j is what is left of a sum whose terms
+    cancel.  Of the three roundings two (of ds, and of what delta is formed from) are of the terms, not of the result: uncorrelated over the terms, each
+    off by 2^-8 / sqrt(3) of itself in the mean square, they give 2^-8 / sqrt(3) scale sqrt(sum ds^2 |k|^2), which is A times 2^-8 / sqrt(3) |dq| with A from
+    the reference's own ds.  The three together: 2^-8 sqrt((1 + 2 A^2) / 3), 2^-8 for A = 1.  (Rounding nothing but the exact ds to bf16 and going
+    on in float64 gives 0.029, 0.053 and 0.086 of dq's norm for the three courses, with A = 17, 31 and 52.)  Float32: the same terms, the same A."""
+    n, d = 700, 64
+    g = torch.Generator(device="cuda").manual_seed(12)
+    j = torch.arange(n, device="cuda")
+    height = {"rises": 22.0 * j / n, "falls": 22.0 - 22.0 * j / n, "jumps": 22.0 * ((j // 32 * 5) % 8) / 8}[course]
+    e = torch.randint(0, 2, (d,), generator=g, device="cuda") * 2.0 - 1.0
+    q = (e / 8 + torch.randn(n, 2, d, generator=g, device="cuda") / 64).to(dtype)
+    k = (height[:, None, None] * e + torch.randn(n, 2, d, generator=g, device="cuda") / 4).to(dtype)
+    v, dout = make(n, 2, 2, d, dtype, seed=13)[2:]
+    want = reference(q, k, v, [n], True, 0.125, dout)
+    q64, k64, v64, d64 = (t.double().cpu().transpose(0, 1).contiguous() for t in (q, k, v, dout))
+    s64 = torch.matmul(q64, k64.transpose(1, 2).contiguous()) * 0.125
+    p64 = torch.softmax(s64.masked_fill(torch.ones(n, n, dtype=torch.bool).triu(1), -math.inf), -1)
+    dp64 = torch.matmul(d64, v64.transpose(1, 2).contiguous())
+    ds2 = (p64 * (dp64 - (p64 * dp64).sum(-1, keepdim=True))) ** 2
+    terms = float(((ds2.sum(1) * (k64 ** 2).sum(-1)).sum()).sqrt()) * 0.125
+    A = terms / float(want[1].norm())
+    q, k, v = (t.requires_grad_(True) for t in (q, k, v))
+    out = packed.attention(q, k, v, packed.PackedSeqs.from_lengths([n], "cuda"), scale=0.125)
+    for what, a, b in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, (q, k, v), dout)), want):
+        if what == "dq":
+            e = float((a.double().cpu() - b).norm() / b.norm())
+            assert e <= TOL[dtype] * math.sqrt((1 + 2 * A * A) / 3), (e, A)
+        else:
+            close(a, b, dtype, what)
+
+
+def test_a_refreshed_layout_refuses_the_backward_pass_of_an_earlier_forward():
+    q, k, v, dout = make(100, 2, 2, 32, torch.bfloat16, seed=14)
+    seqs = packed.PackedSeqs.from_lengths([60, 40], "cuda")
+    q.requires_grad_(True)
+    out = packed.attention(q, k, v, seqs)
+    table = torch.nn.Parameter(torch.randn(50, 32, device="cuda"))
+    emb = packed.embed(torch.arange(100, device="cuda") % 50, table, seqs)
+    both = packed.attention_qkv(torch.cat([q, k, v], 1).view(100, -1), 2, seqs)
+    seqs.refresh()
+    for y in (out, emb, both):
+        with pytest.raises(RuntimeError, match="refreshed between"):
+            y.sum().backward()
+
+
 def test_gradients_against_differences():
     lens, d = [9, 1, 40], 16
     q, k, v, dout = make(sum(lens), 4, 2, d, torch.float32, seed=21)

@@ -65,6 +65,17 @@ def test_packed_tower_equals_the_padded_one(dtype):
         assert rel(g1[k], g0[k]) <= TOL[dtype][1], (k, rel(g1[k], g0[k]))
 
 
+def test_boundaries_outside_the_rows_stay_inside_in_the_tower():
+    """the end marks come from the layout's clamped boundaries: a last one behind the rows is the last row"""
+    model = tower(torch.float32).eval()
+    tokens, seqs = model.pack_captions(captions(4, 24, 300))
+    cu = seqs.cu_seqlens.clone()
+    cu[-1] = 1 << 30
+    with torch.no_grad():
+        want, got = model.encode_packed(tokens, seqs), model.encode_packed(tokens, packed.PackedSeqs(cu, seqs.rows, max_len=24))
+    assert torch.equal(want, got)
+
+
 def test_packed_refusals_of_the_tower():
     model = tower(torch.bfloat16)
     tokens, seqs = model.pack_captions(captions(3, 24, 300))
