@@ -258,7 +258,8 @@ def embed(ids: Tensor, table: Tensor, seqs: Optional[PackedSeqs] = None, pos: Op
     """scale * table[ids] (+ pos[place in the sequence]): ids int64 [rows], table float32 [vocab, e], pos float32 [positions, e] ->
     [rows, e] in ``dtype`` (default: the compute dtype), differentiable in table and pos.  The gradient of the table is dense; it is summed in
     row order (bit-reproducible), and the row of ``padding_idx`` is zero, as with nn.Embedding.  pos needs ``seqs``.  The tokens live on the
-    device and are not read by the host: one outside the table (or a place behind the last position) gives a row of NaN and no gradient."""
+    device and are not read by the host: one outside the table (or a place behind the last position) gives a row of NaN; the gradient of the
+    table leaves out tokens outside it."""
     if ids.dim() != 1 or ids.dtype != torch.int64:
         raise RuntimeError(f"ids must be an int64 vector. Got: {ids.dtype} {list(ids.shape)}")
     if table.dim() != 2 or table.dtype != torch.float32 or table.shape[0] == 0:

@@ -3,8 +3,8 @@ of MIOpen's backward-data solver inside the torch REFERENCE of one kernel test, 
 the end of a segment.  The guard-page allocator (tools/guard_alloc.cpp: every tensor in its own address range, unmapped neighbours, no
 reuse after free) turns any such access into a fault at the launch that does it.  Under it:
   * the kernel tests of the library run clean — no operand is read or written out of bounds, no launch goes through a freed tensor;
-  * the torch-only reproduction of the reference passes with MIOpen off (the suite's configuration, tests/conftest.py).
-The MIOpen-on variant is reported, not asserted (a vendor fix would make it pass)."""
+  * the torch-only reference passes with MIOpen off (the suite's configuration, tests/conftest.py).
+The same reference with MIOpen on is not run: under this allocator its solver faults the GPU, and a fault can take the machine from whoever uses it."""
 import os
 import subprocess
 import sys
@@ -32,10 +32,6 @@ def test_reference_of_bn_eval_mode_is_clean_without_miopen():
     r = subprocess.run([sys.executable, os.path.join(REPO, "tools", "guard_aten_repro.py"), "--no-miopen"], env=_env(), capture_output=True,
                        text=True, timeout=300)
     assert r.returncode == 0 and "PASSED: no fault" in r.stdout, (r.stdout[-800:], r.stderr[-800:])
-    v = subprocess.run([sys.executable, os.path.join(REPO, "tools", "guard_aten_repro.py")], env=_env(), capture_output=True, text=True,
-                       timeout=300)
-    print("[guard] the same reference WITH MIOpen under the guard allocator:",
-          "no fault (vendor kernel fixed?)" if v.returncode == 0 else "faults (" + (v.stderr.strip().splitlines() or ["?"])[0][:120] + ")")
 
 
 @pytest.mark.parametrize("selection", ["tests/test_kernels_gpu.py::test_bn_eval_mode", "tests/test_kernels_gpu.py::test_conv_bn_act",
