@@ -14,7 +14,7 @@
 // double-buffered in LDS and loaded a tile ahead through registers.
 //
 // What bounds it (measured, MI355X): 128 columns, 20 k rows in 3 documents, 16 / 4 heads, causal forward: 613 us = 945 TFLOP/s of the 4 d a pair that have to
-// be computed; about half of the cycles MFMA, the other half softmax arithmetic, which two waves a SIMD overlap only in part.  64 columns, 24.6 k rows,
+// be computed; MFMA 48 %, arithmetic 43 %, LDS 48 % of the cycles, which two waves a SIMD overlap only in part.  Training there: 2640 us.  64 columns, 24.6 k rows,
 // 12 / 4 heads, training: forward 98, dq 130, dk / dv 191 us; a score costs an exponential and three other operations next to 1 / 4 of an MFMA.  128-row
 // workgroups: 4 waves share each staged tile; 64 keys (queries) a tile: at 64 columns 32 cost 20 % and 128 10 % in dk / dv, at 96 and 128 columns 32 cost 5 .. 8 % of
 // a whole training pass.  Captions (5 .. 77 tokens): one wave per 32 rows, 20 + 27 + 22 us for 13 k rows x 8 heads, latency.
@@ -90,9 +90,9 @@ __device__ __forceinline__ float frag_dot(const Frag<float>& a, const Frag<float
 //   cols(k0, col0):  the TRANSPOSE: column col0 + (l & 31), its rows in the order in which a 32x32 accumulator holds them: slot j of lane half h is row
 //                    k0 + 8 (j >> 2) + 4 h + (j & 3).  bf16: two LDS transpose reads (lane 4 r + q of a 16-lane group gives the address of 4 columns of
 //                    block row r and receives column 4 r + q of the 4 x 16 block).
-// bf16 rows are padded so that both kinds of reads find distinct banks: 16 rows x 16 bytes (the pitch an odd number of 16-byte units) and 4 rows x 32
-// bytes (0, 1, 2, 3 pitches at least 32 bytes apart in the 256 bytes of the banks).  16 bytes of padding do for 64 and 96 columns; with 128 they make
-// half of the forward's LDS cycles bank conflicts, 48 bytes none.  (An XOR of the 16-byte chunks with the row does the same without padding, at 30
+// bf16 rows are padded for the row reads, 16 rows x 16 bytes on distinct banks (the pitch an odd number of 16-byte units); the transpose reads, 4 rows x 64
+// bytes, would want another pitch (64 bytes past a multiple of 256) and conflict in a quarter of the LDS cycles, which do not bound the kernels.  16 bytes of
+// padding for 64 and 96 columns, 48 for 128 (half of the LDS cycles were conflicts with 16).  (An XOR of the 16-byte chunks with the row does the same without padding, at 30
 // more registers for the addresses: 164 instead of 128 and spills at 128 columns.)
 typedef short v4s_t __attribute__((ext_vector_type(4)));
 template <typename T, int CP> struct Tile;
