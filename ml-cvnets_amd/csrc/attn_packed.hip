@@ -674,7 +674,7 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
 }
 
 // -----------------------------------------------------------------------------------------------------------------------------------------
-// plan: starts[0 .. seqs] (clamped into 0 .. rows and made monotone, so that no kernel can be led out of its buffers), then the list of
+// plan: starts[0 .. seqs] (from 0, clamped into 0 .. rows and made monotone, so that no kernel can be led out of its buffers), then the list of
 // (sequence, block) pairs by falling block index, the filling blocks behind the last sequence as (-1, block), and (-2, 0) for unused places.
 // One workgroup; LDS counters give the places, whose order among equals does not matter (every item's results are its own).
 // -----------------------------------------------------------------------------------------------------------------------------------------
@@ -685,8 +685,9 @@ __global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(const int* __
   const int tid = threadIdx.x;
   // starts: running maximum over chunks of consecutive entries
   const int n = seqs + 1, per = (n + kPlanThreads - 1) / kPlanThreads, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+  auto boundary = [&](int i) { return i ? min(max(cu[i], 0), rows) : 0; };  // (the first one counts as 0: no row is without an owner)
   int top = 0;
-  for (int i = i0; i < i1; ++i) top = max(top, min(max(cu[i], 0), rows));
+  for (int i = i0; i < i1; ++i) top = max(top, boundary(i));
   part[tid] = top;
   for (int c = tid; c < kClasses; c += kPlanThreads) count[c] = 0;
   __syncthreads();
@@ -698,7 +699,7 @@ __global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(const int* __
   }
   int run = tid ? part[tid - 1] : 0;
   for (int i = i0; i < i1; ++i) {
-    run = max(run, min(max(cu[i], 0), rows));
+    run = max(run, boundary(i));
     plan[i] = run;
   }
   __threadfence_block();

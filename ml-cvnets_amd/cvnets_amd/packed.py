@@ -29,7 +29,8 @@ def _block_rows(rows: int, seqs: int, max_len: int) -> int:
 class PackedSeqs:
     """Boundaries of a batch of packed sequences.
 
-    cu_seqlens: int32 [sequences + 1] on the GPU, sequence b has the rows ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1`` (empty ones are allowed);
+    cu_seqlens: int32 [sequences + 1] on the GPU, sequence b has the rows ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1`` (empty ones are
+    allowed; the first boundary is 0, and counts as 0 whatever stands there);
     rows: the number of rows of the matrices that are used with it (>= cu_seqlens[-1]); max_len: an upper bound of the lengths, if one is
     known on the host - it only chooses the work list's block size, a wrong one costs time and no result.
 

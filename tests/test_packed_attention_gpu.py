@@ -181,6 +181,27 @@ def test_boundaries_from_the_device_are_clamped():
         assert bool((out[a + n:] == 0).all())
 
 
+def test_the_first_boundary_counts_as_zero():
+    """no row is left unwritten in front of the first sequence: attention, its gradients and the embedding equal those from boundary 0"""
+    rows, d = 90, 32
+    q, k, v, dout = make(rows, 2, 1, d, torch.float32, seed=15)
+    table = torch.nn.Parameter(torch.randn(30, 2 * d, device="cuda"))
+    ids = torch.arange(rows, device="cuda") % 30
+    got = []
+    for first in (0, 17):
+        for block in (32, 128):
+            seqs = layout(torch.tensor([first, 40, 75], dtype=torch.int32, device="cuda"), rows, block)
+            junk = torch.full((4 << 20,), float("nan"), device="cuda")  # (freed: what an unwritten result would be made of)
+            del junk
+            t = [x.detach().requires_grad_(True) for x in (q, k, v)]
+            out = packed.attention(*t, seqs)
+            emb = packed.embed(ids, table, seqs, dtype=torch.float32)
+            got.append((out.detach(), *torch.autograd.grad(out, t, dout), emb.detach(), *torch.autograd.grad(emb, (table,), dout.view(rows, -1))))
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert torch.isfinite(b).all() and float((a - b).abs().max()) <= TOL[torch.float32] * float(a.abs().max())
+
+
 def test_offsets_beyond_32_bits():
     """rows 2^17 elements apart: the last sequence lies 5 GB behind the base"""
     rows, stride, d = 20000, 1 << 17, 64
