@@ -454,7 +454,7 @@ typedef struct cvh_packed_attn {
   float scale; /* > 0 */
 } cvh_packed_attn;
 /* Work list of a batch of packed sequences in blocks of 32 or 128 rows: int32 plan[cvh_packed_plan_elems(...)] from cu[seqs + 1] (device, int32).
- * Boundaries outside 0 .. rows are clamped and falling ones lifted to the largest before them, so that no list leads out of the buffers;
+ * cu[0] counts as 0, boundaries outside 0 .. rows are clamped and falling ones lifted to the largest before them: no list leads out of the buffers;
  * `places` of the struct above is rows / block + seqs + 1.  Made once per batch, read by every layer and both directions. */
 long long cvh_packed_plan_elems(int seqs, int rows, int block);
 int cvh_packed_plan(const int* cu, int seqs, int rows, int block, int* plan, void* stream);
