@@ -371,7 +371,8 @@ int cvh_lerp_multi(const long long* table, int n_tensors, long long total, float
 /* A list of matrices, row-major and contiguous: Newton-Schulz steps x <- (a I + b x x^T + c (x x^T)^2) x from x = u / (|u|_F + eps), the shorter
  * side as rows.  cvh_orthogonalize: u = src, dst = x (both of `dtype`; dst may be src).  cvh_muon_step (float32): momentum <- mu momentum + src
  * (src = the gradient), u = src + mu momentum (nesterov) or momentum, param <- (1 - lr wd) param - lr gain x, with {lr, wd} =
- * group_hp[group] on the device.  Coefficients with |a| + |b| + |c| <= 15 whose steps keep singular values below 15.  `mats` is a HOST array (read
+ * group_hp[group] on the device.  Coefficients with |a| + |b| + |c| <= 15 whose steps keep singular values that start in 0 .. 1 below 15 in front of
+ * every step (behind the last one they may be larger): cvh_ns_bounded says 1, others are refused.  `mats` is a HOST array (read
  * during the call only); ws: cvh_ns_workspace_elems float32 of device memory, 256-byte aligned; its contents do not have to survive. */
 typedef struct cvh_ns_matrix {
   const void* src;
@@ -380,6 +381,7 @@ typedef struct cvh_ns_matrix {
   int rows, cols, group;
   float gain;
 } cvh_ns_matrix;
+int cvh_ns_bounded(int steps, float a, float b, float c);
 long long cvh_ns_workspace_elems(const cvh_ns_matrix* mats, int n);
 int cvh_orthogonalize(int dtype, const cvh_ns_matrix* mats, int n, int steps, float a, float b, float c, float eps, float* ws, void* stream);
 int cvh_muon_step(const cvh_ns_matrix* mats, int n, int steps, float a, float b, float c, float eps, float momentum, int nesterov, const float* group_hp,

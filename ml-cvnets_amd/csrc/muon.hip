@@ -5,8 +5,8 @@
 //   result = x   or   w <- (1 - lr wd) w - lr gain x
 //
 // G and P are symmetric and commute: half of their tiles are computed and written twice.  Operands are kept as pairs of fp16 numbers, hi + lo,
-// of the value times a power of two (2^12 for x and G, 2^10 for P: singular values below 16 and |P|_2 below 64 stay under fp16's 65504, and an
-// entry of ordinary size stays far above its subnormals): 22 bits and a sign, and a product is three MFMAs, hi hi + hi lo + lo hi, accumulated in float32 - within a factor of two of a
+// of the value times a power of two (x: 2^12, so that singular values below 16 stay under fp16's 65504 and an entry of ordinary size far above its
+// subnormals; G and P: 2^12 and 2^10, or what the coefficients leave room for, see Bounds): 22 bits and a sign, and a product is three MFMAs, hi hi + hi lo + lo hi, accumulated in float32 - within a factor of two of a
 // float32 product's error, at a third of the fp16 matrix rate instead of the float32 matrix rate (measured on 8192-cubed library products: 1081 / 3
 // = 360 against 154 TFLOP/s).  One fp16 or bf16 product per step would be three times as fast, and its rounding (2^-11 and 2^-8) is multiplied by up to
 // a^steps = 485 in the directions of small singular values.
@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kMats = 32;
 constexpr int kMostRows = 1 << 14, kMostCols = 1 << 20;  // of the shorter and the longer side
-constexpr float kScale = 4096.f, kScaleP = 1024.f;  // of x and G; of P
+constexpr float kScale = 4096.f;  // of x
 typedef _Float16 half_t;
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
@@ -401,8 +401,9 @@ __device__ __forceinline__ void triangle_tile(int at, int n, int& i, int& j) {
   }
 }
 
-// G = x x^T (POLY false) or P = b G + c G G (true): tiles (i, j <= i), written to both halves
-template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVES, 2) void ns_sym_kernel(const Mats* __restrict__ list, int which, float cb, float cc) {
+// G = x x^T (POLY false) or P = b G + c G G (true): tiles (i, j <= i), written to both halves.  scale_g, scale_p: what G and P are stored times.
+template <int TILE, int WAVES, bool POLY>
+__global__ __launch_bounds__(64 * WAVES, 2) void ns_sym_kernel(const Mats* __restrict__ list, int which, float cb, float cc, float scale_g, float scale_p) {
   const Mats& t = *list;
   typedef Product<TILE, TILE, WAVES, false> Prod;
   __shared__ __attribute__((aligned(16))) char smem[Prod::BYTES];
@@ -429,16 +430,17 @@ template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVE
     }
   }
   float* const v = p.spill(tid);  // v[j][i]
+  const float unscale = POLY ? 1.f / scale_g : scale_g / (kScale * kScale), rescale = scale_p / scale_g;  // (powers of two: exact)
 #pragma unroll
   for (int q = 0; q < PIECES; ++q) {
     const int idx = tid + q * Prod::NT, j = idx / (TILE / 8), i = idx % (TILE / 8) * 8;
     const size_t o = place(j0 + j, i0 + i, a.mp);
     float w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = v[j * Prod::OPITCH + i + e] * (1.f / kScale);
+    for (int e = 0; e < 8; ++e) w[e] = v[j * Prod::OPITCH + i + e] * unscale;
     if (POLY) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = (kScaleP / kScale) * (cc * w[e] + cb * ((float)gh[q][e] + (float)gl[q][e]));
+      for (int e = 0; e < 8; ++e) w[e] = rescale * (cc * w[e] + cb * ((float)gh[q][e] + (float)gl[q][e]));
     }
     half8_t hi, lo;
     split8(w, hi, lo);
@@ -466,7 +468,7 @@ template <int TILE, int WAVES, bool POLY> __global__ __launch_bounds__(64 * WAVE
 }
 
 // x <- a x + P x; the last one writes the result instead
-template <int TI, int TJ, int WAVES, typename T, int LAST> __global__ __launch_bounds__(64 * WAVES, 2) void ns_apply_kernel(const Mats* __restrict__ list, int which, float ca, const float* __restrict__ hp) {
+template <int TI, int TJ, int WAVES, typename T, int LAST> __global__ __launch_bounds__(64 * WAVES, 2) void ns_apply_kernel(const Mats* __restrict__ list, int which, float ca, float scale_p, const float* __restrict__ hp) {
   const Mats& t = *list;
   typedef Product<TJ, TI, WAVES, true> Prod;
   __shared__ __attribute__((aligned(16))) char smem[Prod::BYTES];
@@ -490,13 +492,14 @@ template <int TI, int TJ, int WAVES, typename T, int LAST> __global__ __launch_b
   }
   float* const v = p.spill(tid);  // v[i][j]
   ghalf_t* const next = x_of(a, which ^ 1);
+  const float unscale = 1.f / scale_p;
 #pragma unroll
   for (int q = 0; q < PIECES; ++q) {
     const int idx = tid + q * Prod::NT, i = idx / (TJ / 8), j = idx % (TJ / 8) * 8;
     const size_t o = place(i0 + i, j0 + j, a.np);
     float w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = fmaf(ca, (float)xh[q][e] + (float)xl[q][e], v[i * Prod::OPITCH + j + e] * (1.f / kScaleP));
+    for (int e = 0; e < 8; ++e) w[e] = fmaf(ca, (float)xh[q][e] + (float)xl[q][e], v[i * Prod::OPITCH + j + e] * unscale);
     if (LAST == 0) {
       half8_t hi, lo;
       split8(w, hi, lo);
@@ -573,14 +576,61 @@ template <typename F> long long wide_tiles(const Mats& t, F&& tiles) {  // 0: no
 template <int TILE> int sym_tiles(const Mat& q) { return q.mp / TILE * (q.mp / TILE + 1) / 2; }
 template <int TI, int TJ> int all_tiles(const Mat& q) { return q.mp / TI * (q.np / TJ); }
 
-template <int TILE, int WAVES> void run_sym(const Mats* list, int n, int which, float b, float c, hipStream_t st) {
-  ns_sym_kernel<TILE, WAVES, false><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, which, b, c);
-  ns_sym_kernel<TILE, WAVES, true><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, which, b, c);
+// What a step's G and P can reach: the singular values in front of it lie in 0 .. most (1 in front of the first step), those behind it in 0 .. the largest
+// |a s + b s^3 + c s^5| there.  Each is stored times 2^12 (2^10), or times the largest smaller power of two that keeps it under fp16's 65504 (a tenth of
+// it left for rounding): G is the SQUARE of x, 225 where a singular value is 15, and P of the last step whatever the coefficients make of that.  With
+// NS_COEFFICIENTS singular values stay below 1.3, and both scales are the large ones.
+constexpr double kMostSingular = 15.0;
+struct Bounds {
+  double a, b, c, most = 1.0;
+  Bounds(double a_, double b_, double c_) : a(a_), b(b_), c(c_) {}
+  static float scale(double value, float largest) {
+    float s = largest;
+    while (value * s > 60000.0) s *= 0.5f;
+    return s;
+  }
+  float scale_g() const { return scale(most * most, 4096.f); }
+  float scale_p() const {  // of b t + c t^2 for t = s^2: at the end, or at the vertex in front of it
+    const double end = most * most, vertex = c != 0.0 ? -b / (2.0 * c) : -1.0;
+    return scale(fmax(fabs(b * end + c * end * end), vertex > 0.0 && vertex < end ? fabs(b * vertex / 2.0) : 0.0), 1024.f);
+  }
+  void step() {
+    const double end = most * most;
+    double m = fabs(a + b * end + c * end * end) * most;
+    auto at = [&](double t) {  // a place where the derivative a + 3 b t + 5 c t^2 is zero
+      if (t > 0.0 && t < end) m = fmax(m, fabs(a + b * t + c * t * t) * sqrt(t));
+    };
+    const double root = 9.0 * b * b - 20.0 * a * c;
+    if (c == 0.0) {
+      if (b != 0.0) at(-a / (3.0 * b));
+    } else if (root >= 0.0) {
+      const double q = -0.5 * (3.0 * b + (b < 0.0 ? -sqrt(root) : sqrt(root)));
+      at(q / (5.0 * c));
+      if (q != 0.0) at(a / q);
+    }
+    most = m;
+  }
+};
+// singular values stay below kMostSingular in front of every step (behind the last one they may be anything: the result is not an fp16 pair)
+bool stays_small(int steps, double a, double b, double c) {
+  Bounds bounds(a, b, c);
+  for (int s = 1; s < steps; ++s) {
+    const double before = bounds.most;
+    bounds.step();
+    if (!(bounds.most <= kMostSingular)) return false;
+    if (bounds.most == before) break;  // the same interval again, for good
+  }
+  return true;
 }
-template <typename T, int LAST> void run_apply(int tile, const Mats* list, int n, int which, float a, const float* hp, hipStream_t st) {
-  if (tile == SQUARE_128) ns_apply_kernel<128, 128, 8, T, LAST><<<dim3(n), dim3(512), 0, st>>>(list, which, a, hp);
-  else if (tile == TALL) ns_apply_kernel<128, 64, 4, T, LAST><<<dim3(n), dim3(256), 0, st>>>(list, which, a, hp);
-  else ns_apply_kernel<64, 64, 4, T, LAST><<<dim3(n), dim3(256), 0, st>>>(list, which, a, hp);
+
+template <int TILE, int WAVES> void run_sym(const Mats* list, int n, int which, float b, float c, const Bounds& at, hipStream_t st) {
+  ns_sym_kernel<TILE, WAVES, false><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, which, b, c, at.scale_g(), at.scale_p());
+  ns_sym_kernel<TILE, WAVES, true><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, which, b, c, at.scale_g(), at.scale_p());
+}
+template <typename T, int LAST> void run_apply(int tile, const Mats* list, int n, int which, float a, float scale_p, const float* hp, hipStream_t st) {
+  if (tile == SQUARE_128) ns_apply_kernel<128, 128, 8, T, LAST><<<dim3(n), dim3(512), 0, st>>>(list, which, a, scale_p, hp);
+  else if (tile == TALL) ns_apply_kernel<128, 64, 4, T, LAST><<<dim3(n), dim3(256), 0, st>>>(list, which, a, scale_p, hp);
+  else ns_apply_kernel<64, 64, 4, T, LAST><<<dim3(n), dim3(256), 0, st>>>(list, which, a, scale_p, hp);
 }
 template <typename T, bool MOM> int run_list(Mats& t, Mats* list, int steps, float a, float b, float c, float eps, float mu, int nesterov, const float* hp, hipStream_t st) {
   const bool ws = wide_tiles(t, sym_tiles<128>) >= kWideSym;
@@ -593,11 +643,12 @@ template <typename T, bool MOM> int run_list(Mats& t, Mats* list, int steps, flo
   ns_norm_kernel<T, MOM><<<dim3(norms), dim3(256), 0, st>>>(t, list, mu, nesterov);
   ns_scale_kernel<T, MOM><<<dim3(scales), dim3(256), 0, st>>>(list, mu, nesterov, eps);
   constexpr int LAST = MOM ? 2 : 1;
-  for (int s = 0; s < steps; ++s) {
-    if (ws) run_sym<128, 8>(list, syms, s & 1, b, c, st);
-    else run_sym<64, 4>(list, syms, s & 1, b, c, st);
-    if (s + 1 < steps) run_apply<T, 0>(wa, list, applies, s & 1, a, hp, st);
-    else run_apply<T, LAST>(wa, list, applies, s & 1, a, hp, st);
+  Bounds at(a, b, c);
+  for (int s = 0; s < steps; ++s, at.step()) {
+    if (ws) run_sym<128, 8>(list, syms, s & 1, b, c, at, st);
+    else run_sym<64, 4>(list, syms, s & 1, b, c, at, st);
+    if (s + 1 < steps) run_apply<T, 0>(wa, list, applies, s & 1, a, at.scale_p(), hp, st);
+    else run_apply<T, LAST>(wa, list, applies, s & 1, a, at.scale_p(), hp, st);
   }
   CVH_CHECK_LAUNCH();
   return 0;
@@ -631,7 +682,7 @@ int run_all(const cvh_ns_matrix* mats, int n, int steps, float a, float b, float
 }
 
 int check(const cvh_ns_matrix* mats, int n, int steps, float a, float b, float c, float eps, bool step) {
-  if (mats == nullptr || n <= 0 || steps <= 0 || !(eps >= 0.f) || !(fabsf(a) + fabsf(b) + fabsf(c) <= 15.f)) return -2;
+  if (mats == nullptr || n <= 0 || steps <= 0 || !(eps >= 0.f) || !(fabsf(a) + fabsf(b) + fabsf(c) <= 15.f) || !stays_small(steps, a, b, c)) return -2;
   for (int i = 0; i < n; ++i) {
     const cvh_ns_matrix& q = mats[i];
     if (q.rows <= 0 || q.cols <= 0 || (q.rows > kMostRows && q.cols > kMostRows) || q.rows > kMostCols || q.cols > kMostCols || q.src == nullptr) return -2;
@@ -642,6 +693,7 @@ int check(const cvh_ns_matrix* mats, int n, int steps, float a, float b, float c
 
 }  // namespace
 
+extern "C" int cvh_ns_bounded(int steps, float a, float b, float c) { return steps > 0 && stays_small(steps, a, b, c) ? 1 : 0; }
 extern "C" long long cvh_ns_workspace_elems(const cvh_ns_matrix* mats, int n) {
   if (mats == nullptr || n <= 0) return -2;
   long long bytes = (n + kMats - 1) / kMats * kListBytes;

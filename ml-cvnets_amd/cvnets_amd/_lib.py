@@ -144,6 +144,7 @@ SIGNATURES = {
     "cvh_embed_pieces_elems": [I, I, I, I],
     "cvh_embed_packed_fwd": [I, P, P, P, P, I, I, I, I, I, I, I, F, P, P],
     "cvh_embed_packed_bwd": [I, P, P, P, I, I, I, I, L, F, P, I, P, P, P, P],
+    "cvh_ns_bounded": [I, F, F, F],
     "cvh_ns_workspace_elems": [P, I],
     "cvh_orthogonalize": [I, P, I, I, F, F, F, F, P, P],
     "cvh_muon_step": [P, I, I, F, F, F, F, F, I, P, P, P],

@@ -263,6 +263,8 @@ def _check_ns(steps: int, coefficients: Sequence[float], eps: float) -> Tuple[in
         raise ValueError(f"coefficients with |a| + |b| + |c| <= 15 are supported. Got: {tuple(coefficients)}")
     if not 0.0 <= eps < math.inf:
         raise ValueError(f"eps must not be negative. Got: {eps}")
+    if not _lib.query("cvh_ns_bounded", int(steps), a, b, c):
+        raise ValueError(f"coefficients whose steps let singular values grow beyond 15 in front of another step are not supported. Got: {tuple(coefficients)}, {steps} steps")
     return int(steps), a, b, c, float(eps)
 
 
@@ -282,7 +284,7 @@ def orthogonalize(matrices: Union[torch.Tensor, Sequence[torch.Tensor]], steps: 
     """Newton-Schulz orthogonalisation of matrices (one or a list of any shapes, all float32 or all bfloat16): x = u / (|u|_F + eps), then ``steps``
     times x <- (a I + b x x^T + c (x x^T)^2) x, the shorter side as rows.  The products are computed to float32 accuracy whatever the type
     of the matrices; the result has their type.  A list takes as many launches as one matrix.  A NaN or an infinity in a matrix makes its whole
-    result NaN (and no other's).  Coefficients whose steps let singular values grow beyond 15 are not supported."""
+    result NaN (and no other's).  Coefficients whose steps let singular values grow beyond 15 in front of another step are refused."""
     single = isinstance(matrices, torch.Tensor)
     mats = [matrices] if single else list(matrices)
     cfg = _check_ns(steps, coefficients, eps)

@@ -1,0 +1,46 @@
+"""What the orthogonalised update takes and refuses, without a GPU."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from cvnets_amd import _lib, optim
+
+
+def largest(steps, coefficients, points=200001):
+    """the largest singular value in front of the steps 2 .. `steps`, from points of 0 .. 1"""
+    a, b, c = coefficients
+    top, most = 1.0, 1.0
+    for _ in range(steps - 1):
+        s = np.linspace(0.0, top, points)
+        top = float(np.abs(a * s + b * s ** 3 + c * s ** 5).max())
+        most = max(most, top)
+    return most
+
+
+CASES = [(5, optim.NS_COEFFICIENTS), (50, optim.NS_COEFFICIENTS), (12, (1.875, -1.25, 0.375)), (30, (1.5, -0.5, 0.0)), (2, (5.0, -0.1, 0.0)), (3, (5.0, -0.1, 0.0)),
+         (4, (5.0, -0.1, 0.0)), (4, (2.0, 0.0, 0.0)), (6, (2.0, 0.0, 0.0)), (2, (14.0, 0.5, 0.5)), (3, (14.0, 0.5, 0.5)), (1, (0.0, 0.0, -15.0)), (9, (0.0, 0.0, 0.0)),
+         (4, (-3.0, 2.0, 0.1)), (5, (3.0, -3.5, 0.9)), (6, (-1.0, -2.0, 4.0)), (3, (0.0, 3.0, -1.0)), (7, (4.0, -6.0, 3.0))]
+
+
+@pytest.mark.parametrize("steps,coefficients", CASES)
+def test_coefficients_that_let_singular_values_grow_are_refused(steps, coefficients):
+    bounded = largest(steps, coefficients) <= 15.0
+    assert bool(_lib.load().cvh_ns_bounded(steps, *coefficients)) == bounded
+    u = torch.zeros(4, 6)
+    with pytest.raises(RuntimeError if bounded else ValueError):  # (bounded: the next refusal is that of a CPU tensor)
+        optim.orthogonalize(u, steps=steps, coefficients=coefficients)
+    p = torch.nn.Parameter(u)
+    if bounded:
+        optim.Muon([p], ns_steps=steps, ns_coefficients=coefficients)
+    else:
+        with pytest.raises(ValueError, match="grow beyond"):
+            optim.Muon([p], ns_steps=steps, ns_coefficients=coefficients)
+        m = (_lib.NsMatrix * 1)(_lib.NsMatrix(src=256, dst=256, momentum=256, param=256, rows=4, cols=6))
+        assert _lib.load().cvh_orthogonalize(0, ctypes.byref(m), 1, steps, *coefficients, 1e-7, 256, None) == -2
+        assert _lib.load().cvh_muon_step(ctypes.byref(m), 1, steps, *coefficients, 1e-7, 0.9, 1, 256, 256, None) == -2
+
+
+def test_both_sides_of_the_bound_are_among_the_cases():
+    assert {largest(*c) <= 15.0 for c in CASES} == {True, False}
