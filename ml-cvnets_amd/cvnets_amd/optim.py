@@ -410,7 +410,7 @@ class Muon(torch.optim.Optimizer):
         plan = self._plan
         if plan is None or plan["key"] != self._key(entries):
             plan = self._build(entries)
-        if sync_hyperparameters or self._hp is None:
+        if sync_hyperparameters or self._hp is None or len(self._hp) < len(self.param_groups):  # (the kernels read the row of every group)
             self.sync_hyperparameters()
         g0 = self.param_groups[0]
         for g in self.param_groups:  # (they may be rewritten, or loaded)

@@ -1,5 +1,6 @@
 """What the orthogonalised update takes and refuses, without a GPU."""
 import ctypes
+import gc
 
 import numpy as np
 import pytest
@@ -44,3 +45,33 @@ def test_coefficients_that_let_singular_values_grow_are_refused(steps, coefficie
 
 def test_both_sides_of_the_bound_are_among_the_cases():
     assert {largest(*c) <= 15.0 for c in CASES} == {True, False}
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """steps on CPU tensors up to the launch: the arguments that the kernels would get"""
+    seen = []
+    monkeypatch.setattr(optim.ops, "_check_dev", lambda t: None)
+    monkeypatch.setattr(optim.ops, "call_on", lambda dev, name, *args: seen.append((name, *args)))
+    return seen
+
+
+def tensor_at(address):
+    return next(t for t in gc.get_objects() if isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.numel() and t.data_ptr() == address)
+
+
+def with_gradient(*shape):
+    p = torch.nn.Parameter(torch.ones(shape))
+    p.grad = torch.ones(shape)
+    return p
+
+
+def test_the_rates_of_a_group_that_was_added_are_handed_over(launches):
+    """a step without synchronisation behind add_param_group: the kernels read the new group's row of the table, so there has to be one"""
+    opt = optim.Muon([with_gradient(4, 6)], lr=0.5)
+    opt.step()
+    opt.add_param_group({"params": [with_gradient(6, 4)], "lr": 0.25, "weight_decay": 0.125})
+    opt.step(sync_hyperparameters=False)
+    table, rates = launches[-1][1]._obj, tensor_at(launches[-1][-2])
+    assert sorted(table[i].group for i in range(2)) == [0, 1]
+    assert rates[:2].tolist() == [[0.5, 0.0], [0.25, 0.125]]
