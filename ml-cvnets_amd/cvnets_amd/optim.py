@@ -324,8 +324,8 @@ class Muon(torch.optim.Optimizer):
             raise ValueError(f"lr and weight_decay must not be negative, momentum in [0, 1). Got: {lr}, {weight_decay}, {momentum}")
         self._ns = _check_ns(ns_steps, ns_coefficients, eps)
         self._plan = None
-        self._hp = self._hp_host = None
-        self._workspaces = []  # every one that was handed to the kernels: a captured step goes on using its own
+        self._rates = []  # [device table of (lr, weight_decay) by group, its values], the newest last
+        self._workspaces = []  # every one that was handed to the kernels: a captured step goes on using its own (and its own table of rates)
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=bool(nesterov), weight_decay=weight_decay))
 
     def add_param_group(self, param_group) -> None:
@@ -382,14 +382,16 @@ class Muon(torch.optim.Optimizer):
         return [(p.data_ptr(), p.shape, g.data_ptr(), self.state[p]["momentum_buffer"].data_ptr() if "momentum_buffer" in self.state[p] else 0, gi) for p, g, gi in entries]
 
     def sync_hyperparameters(self) -> None:
-        """copy the groups' (lr, weight_decay) to the device table; call after a scheduler changed them (outside graph replay)"""
+        """copy the groups' (lr, weight_decay) to the device tables; call after a scheduler changed them (outside graph replay)"""
         host = [[float(g["lr"]), float(g["weight_decay"])] for g in self.param_groups]
-        if self._hp is None or len(self._hp) != len(host):
-            self._hp = torch.zeros(len(host), 2, dtype=torch.float32, device=self.param_groups[0]["params"][0].device)
-            self._hp_host = None
-        if host != self._hp_host:
-            self._hp.copy_(torch.tensor(host, dtype=torch.float32), non_blocking=True)  # plumbing: 2 floats per group
-            self._hp_host = host
+        if not self._rates or len(self._rates[-1][0]) < len(host):  # (groups were added; a table has room for all of its step's groups)
+            device = next(p.device for g in self.param_groups for p in g["params"])
+            self._rates.append([torch.zeros(len(host), 2, dtype=torch.float32, device=device), None])
+        for entry in self._rates:
+            table, values = entry[0], host[:len(entry[0])]
+            if values != entry[1]:
+                table[:len(values)].copy_(torch.tensor(values, dtype=torch.float32), non_blocking=True)  # plumbing: 2 floats per group
+                entry[1] = values
 
     @torch.no_grad()
     def step(self, closure=None, sync_hyperparameters: bool = True):
@@ -410,12 +412,12 @@ class Muon(torch.optim.Optimizer):
         plan = self._plan
         if plan is None or plan["key"] != self._key(entries):
             plan = self._build(entries)
-        if sync_hyperparameters or self._hp is None or len(self._hp) < len(self.param_groups):  # (the kernels read the row of every group)
+        if sync_hyperparameters or not self._rates or len(self._rates[-1][0]) < len(self.param_groups):  # (the kernels read the row of every group)
             self.sync_hyperparameters()
         g0 = self.param_groups[0]
         for g in self.param_groups:  # (they may be rewritten, or loaded)
             if (g["momentum"], g["nesterov"]) != (g0["momentum"], g0["nesterov"]):
                 raise NotImplementedError("per-group momentum / nesterov are not supported")
-        ops.call_on(dev, "cvh_muon_step", ctypes.byref(plan["table"]), plan["n"], *self._ns, float(g0["momentum"]), int(g0["nesterov"]), _p(self._hp), _p(plan["ws"]))
+        ops.call_on(dev, "cvh_muon_step", ctypes.byref(plan["table"]), plan["n"], *self._ns, float(g0["momentum"]), int(g0["nesterov"]), _p(self._rates[-1][0]), _p(plan["ws"]))
         ops.invalidate_packed()
         return loss

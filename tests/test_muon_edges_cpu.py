@@ -1,6 +1,7 @@
 """What the orthogonalised update takes and refuses, without a GPU."""
 import ctypes
 import gc
+import weakref
 
 import numpy as np
 import pytest
@@ -75,3 +76,19 @@ def test_the_rates_of_a_group_that_was_added_are_handed_over(launches):
     table, rates = launches[-1][1]._obj, tensor_at(launches[-1][-2])
     assert sorted(table[i].group for i in range(2)) == [0, 1]
     assert rates[:2].tolist() == [[0.5, 0.0], [0.25, 0.125]]
+
+
+def test_a_captured_step_keeps_its_table_of_rates(launches):
+    """what a capture holds is the table's address: the table stays, and follows sync_hyperparameters(), after groups were added"""
+    opt = optim.Muon([with_gradient(4, 6)], lr=0.5)
+    opt.step()
+    address = launches[-1][-2]
+    held = weakref.ref(tensor_at(address))
+    opt.add_param_group({"params": [with_gradient(6, 4)], "lr": 0.25})
+    opt.step()
+    gc.collect()
+    assert held() is not None
+    opt.param_groups[0]["lr"], opt.param_groups[0]["weight_decay"] = 0.125, 0.0625
+    opt.sync_hyperparameters()
+    assert tensor_at(address)[0].tolist() == [0.125, 0.0625]
+    assert tensor_at(launches[-1][-2]).tolist() == [[0.125, 0.0625], [0.25, 0.0]]
