@@ -381,11 +381,15 @@ class Muon(torch.optim.Optimizer):
     def _key(self, entries):
         return [(p.data_ptr(), p.shape, g.data_ptr(), self.state[p]["momentum_buffer"].data_ptr() if "momentum_buffer" in self.state[p] else 0, gi) for p, g, gi in entries]
 
+    def _has_rates(self, device) -> bool:
+        """whether the newest table has a row for every group (the kernels read it), where the parameters are"""
+        return bool(self._rates) and len(self._rates[-1][0]) >= len(self.param_groups) and self._rates[-1][0].device == device
+
     def sync_hyperparameters(self) -> None:
         """copy the groups' (lr, weight_decay) to the device tables; call after a scheduler changed them (outside graph replay)"""
         host = [[float(g["lr"]), float(g["weight_decay"])] for g in self.param_groups]
-        if not self._rates or len(self._rates[-1][0]) < len(host):  # (groups were added; a table has room for all of its step's groups)
-            device = next(p.device for g in self.param_groups for p in g["params"])
+        device = next(p.device for g in self.param_groups for p in g["params"])
+        if not self._has_rates(device):
             self._rates.append([torch.zeros(len(host), 2, dtype=torch.float32, device=device), None])
         for entry in self._rates:
             table, values = entry[0], host[:len(entry[0])]
@@ -412,7 +416,7 @@ class Muon(torch.optim.Optimizer):
         plan = self._plan
         if plan is None or plan["key"] != self._key(entries):
             plan = self._build(entries)
-        if sync_hyperparameters or not self._rates or len(self._rates[-1][0]) < len(self.param_groups):  # (the kernels read the row of every group)
+        if sync_hyperparameters or not self._has_rates(dev):
             self.sync_hyperparameters()
         g0 = self.param_groups[0]
         for g in self.param_groups:  # (they may be rewritten, or loaded)

@@ -92,3 +92,15 @@ def test_a_captured_step_keeps_its_table_of_rates(launches):
     opt.sync_hyperparameters()
     assert tensor_at(address)[0].tolist() == [0.125, 0.0625]
     assert tensor_at(launches[-1][-2]).tolist() == [[0.125, 0.0625], [0.25, 0.0]]
+
+
+def test_the_table_of_rates_is_on_the_parameters_device(launches):
+    p = with_gradient(4, 6)
+    opt = optim.Muon([p], lr=0.5)
+    opt.step()
+    with torch.no_grad():
+        moved = torch.nn.Parameter(torch.ones(4, 6, device="meta"))
+        moved.grad = torch.ones(4, 6, device="meta")
+    opt.param_groups[0]["params"][0] = moved  # (what a module's .to(device) leaves behind where it replaces its parameters)
+    opt.step(sync_hyperparameters=False)
+    assert opt._rates[-1][0].device == moved.device
