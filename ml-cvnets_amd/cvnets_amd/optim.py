@@ -379,7 +379,9 @@ class Muon(torch.optim.Optimizer):
         return self._plan
 
     def _key(self, entries):
-        return [(p.data_ptr(), p.shape, g.data_ptr(), self.state[p]["momentum_buffer"].data_ptr() if "momentum_buffer" in self.state[p] else 0, gi) for p, g, gi in entries]
+        """what the plan holds: addresses, and the layouts that stand behind them (a square matrix's transposed view has its address and shape)"""
+        bufs = [self.state[p].get("momentum_buffer") for p, _, _ in entries]
+        return [(p.data_ptr(), p.shape, p.stride(), g.data_ptr(), gi, None if m is None else (m.data_ptr(), m.shape, m.stride(), m.dtype)) for (p, g, gi), m in zip(entries, bufs)]
 
     def _has_rates(self, device) -> bool:
         """whether the newest table has a row for every group (the kernels read it), where the parameters are"""

@@ -104,3 +104,23 @@ def test_the_table_of_rates_is_on_the_parameters_device(launches):
     opt.param_groups[0]["params"][0] = moved  # (what a module's .to(device) leaves behind where it replaces its parameters)
     opt.step(sync_hyperparameters=False)
     assert opt._rates[-1][0].device == moved.device
+
+
+def test_a_transposed_square_parameter_or_momentum_is_refused(launches):
+    """the same address and shape, another matrix"""
+    p = with_gradient(4, 4)
+    opt = optim.Muon([p], lr=0.5)
+    opt.step()
+    p.data = p.data.t()
+    with pytest.raises(RuntimeError, match="another matrix"):
+        opt.step()
+    p.data = p.data.t()
+    opt.step()
+    opt.state[p]["momentum_buffer"] = torch.arange(16.0).view(4, 4).t()  # (a state that somebody else wrote: laid out again, the same values)
+    opt.step()
+    assert opt.state[p]["momentum_buffer"].is_contiguous() and torch.equal(opt.state[p]["momentum_buffer"], torch.arange(16.0).view(4, 4).t())
+    opt.state[p]["momentum_buffer"] = opt.state[p]["momentum_buffer"].t()  # the same address
+    want = opt.state[p]["momentum_buffer"].clone()
+    opt.step()
+    assert opt.state[p]["momentum_buffer"].is_contiguous() and torch.equal(opt.state[p]["momentum_buffer"], want)
+    assert launches[-1][1]._obj[0].momentum == opt.state[p]["momentum_buffer"].data_ptr()
