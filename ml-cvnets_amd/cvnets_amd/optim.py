@@ -344,6 +344,16 @@ class Muon(torch.optim.Optimizer):
             self.param_groups.pop()
             raise
 
+    @torch.no_grad()
+    def load_state_dict(self, state_dict) -> None:
+        """into the momentum that is there (zeros where none is loaded): a captured step goes on reading and writing it"""
+        held = {p: s["momentum_buffer"] for p, s in self.state.items() if "momentum_buffer" in s}
+        super().load_state_dict(state_dict)
+        for p, buf in held.items():
+            new = self.state[p].get("momentum_buffer")
+            if new is None or new.shape == buf.shape:
+                self.state[p]["momentum_buffer"] = buf.zero_() if new is None else buf.copy_(new)
+
     def _entries(self):
         out = []
         for gi, g in enumerate(self.param_groups):

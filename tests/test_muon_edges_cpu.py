@@ -1,4 +1,5 @@
 """What the orthogonalised update takes and refuses, without a GPU."""
+import copy
 import ctypes
 import gc
 import weakref
@@ -124,3 +125,19 @@ def test_a_transposed_square_parameter_or_momentum_is_refused(launches):
     opt.step()
     assert opt.state[p]["momentum_buffer"].is_contiguous() and torch.equal(opt.state[p]["momentum_buffer"], want)
     assert launches[-1][1]._obj[0].momentum == opt.state[p]["momentum_buffer"].data_ptr()
+
+
+def test_a_loaded_state_goes_into_the_momentum_that_a_captured_step_holds(launches):
+    p, q = with_gradient(4, 6), with_gradient(3, 5)
+    opt = optim.Muon([p, q], lr=0.5)
+    opt.step()
+    held = {x: opt.state[x]["momentum_buffer"].data_ptr() for x in (p, q)}
+    saved = copy.deepcopy(opt.state_dict())
+    saved["state"][0]["momentum_buffer"].fill_(3.0)
+    del saved["state"][1]  # a parameter that had not been stepped when the state was saved
+    opt.state[q]["momentum_buffer"].fill_(2.0)
+    opt.load_state_dict(saved)
+    opt.step()
+    assert {x: opt.state[x]["momentum_buffer"].data_ptr() for x in (p, q)} == held
+    assert bool((opt.state[p]["momentum_buffer"] == 3.0).all()) and bool((opt.state[q]["momentum_buffer"] == 0.0).all())
+    assert opt.state[p]["momentum_buffer"].data_ptr() != saved["state"][0]["momentum_buffer"].data_ptr()
