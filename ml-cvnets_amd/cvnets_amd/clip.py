@@ -113,26 +113,30 @@ class TextTransformer(nn.Module):
     @staticmethod
     def pack_captions(text_tokens: Tensor, device=None) -> Tuple[Tensor, packed.PackedSeqs]:
         """[B, S] padded captions -> (tokens [rows], layout): each caption up to and including its end mark (its largest token, as in
-        ``encode_text``).  A host function for the data loader's batch; on a tensor of the device it waits for it."""
+        ``encode_text``); the layout also keeps S, which the positions depend on.  A host function for the data loader's batch; on a tensor of the
+        device it waits for it."""
         if text_tokens.dim() != 2 or text_tokens.numel() == 0:
             raise RuntimeError(f"captions must be [batch, sequence] token ids. Got: {list(text_tokens.shape)}")
         host = text_tokens.cpu()
         lengths = host.argmax(dim=-1) + 1
         rows = host[torch.arange(host.shape[1])[None, :] < lengths[:, None]]
         device = device if device is not None else text_tokens.device if text_tokens.is_cuda else torch.device("cuda", torch.cuda.current_device())
-        return rows.to(device=device, dtype=torch.int64), packed.PackedSeqs.from_lengths(lengths.tolist(), device)
+        return rows.to(device=device, dtype=torch.int64), packed.PackedSeqs.from_lengths(lengths.tolist(), device, context_length=host.shape[1])
 
     def encode_packed(self, text_tokens: Tensor, seqs: packed.PackedSeqs, context_length: Optional[int] = None) -> Tensor:
         """``encode_text`` of packed captions (``pack_captions``): under the causal mask nothing behind a caption's end mark reaches its
         embedding, so the tower runs on the captions' own tokens only.  Every sequence has at least its end mark.  context_length: the
-        padded length whose positional table is meant (default: the table's own)."""
+        padded length whose positional table is meant (default: the layout's, else the table's own); no caption is longer."""
         if not self.causal_masking:
             raise NotImplementedError("packed captions need model.text.transformer.causal_masking: without it the padding tokens take part")
         if context_length is not None and context_length < 1:
             raise ValueError(f"context_length must be positive. Got: {context_length}")
         pos = None
         if self.positional_embedding is not None:
-            pos = self.positional_embedding.table(context_length or self.positional_embedding.pos_embed.num_embeddings)
+            context_length = context_length or seqs.context_length or self.positional_embedding.pos_embed.num_embeddings
+            if seqs.longest is not None and seqs.longest > context_length:
+                raise ValueError(f"a caption of {seqs.longest} tokens has no positions in a table of {context_length}")
+            pos = self.positional_embedding.table(context_length)
         emb = self.embedding_layer
         t = packed.embed(text_tokens, emb.weight, seqs, pos=pos, padding_idx=emb.padding_idx)
         t = self.embedding_dropout(t)

@@ -32,13 +32,14 @@ class PackedSeqs:
     cu_seqlens: int32 [sequences + 1] on the GPU, sequence b has the rows ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1`` (empty ones are
     allowed; the first boundary is 0, and counts as 0 whatever stands there);
     rows: the number of rows of the matrices that are used with it (>= cu_seqlens[-1]); max_len: an upper bound of the lengths, if one is
-    known on the host - it only chooses the work list's block size, a wrong one costs time and no result.
+    known on the host - it only chooses the work list's block size, a wrong one costs time and no result; context_length: the length that the
+    sequences were padded to, for a model whose positions depend on it (None: not known).
 
     The work list is made by one kernel on the current stream, from the boundaries on the device: ``refresh`` makes it again after they were
     changed in place (inside a captured graph, too).  Boundaries that fall or leave 0 .. rows are clamped by that kernel (they are not read by
     the host); ``from_lengths`` checks lengths that the host knows."""
 
-    def __init__(self, cu_seqlens: Tensor, rows: int, max_len: Optional[int] = None):
+    def __init__(self, cu_seqlens: Tensor, rows: int, max_len: Optional[int] = None, context_length: Optional[int] = None):
         if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_contiguous():
             raise RuntimeError(f"cu_seqlens must be a contiguous int32 vector of sequences + 1 boundaries. Got: {cu_seqlens.dtype} {list(cu_seqlens.shape)}")
         rows = int(rows)
@@ -46,9 +47,12 @@ class PackedSeqs:
             raise ValueError(f"rows must be in 1 .. {_MOST_ROWS}. Got: {rows}")
         if max_len is not None and max_len < 0:
             raise ValueError(f"max_len must not be negative. Got: {max_len}")
+        if context_length is not None and context_length < 1:
+            raise ValueError(f"context_length must be positive. Got: {context_length}")
         _check_dev(cu_seqlens)
         self.cu_seqlens, self.rows, self.seqs = cu_seqlens, rows, cu_seqlens.numel() - 1
         self.max_len = rows if max_len is None else min(int(max_len), rows)
+        self.context_length = None if context_length is None else int(context_length)
         self.block = _block_rows(rows, self.seqs, self.max_len)
         self.version = 0  # of the work list: a backward pass with another one than its forward is refused
         self.places = rows // self.block + self.seqs + 1
@@ -56,7 +60,7 @@ class PackedSeqs:
         self.refresh()
 
     @classmethod
-    def from_lengths(cls, lengths: Sequence[int], device, rows: Optional[int] = None) -> "PackedSeqs":
+    def from_lengths(cls, lengths: Sequence[int], device, rows: Optional[int] = None, context_length: Optional[int] = None) -> "PackedSeqs":
         lengths = [int(n) for n in lengths]
         if not lengths or min(lengths) < 0:
             raise ValueError(f"lengths must be one or more non-negative numbers. Got: {lengths[:8]}")
@@ -66,10 +70,13 @@ class PackedSeqs:
         rows = max(total, 1) if rows is None else int(rows)
         if not total <= rows <= _MOST_ROWS:
             raise ValueError(f"{total} rows of sequences do not fit into rows = {rows} (at most {_MOST_ROWS})")
-        return cls(cu.to(torch.int32).to(device), rows, max_len=max(lengths))
+        seqs = cls(cu.to(torch.int32).to(device), rows, max_len=max(lengths), context_length=context_length)
+        seqs.longest = max(lengths)
+        return seqs
 
     def refresh(self) -> None:
         self.version += 1
+        self.longest = None  # of the sequences, where the host knows it
         call_on(self.plan.device, "cvh_packed_plan", _p(self.cu_seqlens), self.seqs, self.rows, self.block, _p(self.plan))
 
     def __repr__(self) -> str:

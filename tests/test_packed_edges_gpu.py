@@ -1,0 +1,109 @@
+"""Packed sequences at the edges of what the operators and the text tower take.  Tolerances are those of the operators' and the tower's own tests:
+float32 attention 128 * 2^-24 (the exponent's argument times 2^-24 in the probabilities and through delta, and as much for sums of up to 700 terms), the
+tower 2e-5 in float32 (2^-24 times a few hundred terms through two layers); bf16 attention 2^-8."""
+import math
+
+import pytest
+import torch
+
+import cvnets_amd
+from cvnets_amd import packed
+
+pytestmark = pytest.mark.gpu
+TOL = {torch.bfloat16: 2.0 ** -8, torch.float32: 128 * 2.0 ** -24}
+
+
+@pytest.fixture(autouse=True)
+def _dtype():
+    yield
+    cvnets_amd.set_compute_dtype(None)
+
+
+def tower(context=24, dim=128, positions=True, seed=0):
+    from cvnets_amd.layers import default_opts
+
+    torch.manual_seed(seed)
+    opts = default_opts(**{"model.text.transformer.model_dim": dim, "model.text.transformer.n_transformer_layers": 2, "model.text.transformer.n_heads_per_layer": 4,
+                           "model.text.transformer.norm_layer": "layer_norm_fp32", "model.text.transformer.causal_masking": True, "model.activation.name": "gelu",
+                           "model.text.transformer.no_pos_embedding": not positions, "dataset.text_vocab_size": 300, "dataset.text_context_length": context,
+                           "dataset.padding_index": 0})
+    cvnets_amd.set_compute_dtype(torch.float32)
+    return cvnets_amd.TextTransformer(opts, projection_dim=64).cuda().train()
+
+
+def captions(n, padded, vocab=300, longest=None, seed=0):
+    """start mark, words, end mark (the largest token), padding"""
+    g = torch.Generator().manual_seed(seed)
+    t = torch.zeros(n, padded, dtype=torch.int64)
+    for i in range(n):
+        words = int(torch.randint(0, (longest or padded) - 1, (1,), generator=g))
+        t[i, :words + 1] = torch.randint(1, vocab - 2, (words + 1,), generator=g)
+        t[i, 0] = vocab - 2
+        t[i, words + 1] = vocab - 1
+    return t
+
+
+def rel(a, b):
+    return float((a.double() - b.double()).norm() / b.double().norm().clamp(min=1e-30))
+
+
+@pytest.mark.parametrize("padded", [9, 16, 24, 40, 77])
+def test_captions_padded_to_another_length_than_the_table(padded):
+    """the padded tower resizes its positional table to the padded length; the packed one has to take the same rows of it"""
+    model, text = tower(), captions(23, padded)
+    tokens, seqs = model.pack_captions(text)
+    dy = torch.randn(23, 64, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    got = []
+    for run in (lambda: model(text.cuda()), lambda: model.encode_packed(tokens, seqs)):
+        model.zero_grad(set_to_none=True)
+        y = run()
+        y.backward(dy)
+        got.append((y.detach(), {k: p.grad.clone() for k, p in model.named_parameters()}))
+    (y0, g0), (y1, g1) = got
+    assert rel(y1, y0) <= 2e-5
+    for k in g0:
+        assert rel(g1[k], g0[k]) <= 1e-4, k
+
+
+@pytest.mark.parametrize("padded", [16, 40])
+def test_clip_takes_packed_captions_of_another_padded_length(padded):
+    cvnets_amd.set_compute_dtype(torch.float32)
+    torch.manual_seed(0)
+    model = cvnets_amd.build_clip(**{"model.classification.vit.mode": "tiny", "model.text.transformer.model_dim": 128, "model.text.transformer.n_transformer_layers": 1,
+                                     "model.text.transformer.n_heads_per_layer": 4, "dataset.text_vocab_size": 300, "dataset.text_context_length": 24,
+                                     "model.multi_modal_image_text.clip.projection_dim": 64}).cuda().eval()
+    image, text = torch.randn(5, 3, 64, 64, generator=torch.Generator().manual_seed(0)).cuda(), captions(5, padded)
+    tokens, seqs = model.text_encoder.pack_captions(text)
+    with torch.no_grad():
+        a, b = model({"image": image, "text": text.cuda()}), model({"image": image, "text": tokens, "text_seqs": seqs})
+    assert rel(b["text"], a["text"]) <= 2e-5
+
+
+def test_the_padded_length_given_and_kept():
+    model, text = tower(), captions(7, 40, longest=12)
+    tokens, seqs = model.pack_captions(text)
+    assert seqs.context_length == 40
+    lengths = (text.argmax(-1) + 1).tolist()
+    with torch.no_grad():
+        want = model(text.cuda())
+        bare = packed.PackedSeqs.from_lengths(lengths, "cuda")
+        assert rel(model.encode_packed(tokens, bare, context_length=40), want) <= 2e-5
+        assert rel(model.encode_packed(tokens, packed.PackedSeqs(seqs.cu_seqlens, seqs.rows, context_length=40)), want) <= 2e-5
+        short = torch.nn.functional.pad(text[:, :20], (0, 4)).cuda()  # the same captions padded to the table's length
+        assert rel(model.encode_packed(tokens, bare), model(short)) <= 2e-5
+        assert rel(model.encode_packed(tokens, seqs, context_length=24), model(short)) <= 2e-5  # (the argument comes first)
+        seqs.refresh()
+        assert seqs.context_length == 40 and rel(model.encode_packed(tokens, seqs), want) <= 2e-5
+
+
+def test_captions_longer_than_the_positions_are_refused():
+    model = tower()
+    ids = torch.ones(30, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="no positions"):
+        model.encode_packed(ids, packed.PackedSeqs.from_lengths([25, 5], "cuda"))
+    with pytest.raises(ValueError, match="no positions"):
+        model.encode_packed(ids, packed.PackedSeqs.from_lengths([20, 10], "cuda"), context_length=19)
+    with pytest.raises(ValueError, match="context_length"):
+        packed.PackedSeqs(torch.tensor([0, 5], dtype=torch.int32, device="cuda"), 5, context_length=0)
+    without = tower(positions=False)
+    assert torch.isfinite(without.encode_packed(ids, packed.PackedSeqs.from_lengths([25, 5], "cuda"))).all()
