@@ -131,12 +131,16 @@ class TextTransformer(nn.Module):
             raise NotImplementedError("packed captions need model.text.transformer.causal_masking: without it the padding tokens take part")
         if context_length is not None and context_length < 1:
             raise ValueError(f"context_length must be positive. Got: {context_length}")
+        context_length = context_length or seqs.context_length
         pos = None
         if self.positional_embedding is not None:
-            context_length = context_length or seqs.context_length or self.positional_embedding.pos_embed.num_embeddings
+            context_length = context_length or self.positional_embedding.pos_embed.num_embeddings
             if seqs.longest is not None and seqs.longest > context_length:
                 raise ValueError(f"a caption of {seqs.longest} tokens has no positions in a table of {context_length}")
             pos = self.positional_embedding.table(context_length)
+        if context_length == self.model_dim and any(isinstance(m, nn.LayerNorm) and getattr(m, "reference_quirk", True) for m in self.modules()):
+            raise NotImplementedError(f"captions padded to the model's width ({context_length}): the LayerNorms of the padded tower then normalise over the padded "
+                                      "sequence, which packed rows do not have (LayerNorm.reference_quirk = False: over the width, for both)")
         emb = self.embedding_layer
         t = packed.embed(text_tokens, emb.weight, seqs, pos=pos, padding_idx=emb.padding_idx)
         t = self.embedding_dropout(t)

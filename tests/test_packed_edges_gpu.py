@@ -107,3 +107,22 @@ def test_captions_longer_than_the_positions_are_refused():
         packed.PackedSeqs(torch.tensor([0, 5], dtype=torch.int32, device="cuda"), 5, context_length=0)
     without = tower(positions=False)
     assert torch.isfinite(without.encode_packed(ids, packed.PackedSeqs.from_lengths([25, 5], "cuda"))).all()
+
+
+def test_a_padded_length_equal_to_the_width_is_refused():
+    """the padded tower's LayerNorm then normalises over the (padded) sequence: packed rows have no such sequence"""
+    model, text = tower(context=64, dim=64), captions(9, 64)
+    tokens, seqs = model.pack_captions(text)
+    with pytest.raises(NotImplementedError, match="reference_quirk"):
+        model.encode_packed(tokens, seqs)
+    model = tower(context=24, dim=64)
+    with torch.no_grad():
+        with pytest.raises(NotImplementedError, match="reference_quirk"):
+            model.encode_packed(tokens, seqs)
+        for m in model.modules():
+            if isinstance(m, torch.nn.LayerNorm):
+                m.reference_quirk = False  # the documented LayerNorm, whatever the length
+        assert rel(model.encode_packed(tokens, seqs), model(text.cuda())) <= 2e-5
+    model = tower(context=24, dim=64)
+    tokens, seqs = model.pack_captions(captions(9, 24))
+    assert torch.isfinite(model.encode_packed(tokens, seqs)).all()
