@@ -343,7 +343,8 @@ int cvh_ln_seq_bwd(int dtype, const void* x, const void* dy, const float* gamma,
 
 /* ---- CLIP heads and loss ------------------------------------------------------------------------- */
 /* dst[r] = src[idx[r]] (scatter == 0) / dst[idx[r]] = src[r] (scatter == 1, dst pre-zeroed): the EOT-token gather
- * token_emb[arange(B), text_tokens.argmax(-1)] (cvnets/text_encoders/transformer.py:413-421) and its adjoint. */
+ * token_emb[arange(B), text_tokens.argmax(-1)] (cvnets/text_encoders/transformer.py:413-421) and its adjoint.  idx[r] < 0: no row (zeros; nothing
+ * is scattered); src has at least one row, and the indices from 0 on are distinct where scatter == 1. */
 int cvh_rows_gather_idx(int dtype, const void* src, const long long* idx, void* dst, int R, int C, int scatter, void* stream);
 /* F.normalize(x, dim=-1) (simple_projection_head.py:83-84, text_encoders/transformer.py:424-425); inv_norm[R] is saved for bwd */
 int cvh_l2norm_fwd(int dtype, const void* x, void* y, float* inv_norm, int R, int C, float eps, void* stream);

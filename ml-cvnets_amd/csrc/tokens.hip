@@ -118,7 +118,8 @@ __global__ void embed_lookup_bwd_kernel(const long long* __restrict__ tok, const
   }
 }
 
-// dst[b][:] = src[idx[b]][:]  (EOT-token rows, text_encoders/transformer.py:413-421) ; scatter form for the backward (dst pre-zeroed)
+// dst[b][:] = src[idx[b]][:]  (EOT-token rows, text_encoders/transformer.py:413-421) ; scatter form for the backward (dst pre-zeroed).  An index below 0
+// names no row: zeros, and nothing is scattered.  (The other indices are distinct: the scatter's stores are plain ones.)
 template <typename T>
 __global__ void rows_gather_idx_kernel(const T* __restrict__ src, const long long* __restrict__ idx, T* __restrict__ dst, int R, int C, int scatter) {
   const int cg = C / 8;
@@ -126,9 +127,12 @@ __global__ void rows_gather_idx_kernel(const T* __restrict__ src, const long lon
   for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
     const int c0 = (int)(i % cg) * 8;
     const size_t r = i / cg;
-    const size_t sr = (size_t)idx[r];
-    if (scatter) v8_store<T>(dst + sr * C + c0, v8_load<T>(src + r * C + c0));
-    else v8_store<T>(dst + r * C + c0, v8_load<T>(src + sr * C + c0));
+    const long long sr = idx[r];
+    if (scatter) {
+      if (sr >= 0) v8_store<T>(dst + (size_t)sr * C + c0, v8_load<T>(src + r * C + c0));
+    } else {
+      v8_store<T>(dst + r * C + c0, v8_mask(v8_load<T>(src + (size_t)(sr < 0 ? 0 : sr) * C + c0), sr >= 0));
+    }
   }
 }
 

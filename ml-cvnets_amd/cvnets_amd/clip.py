@@ -125,7 +125,7 @@ class TextTransformer(nn.Module):
 
     def encode_packed(self, text_tokens: Tensor, seqs: packed.PackedSeqs, context_length: Optional[int] = None) -> Tensor:
         """``encode_text`` of packed captions (``pack_captions``): under the causal mask nothing behind a caption's end mark reaches its
-        embedding, so the tower runs on the captions' own tokens only.  Every sequence has at least its end mark.  context_length: the
+        embedding, so the tower runs on the captions' own tokens only.  An empty sequence's embedding is zero, and no gradient comes from it.  context_length: the
         padded length whose positional table is meant (default: the layout's, else the table's own); no caption is longer."""
         if not self.causal_masking:
             raise NotImplementedError("packed captions need model.text.transformer.causal_masking: without it the padding tokens take part")
@@ -147,7 +147,8 @@ class TextTransformer(nn.Module):
         for layer in self.transformer:
             t = layer.forward_tokens(t, ops.NO_SEQMAP, causal=True, seqs=seqs)
         t = ops.layer_norm_tokens(t, self.final_layer_norm, ops.NO_SEQMAP)
-        ends = (seqs.plan[1:seqs.seqs + 1].long() - 1).clamp(min=0)  # plumbing: EOT index arithmetic, on the clamped boundaries
+        start, end = seqs.plan[:seqs.seqs], seqs.plan[1:seqs.seqs + 1]  # the clamped boundaries
+        ends = torch.where(end > start, end - 1, -1).long()  # plumbing: EOT index arithmetic; empty sequences have no row
         return ops.l2_normalize(ops.linear(ops.RowsGatherIdx.apply(t, ends), self.projection_layer.t()))
 
     def forward_zero_shot(self, text_tokens: Tensor, key_padding_mask: Optional[Tensor] = None, *args, **kwargs) -> Tensor:

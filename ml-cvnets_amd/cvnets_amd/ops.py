@@ -1712,7 +1712,8 @@ class EmbedLookup(torch.autograd.Function):
 
 
 class RowsGatherIdx(torch.autograd.Function):
-    """x [R_src, C], rows int64 [R] -> x[rows]  (EOT-token embeddings, text_encoders/transformer.py:413-421)."""
+    """x [R_src, C], rows int64 [R] -> x[rows]  (EOT-token embeddings, text_encoders/transformer.py:413-421); a row below 0 is none: zeros, no
+    gradient.  The others are distinct."""
 
     @staticmethod
     def forward(ctx, x, rows):

@@ -126,3 +126,36 @@ def test_a_padded_length_equal_to_the_width_is_refused():
     model = tower(context=24, dim=64)
     tokens, seqs = model.pack_captions(captions(9, 24))
     assert torch.isfinite(model.encode_packed(tokens, seqs)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_that_name_nothing_are_zeros_without_gradient(dtype):
+    x = torch.randn(9, 40, device="cuda").to(dtype).requires_grad_(True)
+    rows = torch.tensor([3, -1, 8, -1, 0], device="cuda")
+    y = cvnets_amd.ops.RowsGatherIdx.apply(x, rows)
+    assert torch.equal(y[[0, 2, 4]], x.detach()[[3, 8, 0]]) and bool((y[[1, 3]] == 0).all())
+    dy = torch.randn(5, 40, device="cuda").to(dtype)
+    (dx,) = torch.autograd.grad(y, (x,), dy)
+    want = torch.zeros_like(dx)
+    want[[3, 8, 0]] = dy[[0, 2, 4]]
+    assert torch.equal(dx, want)
+
+
+@pytest.mark.parametrize("lengths", [[0, 5, 9], [5, 0, 0, 9], [5, 9, 0], [0, 0, 5, 0, 9, 0]])
+def test_empty_captions_have_zero_embeddings_and_take_no_gradient_away(lengths):
+    """a batch of fewer captions than places: the captions' embeddings and all gradients are those of the batch without the empty places"""
+    model = tower()
+    ids = torch.randint(1, 298, (14,), generator=torch.Generator().manual_seed(3)).cuda()
+    live = [i for i, n in enumerate(lengths) if n]
+    dy = torch.randn(len(lengths), 64, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    got = []
+    for lens, d in ((lengths, dy), ([5, 9], dy[live])):
+        model.zero_grad(set_to_none=True)
+        y = model.encode_packed(ids, packed.PackedSeqs.from_lengths(lens, "cuda", context_length=24))
+        y.backward(d)
+        got.append((y.detach(), {k: p.grad.clone() for k, p in model.named_parameters()}))
+    (y0, g0), (y1, g1) = got
+    assert rel(y0[live], y1) <= 2e-5
+    assert bool((y0[[i for i in range(len(lengths)) if i not in live]] == 0).all())
+    for k in g1:
+        assert torch.isfinite(g0[k]).all() and rel(g0[k], g1[k]) <= 1e-4, k
