@@ -9,6 +9,7 @@ import math
 from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 from .ops import _p, _stream
@@ -284,7 +285,7 @@ def orthogonalize(matrices: Union[torch.Tensor, Sequence[torch.Tensor]], steps: 
     """Newton-Schulz orthogonalisation of matrices (one or a list of any shapes, all float32 or all bfloat16): x = u / (|u|_F + eps), then ``steps``
     times x <- (a I + b x x^T + c (x x^T)^2) x, the shorter side as rows.  The products are computed to float32 accuracy whatever the type
     of the matrices; the result has their type.  A list takes as many launches as one matrix.  A NaN or an infinity in a matrix makes its whole
-    result NaN (and no other's).  Coefficients whose steps let singular values grow beyond 15 in front of another step are refused."""
+    result NaN (and no other's).  Not differentiable: the result is detached.  Coefficients whose steps let singular values grow beyond 15 in front of another step are refused."""
     single = isinstance(matrices, torch.Tensor)
     mats = [matrices] if single else list(matrices)
     cfg = _check_ns(steps, coefficients, eps)
@@ -292,6 +293,8 @@ def orthogonalize(matrices: Union[torch.Tensor, Sequence[torch.Tensor]], steps: 
         if t.dim() != 2 or t.dtype not in (torch.float32, torch.bfloat16) or t.dtype != mats[0].dtype:
             raise RuntimeError(f"orthogonalize takes float32 or bfloat16 matrices of one dtype. Got: {t.dtype} {list(t.shape)}")
         _check_matrix(*t.shape)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in mats):
+        raise NotImplementedError("orthogonalize has no forward-mode derivatives")
     for t in mats:
         ops._check_dev(t)
         if t.device != mats[0].device:

@@ -9,6 +9,7 @@ from typing import Optional, Sequence
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -81,6 +82,16 @@ class PackedSeqs:
 
     def __repr__(self) -> str:
         return f"PackedSeqs(sequences={self.seqs}, rows={self.rows}, max_len={self.max_len})"
+
+
+def _has_tangent(*tensors: Optional[Tensor]) -> bool:
+    """whether forward-mode differentiation runs through one of them"""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _differentiated(*tensors: Optional[Tensor]) -> bool:
+    """whether the autograd function is needed: in reverse mode it gives the gradients, in forward mode it says that it has no derivatives of that kind"""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or _has_tangent(*tensors)
 
 
 def _check_version(seqs: PackedSeqs, version: int) -> None:
@@ -198,7 +209,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, seqs: PackedSeqs, causal: bool = 
     d contiguous and rows on 16 bytes are read in place.  scale: default d ** -0.5.  causal: token i sees the tokens 0 .. i of its sequence.
     A NaN or infinity reaches the results of its own sequence only (under the causal mask: of its 32-row block and behind it)."""
     scale = _check_heads(q, k, v, seqs, scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _differentiated(q, k, v):
         return PackedAttentionFn.apply(q, k, v, seqs, bool(causal), scale)
     return _forward(_loadable(q), _loadable(k), _loadable(v), seqs, bool(causal), scale, False)[0]
 
@@ -214,7 +225,7 @@ def attention_qkv(qkv: Tensor, heads: int, seqs: PackedSeqs, kv_heads: Optional[
     scale = _check_heads(q, k, v, seqs, scale)
     if qkv.shape[1] > _MOST_ROW:
         raise NotImplementedError(f"packed attention: rows of more than {_MOST_ROW} elements. Got: {qkv.shape[1]}")
-    if torch.is_grad_enabled() and qkv.requires_grad:
+    if _differentiated(qkv):
         return PackedAttentionQKVFn.apply(qkv, int(heads), kv_heads, seqs, bool(causal), scale)
     return _forward(q, k, v, seqs, bool(causal), scale, False)[0].view(qkv.shape[0], -1)
 
@@ -298,6 +309,6 @@ def embed(ids: Tensor, table: Tensor, seqs: Optional[PackedSeqs] = None, pos: Op
     if pos is not None and (not pos.is_contiguous() or pos.data_ptr() % 16):
         pos = pos.contiguous() if not pos.is_contiguous() else pos.clone()
     ids = ids.contiguous()
-    if torch.is_grad_enabled() and (table.requires_grad or (pos is not None and pos.requires_grad)):
+    if _differentiated(table, pos):
         return PackedEmbedFn.apply(table, pos, ids, seqs, float(scale), padding_idx, dtype)
     return _lookup(table, pos, ids, seqs, float(scale), dtype)

@@ -1,0 +1,41 @@
+"""Packed sequences without a GPU: what comes before a launch.  Where a test goes further, the launches themselves are left out."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from cvnets_amd import _lib, optim, packed
+
+
+def layout(rows=10, places=2):
+    return SimpleNamespace(rows=rows, places=places, seqs=1, block=32, plan=torch.zeros(4, dtype=torch.int32), version=1)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    seen = []
+    for module in (packed, optim.ops):
+        monkeypatch.setattr(module, "_check_dev", lambda t: None)
+        monkeypatch.setattr(module, "call_on", lambda dev, name, *args: seen.append((name, *args)))
+    return seen
+
+
+def dual(*shape):
+    return forward_ad.make_dual(torch.zeros(shape), torch.ones(shape))
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused_not_dropped(launches, grad):
+    q, k, ids = torch.zeros(10, 4, 16), torch.zeros(10, 2, 16), torch.zeros(10, dtype=torch.int64)
+    table, pos = torch.zeros(7, 16), torch.zeros(12, 16)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        for call in (lambda: packed.attention(dual(10, 4, 16), k, k, layout()), lambda: packed.attention(q, dual(10, 2, 16), k, layout()),
+                     lambda: packed.attention(q, k, dual(10, 2, 16), layout()), lambda: packed.attention_qkv(dual(10, 48), 1, layout()),
+                     lambda: packed.embed(ids, dual(7, 16), dtype=torch.float32), lambda: packed.embed(ids, table, layout(), pos=dual(12, 16), dtype=torch.float32),
+                     lambda: optim.orthogonalize(dual(4, 6)), lambda: optim.orthogonalize([torch.zeros(4, 6), dual(4, 6)])):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert packed.attention(q, k, k, layout()).shape == q.shape  # (no tangent: as outside)
+        assert packed.embed(ids, table, layout(), pos=pos, dtype=torch.float32).shape == (10, 16)
+        assert optim.orthogonalize(torch.zeros(4, 6)).shape == (4, 6)
