@@ -106,7 +106,7 @@ def _loadable(t: Tensor) -> Tensor:
     """[rows, heads, d] as the kernels read it: d contiguous, base and strides on 16 bytes (any other layout is copied)"""
     n = 16 // t.element_size()
     ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % n == 0 and t.stride(1) % n == 0 and t.stride(1) >= 0 and 0 <= t.stride(0) <= _MOST_ROW
-    return t if ok else t.contiguous() if not t.is_contiguous() else t.clone()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)  # (contiguous() leaves the stride of a dimension of one as it is)
 
 
 def _launch(name: str, seqs: PackedSeqs, scale: float, causal: bool, q, k, v, out, out_lo, lse, delta=None, dout=None, dq=None, dk=None, dv=None) -> None:
@@ -219,8 +219,8 @@ def attention_qkv(qkv: Tensor, heads: int, seqs: PackedSeqs, kv_heads: Optional[
     kv_heads = heads if kv_heads is None else int(kv_heads)
     if qkv.dim() != 2 or heads <= 0 or kv_heads <= 0 or qkv.shape[1] % (heads + 2 * kv_heads):
         raise RuntimeError(f"qkv must be [rows, ({heads} + 2 x {kv_heads}) heads x d]. Got: {list(qkv.shape)}")
-    if not qkv.is_contiguous() or qkv.data_ptr() % 16:
-        qkv = qkv.contiguous() if not qkv.is_contiguous() else qkv.clone()
+    if qkv.stride() != (qkv.shape[1], 1) or qkv.data_ptr() % 16:
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
     q, k, v = _split_heads(qkv, int(heads), kv_heads)
     scale = _check_heads(q, k, v, seqs, scale)
     if qkv.shape[1] > _MOST_ROW:

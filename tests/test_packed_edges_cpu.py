@@ -39,3 +39,32 @@ def test_forward_mode_derivatives_are_refused_not_dropped(launches, grad):
         assert packed.attention(q, k, k, layout()).shape == q.shape  # (no tangent: as outside)
         assert packed.embed(ids, table, layout(), pos=pos, dtype=torch.float32).shape == (10, 16)
         assert optim.orthogonalize(torch.zeros(4, 6)).shape == (4, 6)
+
+
+def strides_ok(t):
+    n = 16 // t.element_size()
+    return t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(t.stride(i) % n == 0 and t.stride(i) >= 0 for i in (0, 1)) and t.stride(0) <= 1 << 21
+
+
+def odd_rows(dtype):
+    """one row, or one head, of a larger matrix: contiguous whatever the stride of that dimension"""
+    wide = torch.arange(4 * 1001, dtype=torch.float32).to(dtype).view(4, 1001)
+    far = torch.arange(64.0).to(dtype).as_strided((1, 2, 32), (1 << 22, 32, 1))
+    return {"odd row stride": wide[:, :512].view(4, 8, 64)[:1], "large row stride": far, "one head": wide[:, :64].contiguous().unsqueeze(-1).transpose(1, 2)}
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("name", ["odd row stride", "large row stride", "one head"])
+def test_single_rows_and_heads_are_laid_out_as_the_kernels_read_them(dtype, name):
+    t = odd_rows(dtype)[name]
+    assert t.is_contiguous() and not strides_ok(t)
+    got = packed._loadable(t)
+    assert strides_ok(got) and torch.equal(got, t)
+
+
+def test_one_row_of_a_projection(launches):
+    qkv = torch.arange(4 * 1001.0).view(4, 1001)[:1, :384]
+    assert qkv.is_contiguous() and qkv.stride(0) == 1001
+    packed.attention_qkv(qkv, 2, layout(rows=1), kv_heads=2)
+    args = _lib.PackedAttn.from_buffer_copy(launches[-1][2])
+    assert (args.q_row, args.q_head) == (384, 64)

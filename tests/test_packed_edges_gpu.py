@@ -159,3 +159,23 @@ def test_empty_captions_have_zero_embeddings_and_take_no_gradient_away(lengths):
     assert bool((y0[[i for i in range(len(lengths)) if i not in live]] == 0).all())
     for k in g1:
         assert torch.isfinite(g0[k]).all() and rel(g0[k], g1[k]) <= 1e-4, k
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_one_row_of_a_larger_matrix(dtype):
+    """a softmax over one key: the output is v, and dv the incoming gradient, to the bit; dq and dk are zeros"""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    wide = torch.randn(3, 4, 1001, generator=g, device="cuda").to(dtype)
+    q, k, v = (w[:, :512].view(4, 8, 64)[1:2].detach().requires_grad_(True) for w in wide)
+    dout = torch.randn(4, 1001, generator=g, device="cuda").to(dtype)[:, :512].view(4, 8, 64)[2:3]
+    seqs = packed.PackedSeqs.from_lengths([1], "cuda")
+    out = packed.attention(q, k, v, seqs)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), dout)
+    assert torch.equal(out, v) and torch.equal(dv, dout)
+    assert float(dq.abs().max()) <= TOL[dtype] * 64 and float(dk.abs().max()) <= TOL[dtype] * 64
+    qkv = wide[0][:, :384][3:4].detach().requires_grad_(True)
+    both = packed.attention_qkv(qkv, 2, seqs)
+    assert torch.equal(both, qkv[:, 256:])
+    one_head = torch.randn(70, 64, generator=g, device="cuda").to(dtype).unsqueeze(-1).transpose(1, 2)
+    assert torch.equal(packed.attention(*(one_head,) * 3, packed.PackedSeqs.from_lengths([50, 20], "cuda")),
+                       packed.attention(*(one_head.clone(memory_format=torch.contiguous_format),) * 3, packed.PackedSeqs.from_lengths([50, 20], "cuda")))
