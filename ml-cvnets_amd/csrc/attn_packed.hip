@@ -384,13 +384,15 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
       }
     l += sum;  // this lane's half of the keys; the halves are joined once, at the end
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b) {
+      if (b > 0 && p.causal && k0 + 32 * b > q0 + 31) continue;  // all zeros; and 0 times a NaN of the future would not be
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const Frag<T> pf = acc_frag<T>(s[b], h);
 #pragma unroll
         for (int f = 0; f < NF; ++f) mma32(o[f], tile.cols(Vt, 32 * b + 16 * h, 32 * f), pf);
       }
+    }
     if (ST == 1) advance();
   }
   l = both_halves_sum(l);
@@ -487,6 +489,7 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
     const bool masked = k0 + KB > w.len || (p.causal && k0 + KB - 1 > q0);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+      if (b > 0 && p.causal && k0 + 32 * b > q0 + 31) continue;  // (as in the forward)
       f32x16_t s = acc_zero(), dp = minus_delta;
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
@@ -610,6 +613,7 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
     const bool masked = q0 + QB > w.len || (p.causal && q0 < k0 + 31);
 #pragma unroll
     for (int b0 = 0; b0 < NB; b0 += SB) {
+      if (SB == 1 && b0 + 1 < NB && p.causal && q0 + 32 * b0 + 31 < k0) continue;  // none of these queries sees a key of this wave
       f32x16_t s[SB], dp[SB];  // dp starts from -delta
 #pragma unroll
       for (int b = 0; b < SB; ++b) {
@@ -650,7 +654,8 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
         }
       }
 #pragma unroll
-      for (int b = 0; b < SB; ++b)
+      for (int b = 0; b < SB; ++b) {
+        if (b + 1 < SB && p.causal && q0 + 32 * b + 31 < k0) continue;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const Frag<T> pf = acc_frag<T>(s[b], h), sf = acc_frag<T>(dp[b], h);
@@ -660,6 +665,7 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
             mma32(ak[f], tile.cols(Qt, 32 * (b0 + b) + 16 * h, 32 * f), sf);
           }
         }
+      }
     }
     if (ST == 1) advance();
   }

@@ -207,7 +207,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, seqs: PackedSeqs, causal: bool = 
     """Softmax attention inside each sequence: q [rows, heads, d], k and v [rows, kv_heads, d] (heads a multiple of kv_heads: consecutive query
     heads share a key head) -> [rows, heads, d], differentiable in q, k and v.  float32 or bfloat16, d a multiple of 8 up to 128; views with
     d contiguous and rows on 16 bytes are read in place.  scale: default d ** -0.5.  causal: token i sees the tokens 0 .. i of its sequence.
-    A NaN or infinity reaches the results of its own sequence only (under the causal mask: of its 32-row block and behind it)."""
+    A NaN or infinity reaches the results of its own sequence only.  Under the causal mask it reaches the outputs and the gradient of q from its 32-row
+    block on (rows 32 i .. 32 i + 31 of the sequence), and one of q or of the incoming gradient those of k and v up to its block."""
     scale = _check_heads(q, k, v, seqs, scale)
     if _differentiated(q, k, v):
         return PackedAttentionFn.apply(q, k, v, seqs, bool(causal), scale)

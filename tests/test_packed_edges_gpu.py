@@ -179,3 +179,37 @@ def test_one_row_of_a_larger_matrix(dtype):
     one_head = torch.randn(70, 64, generator=g, device="cuda").to(dtype).unsqueeze(-1).transpose(1, 2)
     assert torch.equal(packed.attention(*(one_head,) * 3, packed.PackedSeqs.from_lengths([50, 20], "cuda")),
                        packed.attention(*(one_head.clone(memory_format=torch.contiguous_format),) * 3, packed.PackedSeqs.from_lengths([50, 20], "cuda")))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("block", [32, 128])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_a_nan_of_the_future_stays_in_its_block(dtype, d, block, value, monkeypatch):
+    """one bad token inside a causal sequence: rows that cannot see it, but for its own 32, keep their results to the bit, with either size of blocks"""
+    monkeypatch.setattr(packed, "_block_rows", lambda *_: block)
+    n = 300
+    g = torch.Generator(device="cuda").manual_seed(d)
+    clean = [torch.randn(n + 20, h, d, generator=g, device="cuda").to(dtype) for h in (4, 2, 2, 4)]
+    seqs = packed.PackedSeqs(torch.tensor([0, 20, n + 20], dtype=torch.int32, device="cuda"), n + 20)
+
+    def run(q, k, v, dout):
+        t = [x.detach().clone().requires_grad_(True) for x in (q, k, v)]
+        out = packed.attention(*t, seqs)
+        return [x[20:] for x in (out.detach(), *torch.autograd.grad(out, t, dout))]
+
+    want = run(*clean)
+    for at in (40, 100, 159, 161, 256):
+        lo, hi = at // 32 * 32, at // 32 * 32 + 32
+        for which in range(4):
+            dirty = [x.clone() for x in clean]
+            dirty[which][20 + at, 0, d // 2] = value
+            got = run(*dirty)
+            assert not torch.isfinite(torch.stack([x.double().sum() for x in got])).all()
+            for i, (a, b) in enumerate(zip(got, want)):  # out, dq, dk, dv
+                if i < 2:
+                    assert torch.equal(a[:lo], b[:lo]), (at, which, i)
+                elif which in (0, 3):
+                    assert torch.equal(a[hi:], b[hi:]), (at, which, i)
+                if i == 0 and which == 3:
+                    assert torch.equal(a, b)
