@@ -467,7 +467,7 @@ int cvh_packed_attn_bwd(int dtype, const cvh_packed_attn* p, void* stream);
 /* ---- token embedding on packed rows, its gradient by sorted tokens ------------------------------- */
 /* out[r] = scale * table[ids[r]] + pos[place of r in its sequence] (pos nullable), table / pos float32, e % 8 == 0.  plan: the work list of
  * cvh_packed_plan (rows behind its last sequence become zeros), or NULL: every row counts and pos must be NULL.  A token outside 0 .. vocab - 1 or a
- * place at or behind `positions` gives a row of NaN (never a read out of bounds).
+ * place at or behind `positions` (at most 2^22) gives a row of NaN (never a read out of bounds).
  * bwd: dtable[vocab][e] = scale * the sums of dout over the rows of each token, in row order (padding_idx's row: zero), every row written once;
  * dpos[positions][e] = the sums over the sequences; either may be NULL.  sort / pieces: scratch of cvh_embed_sort_elems int32 /
  * cvh_embed_pieces_elems float32.  No atomics on values: bit-reproducible. */

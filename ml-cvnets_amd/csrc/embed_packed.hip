@@ -19,6 +19,7 @@ constexpr int kItems = 1024;   // rows a sort workgroup takes: 4 waves x 4 round
 constexpr int kChunk = 32;     // sorted rows that are summed by one group of lanes
 constexpr int kTableRows = 32;  // rows of the table a workgroup writes
 constexpr int kMostRows = 0x7fffffff - 4096, kMostBlocks = 1 << 24;  // (a grid has fewer than 2^32 threads)
+constexpr int kMostPositions = 1 << 22;
 
 // sort key of row r: its token, or `vocab` (sorted behind everything) where the row adds nothing: behind the last sequence, the padding token,
 // a token outside the table
@@ -375,7 +376,8 @@ int sort_passes(int vocab) {
 }
 long long sort_blocks(long long n) { return (n + kItems - 1) / kItems; }
 long long padded(long long n) { return (n + kChunk - 1) / kChunk * kChunk; }
-int pos_split(int seqs) { return seqs <= 64 ? 1 : seqs >= 1024 ? 16 : (seqs + 63) / 64; }  // 64 sequences a workgroup, while that is at most 16 parts
+// 64 sequences a workgroup, while that is at most 16 parts; one part where the positions alone are more workgroups than the card takes at a time
+int pos_split(int seqs, int positions) { return seqs <= 64 || positions > 1 << 18 ? 1 : seqs >= 1024 ? 16 : (seqs + 63) / 64; }
 
 }  // namespace
 
@@ -386,14 +388,14 @@ extern "C" long long cvh_embed_sort_elems(int rows) {
 }
 // float32 scratch: two pieces a chunk, the parts of the positions' sums
 extern "C" long long cvh_embed_pieces_elems(int rows, int e, int positions, int seqs) {
-  if (rows <= 0 || rows > kMostRows || e <= 0 || positions < 0 || seqs < 0) return -2;
-  const int split = pos_split(seqs);
+  if (rows <= 0 || rows > kMostRows || e <= 0 || positions < 0 || positions > kMostPositions || seqs < 0) return -2;
+  const int split = pos_split(seqs, positions);
   return (padded(rows) / kChunk * 2 + (split > 1 ? (long long)split * positions : 0)) * e;
 }
 extern "C" int cvh_embed_packed_fwd(int dtype, const long long* ids, const float* table, const float* pos, const int* plan, int seqs, int block, int places,
                                     int rows, int vocab, int positions, int e, float scale, void* out, void* stream) {
   if (dtype != CVH_DT_F32 && dtype != CVH_DT_BF16) return -1;
-  if (ids == nullptr || table == nullptr || out == nullptr || rows <= 0 || rows > kMostRows || vocab <= 0 || e <= 0 || e % 8 || (pos != nullptr && (plan == nullptr || positions <= 0))) return -2;
+  if (ids == nullptr || table == nullptr || out == nullptr || rows <= 0 || rows > kMostRows || vocab <= 0 || e <= 0 || e % 8 || (pos != nullptr && (plan == nullptr || positions <= 0 || positions > kMostPositions))) return -2;
   if (plan != nullptr && (seqs <= 0 || (block != 32 && block != 128) || places != rows / block + seqs + 1)) return -2;
   if (plan == nullptr) {
     block = 32;
@@ -415,7 +417,7 @@ extern "C" int cvh_embed_packed_fwd(int dtype, const long long* ids, const float
 extern "C" int cvh_embed_packed_bwd(int dtype, const long long* ids, const void* dout, const int* plan, int seqs, int rows, int vocab, int e, long long padding_idx,
                                     float scale, float* dtable, int positions, float* dpos, int* sort, float* pieces, void* stream) {
   if (dtype != CVH_DT_F32 && dtype != CVH_DT_BF16) return -1;
-  if (dout == nullptr || rows <= 0 || rows > kMostRows || e <= 0 || e % 8 || (dpos != nullptr && (plan == nullptr || positions <= 0 || positions > kMostBlocks / 64 || pieces == nullptr)) || (plan != nullptr && seqs <= 0)) return -2;
+  if (dout == nullptr || rows <= 0 || rows > kMostRows || e <= 0 || e % 8 || (dpos != nullptr && (plan == nullptr || positions <= 0 || positions > kMostPositions || pieces == nullptr)) || (plan != nullptr && seqs <= 0)) return -2;
   if (dtable != nullptr && (ids == nullptr || sort == nullptr || pieces == nullptr || vocab <= 0 || vocab / kTableRows >= kMostBlocks / 2)) return -2;
   hipStream_t st = (hipStream_t)stream;
   Grad g = {};
@@ -446,10 +448,11 @@ extern "C" int cvh_embed_packed_bwd(int dtype, const long long* ids, const void*
   }
   g.pos_split = 1;
   if (dpos != nullptr) {
-    g.pos_split = pos_split(seqs);
+    g.pos_split = pos_split(seqs, positions);
     g.pos_blocks = positions * g.pos_split;
     g.pos_part = pieces + (long long)padded(rows) / kChunk * 2 * e;
   }
+  if ((long long)g.chunk_blocks + g.pos_blocks + zero_blocks >= kMostBlocks) return -2;
   const dim3 grid(g.chunk_blocks + g.pos_blocks + zero_blocks);
   if (grid.x == 0) return 0;
   if (dtype == CVH_DT_BF16) hipLaunchKernelGGL(embed_grad_kernel<bf16_t>, grid, dim3(256), 0, st, g, (const bf16_t*)dout);

@@ -18,6 +18,7 @@ from .ops import _check_dev, _dt, _p, call_on, compute_dtype
 _MOST_ROWS = 2 ** 31 - 4097  # rows are counted in 32 bits
 _MOST_BLOCKS = (1 << 24) - 1  # a grid has fewer than 2^32 threads
 _MOST_ROW = 1 << 21  # elements between two rows
+_MOST_POSITIONS = 1 << 22
 
 
 def _block_rows(rows: int, seqs: int, max_len: int) -> int:
@@ -294,6 +295,8 @@ def embed(ids: Tensor, table: Tensor, seqs: Optional[PackedSeqs] = None, pos: Op
             raise RuntimeError(f"pos must be float32 [positions, {e}]. Got: {pos.dtype} {list(pos.shape)}")
         if seqs is None:
             raise RuntimeError("pos needs the layout of the sequences (seqs)")
+        if pos.shape[0] > _MOST_POSITIONS:
+            raise NotImplementedError(f"packed embedding: up to {_MOST_POSITIONS} positions are supported. Got: {pos.shape[0]}")
     if seqs is not None and seqs.rows != ids.shape[0]:
         raise RuntimeError(f"the layout is of {seqs.rows} rows, ids has {ids.shape[0]}")
     if padding_idx is not None and not 0 <= padding_idx < vocab:

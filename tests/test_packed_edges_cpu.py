@@ -68,3 +68,20 @@ def test_one_row_of_a_projection(launches):
     packed.attention_qkv(qkv, 2, layout(rows=1), kv_heads=2)
     args = _lib.PackedAttn.from_buffer_copy(launches[-1][2])
     assert (args.q_row, args.q_head) == (384, 64)
+
+
+def test_more_positions_than_the_gradient_takes_are_refused_by_the_forward(launches):
+    """what is refused is refused before the forward pass, not by its backward"""
+    lib = _lib.load()
+    ids, table = torch.zeros(10, dtype=torch.int64), torch.zeros(7, 8)
+    most = 1 << 22
+    pos = torch.zeros(1, 8).expand(most + 1, 8).detach().requires_grad_(True)  # (never copied: refused)
+    with pytest.raises(NotImplementedError, match="positions"):
+        packed.embed(ids, table, layout(), pos=pos, dtype=torch.float32)
+    for positions, rc in ((most + 1, -2), (0, -2)):
+        assert lib.cvh_embed_packed_fwd(1, 256, 256, 256, 256, 1, 32, 2, 10, 7, positions, 8, 1.0, 256, None) == rc
+        assert lib.cvh_embed_packed_bwd(1, 256, 256, 256, 1, 10, 7, 8, -1, 1.0, 256, positions, 256, 256, 256, None) == rc
+    # the scratch of the sums: a part of the positions' sums for every 64 sequences, where 16 parts of them are not too many
+    assert lib.cvh_embed_pieces_elems(10, 8, 1000, 128) == (2 + 2 * 1000) * 8
+    assert lib.cvh_embed_pieces_elems(10, 8, most, 128) == (2 + 0) * 8
+    assert lib.cvh_embed_pieces_elems(10, 8, most + 1, 128) == -2

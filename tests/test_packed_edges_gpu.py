@@ -213,3 +213,20 @@ def test_a_nan_of_the_future_stays_in_its_block(dtype, d, block, value, monkeypa
                     assert torch.equal(a[hi:], b[hi:]), (at, which, i)
                 if i == 0 and which == 3:
                     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("positions,seqs", [((1 << 18) + 5, 200), (1 << 22, 3)])
+def test_many_positions(positions, seqs):
+    """long tables of positions: what lies behind the longest sequence has no gradient, the rest is the sums over the sequences (of small whole numbers: exact)"""
+    lens = [5 + 7 * (i % 11) for i in range(seqs)]
+    rows = sum(lens)
+    table = torch.zeros(9, 8, device="cuda")
+    pos = torch.zeros(positions, 8, device="cuda").requires_grad_(True)
+    ids = torch.arange(rows, device="cuda") % 9
+    dy = torch.randint(-3, 4, (rows, 8), generator=torch.Generator(device="cuda").manual_seed(5), device="cuda").float()
+    out = packed.embed(ids, table, packed.PackedSeqs.from_lengths(lens, "cuda"), pos=pos, dtype=torch.float32)
+    (dpos,) = torch.autograd.grad(out, (pos,), dy)
+    want = torch.zeros(max(lens), 8, dtype=torch.float64)
+    want.index_add_(0, torch.cat([torch.arange(n) for n in lens]), dy.double().cpu())
+    assert torch.equal(dpos[:max(lens)].double().cpu(), want)
+    assert bool((dpos[max(lens):] == 0).all())
