@@ -20,6 +20,10 @@ constexpr int kChunk = 32;     // sorted rows that are summed by one group of la
 constexpr int kTableRows = 32;  // rows of the table a workgroup writes
 constexpr int kMostRows = 0x7fffffff - 4096, kMostBlocks = 1 << 24;  // (a grid has fewer than 2^32 threads)
 constexpr int kMostPositions = 1 << 22;
+// A scatter workgroup reads the counts of all workgroups where there are at most so many, which costs less than the launch that scans them; beyond, that
+// would grow with the square of the rows (forward and gradient of 64, 128, 256, 1024, 4096 k rows x 32, a token each of 50000: 52 / 54, 69 / 67, 96 / 82,
+// 332 / 222, 2286 / 642 us).
+constexpr int kAllCounts = 96;
 
 // sort key of row r: its token, or `vocab` (sorted behind everything) where the row adds nothing: behind the last sequence, the padding token,
 // a token outside the table
@@ -52,9 +56,40 @@ __global__ __launch_bounds__(256) void sort_count_kernel(SortIn s, int* __restri
   count[blockIdx.x * 256 + threadIdx.x] = c[threadIdx.x];
 }
 
+// The counts turned into places, in place: of each digit, the rows in earlier workgroups; behind the last workgroup's line: the rows of each digit in all.  A
+// workgroup takes 32 digits, 32 lanes a line; each of its 32 groups of lanes a run of consecutive workgroups' counts.
+__global__ __launch_bounds__(1024) void sort_scan_kernel(int* __restrict__ count, int blocks) {
+  __shared__ int sum[32][32];
+  const int digit = threadIdx.x & 31, group = threadIdx.x >> 5;
+  int* const at = count + blockIdx.x * 32 + digit;
+  const int per = (blocks + 31) / 32, b0 = min(group * per, blocks), b1 = min(b0 + per, blocks);
+  int s = 0;
+#pragma unroll 8
+  for (int b = b0; b < b1; ++b) s += at[(size_t)b * 256];
+  sum[group][digit] = s;
+  __syncthreads();
+  int run = 0, total = 0;
+  for (int g = 0; g < 32; ++g) {
+    if (g == group) run = total;
+    total += sum[g][digit];
+  }
+  for (int b = b0; b < b1; b += 8) {
+    int v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = at[(size_t)min(b + j, b1 - 1) * 256];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (b + j < b1) at[(size_t)(b + j) * 256] = run;
+      run += v[j];
+    }
+  }
+  if (group == 0) at[(size_t)blocks * 256] = total;
+}
+
 // stable scatter of one pass.  A wave's rows are consecutive; a lane's place = rows of smaller digits + of this digit in earlier workgroups, waves
 // and rounds + in lower lanes of its round (8 ballots find the lanes with the same digit).
-__global__ __launch_bounds__(256) void sort_scatter_kernel(SortIn s, const int* __restrict__ count, unsigned* __restrict__ keys_out, int* __restrict__ rows_out) {
+// count: the workgroups' counts, or (scanned) what sort_scan_kernel made of them.
+__global__ __launch_bounds__(256) void sort_scatter_kernel(SortIn s, const int* __restrict__ count, int scanned, unsigned* __restrict__ keys_out, int* __restrict__ rows_out) {
   __shared__ int at[4][256];  // counts, then next place, of each wave and digit
   __shared__ int scan[256];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -73,6 +108,9 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(SortIn s, const int* 
   int before = 0, total = 0;  // digit `tid`: rows in earlier workgroups, rows in all
   if (gridDim.x == 1) {
     total = at[0][tid] + at[1][tid] + at[2][tid] + at[3][tid];
+  } else if (scanned) {
+    before = count[(size_t)blockIdx.x * 256 + tid];
+    total = count[(size_t)gridDim.x * 256 + tid];
   } else {
     for (int b0 = 0; b0 < (int)gridDim.x; b0 += 16) {
       int v[16];
@@ -384,7 +422,7 @@ int pos_split(int seqs, int positions) { return seqs <= 64 || positions > 1 << 1
 // int32 scratch: two key and two row arrays (in whole chunks), the digit counts
 extern "C" long long cvh_embed_sort_elems(int rows) {
   if (rows <= 0 || rows > kMostRows) return -2;
-  return 4 * padded(rows) + sort_blocks(rows) * 256;
+  return 4 * padded(rows) + (sort_blocks(rows) + 1) * 256;
 }
 // float32 scratch: two pieces a chunk, the parts of the positions' sums
 extern "C" long long cvh_embed_pieces_elems(int rows, int e, int positions, int seqs) {
@@ -436,7 +474,9 @@ extern "C" int cvh_embed_packed_bwd(int dtype, const long long* ids, const void*
     for (int p = 0; p < passes; ++p) {
       s.shift = 8 * p;
       if (blocks > 1) hipLaunchKernelGGL(sort_count_kernel, dim3(blocks), dim3(256), 0, st, s, count);
-      hipLaunchKernelGGL(sort_scatter_kernel, dim3(blocks), dim3(256), 0, st, s, count, keys[p & 1], order[p & 1]);
+      const int scanned = blocks > kAllCounts;
+      if (scanned) hipLaunchKernelGGL(sort_scan_kernel, dim3(8), dim3(1024), 0, st, count, blocks);
+      hipLaunchKernelGGL(sort_scatter_kernel, dim3(blocks), dim3(256), 0, st, s, count, scanned, keys[p & 1], order[p & 1]);
       s.keys = keys[p & 1];
       s.rows = order[p & 1];
     }

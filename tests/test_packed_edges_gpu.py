@@ -230,3 +230,17 @@ def test_many_positions(positions, seqs):
     want.index_add_(0, torch.cat([torch.arange(n) for n in lens]), dy.double().cpu())
     assert torch.equal(dpos[:max(lens)].double().cpu(), want)
     assert bool((dpos[max(lens):] == 0).all())
+
+
+@pytest.mark.parametrize("rows", [96 * 1024, 96 * 1024 + 1, 130001, 1 << 20])
+@pytest.mark.parametrize("vocab", [200, 70000])
+def test_sorting_many_rows(rows, vocab):
+    """both ways to the places of the sorted rows, in one pass of the sort and in three; whole numbers: the sums are exact"""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    ids = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    ids[::7] = vocab - 1
+    dy = torch.randint(-3, 4, (rows, 16), generator=g, device="cuda").to(torch.bfloat16)
+    table = torch.zeros(vocab, 16, device="cuda").requires_grad_(True)
+    (dtable,) = torch.autograd.grad(packed.embed(ids, table, dtype=torch.bfloat16), (table,), dy)
+    want = torch.zeros(vocab, 16, dtype=torch.float64, device="cuda").index_add_(0, ids, dy.double())
+    assert torch.equal(dtable.double(), want)
