@@ -318,9 +318,10 @@ template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(G
 __global__ __launch_bounds__(256) void embed_join_kernel(Grad g, int chunks) {
   __shared__ __attribute__((aligned(16))) float joined[2048];
   __shared__ int run_end;
-  const int tid = threadIdx.x, G = g.group, per = 256 / G, sub = tid / G, sl = tid % G;
-  if ((int)blockIdx.x >= chunks) {
-    const int t = blockIdx.x - chunks, positions = g.pos_blocks / g.pos_split;
+  const int tid = threadIdx.x, G = g.group, per = 256 / G, sub = tid / G, sl = tid % G, item = blockIdx.y * gridDim.x + blockIdx.x;
+  if (item >= chunks) {
+    const int t = item - chunks, positions = g.pos_blocks / g.pos_split;
+    if (g.pos_split == 1 || t >= positions) return;  // (the last line of the grid)
     for (int c = tid; c < g.e; c += 256) {
       float s = 0.f;
 #pragma unroll 8
@@ -329,7 +330,7 @@ __global__ __launch_bounds__(256) void embed_join_kernel(Grad g, int chunks) {
     }
     return;
   }
-  const int chunk = blockIdx.x, a = chunk * kChunk, b = a + kChunk;
+  const int chunk = item, a = chunk * kChunk, b = a + kChunk;
   if (b >= g.n) return;
   const unsigned v = g.keys[b - 1];
   if (v >= (unsigned)g.vocab || g.keys[b] != v || (a > 0 && g.keys[a - 1] == v)) return;  // does not go on, or came in (the same for all threads)
@@ -434,9 +435,9 @@ extern "C" int cvh_embed_packed_fwd(int dtype, const long long* ids, const float
                                     int rows, int vocab, int positions, int e, float scale, void* out, void* stream) {
   if (dtype != CVH_DT_F32 && dtype != CVH_DT_BF16) return -1;
   if (ids == nullptr || table == nullptr || out == nullptr || rows <= 0 || rows > kMostRows || vocab <= 0 || e <= 0 || e % 8 || (pos != nullptr && (plan == nullptr || positions <= 0 || positions > kMostPositions))) return -2;
-  if (plan != nullptr && (seqs <= 0 || (block != 32 && block != 128) || places != rows / block + seqs + 1)) return -2;
+  if (plan != nullptr && (seqs <= 0 || (block != 32 && block != 128) || places != (long long)rows / block + seqs + 1)) return -2;
   if (plan == nullptr) {
-    block = 32;
+    block = rows < 1 << 28 ? 32 : 128;
     places = (rows + block - 1) / block;
   }
   if (places >= kMostBlocks) return -2;
@@ -498,7 +499,8 @@ extern "C" int cvh_embed_packed_bwd(int dtype, const long long* ids, const void*
   if (dtype == CVH_DT_BF16) hipLaunchKernelGGL(embed_grad_kernel<bf16_t>, grid, dim3(256), 0, st, g, (const bf16_t*)dout);
   else hipLaunchKernelGGL(embed_grad_kernel<float>, grid, dim3(256), 0, st, g, (const float*)dout);
   const int joins = (chunks > 1 ? chunks : 0) + (g.pos_split > 1 ? positions : 0);
-  if (joins > 0) hipLaunchKernelGGL(embed_join_kernel, dim3(joins), dim3(256), 0, st, g, chunks > 1 ? chunks : 0);
+  constexpr int kLine = 1 << 22;  // (2^26 chunks of 2^31 rows: lines of a grid)
+  if (joins > 0) hipLaunchKernelGGL(embed_join_kernel, dim3(joins < kLine ? joins : kLine, (joins + kLine - 1) / kLine), dim3(256), 0, st, g, chunks > 1 ? chunks : 0);
   CVH_CHECK_LAUNCH();
   return 0;
 }

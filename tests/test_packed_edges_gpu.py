@@ -244,3 +244,19 @@ def test_sorting_many_rows(rows, vocab):
     (dtable,) = torch.autograd.grad(packed.embed(ids, table, dtype=torch.bfloat16), (table,), dy)
     want = torch.zeros(vocab, 16, dtype=torch.float64, device="cuda").index_add_(0, ids, dy.double())
     assert torch.equal(dtable.double(), want)
+
+
+def test_more_rows_than_one_line_of_workgroups():
+    """2^29 rows and more (34 GB): every run of a token crosses millions of chunks; few rows have a gradient, so that the sums are exact"""
+    rows, vocab = (1 << 29) + 1000, 5
+    table = torch.randn(vocab, 8, device="cuda").requires_grad_(True)
+    ids = torch.arange(rows, device="cuda", dtype=torch.int64).remainder_(vocab)
+    out = packed.embed(ids, table, dtype=torch.bfloat16)
+    for a in (0, 1 << 28, rows - 1000):
+        assert torch.equal(out[a:a + 1000], table.detach()[ids[a:a + 1000]].to(torch.bfloat16))
+    dy = torch.zeros(rows, 8, dtype=torch.bfloat16, device="cuda")
+    some = torch.randint(0, rows, (5000,), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").unique()
+    some = torch.cat([some, torch.tensor([rows - 1], device="cuda")]).unique()
+    dy[some] = torch.randint(-3, 4, (some.numel(), 8), generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").to(torch.bfloat16)
+    (dtable,) = torch.autograd.grad(out, (table,), dy)
+    assert torch.equal(dtable.double(), torch.zeros(vocab, 8, dtype=torch.float64, device="cuda").index_add_(0, ids[some], dy[some].double()))
