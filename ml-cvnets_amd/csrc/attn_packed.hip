@@ -794,7 +794,7 @@ int check(int dtype, const PA* p, int backward) {
   if (p == nullptr || p->plan == nullptr) return -2;
   if (p->rows <= 0 || p->rows > kMostRows || p->seqs <= 0 || p->seqs > kMostRows || p->heads_q <= 0 || p->heads_kv <= 0 || p->heads_q % p->heads_kv || p->d <= 0 || p->d > 128 || p->d % 8) return -2;
   if (!(p->scale > 0.f) || (p->block != 32 && p->block != 128)) return -2;
-  if (p->places != p->rows / p->block + p->seqs + 1 || (long long)p->places * p->heads_q >= (1 << 24)) return -2;  // (a grid has fewer than 2^32 threads)
+  if (p->places != (long long)p->rows / p->block + p->seqs + 1 || (long long)p->places * p->heads_q >= (1 << 24)) return -2;  // (a grid has fewer than 2^32 threads)
   if (!strides_ok(dtype, p->q, p->q_row, p->q_head) || !strides_ok(dtype, p->k, p->k_row, p->k_head) || !strides_ok(dtype, p->v, p->v_row, p->v_head) ||
       !strides_ok(dtype, p->out, p->o_row, p->o_head))
     return -2;
@@ -813,6 +813,7 @@ extern "C" long long cvh_packed_plan_elems(int seqs, int rows, int block) {
 }
 extern "C" int cvh_packed_plan(const int* cu, int seqs, int rows, int block, int* plan, void* stream) {
   if (cu == nullptr || plan == nullptr || seqs <= 0 || seqs > kMostRows || rows <= 0 || rows > kMostRows || (block != 32 && block != 128)) return -2;
+  if ((long long)rows / block + seqs + 1 >= 1 << 24) return -2;  // more than any launch over the list takes
   hipLaunchKernelGGL(packed_plan_kernel, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, cu, seqs, rows, block, plan, rows / block + seqs + 1);
   CVH_CHECK_LAUNCH();
   return 0;

@@ -51,13 +51,15 @@ class PackedSeqs:
             raise ValueError(f"max_len must not be negative. Got: {max_len}")
         if context_length is not None and context_length < 1:
             raise ValueError(f"context_length must be positive. Got: {context_length}")
-        _check_dev(cu_seqlens)
         self.cu_seqlens, self.rows, self.seqs = cu_seqlens, rows, cu_seqlens.numel() - 1
         self.max_len = rows if max_len is None else min(int(max_len), rows)
         self.context_length = None if context_length is None else int(context_length)
         self.block = _block_rows(rows, self.seqs, self.max_len)
         self.version = 0  # of the work list: a backward pass with another one than its forward is refused
         self.places = rows // self.block + self.seqs + 1
+        if self.places > _MOST_BLOCKS:
+            raise ValueError(f"{self.seqs} sequences in {rows} rows are more than one launch takes ({self.places} blocks, at most {_MOST_BLOCKS})")
+        _check_dev(cu_seqlens)
         self.plan = torch.empty(_lib.query("cvh_packed_plan_elems", self.seqs, rows, self.block), dtype=torch.int32, device=cu_seqlens.device)
         self.refresh()
 

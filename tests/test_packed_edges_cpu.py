@@ -85,3 +85,13 @@ def test_more_positions_than_the_gradient_takes_are_refused_by_the_forward(launc
     assert lib.cvh_embed_pieces_elems(10, 8, 1000, 128) == (2 + 2 * 1000) * 8
     assert lib.cvh_embed_pieces_elems(10, 8, most, 128) == (2 + 0) * 8
     assert lib.cvh_embed_pieces_elems(10, 8, most + 1, 128) == -2
+
+
+def test_a_layout_that_no_launch_takes_is_refused_when_it_is_made():
+    lib = _lib.load()
+    for seqs, rows, block in ((1 << 24, 1000, 32), ((1 << 24) - 1, 100, 128), (1, (1 << 29), 32), (2 ** 31 - 4097, 2 ** 31 - 4097, 32)):
+        assert rows // block + seqs + 1 >= 1 << 24 and lib.cvh_packed_plan(256, seqs, rows, block, 256, None) == -2
+    with pytest.raises(ValueError, match="more than one launch"):
+        packed.PackedSeqs(torch.zeros((1 << 24) + 1, dtype=torch.int32), 1000)
+    with pytest.raises(ValueError, match="more than one launch"):
+        packed.PackedSeqs(torch.zeros(40, dtype=torch.int32), 2 ** 31 - 4097)
