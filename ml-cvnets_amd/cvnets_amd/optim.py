@@ -327,8 +327,7 @@ class Muon(torch.optim.Optimizer):
             raise ValueError(f"lr and weight_decay must not be negative, momentum in [0, 1). Got: {lr}, {weight_decay}, {momentum}")
         self._ns = _check_ns(ns_steps, ns_coefficients, eps)
         self._plan = None
-        self._rates = []  # [device table of (lr, weight_decay) by group, its values], the newest last
-        self._workspaces = []  # every one that was handed to the kernels: a captured step goes on using its own (and its own table of rates)
+        self._rates = []  # [device table of (lr, weight_decay) by group, its values], the newest last; a captured step goes on reading its own
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=bool(nesterov), weight_decay=weight_decay))
 
     def add_param_group(self, param_group) -> None:
@@ -383,12 +382,7 @@ class Muon(torch.optim.Optimizer):
         rows = [_lib.NsMatrix(src=_p(entries[i][1]), momentum=_p(self.state[entries[i][0]]["momentum_buffer"]), param=_p(entries[i][0]), rows=sizes[i][0],
                               cols=sizes[i][1], group=entries[i][2], gain=math.sqrt(max(1.0, sizes[i][0] / sizes[i][1]))) for i in _by_cost(sizes)]
         table = (_lib.NsMatrix * len(rows))(*rows)
-        need = _lib.query("cvh_ns_workspace_elems", ctypes.byref(table), len(rows))
-        ws = next((w for w in self._workspaces if w.numel() >= need and w.device == dev), None)
-        if ws is None:
-            ws = torch.empty(need, dtype=torch.float32, device=dev)
-            self._workspaces.append(ws)
-        self._plan = {"table": table, "n": len(rows), "ws": ws, "key": self._key(entries)}
+        self._plan = {"table": table, "n": len(rows), "need": _lib.query("cvh_ns_workspace_elems", ctypes.byref(table), len(rows)), "key": self._key(entries)}
         return self._plan
 
     def _key(self, entries):
@@ -437,6 +431,8 @@ class Muon(torch.optim.Optimizer):
         for g in self.param_groups:  # (they may be rewritten, or loaded)
             if (g["momentum"], g["nesterov"]) != (g0["momentum"], g0["nesterov"]):
                 raise NotImplementedError("per-group momentum / nesterov are not supported")
-        ops.call_on(dev, "cvh_muon_step", ctypes.byref(plan["table"]), plan["n"], *self._ns, float(g0["momentum"]), int(g0["nesterov"]), _p(self._rates[-1][0]), _p(plan["ws"]))
+        # a workspace of this step's own, on its stream: a graph takes one from its own memory, so that two of them may be replayed side by side
+        ws = torch.empty(plan["need"], dtype=torch.float32, device=dev)
+        ops.call_on(dev, "cvh_muon_step", ctypes.byref(plan["table"]), plan["n"], *self._ns, float(g0["momentum"]), int(g0["nesterov"]), _p(self._rates[-1][0]), _p(ws))
         ops.invalidate_packed()
         return loss

@@ -57,3 +57,38 @@ def test_singular_values_beyond_4(dtype, shape, coefficients, steps):
     assert torch.isfinite(got).all()
     rounding = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
     assert float((got - want).norm() / want.norm()) <= error / s + rounding
+
+
+def test_two_captured_steps_side_by_side():
+    """one optimizer, a graph for each half of its parameters, replayed on two streams at a time: the same weights as eager steps, to the bit"""
+    def make():
+        g = torch.Generator(device="cuda").manual_seed(3)
+        ps = [torch.nn.Parameter(torch.randn(s, generator=g, device="cuda")) for s in ((600, 500), (500, 620), (640, 510), (512, 512))]
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=g, device="cuda")
+        return ps, optim.Muon(ps, lr=0.1)
+
+    (ps, opt), (twins, eager) = make(), make()
+    grads = [p.grad for p in ps]
+    opt.step()
+    eager.step()
+    graphs = []
+    for half in ((0, 1), (2, 3)):
+        for i, p in enumerate(ps):
+            p.grad = grads[i] if i in half else None
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step(sync_hyperparameters=False)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for it in range(6):
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        eager.step()
+        torch.cuda.synchronize()
+        for p, q in zip(ps, twins):
+            assert torch.equal(p, q), it
+            assert torch.equal(opt.state[p]["momentum_buffer"], eager.state[q]["momentum_buffer"]), it
