@@ -310,6 +310,10 @@ def orthogonalize(matrices: Union[torch.Tensor, Sequence[torch.Tensor]], steps: 
     return out[0] if single else out
 
 
+def _capturing(device: torch.device) -> bool:
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 class Muon(torch.optim.Optimizer):
     """Momentum whose update is orthogonalised, for the matrices of a model (dimensions behind the first are flattened, as in a convolution's
     [out, in, kh, kw]); vectors, embeddings and heads stay with ``AdamW``:
@@ -319,7 +323,7 @@ class Muon(torch.optim.Optimizer):
 
     ``param_groups`` with their own lr and weight_decay, which a scheduler may rewrite; ``state[p]["momentum_buffer"]`` and the usual state dict.
     One step is 2 + 3 ns_steps launches for up to 32 matrices.  Rates live on the device: a captured ``step(sync_hyperparameters=False)``
-    follows ``sync_hyperparameters()`` calls between replays."""
+    follows ``sync_hyperparameters()`` calls between replays.  A step is captured after an eager one with the same parameters."""
 
     def __init__(self, params: Iterable, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, ns_steps: int = 5,
                  ns_coefficients: Sequence[float] = NS_COEFFICIENTS, eps: float = 1e-7):
@@ -377,6 +381,8 @@ class Muon(torch.optim.Optimizer):
                 raise RuntimeError(f"a parameter became another matrix: {list(p.shape)}, contiguous {p.is_contiguous()}, its momentum {None if buf is None else list(buf.shape)}")
             _check_matrix(p.shape[0], p.numel() // max(1, p.shape[0]))
             if buf is None or buf.dtype != torch.float32 or not buf.is_contiguous() or buf.device != dev:  # (a loaded state may be another type's)
+                if _capturing(dev):  # every replay would make it again
+                    raise RuntimeError("a captured step needs the momentum of its parameters: take an eager step with them before the capture")
                 self.state[p]["momentum_buffer"] = torch.zeros_like(p) if buf is None else buf.to(device=dev, dtype=torch.float32).contiguous()
         sizes = [(p.shape[0], p.numel() // p.shape[0]) for p, _, _ in entries]
         rows = [_lib.NsMatrix(src=_p(entries[i][1]), momentum=_p(self.state[entries[i][0]]["momentum_buffer"]), param=_p(entries[i][0]), rows=sizes[i][0],
@@ -398,6 +404,10 @@ class Muon(torch.optim.Optimizer):
         """copy the groups' (lr, weight_decay) to the device tables; call after a scheduler changed them (outside graph replay)"""
         host = [[float(g["lr"]), float(g["weight_decay"])] for g in self.param_groups]
         device = next(p.device for g in self.param_groups for p in g["params"])
+        if _capturing(device):  # what is copied to the device comes from a temporary of the host's
+            if not self._has_rates(device) or any(values != host[:len(table)] for table, values in self._rates):
+                raise RuntimeError("the groups' rates changed: call sync_hyperparameters() before the capture, not in it")
+            return
         if not self._has_rates(device):
             self._rates.append([torch.zeros(len(host), 2, dtype=torch.float32, device=device), None])
         for entry in self._rates:

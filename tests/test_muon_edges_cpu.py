@@ -141,3 +141,30 @@ def test_a_loaded_state_goes_into_the_momentum_that_a_captured_step_holds(launch
     assert {x: opt.state[x]["momentum_buffer"].data_ptr() for x in (p, q)} == held
     assert bool((opt.state[p]["momentum_buffer"] == 3.0).all()) and bool((opt.state[q]["momentum_buffer"] == 0.0).all())
     assert opt.state[p]["momentum_buffer"].data_ptr() != saved["state"][0]["momentum_buffer"].data_ptr()
+
+
+def test_nothing_of_the_host_is_captured(launches, monkeypatch):
+    """a capture would hold the address of a temporary for the rates, and would set the momentum to zero with every replay"""
+    opt = optim.Muon([with_gradient(4, 6)], lr=0.5)
+    capturing = [True]
+    monkeypatch.setattr(optim, "_capturing", lambda device: capturing[0])
+    with pytest.raises(RuntimeError, match="eager step"):
+        opt.step(sync_hyperparameters=False)
+    assert not launches
+    capturing[0] = False
+    opt.step()
+    capturing[0] = True
+    opt.step()  # nothing changed: nothing is copied
+    opt.step(sync_hyperparameters=False)
+    opt.param_groups[0]["lr"] = 0.25
+    with pytest.raises(RuntimeError, match="sync_hyperparameters"):
+        opt.step()
+    opt.step(sync_hyperparameters=False)
+    opt.add_param_group({"params": [torch.nn.Parameter(torch.ones(3, 5))]})
+    with pytest.raises(RuntimeError, match="sync_hyperparameters"):
+        opt.step(sync_hyperparameters=False)  # (no row of rates for the new group)
+    capturing[0] = False
+    opt.sync_hyperparameters()
+    capturing[0] = True
+    opt.step(sync_hyperparameters=False)
+    assert len(launches) == 5

@@ -92,3 +92,26 @@ def test_two_captured_steps_side_by_side():
         for p, q in zip(ps, twins):
             assert torch.equal(p, q), it
             assert torch.equal(opt.state[p]["momentum_buffer"], eager.state[q]["momentum_buffer"]), it
+
+
+def test_a_capture_without_an_eager_step_is_refused():
+    p = torch.nn.Parameter(torch.randn(20, 30, device="cuda"))
+    p.grad = torch.randn(20, 30, device="cuda")
+    opt, before = optim.Muon([p], lr=0.1), p.detach().clone()
+    opt.sync_hyperparameters()
+    for lr in (0.2, None):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="before the capture"):
+            with torch.cuda.graph(graph):
+                opt.step()
+        assert torch.equal(p, before)
+        opt.step()
+        before = p.detach().clone()
+        opt.param_groups[0]["lr"] = lr or 0.1
+    opt.sync_hyperparameters()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not torch.equal(p, before)
