@@ -6,8 +6,8 @@
 //
 // G and P are symmetric and commute: half of their tiles are computed and written twice.  Operands are kept as pairs of fp16 numbers, hi + lo,
 // of the value times a power of two (x: 2^12, so that singular values below 16 stay under fp16's 65504 and an entry of ordinary size far above its
-// subnormals; G and P: 2^12 and 2^10, or what the coefficients leave room for, see Bounds): 22 bits and a sign, and a product is three MFMAs, hi hi + hi lo + lo hi, accumulated in float32 - within a factor of two of a
-// float32 product's error, at a third of the fp16 matrix rate instead of the float32 matrix rate (measured on 8192-cubed library products: 1081 / 3
+// subnormals; G and P: 2^12 and 2^10, or what the coefficients leave room for, see Bounds): 22 bits and a sign, and a product is three MFMAs, hi hi + hi lo + lo hi, accumulated in float32 -
+// results as near to the exact ones as those of float32 products (from 41 rows on, see few rows), at a third of the fp16 matrix rate instead of the float32 matrix rate (measured on 8192-cubed library products: 1081 / 3
 // = 360 against 154 TFLOP/s).  One fp16 or bf16 product per step would be three times as fast, and its rounding (2^-11 and 2^-8) is multiplied by up to
 // a^steps = 485 in the directions of small singular values.
 //
@@ -47,7 +47,8 @@ enum { NORM, SCALE, SYM, APPLY, PHASES };
 struct Mats {
   Mat mat[kMats];
   int first[PHASES][kMats + 1];  // prefixes of workgroups; behind the last matrix: their number
-  int count;
+  int count, steps, nesterov;
+  float a, b, c, eps, mu;
 };
 // the matrix that workgroup `wg` of a phase works on, for all of its waves: lane i compares the end of matrix i
 __device__ __forceinline__ int find(const Mats& t, int phase, int wg) {
@@ -137,14 +138,227 @@ template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_norm_k
 }
 
 // -----------------------------------------------------------------------------------------------------------------------------------------
+// Matrices of few rows.  All steps are one polynomial of u u^T, and with few rows that is small enough for 64 bits: G = u u^T from partial sums (in the
+// scale kernel), Q = the product of the steps' a I + b G + c G^2, G <- (..) G (..) (one workgroup, in the first launch for x x^T), result = Q u / (|u| + eps)
+// (in the first launch of P x): no launch more, and none behind the first step where all matrices of a list are such.  Not for speed: one singular direction
+// is a large part of such a matrix, and pairs of 22 bits through five steps leave an error that nothing averages: 1 .. 16 rows 0.8 .. 1.7e-6 where float32
+// products leave 0.5 .. 1.1e-6, now 0.4 .. 0.6e-7; from 40 rows on the pairs leave 0.7 .. 1.5e-6 where those leave 0.8 .. 3.1e-6.  (In the chain of
+// products / so: 1 x 640 86 / 24 us, 16 x 2500 160 / 31, 40 x 40 63 / 57, 40 x 100000 3765 / 198; eight 16 x 144 next to eight 192 x 576 130 / 133.)
+// In the workspace: partial sums [chunk][pair i >= j], then Q.
+// -----------------------------------------------------------------------------------------------------------------------------------------
+constexpr int kFewRows = 40, kFewCols = 64, kFewChunks = 256;  // columns of a workgroup of the result; most chunks of the partial sums, 64 columns and more each
+typedef GLOBAL double gdouble_t;
+__host__ __device__ __forceinline__ bool few(const Mat& a) { return a.m <= kFewRows; }
+__host__ __device__ __forceinline__ int few_chunks(const Mat& a) { return a.n < 64 * kFewChunks ? (a.n + 63) / 64 : kFewChunks; }
+__device__ __forceinline__ int pairs_of(int m) { return m * (m + 1) / 2; }
+__device__ __forceinline__ gdouble_t* few_parts(const Mat& a) { return (gdouble_t*)a.ws; }
+__device__ __forceinline__ gdouble_t* few_q(const Mat& a) { return few_parts(a) + (size_t)few_chunks(a) * pairs_of(a.m); }
+__device__ __forceinline__ void pair_at(int p, int& i, int& j) {
+  for (i = 0; p > i; ++i) p -= i + 1;
+  j = p;
+}
+
+template <typename T, bool MOM> __device__ __forceinline__ void few_gram(const Mat& a, int chunk, float (*tile)[65], double* red, float mu, int nesterov) {
+  constexpr int MOST = (kFewRows * (kFewRows + 1) / 2 + 255) / 256, LOADS = 5;  // pairs of a thread, elements that it loads at a time
+  const int tid = threadIdx.x, m = a.m, n = a.n, pairs = pairs_of(m), chunks = few_chunks(a);
+  const int per = ((n + chunks - 1) / chunks + 63) & ~63, c0 = chunk * per, c1 = min(c0 + per, n);
+  int slices = 1;  // of the columns, where there are fewer pairs than threads
+  while (slices * 2 * pairs <= 256) slices *= 2;
+  const bool narrow = pairs <= 256;
+  const int mine = narrow ? tid % pairs : tid, slice = narrow ? tid / pairs : 0;
+  int pi[MOST], pj[MOST];
+  double sum[MOST];
+#pragma unroll
+  for (int q = 0; q < MOST; ++q) {
+    pair_at(mine + 256 * q < pairs ? mine + 256 * q : 0, pi[q], pj[q]);
+    sum[q] = 0.0;
+  }
+  const bool flip = a.rows > a.cols;
+  for (int c = c0; c < c1; c += 64) {
+#pragma unroll 1
+    for (int base = tid; base < 64 * m; base += 256 * LOADS) {
+      float v[LOADS];  // in flight together (what is not there: the first element)
+#pragma unroll
+      for (int q = 0; q < LOADS; ++q) {
+        const int idx = base + 256 * q, i = flip ? idx % m : idx >> 6, j = flip ? idx / m : idx & 63;
+        const bool here = idx < 64 * m && c + j < c1;
+        v[q] = update_of<T, MOM>(a, !here ? 0 : flip ? (size_t)(c + j) * m + i : (size_t)i * n + c + j, mu, nesterov);
+        v[q] = here ? v[q] : 0.f;
+      }
+#pragma unroll
+      for (int q = 0; q < LOADS; ++q) {
+        const int idx = base + 256 * q;
+        if (idx < 64 * m) tile[flip ? idx % m : idx >> 6][flip ? idx / m : idx & 63] = v[q];
+      }
+    }
+    __syncthreads();
+    if (slice < slices) {
+#pragma unroll
+      for (int q = 0; q < MOST; ++q) {
+        if (q > 0 && 256 * q >= pairs) continue;
+        const float *x = tile[pi[q]], *y = tile[pj[q]];
+#pragma unroll 4
+        for (int k = slice; k < 64; k += slices) sum[q] += (double)x[k] * (double)y[k];
+      }
+    }
+    __syncthreads();
+  }
+  gdouble_t* const out = few_parts(a) + (size_t)chunk * pairs;
+  if (narrow) {
+    red[tid] = sum[0];
+    __syncthreads();
+    if (tid < pairs) {
+      double s = 0.0;
+      for (int k = 0; k < slices; ++k) s += red[k * pairs + tid];
+      out[tid] = s;
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < MOST; ++q)
+      if (tid + 256 * q < pairs) out[tid + 256 * q] = sum[q];
+  }
+}
+
+// Q by one workgroup.  G, Q and the matrices between them are polynomials of one symmetric matrix: they commute, and their products are symmetric; 2 x 2
+// elements at or below the diagonal a thread, rows and columns up to a multiple of 4 stay zero.  Reading the LDS bounds it (4 x 4 elements a thread: half the
+// reads, but half of the card's units for doubles of this workgroup idle, and slower).
+constexpr size_t kFewBytes = 3 * sizeof(double) * kFewRows * (kFewRows + 2);
+__device__ __forceinline__ void few_solve(const Mats& t, const Mat& a, double* lds) {
+  static_assert(kFewRows % 4 == 0 && kFewRows / 2 * (kFewRows / 2 + 1) / 2 <= 256, "a square of a product a thread");
+  const int tid = threadIdx.x, m = a.m, size = (m + 3) & ~3, half = size / 2, ld = size + 2, pairs = pairs_of(m), chunks = few_chunks(a);
+  double *const G = lds, *const Q = G + size * ld, *const M = Q + size * ld;
+  for (int i = tid; i < 3 * size * ld; i += 256) lds[i] = 0.0;
+  __syncthreads();
+  const gdouble_t* const parts = few_parts(a);
+  for (int p = tid; p < pairs; p += 256) {
+    double s = 0.0;
+#pragma unroll 8
+    for (int c = 0; c < chunks; ++c) s += parts[(size_t)c * pairs + p];
+    int i, j;
+    pair_at(p, i, j);
+    G[i * ld + j] = G[j * ld + i] = s;
+  }
+  if (tid < m) Q[tid * ld + tid] = 1.0;
+  __syncthreads();
+  double total = 0.0;
+  for (int i = 0; i < m; ++i) total += G[i * ld + i];
+  const double inv = 1.0 / (sqrt(total) + (double)t.eps);
+  __syncthreads();
+  for (int i = tid; i < size * ld; i += 256) G[i] *= inv * inv;
+  __syncthreads();
+  const bool in = tid < half * (half + 1) / 2;
+  int i0, j0;
+  pair_at(in ? tid : 0, i0, j0);
+  i0 *= 2;
+  j0 *= 2;
+  struct Out {
+    double v[2][2];
+  };
+  auto multiply = [&](const double* A, const double* B) {
+    Out o = {};
+    if (!in) return o;
+    for (int k = 0; k < size; k += 4) {
+      double x[4][2], y[4][2];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          x[e][f] = A[(i0 + f) * ld + k + e];
+          y[e][f] = B[(k + e) * ld + j0 + f];
+        }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) o.v[r][c] += x[e][r] * y[e][c];
+    }
+    return o;
+  };
+  auto put = [&](double* D, const Out& o) {  // (a square on the diagonal: its lower three)
+    if (!in) return;
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        if (j0 + c <= i0 + r) D[(i0 + r) * ld + j0 + c] = D[(j0 + c) * ld + i0 + r] = o.v[r][c];
+  };
+  for (int s = 0; s < t.steps; ++s) {
+    Out o = multiply(G, G);
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const double g = in ? G[(i0 + r) * ld + j0 + c] : 0.0;
+        o.v[r][c] = (i0 + r == j0 + c && i0 + r < m ? (double)t.a : 0.0) + (double)t.b * g + (double)t.c * o.v[r][c];
+      }
+    put(M, o);
+    __syncthreads();
+    if (s > 0) o = multiply(M, Q);  // (Q is one)
+    if (s + 1 == t.steps) {
+      __syncthreads();
+      put(Q, o);
+      break;
+    }
+    const Out w = multiply(M, G);
+    __syncthreads();
+    put(Q, o);
+    put(G, w);
+    __syncthreads();
+    o = multiply(G, M);
+    __syncthreads();
+    put(G, o);
+    __syncthreads();
+  }
+  __syncthreads();
+  gdouble_t* const out = few_q(a);
+  for (int i = tid; i < m * m; i += 256) out[i] = Q[i / m * ld + i % m] * inv;
+}
+
+// result = Q u: 64 columns, a lane a column, the rows dealt out to the four waves
+template <typename T> __device__ __forceinline__ void few_apply(const Mats& t, const Mat& a, int part, double* lds, const float* __restrict__ hp) {
+  const int tid = threadIdx.x, m = a.m, n = a.n, j = part * kFewCols + (tid & 63);
+  const bool flip = a.rows > a.cols;
+  auto place_of = [&](int i) { return flip ? (size_t)min(j, n - 1) * m + i : (size_t)i * n + min(j, n - 1); };
+  double u[kFewRows];
+#pragma unroll
+  for (int k = 0; k < kFewRows; ++k) {
+    const size_t at = place_of(min(k, m - 1));  // (all loads in flight)
+    u[k] = k < m ? (double)(a.mom != nullptr ? update_of<float, true>(a, at, t.mu, t.nesterov) : update_of<T, false>(a, at, 0.f, 0)) : 0.0;
+  }
+  const gdouble_t* const q = few_q(a);
+#pragma unroll 4
+  for (int i = tid; i < m * kFewRows; i += 256) {
+    const double v = q[i / kFewRows * m + min(i % kFewRows, m - 1)];
+    lds[i] = i % kFewRows < m ? v : 0.0;
+  }
+  __syncthreads();  // (u is read: the result may be written over it)
+  if (j >= n) return;
+  const float lr = a.par != nullptr ? hp[2 * a.group] : 0.f, keep = a.par != nullptr ? 1.f - lr * hp[2 * a.group + 1] : 0.f, step = lr * a.gain;
+  for (int i = tid >> 6; i < m; i += 4) {
+    const float old = a.par != nullptr ? gvalue<float>(a.par, place_of(i)) : 0.f;
+    double y[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int k = 0; k < kFewRows; ++k) y[k & 3] += lds[i * kFewRows + k] * u[k];
+    const float v = (float)((y[0] + y[1]) + (y[2] + y[3]));
+    if (a.par != nullptr) gput<float>(a.par, place_of(i), old * keep - step * v);
+    else gput<T>(a.dst, place_of(i), v);
+  }
+}
+
+// -----------------------------------------------------------------------------------------------------------------------------------------
 // x = u / (|u| + eps), 64 x 64 elements (of the padded matrix) a workgroup; through LDS where the matrix is taller than wide
 // -----------------------------------------------------------------------------------------------------------------------------------------
 template <typename T, bool MOM> __global__ __launch_bounds__(256) void ns_scale_kernel(const Mats* __restrict__ list, float mu, int nesterov, float eps) {
   const Mats& t = *list;
   __shared__ float tile[64][65];
-  __shared__ double total;
+  __shared__ double total, red[256];
   const int k = find(t, SCALE, blockIdx.x), at = blockIdx.x - t.first[SCALE][k], tid = threadIdx.x;
   const Mat& a = t.mat[k];
+  if (few(a)) {
+    few_gram<T, MOM>(a, at, tile, red, mu, nesterov);
+    return;
+  }
   const int tn = a.np / 64, i0 = at / tn * 64, j0 = at % tn * 64;
   const bool flip = a.rows > a.cols;  // x[i][j] = u[j][i]
   float v[16];
@@ -403,12 +617,19 @@ __device__ __forceinline__ void triangle_tile(int at, int n, int& i, int& j) {
 
 // G = x x^T (POLY false) or P = b G + c G G (true): tiles (i, j <= i), written to both halves.  scale_g, scale_p: what G and P are stored times.
 template <int TILE, int WAVES, bool POLY>
-__global__ __launch_bounds__(64 * WAVES, 2) void ns_sym_kernel(const Mats* __restrict__ list, int which, float cb, float cc, float scale_g, float scale_p) {
+__global__ __launch_bounds__(64 * WAVES, 2) void ns_sym_kernel(const Mats* __restrict__ list, int step, float cb, float cc, float scale_g, float scale_p) {
   const Mats& t = *list;
   typedef Product<TILE, TILE, WAVES, false> Prod;
   __shared__ __attribute__((aligned(16))) char smem[Prod::BYTES];
-  const int block = near_tiles(blockIdx.x, gridDim.x), k = find(t, SYM, block), tid = threadIdx.x;
+  const int block = near_tiles(blockIdx.x, gridDim.x), k = find(t, SYM, block), tid = threadIdx.x, which = step & 1;
   const Mat a = t.mat[k];
+  if constexpr (TILE == 64) {  // (a list with such a matrix takes the small tiles: its sides are not multiples of 128)
+    static_assert(Prod::BYTES >= kFewBytes, "three matrices of doubles");
+    if (few(a)) {
+      if (!POLY && step == 0) few_solve(t, a, reinterpret_cast<double*>(smem));
+      return;
+    }
+  }
   int ti, tj;
   triangle_tile(block - t.first[SYM][k], a.mp / TILE, ti, tj);
   const int i0 = ti * TILE, j0 = tj * TILE;
@@ -468,12 +689,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ns_sym_kernel(const Mats* __res
 }
 
 // x <- a x + P x; the last one writes the result instead
-template <int TI, int TJ, int WAVES, typename T, int LAST> __global__ __launch_bounds__(64 * WAVES, 2) void ns_apply_kernel(const Mats* __restrict__ list, int which, float ca, float scale_p, const float* __restrict__ hp) {
+template <int TI, int TJ, int WAVES, typename T, int LAST> __global__ __launch_bounds__(64 * WAVES, 2) void ns_apply_kernel(const Mats* __restrict__ list, int step, float ca, float scale_p, const float* __restrict__ hp) {
   const Mats& t = *list;
   typedef Product<TJ, TI, WAVES, true> Prod;
   __shared__ __attribute__((aligned(16))) char smem[Prod::BYTES];
-  const int block = near_tiles(blockIdx.x, gridDim.x), k = find(t, APPLY, block), tid = threadIdx.x;
+  const int block = near_tiles(blockIdx.x, gridDim.x), k = find(t, APPLY, block), tid = threadIdx.x, which = step & 1;
   const Mat a = t.mat[k];
+  if constexpr (TI == 64 && TJ == 64) {
+    if (few(a)) {
+      if (step == 0) few_apply<T>(t, a, block - t.first[APPLY][k], reinterpret_cast<double*>(smem), hp);
+      return;
+    }
+  }
   int ti, tj;
   square_tile(block - t.first[APPLY][k], a.mp / TI, a.np / TJ, ti, tj);
   const int i0 = ti * TI, j0 = tj * TJ;
@@ -513,7 +740,7 @@ template <int TI, int TJ, int WAVES, typename T, int LAST> __global__ __launch_b
   if (LAST == 0) return;
   __syncthreads();
   const bool flip = a.rows > a.cols;
-  const float lr = LAST == 2 ? hp[2 * a.group] : 0.f, keep = LAST == 2 ? 1.f - lr * hp[2 * a.group + 1] : 0.f, step = lr * a.gain;
+  const float lr = LAST == 2 ? hp[2 * a.group] : 0.f, keep = LAST == 2 ? 1.f - lr * hp[2 * a.group + 1] : 0.f, rate = lr * a.gain;
   const int across = flip ? TI : TJ;
   constexpr int IN_FLIGHT = 8;
   for (int base = tid; base < TI * TJ; base += Prod::NT * IN_FLIGHT) {
@@ -533,7 +760,7 @@ template <int TI, int TJ, int WAVES, typename T, int LAST> __global__ __launch_b
       const float y = flip ? v[fast * Prod::OPITCH + slow] : v[slow * Prod::OPITCH + fast];
       if (!in[q]) continue;
       if (LAST == 1) gput<T>(a.dst, o[q], y);
-      else gput<float>(a.par, o[q], old[q] * keep - step * y);
+      else gput<float>(a.par, o[q], old[q] * keep - rate * y);
     }
   }
 }
@@ -573,8 +800,9 @@ template <typename F> long long wide_tiles(const Mats& t, F&& tiles) {  // 0: no
   }
   return n;
 }
-template <int TILE> int sym_tiles(const Mat& q) { return q.mp / TILE * (q.mp / TILE + 1) / 2; }
-template <int TI, int TJ> int all_tiles(const Mat& q) { return q.mp / TI * (q.np / TJ); }
+template <int TILE> int sym_tiles(const Mat& q) { return few(q) ? 1 : q.mp / TILE * (q.mp / TILE + 1) / 2; }
+template <int TI, int TJ> int all_tiles(const Mat& q) { return few(q) ? (q.n + kFewCols - 1) / kFewCols : q.mp / TI * (q.np / TJ); }
+int scale_tiles(const Mat& q) { return few(q) ? few_chunks(q) : all_tiles<64, 64>(q); }
 
 // What a step's G and P can reach: the singular values in front of it lie in 0 .. most (1 in front of the first step), those behind it in 0 .. the largest
 // |a s + b s^3 + c s^5| there.  Each is stored times 2^12 (2^10), or times the largest smaller power of two that keeps it under fp16's 65504 (a tenth of
@@ -623,32 +851,35 @@ bool stays_small(int steps, double a, double b, double c) {
   return true;
 }
 
-template <int TILE, int WAVES> void run_sym(const Mats* list, int n, int which, float b, float c, const Bounds& at, hipStream_t st) {
-  ns_sym_kernel<TILE, WAVES, false><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, which, b, c, at.scale_g(), at.scale_p());
-  ns_sym_kernel<TILE, WAVES, true><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, which, b, c, at.scale_g(), at.scale_p());
+template <int TILE, int WAVES> void run_sym(const Mats* list, int n, int step, bool poly, float b, float c, const Bounds& at, hipStream_t st) {
+  ns_sym_kernel<TILE, WAVES, false><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, step, b, c, at.scale_g(), at.scale_p());
+  if (poly) ns_sym_kernel<TILE, WAVES, true><<<dim3(n), dim3(64 * WAVES), 0, st>>>(list, step, b, c, at.scale_g(), at.scale_p());
 }
-template <typename T, int LAST> void run_apply(int tile, const Mats* list, int n, int which, float a, float scale_p, const float* hp, hipStream_t st) {
-  if (tile == SQUARE_128) ns_apply_kernel<128, 128, 8, T, LAST><<<dim3(n), dim3(512), 0, st>>>(list, which, a, scale_p, hp);
-  else if (tile == TALL) ns_apply_kernel<128, 64, 4, T, LAST><<<dim3(n), dim3(256), 0, st>>>(list, which, a, scale_p, hp);
-  else ns_apply_kernel<64, 64, 4, T, LAST><<<dim3(n), dim3(256), 0, st>>>(list, which, a, scale_p, hp);
+template <typename T, int LAST> void run_apply(int tile, const Mats* list, int n, int step, float a, float scale_p, const float* hp, hipStream_t st) {
+  if (tile == SQUARE_128) ns_apply_kernel<128, 128, 8, T, LAST><<<dim3(n), dim3(512), 0, st>>>(list, step, a, scale_p, hp);
+  else if (tile == TALL) ns_apply_kernel<128, 64, 4, T, LAST><<<dim3(n), dim3(256), 0, st>>>(list, step, a, scale_p, hp);
+  else ns_apply_kernel<64, 64, 4, T, LAST><<<dim3(n), dim3(256), 0, st>>>(list, step, a, scale_p, hp);
 }
 template <typename T, bool MOM> int run_list(Mats& t, Mats* list, int steps, float a, float b, float c, float eps, float mu, int nesterov, const float* hp, hipStream_t st) {
   const bool ws = wide_tiles(t, sym_tiles<128>) >= kWideSym;
   const long long wide = wide_tiles(t, all_tiles<128, 128>);
   const int wa = wide < kTallLeast ? SQUARE_64 : wide < kSquareLeast || wide > kSquareMost ? TALL : SQUARE_128;
   const int norms = prefix(t, NORM, [](const Mat& q) { return (int)(((long long)q.m * q.n + kNormItems - 1) / kNormItems); });
-  const int scales = prefix(t, SCALE, all_tiles<64, 64>);
+  const int scales = prefix(t, SCALE, scale_tiles);
   const int syms = ws ? prefix(t, SYM, sym_tiles<128>) : prefix(t, SYM, sym_tiles<64>);
   const int applies = wa == SQUARE_128 ? prefix(t, APPLY, all_tiles<128, 128>) : wa == TALL ? prefix(t, APPLY, all_tiles<128, 64>) : prefix(t, APPLY, all_tiles<64, 64>);
+  bool all_few = true;
+  for (int i = 0; i < t.count; ++i) all_few = all_few && few(t.mat[i]);
+  t.steps = steps; t.nesterov = nesterov; t.a = a; t.b = b; t.c = c; t.eps = eps; t.mu = mu;
   ns_norm_kernel<T, MOM><<<dim3(norms), dim3(256), 0, st>>>(t, list, mu, nesterov);
   ns_scale_kernel<T, MOM><<<dim3(scales), dim3(256), 0, st>>>(list, mu, nesterov, eps);
   constexpr int LAST = MOM ? 2 : 1;
   Bounds at(a, b, c);
-  for (int s = 0; s < steps; ++s, at.step()) {
-    if (ws) run_sym<128, 8>(list, syms, s & 1, b, c, at, st);
-    else run_sym<64, 4>(list, syms, s & 1, b, c, at, st);
-    if (s + 1 < steps) run_apply<T, 0>(wa, list, applies, s & 1, a, at.scale_p(), hp, st);
-    else run_apply<T, LAST>(wa, list, applies, s & 1, a, at.scale_p(), hp, st);
+  for (int s = 0; s < (all_few ? 1 : steps); ++s, at.step()) {
+    if (ws) run_sym<128, 8>(list, syms, s, !all_few, b, c, at, st);
+    else run_sym<64, 4>(list, syms, s, !all_few, b, c, at, st);
+    if (s + 1 < steps) run_apply<T, 0>(wa, list, applies, s, a, at.scale_p(), hp, st);
+    else run_apply<T, LAST>(wa, list, applies, s, a, at.scale_p(), hp, st);
   }
   CVH_CHECK_LAUNCH();
   return 0;

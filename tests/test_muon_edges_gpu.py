@@ -115,3 +115,61 @@ def test_a_capture_without_an_eager_step_is_refused():
     graph.replay()
     torch.cuda.synchronize()
     assert not torch.equal(p, before)
+
+
+def rounded(coefficients):
+    return tuple(torch.tensor(c, dtype=torch.float32).item() for c in coefficients)
+
+
+FEW = [(1, 1), (1, 2500), (2, 7), (3, 50), (16, 33), (17, 300), (22, 22), (23, 1000), (33, 66000), (39, 41), (40, 40), (40, 2500), (5, 70001)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", FEW)
+def test_few_rows(dtype, shape):
+    """up to 40 rows everything but the result is held in 64 bits: one rounding to the result's type (coefficients and eps are float32 numbers)"""
+    coefficients, eps = rounded(optim.NS_COEFFICIENTS), rounded([1e-7])[0]
+    for r, c in (shape, shape[::-1]):
+        g = torch.Generator(device="cuda").manual_seed(r)
+        u = (torch.randn(r, c, generator=g, device="cuda") * torch.logspace(0, -3, c, device="cuda")).to(dtype)
+        for steps in (1, 5):
+            got, want = optim.orthogonalize(u, steps=steps), steps64(u, steps, coefficients, eps)
+            off = (got.double().cpu() - want).abs()
+            assert bool((off <= want.abs() * (torch.finfo(dtype).eps / 2) + 1e-13).all()), float((off / want.abs().clamp(min=1e-30)).max())
+
+
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_few_rows_among_others_and_in_the_optimizer(nesterov):
+    """lists of few and many rows, each result that of its matrix alone; steps with momentum, rates and decay"""
+    shapes = [(1, 300), (300, 2), (100, 130), (40, 700), (41, 60), (64, 7, 3, 3), (8, 1, 3, 3), (500, 33)]
+    g = torch.Generator(device="cuda").manual_seed(7)
+    mats = [torch.randn(s[0], math.prod(s[1:]), generator=g, device="cuda") for s in shapes]
+    for x, u in zip(optim.orthogonalize(mats), mats):
+        assert torch.equal(x, optim.orthogonalize(u))
+    params = [torch.nn.Parameter(torch.randn(s, generator=g, device="cuda") * 0.1) for s in shapes]
+    opt = optim.Muon([{"params": params[::2], "lr": 0.05, "weight_decay": 0.1}, {"params": params[1::2]}], lr=0.01, momentum=0.9, nesterov=nesterov)
+    want = [p.detach().double().cpu() for p in params]
+    mom = [torch.zeros_like(w) for w in want]
+    for _ in range(3):
+        for i, p in enumerate(params):
+            p.grad = torch.randn(p.shape, generator=g, device="cuda")
+            g64 = p.grad.double().cpu()
+            mom[i] = 0.9 * mom[i] + g64
+            u = g64 + 0.9 * mom[i] if nesterov else mom[i]
+            lr, wd = (0.05, 0.1) if i % 2 == 0 else (0.01, 0.0)
+            x = steps64(u.reshape(p.shape[0], -1), 5, optim.NS_COEFFICIENTS)
+            want[i] = want[i] * (1 - lr * wd) - lr * max(1.0, p.shape[0] / x.shape[1]) ** 0.5 * x.view(p.shape)
+        opt.step()
+    for p, w, m in zip(params, want, mom):
+        assert float((p.detach().double().cpu() - w).norm() / w.norm()) <= 2.0 ** -17
+        assert float((opt.state[p]["momentum_buffer"].double().cpu() - m).norm() / m.norm()) <= 2.0 ** -22
+
+
+def test_few_rows_of_zeros_and_without_finite_values():
+    z, bad, u = torch.zeros(7, 90, device="cuda"), torch.ones(30, 50, device="cuda"), torch.randn(9, 40, device="cuda")
+    bad[3, 4] = float("inf")
+    x = optim.orthogonalize([z, bad, u])
+    assert torch.equal(x[0], z) and torch.isnan(x[1]).all() and torch.equal(x[2], optim.orthogonalize(u))
+    for s in (1e-30, 1e25):  # squares outside float32
+        want = steps64(u.double() * s, 5, rounded(optim.NS_COEFFICIENTS), 0.0)
+        assert float(((optim.orthogonalize(u * s, eps=0.0).double().cpu() - want).norm() / want.norm())) <= 2.0 ** -22
