@@ -13,11 +13,11 @@
 // from accumulator to operand registers and never touch LDS.  The waves of a workgroup share the staged K / V (or Q / dO) tiles, which are
 // double-buffered in LDS and loaded a tile ahead through registers.
 //
-// What bounds it (measured, MI355X): 128 columns, 20 k rows in 3 documents, 16 / 4 heads, causal forward: 613 us = 945 TFLOP/s of the 4 d a pair that have to
-// be computed; MFMA 48 %, arithmetic 43 %, LDS 48 % of the cycles, which two waves a SIMD overlap only in part.  Training there: 2640 us.  64 columns, 24.6 k rows,
-// 12 / 4 heads, training: forward 98, dq 130, dk / dv 191 us; a score costs an exponential and three other operations next to 1 / 4 of an MFMA.  128-row
+// What bounds it (measured, MI355X): 128 columns, 20 k rows in 3 documents, 16 / 4 heads, causal forward: 600 .. 640 us (cards differ) = 966 .. 905
+// TFLOP/s of the 4 d a pair that have to be computed; MFMA 48 %, arithmetic 43 %, LDS 48 % of the cycles, which two waves a SIMD overlap only in part.  Training
+// there: 2800 .. 2930 us.  64 columns, 24.6 k rows, 12 / 4 heads, training: forward 93, dq 134, dk / dv 169 us; a score costs an exponential and three other operations next to 1 / 4 of an MFMA.  128-row
 // workgroups: 4 waves share each staged tile; 64 keys (queries) a tile: at 64 columns 32 cost 20 % and 128 10 % in dk / dv, at 96 and 128 columns 32 cost 5 .. 8 % of
-// a whole training pass.  Captions (5 .. 77 tokens): one wave per 32 rows, 20 + 27 + 22 us for 13 k rows x 8 heads, latency.
+// a whole training pass.  Captions (5 .. 77 tokens): one wave per 32 rows, 20 + 27 + 21 us for 13 k rows x 8 heads, latency.
 //
 // Work items come from a plan (packed_plan_kernel) made once per batch: (sequence, block) pairs, most expensive first, so that the last
 // workgroups to start are the short ones; the list also has the rows behind the last sequence, whose results are written as zeros.

@@ -18,8 +18,8 @@
 // LDS, so that global memory sees whole rows.  Sides are padded to the tile with zeros, which the products keep zero: the main loop has no bounds.
 // All matrices of a list go through one launch per product: 2 + 3 steps launches for up to kMats matrices.
 //
-// Measured: 24 matrices of a 6-layer text tower of 512 (1536 x 512 .. 512 x 2048, float32): 870 us, of 526 at the library's rates; 4096 x 2048 in bf16: 1205 of
-// 842 us (P x at 815 TFLOP/s of MFMA; x x^T has 136 tiles for 256 units); 21 matrices of 144 .. 720: 160 us, 17 dependent launches of 7 .. 14 us.
+// Measured: 24 matrices of a 6-layer text tower of 512 (1536 x 512 .. 512 x 2048, float32): 830 .. 900 us (cards differ), of 526 at the library's rates; 4096 x 2048 in
+// bf16: 1175 .. 1280 of 842 us (P x at 880 TFLOP/s of MFMA; x x^T has 136 tiles for 256 units); 21 matrices of 144 .. 720: 161 us, 17 dependent launches of 7 .. 14 us.
 #include "common.hpp"
 #include "cvnets_hip.h"
 

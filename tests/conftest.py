@@ -35,8 +35,8 @@ def _references_without_miopen():
     [2, 16, 6, 6] x [24, 16, 1, 1] of tests/test_kernels_gpu.py::test_bn_eval_mode, MIOpen's backward-data solver
     `igemm_bwd_gtcx35_nhwc_fp32_bx0_ex1_bt128x32x8_...` reads past the end of its operands.  Inside the caching allocator's segments that is
     invisible; when the tensor happens to end a segment that is followed by an unmapped range (allocation history = test order) the GPU
-    faults.  tools/guard_aten_repro.py reproduces it with torch alone (no kernel of this repository runs) under the guard-page allocator
-    and passes with MIOpen off; profiles/r05_fault_root_cause.txt has the runs.  The product never calls MIOpen."""
+    faults.  Runs of that reference with torch alone (no kernel of this repository) under the guard-page allocator faulted with MIOpen and were clean
+    without it (profiles/r05_fault_root_cause.txt); tools/guard_aten_repro.py makes the clean one only.  The product never calls MIOpen."""
     try:
         import torch
         torch.backends.cudnn.enabled = False  # ("cudnn" is MIOpen on ROCm): ATen's native convolution / batch-norm kernels instead
