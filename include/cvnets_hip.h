@@ -447,7 +447,8 @@ int cvh_embed_lookup_bwd(int dtype, const long long* tok, const void* dout, floa
 typedef struct cvh_packed_attn {
   const void *q, *k, *v;
   void* out;    /* forward: written; backward: the forward's result */
-  void* out_lo; /* bf16, nullable: what the rounding of out left over, in out's layout; the backward's row sums dout . out are formed from both */
+  void* out_lo; /* nullable; the same in both directions.  bf16: what the rounding of out left over, in out's layout; the backward's row sums dout . out are formed
+                   from both.  float32: [heads_q][rows] float32, log2 of the softmax sums; lse then holds the maxima (times scale log2(e)) alone */
   const void* dout;
   void *dq, *dk, *dv;
   float *lse, *delta;

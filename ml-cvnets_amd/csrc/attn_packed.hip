@@ -249,6 +249,12 @@ template <bool ONE_WAVE, int N> __device__ __forceinline__ void accumulators(f32
 // share a unit (captions of 5 .. 77 tokens, 21 k rows, forward: bf16 26.9 -> 24.3 us, float32 65.6 -> 50.8 us; training 107 -> 105, 248 -> 227 us).
 constexpr int stages(int waves) { return waves == 1 ? 1 : 2; }
 
+// The softmax statistics that the backward pass takes up: one number a query, its maximum + log2 of its sum; in float32 the two by themselves where the caller has
+// room for them.  Their sum is rounded by 2^-24 of the maximum, which is an error of all probabilities of the query: with scores of 4096 dv was 4.7e-5 of its norm
+// off, with the two numbers 4.4e-6 (32-bit elementary operations: 3.1e-6), for 0 .. 2 % of a training pass.  (To the 8 bits of a bf16 probability it is nothing.)
+template <typename T> constexpr int statistics = sizeof(T) == 4 ? 3 : 2;  // of a query in the dk / dv kernel's LDS, with delta
+template <typename T> __device__ __forceinline__ float* log_sums(const PA& p) { return sizeof(T) == 4 ? reinterpret_cast<float*>(p.out_lo) : nullptr; }
+
 struct Item {
   int seq, block, head, start, len;
 };
@@ -398,10 +404,15 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
   l = both_halves_sum(l);
   const float inv = 1.0f / l;
   const long long row = w.start + (q_ok ? my_q : 0);
-  T* const lo = p.out_lo != nullptr ? reinterpret_cast<T*>(p.out_lo) + w.head * p.o_head + row * p.o_row : nullptr;
+  T* const lo = sizeof(T) == 2 && p.out_lo != nullptr ? reinterpret_cast<T*>(p.out_lo) + w.head * p.o_head + row * p.o_row : nullptr;
 #pragma unroll
   for (int f = 0; f < NF; ++f) store_rows(out + row * p.o_row, lo, o[f], inv, 32 * f, p.d, lane, q_ok);
-  if (lane < 32 && q_ok && p.lse != nullptr) p.lse[(long long)w.head * p.rows + row] = fmaf(m, c, __log2f(l));
+  if (lane < 32 && q_ok && p.lse != nullptr) {
+    const long long at = (long long)w.head * p.rows + row;
+    float* const sums = log_sums<T>(p);
+    p.lse[at] = sums != nullptr ? m * c : fmaf(m, c, __log2f(l));
+    if (sums != nullptr) sums[at] = __log2f(l);
+  }
 }
 
 // -----------------------------------------------------------------------------------------------------------------------------------------
@@ -427,7 +438,8 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
   const T* const qb = reinterpret_cast<const T*>(p.q) + (long long)w.start * p.q_row + w.head * p.q_head;
   const T* const db = reinterpret_cast<const T*>(p.dout) + (long long)w.start * p.do_row + w.head * p.do_head;
   const T* const ob = reinterpret_cast<const T*>(p.out) + (long long)w.start * p.o_row + w.head * p.o_head;
-  const T* const lb = reinterpret_cast<const T*>(p.out_lo != nullptr ? p.out_lo : p.out) + (long long)w.start * p.o_row + w.head * p.o_head;
+  const bool two = sizeof(T) == 2 && p.out_lo != nullptr;
+  const T* const lb = reinterpret_cast<const T*>(two ? p.out_lo : p.out) + (long long)w.start * p.o_row + w.head * p.o_head;
   const T* const kb = reinterpret_cast<const T*>(p.k) + (long long)w.start * p.k_row + kv_head * p.k_head;
   const T* const vb = reinterpret_cast<const T*>(p.v) + (long long)w.start * p.v_row + kv_head * p.v_head;
   const int keys = p.causal ? min(w.len, first + 32 * NW) : w.len;
@@ -448,7 +460,7 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
   float delta = 0.f;
   {
     const rsrc_t rq = tile_rows(qb, p.q_row, q0, w.len, p.d), rd = tile_rows(db, p.do_row, q0, w.len, p.d), ro = tile_rows(ob, p.o_row, q0, w.len, p.d);
-    const rsrc_t rl = p.out_lo != nullptr ? tile_rows(lb, p.o_row, q0, w.len, p.d) : rows_of(lb, 0);
+    const rsrc_t rl = two ? tile_rows(lb, p.o_row, q0, w.len, p.d) : rows_of(lb, 0);
     const int r = (lane & 31) * (int)sizeof(T), oq = r * (int)p.q_row, od = r * (int)p.do_row, oo = r * (int)p.o_row;
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
@@ -460,7 +472,8 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
   }
   delta = both_halves_sum(delta);
   const long long row = w.start + (q_ok ? my_q : 0), at = (long long)w.head * p.rows + row;
-  const float lse = p.lse[at];
+  const float* const sums = log_sums<T>(p);
+  const float lse = p.lse[at], log_sum = sums != nullptr ? sums[at] : 0.f;
   if (lane < 32 && q_ok) p.delta[at] = delta;  // read by the dk / dv kernel behind this one
   kt.store(Kl, tid);
   vt.store(Vl, tid);
@@ -497,7 +510,7 @@ template <typename T, int CP, int NW, int KB, int OCC> __global__ __launch_bound
         mma32(dp, tile.rows(Vt, 32 * b, 16 * k), df[k]);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = pexp2(fmaf(s[r], c, -lse)) * dp[r];
+      for (int r = 0; r < 16; ++r) s[r] = pexp2(sizeof(T) == 4 ? fmaf(s[r], c, -lse) - log_sum : fmaf(s[r], c, -lse)) * dp[r];
       if (masked) {
         const int last = (p.causal ? min(my_q, w.len - 1) : w.len - 1) - k0 - 32 * b - 4 * (lane >> 5);
 #pragma unroll
@@ -528,7 +541,8 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* const Ql = reinterpret_cast<T*>(smem);
   T* const Dl = Ql + ST * QB * PT;
-  float* const Ll = reinterpret_cast<float*>(Dl + ST * QB * PT);  // [ST][2][NT]: log-sums and -deltas of a tile's queries
+  constexpr int NL = statistics<T>;
+  float* const Ll = reinterpret_cast<float*>(Dl + ST * QB * PT);  // [ST][NL][NT]: log-sums (maxima), -deltas, (log-sums) of a tile's queries
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Item w = work_item(p, p.heads_kv);
   if (w.seq < -1) return;
@@ -553,7 +567,8 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
   qt.place(p.q_row, p.d, tid);
   dt.place(p.do_row, p.d, tid);
   const Tile<T, CP> tile(lane);
-  float lse, delta;
+  float lse, delta, log_sum = 0.f;
+  const float* const sums = log_sums<T>(p);
   int next_head = w.head * group, next_q = w.len;  // of the tile that is requested next; behind a head's last one: start the next head
   const int end_head = next_head + group, offset = tid < QB ? tid * 4 : kBeyond;
   auto request = [&]() {
@@ -570,13 +585,15 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
     const long long bytes = next_head <= end_head ? (long long)(w.len - next_q) * 4 : 0;
     lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows_of(p.lse + at, bytes), offset, 0, 0));
     delta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows_of(p.delta + at, bytes), offset, 0, 0));
+    if (sizeof(T) == 4) log_sum = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows_of(sums + (sums != nullptr ? at : 0), sums != nullptr ? bytes : 0), offset, 0, 0));
     next_q += QB;
   };
   auto store = [&](int t) {
     qt.store(Ql + t % ST * QB * PT, tid);
     dt.store(Dl + t % ST * QB * PT, tid);
-    Ll[t % ST * 2 * NT + tid] = lse;
-    Ll[t % ST * 2 * NT + NT + tid] = -delta;
+    Ll[t % ST * NL * NT + tid] = lse;
+    Ll[t % ST * NL * NT + NT + tid] = -delta;
+    if (NL == 3) Ll[t % ST * NL * NT + 2 * NT + tid] = log_sum;
   };
   request();
   Frag<T> kf[NK], vf[NK];
@@ -608,7 +625,7 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
     if (ST > 1) advance();
     const T* const Qt = Ql + t % ST * QB * PT;
     const T* const Dt = Dl + t % ST * QB * PT;
-    const float* const Lt = Ll + t % ST * 2 * NT;
+    const float* const Lt = Ll + t % ST * NL * NT;
     if (NW > 1 && (k0 >= w.len || (p.causal && q0 + QB - 1 < k0))) continue;  // no key of this wave, or none of the tile's queries sees one
     const bool masked = q0 + QB > w.len || (p.causal && q0 < k0 + 31);
 #pragma unroll
@@ -632,9 +649,13 @@ template <typename T, int CP, int NW, int QB, int OCC> __global__ __launch_bound
         for (int i = 0; i < 4; ++i) {
           const float4 ls = *reinterpret_cast<const float4*>(Lt + 32 * (b0 + b) + 8 * i + 4 * (lane >> 5));
           const float lv[4] = {ls.x, ls.y, ls.z, ls.w};
+          float4 lg = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (NL == 3) lg = *reinterpret_cast<const float4*>(Lt + 2 * NT + 32 * (b0 + b) + 8 * i + 4 * (lane >> 5));
+          const float gv[4] = {lg.x, lg.y, lg.z, lg.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            s[b][4 * i + e] = pexp2(fmaf(s[b][4 * i + e], c, -lv[e]));
+            const float x = fmaf(s[b][4 * i + e], c, -lv[e]);
+            s[b][4 * i + e] = pexp2(NL == 3 ? x - gv[e] : x);
             dp[b][4 * i + e] *= s[b][4 * i + e];
           }
         }
@@ -762,7 +783,7 @@ template <typename T, int CP, int NW, int KB> int launch_bwd(const PA& p, hipStr
   constexpr auto dkv = packed_attn_dkv_kernel<T, CP, NW, QB, occ<T, CP, NW>(true)>;
   static DynSmemAttr aq, ak;
   constexpr int tiles = 2 * stages(NW);
-  const size_t sq = (size_t)tiles * KB * Tile<T, CP>::PT * sizeof(T), sk = (size_t)tiles * QB * Tile<T, CP>::PT * sizeof(T) + tiles * 64 * NW * sizeof(float);
+  const size_t sq = (size_t)tiles * KB * Tile<T, CP>::PT * sizeof(T), sk = (size_t)tiles * QB * Tile<T, CP>::PT * sizeof(T) + stages(NW) * statistics<T> * 64 * NW * sizeof(float);
   if (hipError_t e = aq.ensure((const void*)dq, sq)) return (int)e;
   if (hipError_t e = ak.ensure((const void*)dkv, sk)) return (int)e;
   dq<<<dim3((unsigned)(p.places * p.heads_q)), dim3(64 * NW), sq, st>>>(p);
@@ -798,7 +819,7 @@ int check(int dtype, const PA* p, int backward) {
   if (!strides_ok(dtype, p->q, p->q_row, p->q_head) || !strides_ok(dtype, p->k, p->k_row, p->k_head) || !strides_ok(dtype, p->v, p->v_row, p->v_head) ||
       !strides_ok(dtype, p->out, p->o_row, p->o_head))
     return -2;
-  if (p->out_lo != nullptr && (dtype != CVH_DT_BF16 || (reinterpret_cast<uintptr_t>(p->out_lo) & 15))) return -2;
+  if (p->out_lo != nullptr && (reinterpret_cast<uintptr_t>(p->out_lo) & 15)) return -2;
   if (backward && (p->lse == nullptr || p->delta == nullptr || !strides_ok(dtype, p->dout, p->do_row, p->do_head) || !strides_ok(dtype, p->dq, p->dq_row, p->dq_head) ||
                    !strides_ok(dtype, p->dk, p->dk_row, p->dk_head) || !strides_ok(dtype, p->dv, p->dv_row, p->dv_head)))
     return -2;

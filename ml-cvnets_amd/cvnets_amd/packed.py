@@ -123,10 +123,11 @@ def _launch(name: str, seqs: PackedSeqs, scale: float, causal: bool, q, k, v, ou
 
 
 def _forward(q: Tensor, k: Tensor, v: Tensor, seqs: PackedSeqs, causal: bool, scale: float, grad: bool):
-    """(out, out_lo, lse); the last two are for the backward only: in bf16 the row sums dout . out are formed from 16 bits of out, not 8"""
+    """(out, out_lo, lse); the last two are for the backward only: in bf16 the row sums dout . out are formed from 16 bits of out, not 8; in float32 out_lo is
+    the second part of the softmax statistics"""
     rows, heads, d = q.shape
     out = torch.empty((rows, heads, d), dtype=q.dtype, device=q.device)
-    out_lo = torch.empty((rows, heads, d), dtype=q.dtype, device=q.device) if grad and q.dtype == torch.bfloat16 else None
+    out_lo = torch.empty((rows, heads, d) if q.dtype == torch.bfloat16 else (heads, rows), dtype=q.dtype, device=q.device) if grad else None
     lse = torch.empty((heads, rows), dtype=torch.float32, device=q.device) if grad else None
     _launch("cvh_packed_attn_fwd", seqs, scale, causal, q, k, v, out, out_lo, lse)
     return out, out_lo, lse

@@ -260,3 +260,51 @@ def test_more_rows_than_one_line_of_workgroups():
     dy[some] = torch.randint(-3, 4, (some.numel(), 8), generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").to(torch.bfloat16)
     (dtable,) = torch.autograd.grad(out, (table,), dy)
     assert torch.equal(dtable.double(), torch.zeros(vocab, 8, dtype=torch.float64, device="cuda").index_add_(0, ids[some], dy[some].double()))
+    del out, dy, ids
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("block", [32, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("height", [1.0, 64.0, 8192.0])
+def test_float32_gradients_of_large_scores(block, causal, height, monkeypatch):
+    """equal keys: every probability is one over the number of keys, whatever the scores are.  The exponent's argument, behind the maximum and the log-sum, is
+    at most 8, so that the tolerance of ordinary scores holds (with maximum and log-sum added up first it was 2^-24 of 1.44 times 8192)"""
+    monkeypatch.setattr(packed, "_block_rows", lambda *_: block)
+    lens, d = [200, 1, 77], 64
+    g = torch.Generator(device="cuda").manual_seed(2)
+    e = torch.randint(0, 2, (d,), generator=g, device="cuda") * 2.0 - 1.0  # e . e = 64
+    q = e.expand(278, 4, d).contiguous().requires_grad_(True)
+    k = (e * (height / 64)).expand(278, 2, d).contiguous().requires_grad_(True)
+    v, dout = (torch.randn(278, h, d, generator=g, device="cuda") for h in (2, 4))
+    v.requires_grad_(True)
+    out = packed.attention(q, k, v, packed.PackedSeqs.from_lengths(lens, "cuda"), causal=causal, scale=1.0)
+    (dv,) = torch.autograd.grad(out, (v,), dout)
+    want_out, want_dv, a = torch.zeros(278, 4, d, dtype=torch.float64, device="cuda"), torch.zeros(278, 2, d, dtype=torch.float64, device="cuda"), 0
+    for n in lens:
+        p = torch.ones(n, n, dtype=torch.float64, device="cuda")
+        p = p.tril() if causal else p
+        p = p / p.sum(1, keepdim=True)
+        for h in range(4):
+            want_out[a:a + n, h] = p @ v.detach()[a:a + n, h // 2].double()
+            want_dv[a:a + n, h // 2] += p.t().contiguous() @ dout[a:a + n, h].double()
+        a += n
+    assert rel(out.detach(), want_out) <= TOL[torch.float32] and rel(dv, want_dv) <= TOL[torch.float32]
+
+
+def test_float32_statistics_in_one_number():
+    """callers of the C entry without room for the second part: one number a query, as in bf16"""
+    rows, d = 261, 64
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q, k, v, dout = (torch.randn(rows, h, d, generator=g, device="cuda") for h in (4, 2, 2, 4))
+    seqs = packed.PackedSeqs.from_lengths([70, 1, 190], "cuda")
+    t = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    out = packed.attention(*t, seqs)
+    want = torch.autograd.grad(out, t, dout)
+    one, lse = torch.empty_like(q), torch.empty(4, rows, device="cuda")
+    packed._launch("cvh_packed_attn_fwd", seqs, d ** -0.5, True, q, k, v, one, None, lse)
+    got = [torch.empty_like(x) for x in (q, k, v)]
+    packed._launch("cvh_packed_attn_bwd", seqs, d ** -0.5, True, q, k, v, one, None, lse, torch.empty_like(lse), dout, *got)
+    assert torch.equal(one, out.detach())
+    for a, b in zip(got, want):
+        assert rel(a, b) <= 2 * TOL[torch.float32]
