@@ -148,7 +148,7 @@ class TextTransformer(nn.Module):
             t = layer.forward_tokens(t, ops.NO_SEQMAP, causal=True, seqs=seqs)
         t = ops.layer_norm_tokens(t, self.final_layer_norm, ops.NO_SEQMAP)
         start, end = seqs.plan[:seqs.seqs], seqs.plan[1:seqs.seqs + 1]  # the clamped boundaries
-        ends = torch.where(end > start, end - 1, -1).long()  # plumbing: EOT index arithmetic; empty sequences have no row
+        ends = (end * (end > start) - 1).long()  # plumbing: EOT index arithmetic; -1: an empty sequence has no row
         return ops.l2_normalize(ops.linear(ops.RowsGatherIdx.apply(t, ends), self.projection_layer.t()))
 
     def forward_zero_shot(self, text_tokens: Tensor, key_padding_mask: Optional[Tensor] = None, *args, **kwargs) -> Tensor:

@@ -308,3 +308,47 @@ def test_float32_statistics_in_one_number():
     assert torch.equal(one, out.detach())
     for a, b in zip(got, want):
         assert rel(a, b) <= 2 * TOL[torch.float32]
+
+
+def test_a_captured_tower_follows_captions_that_come_and_go():
+    """forward and gradients of one graph over batches with other captions, places and rows, some of them empty: those of the eager tower, to the bit"""
+    model = tower()
+    for p in model.parameters():
+        p.grad = torch.zeros_like(p)
+    rows, places = 90, 6
+    ids = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    cu = torch.zeros(places + 1, dtype=torch.int32, device="cuda")
+    dy = torch.randn(places, 64, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    seqs = packed.PackedSeqs(cu, rows, context_length=24)
+
+    def fill(lengths, seed):
+        cu.copy_(torch.tensor([sum(lengths[:i]) for i in range(places + 1)], dtype=torch.int32))
+        ids.copy_(torch.randint(1, 298, (rows,), generator=torch.Generator().manual_seed(seed)))
+
+    def step():
+        for p in model.parameters():
+            p.grad.zero_()
+        seqs.refresh()
+        y = model.encode_packed(ids, seqs)
+        y.backward(dy)
+        return y.detach()
+
+    fill([5, 9, 24, 1, 7, 3], 0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i, lengths in enumerate(([5, 0, 24, 0, 0, 3], [0, 0, 0, 0, 0, 8], [1, 24, 24, 24, 0, 17], [0, 0, 0, 0, 0, 0], [5, 9, 24, 1, 7, 3])):
+        fill(lengths, i)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [held.clone()] + [p.grad.clone() for p in model.parameters()]
+        want = [step()] + [p.grad for p in model.parameters()]
+        torch.cuda.synchronize()
+        assert bool((got[0][[j for j, n in enumerate(lengths) if n == 0]] == 0).all())
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), lengths
